@@ -1,0 +1,39 @@
+/*
+ * aclnnMoeAddRmsNormQuant — residual addition, RMS norm and dynamic quantisation of rows in one pass.
+ * An operator of this library without a counterpart among the entry points it replaces: what stands in front of every MoE
+ * block.  yOut and scaleOut are the int8 rows and scales that aclnnMoeInitRoutingV2 / V3 route, normOut the rows that
+ * aclnnMoeRouterLogits multiplies, sumOut the residual of the next block.
+ *
+ * Per row of H values:
+ *   s = x + residual, rounded to x's type (s = x without a residual)                              -> sumOutOptional
+ *   n = s * (1 / sqrt(mean(s^2) + epsilon)) * gamma, in fp32                                       -> normOutOptional (rounded)
+ *   v = n * smoothScale;  scale = max|v| / 127;  y = round_half_even(v / scale) in [-127, 127]     -> yOut, scaleOut
+ * A row with scale 0 (zeros, or squares whose sum passes fp32) gives zeros; one with a NaN or an infinity gives scale NaN and zeros in y.
+ *
+ * x, residualOptional, sumOutOptional, normOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents;
+ * gamma [H] of x's type or FLOAT; smoothScaleOptional FLOAT [H]; yOutOptional INT8 of x's extents with scaleOutOptional FLOAT of x's
+ * extents without the last (both or neither; without them the operator is a plain RMS norm); at least one of normOut and yOut.
+ * Inputs may be strided views; outputs are contiguous.  sumOut may be x's or residual's own memory, entirely; no other output
+ * may share memory with an input or another output.
+ */
+#ifndef OPS_TRANSFORMER_AMD_ACLNN_MOE_ADD_RMS_NORM_QUANT_H_
+#define OPS_TRANSFORMER_AMD_ACLNN_MOE_ADD_RMS_NORM_QUANT_H_
+
+#include "acl/acl.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+ACLNN_API aclnnStatus aclnnMoeAddRmsNormQuantGetWorkspaceSize(
+    const aclTensor* x, const aclTensor* residualOptional, const aclTensor* gamma, const aclTensor* smoothScaleOptional,
+    double epsilon, const aclTensor* yOutOptional, const aclTensor* scaleOutOptional, const aclTensor* normOutOptional,
+    const aclTensor* sumOutOptional, uint64_t* workspaceSize, aclOpExecutor** executor);
+
+ACLNN_API aclnnStatus aclnnMoeAddRmsNormQuant(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                              aclrtStream stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

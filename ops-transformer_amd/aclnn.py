@@ -61,6 +61,12 @@ _PHASE1_SIGNATURES = {
         [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, ctypes.c_bool, _I64, _VP, _VP, _VP, _VP, _VP, _U64P, _VPP],
     "aclnnMoeGatingTopKSoftmaxV2GetWorkspaceSize":
         [_VP, _VP, _I64, _I64, ctypes.c_bool, _VP, _VP, _VP, _U64P, _VPP],
+    "aclnnMoeAddRmsNormQuantGetWorkspaceSize":
+        [_VP, _VP, _VP, _VP, ctypes.c_double, _VP, _VP, _VP, _VP, _U64P, _VPP],
+    "aclnnMoeRouterLogitsGetWorkspaceSize":
+        [_VP, _VP, _VP, _U64P, _VPP],
+    "aclnnMoeGatingTopKGroupedGetWorkspaceSize":
+        [_VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_double, ctypes.c_double, _VP, _VP, _VP, _U64P, _VPP],
     "aclnnMoeInitRoutingV3GetWorkspaceSize":
         [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, ctypes.c_bool, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _U64P, _VPP],
     "aclnnGroupedMatmulSwigluQuantGetWorkspaceSize":
@@ -89,7 +95,7 @@ _PHASE1_SIGNATURES = {
 _PHASE2 = ["aclnnMoeInitRoutingQuantV2", "aclnnGroupedMatmulSwigluQuantWeightNZ", "aclnnGroupedMatmulWeightNz",
            "aclnnGroupedMatmulFinalizeRoutingWeightNz", "aclnnGroupedMatmulFinalizeRoutingWeightNzV2", "aclnnGroupedMatmulFinalizeRouting", "aclnnGroupedMatmulFinalizeRoutingV2", "aclnnGroupedMatmulFinalizeRoutingV3",
            "aclnnMoeGatingTopKSoftmaxV2", "aclnnMoeInitRoutingV2", "aclnnMoeInitRoutingV3", "aclnnGroupedMatmulSwigluQuant", "aclnnGroupedMatmulV4", "aclnnGroupedMatmulV5",
-           "aclnnMoeFinalizeRoutingV2"]
+           "aclnnMoeFinalizeRoutingV2", "aclnnMoeAddRmsNormQuant", "aclnnMoeRouterLogits", "aclnnMoeGatingTopKGrouped"]
 
 
 def lib():
@@ -282,8 +288,10 @@ def _run_two_phase(api, args, device, workspace=None, static_workspace_api=None)
 
 # Operators of opapiPlanPacked (include/opapi_descriptor.h), by number.
 _PLANNED = ("aclnnMoeGatingTopKSoftmaxV2", "aclnnMoeInitRoutingV2", "aclnnMoeInitRoutingQuantV2", "aclnnMoeInitRoutingV3",
-            "aclnnGroupedMatmulSwigluQuant", "aclnnGroupedMatmulV4", "aclnnMoeFinalizeRoutingV2")
-(_GATING, _ROUTING_V2, _ROUTING_QUANT_V2, _ROUTING_V3, _SWIGLU_QUANT, _GROUPED_MATMUL_V4, _FINALIZE_V2) = range(7)
+            "aclnnGroupedMatmulSwigluQuant", "aclnnGroupedMatmulV4", "aclnnMoeFinalizeRoutingV2", "aclnnMoeAddRmsNormQuant",
+            "aclnnMoeRouterLogits", "aclnnMoeGatingTopKGrouped")
+(_GATING, _ROUTING_V2, _ROUTING_QUANT_V2, _ROUTING_V3, _SWIGLU_QUANT, _GROUPED_MATMUL_V4, _FINALIZE_V2, _ADD_RMS_NORM_QUANT, _ROUTER_LOGITS,
+ _GATING_GROUPED) = range(10)
 
 
 def _packed(t):
@@ -419,6 +427,66 @@ def moe_gating_top_k_softmax_v2(x, k, renorm=0, finished=None, output_softmax=Fa
         sm = torch.empty(tuple(x.shape), dtype=torch.float32, device=dev) if (output_softmax and renorm == 0) else None
     _run_packed(_GATING, (k, renorm, bool(output_softmax)), (x, finished, y, idx, sm), dev)
     return y, idx, sm
+
+
+def _check_device(api, device, *tensors):
+    """The kernels run on the current device, on its current stream: tensors of another device, or of the host, are refused."""
+    if device.type != "cuda" or device.index != torch.cuda.current_device():
+        raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s, not on the current GPU" % device)
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s and %s" % (device, t.device))
+
+
+def _bits(value):
+    """A double as opapiPlanPacked takes it among whole numbers."""
+    return _REAL_AS_WHOLE.unpack(_REAL.pack(value))[0]
+
+
+_REAL, _REAL_AS_WHOLE = struct.Struct("d"), struct.Struct("q")
+
+
+def moe_add_rms_norm_quant(x, gamma, residual=None, smooth_scale=None, epsilon=1e-6, quantise=True, output_norm=True, output_sum=True,
+                           out=None, workspace=None):
+    """aclnnMoeAddRmsNormQuant.  Returns (y int8, scale fp32, norm, sum) of the rows x + residual: the RMS norm of the sum in x's dtype, its
+    int8 rows with a scale each (None, None with quantise=False) and the sum itself (None without a residual).  ``out`` may carry
+    the outputs in that order, None for those that are not wanted; its sum may be x or residual."""
+    if out is not None:
+        y, scale, norm, total = out
+    else:
+        y = torch.empty(x.shape, dtype=torch.int8, device=x.device) if quantise else None
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantise else None
+        norm = torch.empty(x.shape, dtype=x.dtype, device=x.device) if output_norm else None
+        total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if output_sum and residual is not None else None
+    _check_device("aclnnMoeAddRmsNormQuant", x.device, gamma, residual, smooth_scale, y, scale, norm, total)
+    _run_packed(_ADD_RMS_NORM_QUANT, (_bits(epsilon),), (x, residual, gamma, smooth_scale, y, scale, norm, total), x.device, workspace)
+    return y, scale, norm, total
+
+
+def moe_router_logits(x, weight, out=None, workspace=None):
+    """aclnnMoeRouterLogits.  Returns logits fp32 [..., E] of x [..., H] and weight [E, H] (x's dtype or fp32)."""
+    if out is None:
+        out = torch.empty(x.shape[:-1] + weight.shape[:1], dtype=torch.float32, device=x.device)
+    _check_device("aclnnMoeRouterLogits", x.device, weight, out)
+    _run_packed(_ROUTER_LOGITS, (), (x, weight, out), x.device, workspace)
+    return out
+
+
+def moe_gating_top_k_grouped(x, k, bias=None, finished=None, k_group=1, group_count=1, group_select_mode=0, score_type=0, renorm=0,
+                             routed_scaling_factor=1.0, eps=1e-20, y_dtype=None, output_scores=False, out=None, workspace=None):
+    """aclnnMoeGatingTopKGrouped.  Returns (y [..., k] in y_dtype (x's or fp32; x's when not given), expertIdx int32 [..., k], scores fp32
+    [..., E] or None).  score_type 0 softmax, 1 sigmoid; group_select_mode 0 largest, 1 sum of the two largest."""
+    if out is not None:
+        y, idx, scores = out
+    else:
+        lead = x.shape[:-1]
+        y = torch.empty(lead + (k,), dtype=x.dtype if y_dtype is None else y_dtype, device=x.device)
+        idx = torch.empty(lead + (k,), dtype=torch.int32, device=x.device)
+        scores = torch.empty(x.shape, dtype=torch.float32, device=x.device) if output_scores else None
+    _check_device("aclnnMoeGatingTopKGrouped", x.device, bias, finished, y, idx, scores)
+    _run_packed(_GATING_GROUPED, (k, k_group, group_count, group_select_mode, score_type, renorm, _bits(routed_scaling_factor), _bits(eps)),
+                (x, bias, finished, y, idx, scores), x.device, workspace)
+    return y, idx, scores
 
 
 def moe_init_routing_v3(x, expert_idx, scale=None, expert_num=0, expert_tokens_num_type=1, quant_mode=-1,

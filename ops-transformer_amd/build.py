@@ -22,6 +22,9 @@ EXPORTS = os.path.join(CSRC, "exports.map")  # linker version script: only the C
 SOURCES = [
     "acl_runtime.cpp",
     "moe_gating_top_k_softmax_v2.hip",
+    "moe_add_rms_norm_quant.hip",
+    "moe_router_logits.hip",
+    "moe_gating_top_k_grouped.hip",
     "moe_init_routing.hip",
     "grouped_gemm_i8.hip",
     "grouped_gemm_i8_int32.hip",

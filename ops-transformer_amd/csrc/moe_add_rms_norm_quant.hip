@@ -1,0 +1,234 @@
+// aclnnMoeAddRmsNormQuant for gfx950: s = x + residual, n = rms_norm(s) * gamma, int8 rows of n * smooth with a scale each.
+//
+// With r = 1 / sqrt(mean(s^2) + eps) the scale's maximum is max|s r gamma smooth| = r max|s gamma smooth|, and r cancels in
+// v / scale: y = round(127 w / max|w|) with w = s gamma smooth.  So one reduction over the row yields the sum of squares and the
+// maximum together, and the row is done after a single exchange between its waves.  Sums, r, n and w are fp32; what is rounded is s
+// (to the stream's type, and that rounded value is what is normalised: norm and sum agree whether or not the sum is asked for), n where
+// it leaves, and y.
+#include "moe_front.h"
+
+#include <cmath>
+
+#include "aclnnop/aclnn_moe_add_rms_norm_quant.h"
+
+namespace {
+
+using namespace moe_front;
+
+struct NormArgs {
+    const void* x;
+    const void* residual;  // optional
+    const void* gamma;
+    const float* smooth;   // optional
+    int8_t* y;             // optional, with scale
+    float* scale;
+    void* norm;            // optional
+    void* sum;             // optional; may be x's or residual's memory
+    int64_t rows;
+    int64_t cols;
+    float eps;
+};
+
+// What a row's reduction settles.
+struct RowScales {
+    float r;      // of the norm
+    float scale;  // of the int8 row
+    float up;     // w is taken times `up` before `inv`, so that 127 / max|w| stays finite for rows of tiny values
+    float inv;    // 0 where the row's int8 values are zeros
+};
+
+// sumSquares and maxBits (the bits of max|w|, whose order as unsigned numbers is that of the values, NaN last) are the row's.
+__device__ __forceinline__ RowScales ScalesOf(float sumSquares, uint32_t maxBits, int64_t cols, float eps) {
+    RowScales s;
+    const float mean = sumSquares / static_cast<float>(cols) + eps;
+    s.r = mean == 0.f ? 0.f : 1.f / sqrtf(mean);
+    const float m = __uint_as_float(maxBits);
+    s.scale = m * s.r / 127.f;
+    s.up = m < 0x1p-100f ? 0x1p100f : 1.f;
+    s.inv = s.scale > 0.f && s.scale < INFINITY ? 127.f / (m * s.up) : 0.f;
+    return s;
+}
+
+__device__ __forceinline__ int32_t Quantised(float w, const RowScales& s) {
+    return s.inv == 0.f ? 0 : static_cast<int32_t>(fminf(fmaxf(rintf(w * s.up * s.inv), -127.f), 127.f));
+}
+
+template <int kWaves>
+__device__ __forceinline__ void ReduceRow(float& sumSquares, uint32_t& maxBits) {
+    sumSquares = WaveSum(sumSquares);
+    maxBits = WaveMax(maxBits);
+    if constexpr (kWaves > 1) {
+        __shared__ float sums[kWaves];
+        __shared__ uint32_t maxima[kWaves];
+        if (threadIdx.x % kWave == 0) {
+            sums[threadIdx.x / kWave] = sumSquares;
+            maxima[threadIdx.x / kWave] = maxBits;
+        }
+        __syncthreads();
+        sumSquares = sums[0];
+        maxBits = maxima[0];
+        for (int w = 1; w < kWaves; ++w) {
+            sumSquares += sums[w];
+            maxBits = max(maxBits, maxima[w]);
+        }
+    }
+}
+
+// Rows of any length and alignment: a workgroup per row, one element at a time, the row read again for the outputs (from the sum where that
+// was written, by the same lane: it may lie in x's memory).
+constexpr int kAnyThreads = 256;
+
+template <typename Codec, typename Gamma>
+__global__ __launch_bounds__(kAnyThreads) void NormQuantAnyKernel(NormArgs a) {
+    using S = typename Codec::Storage;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * a.cols;
+    const S* const x = static_cast<const S*>(a.x) + at;
+    const S* const residual = a.residual == nullptr ? nullptr : static_cast<const S*>(a.residual) + at;
+    S* const sum = a.sum == nullptr ? nullptr : static_cast<S*>(a.sum) + at;
+    const typename Gamma::Storage* const gamma = static_cast<const typename Gamma::Storage*>(a.gamma);
+    float sumSquares = 0.f;
+    uint32_t maxBits = 0;
+    auto rounded = [&](int64_t c) { return residual == nullptr ? x[c] : Codec::Store(Codec::Load(x[c]) + Codec::Load(residual[c])); };
+    auto weight = [&](int64_t c) { return a.smooth == nullptr ? 1.f : a.smooth[c]; };
+    for (int64_t c = threadIdx.x; c < a.cols; c += kAnyThreads) {
+        const S raw = rounded(c);
+        if (sum != nullptr) sum[c] = raw;
+        const float s = Codec::Load(raw);
+        sumSquares = fmaf(s, s, sumSquares);
+        maxBits = max(maxBits, __float_as_uint(fabsf(s * Gamma::Load(gamma[c]) * weight(c))));
+    }
+    ReduceRow<kAnyThreads / kWave>(sumSquares, maxBits);
+    const RowScales scales = ScalesOf(sumSquares, maxBits, a.cols, a.eps);
+    if (a.scale != nullptr && threadIdx.x == 0) a.scale[blockIdx.x] = scales.scale;
+    for (int64_t c = threadIdx.x; c < a.cols; c += kAnyThreads) {
+        const float s = Codec::Load(sum != nullptr ? sum[c] : rounded(c));
+        const float g = Gamma::Load(gamma[c]);
+        if (a.norm != nullptr) static_cast<S*>(a.norm)[at + c] = Codec::Store(s * scales.r * g);
+        if (a.y != nullptr) a.y[at + c] = static_cast<int8_t>(Quantised(s * g * weight(c), scales));
+    }
+}
+
+class NormQuantExecutor : public aclOpExecutor {
+   public:
+    NormArgs args{};
+    aclDataType dtype = ACL_FLOAT;
+    aclDataType gammaType = ACL_FLOAT;
+
+    template <typename Codec, typename Gamma>
+    void Launch(hipStream_t stream) const {
+        hipLaunchKernelGGL((NormQuantAnyKernel<Codec, Gamma>), dim3(static_cast<unsigned>(args.rows)), dim3(kAnyThreads), 0, stream, args);
+    }
+
+    template <typename Codec>
+    void LaunchFor(hipStream_t stream) const {
+        if (gammaType == Codec::kType) Launch<Codec, Codec>(stream);
+        else Launch<Codec, F32>(stream);
+    }
+
+    aclnnStatus Run(void*, hipStream_t stream) override {
+        if (args.rows == 0) return ACLNN_SUCCESS;
+        opapi::KernelTimer timer("add_rms_norm_quant", stream);
+        if (dtype == ACL_FLOAT) Launch<F32, F32>(stream);
+        else if (dtype == ACL_FLOAT16) LaunchFor<F16>(stream);
+        else LaunchFor<Bf16>(stream);
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) {
+            opapi::SetError("aclnnMoeAddRmsNormQuant: launch failed: %s", hipGetErrorString(err));
+            return ACLNN_ERR_RUNTIME_ERROR;
+        }
+        return ACLNN_SUCCESS;
+    }
+};
+
+}  // namespace
+
+extern "C" aclnnStatus aclnnMoeAddRmsNormQuantGetWorkspaceSize(
+    const aclTensor* x, const aclTensor* residualOptional, const aclTensor* gamma, const aclTensor* smoothScaleOptional,
+    double epsilon, const aclTensor* yOutOptional, const aclTensor* scaleOutOptional, const aclTensor* normOutOptional,
+    const aclTensor* sumOutOptional, uint64_t* workspaceSize, aclOpExecutor** executor) try {
+    using namespace opapi;
+    ClearError();
+    OPAPI_CHECK_NOTNULL(x, "x");
+    OPAPI_CHECK_NOTNULL(gamma, "gamma");
+    OPAPI_CHECK_NOTNULL(workspaceSize, "workspaceSize");
+    OPAPI_CHECK_NOTNULL(executor, "executor");
+    OPAPI_CHECK_EXTENTS(x, residualOptional, gamma, smoothScaleOptional, yOutOptional, scaleOutOptional, normOutOptional, sumOutOptional);
+
+    constexpr aclnnStatus kInvalid = ACLNN_ERR_PARAM_INVALID;
+    OPAPI_CHECK(IsFloating(x), kInvalid, "x must be FLOAT, FLOAT16 or BF16");
+    OPAPI_CHECK(x->dims.size() == 2 || x->dims.size() == 3, kInvalid, "x must have rank 2 or 3, not %zu", x->dims.size());
+    for (int64_t d : x->dims) OPAPI_CHECK(d <= 2147483647ll, kInvalid, "an extent of x is larger than 2147483647");
+    const int64_t cols = x->dims.back();
+    OPAPI_CHECK(cols > 0, kInvalid, "the last extent of x is zero");
+    const int64_t rows = RowsOf(x);
+    OPAPI_CHECK(rows >= 0, kInvalid, "x has more than 2147483647 rows");
+    OPAPI_CHECK((gamma->dtype == x->dtype || gamma->dtype == ACL_FLOAT) && gamma->dims.size() == 1 && gamma->dims[0] == cols, kInvalid,
+                "gamma must be [%lld] of x's type or FLOAT", (long long)cols);
+    OPAPI_CHECK(smoothScaleOptional == nullptr || (smoothScaleOptional->dtype == ACL_FLOAT && smoothScaleOptional->dims.size() == 1 &&
+                                                   smoothScaleOptional->dims[0] == cols),
+                kInvalid, "smoothScale must be FLOAT [%lld]", (long long)cols);
+    OPAPI_CHECK(epsilon >= 0 && epsilon <= 1e30, kInvalid, "epsilon must be a number of at least 0");
+    OPAPI_CHECK((yOutOptional == nullptr) == (scaleOutOptional == nullptr), ACLNN_ERR_PARAM_NULLPTR, "yOut and scaleOut belong together");
+    OPAPI_CHECK(yOutOptional != nullptr || normOutOptional != nullptr, ACLNN_ERR_PARAM_NULLPTR, "neither yOut nor normOut is given");
+    OPAPI_CHECK(yOutOptional != nullptr || smoothScaleOptional == nullptr, kInvalid, "smoothScale goes into yOut, which is not given");
+    if (residualOptional != nullptr) {
+        OPAPI_CHECK(residualOptional->dtype == x->dtype && SameButLast(residualOptional, x, cols), kInvalid,
+                    "residual %s must have x's type and extents %s", ShapeStr(residualOptional).c_str(), ShapeStr(x).c_str());
+    }
+    for (const aclTensor* t : {normOutOptional, sumOutOptional}) {
+        OPAPI_CHECK(t == nullptr || (t->dtype == x->dtype && SameButLast(t, x, cols)), kInvalid,
+                    "%s %s must have x's type and extents %s", t == normOutOptional ? "normOut" : "sumOut", ShapeStr(t).c_str(),
+                    ShapeStr(x).c_str());
+    }
+    if (yOutOptional != nullptr) {
+        OPAPI_CHECK(yOutOptional->dtype == ACL_INT8 && SameButLast(yOutOptional, x, cols), kInvalid, "yOut %s must be INT8 of x's extents %s",
+                    ShapeStr(yOutOptional).c_str(), ShapeStr(x).c_str());
+        OPAPI_CHECK(scaleOutOptional->dtype == ACL_FLOAT && SameButLast(scaleOutOptional, x, -1), kInvalid,
+                    "scaleOut %s must be FLOAT of x's extents %s without the last", ShapeStr(scaleOutOptional).c_str(), ShapeStr(x).c_str());
+    }
+    const aclTensor* const ins[] = {x, residualOptional, gamma, smoothScaleOptional};
+    const aclTensor* const outs[] = {sumOutOptional, normOutOptional, yOutOptional, scaleOutOptional};
+    for (int o = 0; o < 4; ++o) {
+        if (outs[o] == nullptr) continue;
+        OPAPI_CHECK(InOrder(outs[o]), kInvalid, "the outputs must be contiguous");
+        OPAPI_CHECK(rows == 0 || outs[o]->data != nullptr, ACLNN_ERR_PARAM_NULLPTR, "an output carries no device memory");
+        for (int p = 0; p < o; ++p) OPAPI_CHECK(!Overlap(outs[o], outs[p]), kInvalid, "two outputs share memory");
+    }
+    for (int i = 0; i < 4; ++i) {
+        if (ins[i] == nullptr) continue;
+        OPAPI_CHECK(rows == 0 || ins[i]->data != nullptr, ACLNN_ERR_PARAM_NULLPTR, "an input carries no device memory");
+        if (!IsContiguous(ins[i])) continue;  // read from a copy that is made first
+        for (int o = 0; o < 4; ++o) {
+            const bool inPlace = o == 0 && i < 2 && outs[o] != nullptr && DataPtr(outs[o]) == DataPtr(ins[i]);
+            OPAPI_CHECK(inPlace || !Overlap(outs[o], ins[i]), kInvalid, "an output shares memory with an input");
+        }
+    }
+
+    auto* ex = new (std::nothrow) NormQuantExecutor();
+    OPAPI_CHECK(ex != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "out of host memory");
+    ex->dtype = x->dtype;
+    ex->gammaType = gamma->dtype;
+    OPAPI_BIND(ex, x, &ex->args.x);
+    OPAPI_BIND(ex, residualOptional, &ex->args.residual);
+    OPAPI_BIND(ex, gamma, &ex->args.gamma);
+    OPAPI_BIND(ex, smoothScaleOptional, &ex->args.smooth);
+    ex->args.y = reinterpret_cast<int8_t*>(DataPtr(yOutOptional));
+    ex->args.scale = reinterpret_cast<float*>(DataPtr(scaleOutOptional));
+    ex->args.norm = DataPtr(normOutOptional);
+    ex->args.sum = DataPtr(sumOutOptional);
+    ex->args.rows = rows;
+    ex->args.cols = cols;
+    ex->args.eps = static_cast<float>(epsilon);
+    ex->SealWorkspace(0);
+    *workspaceSize = ex->workspaceBytes;
+    *executor = ex;
+    return ACLNN_SUCCESS;
+} catch (...) {  // no exception may cross the C boundary
+    opapi::SetError("out of host memory");
+    return ACLNN_ERR_INNER;
+}
+
+extern "C" aclnnStatus aclnnMoeAddRmsNormQuant(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor,
+                                               aclrtStream stream) {
+    return opapi::RunAndRelease(workspace, workspaceSize, executor, stream);
+}

@@ -3,19 +3,23 @@
 
 #include "aclnnop/aclnn_grouped_matmul_swiglu_quant.h"
 #include "aclnnop/aclnn_grouped_matmul_v4.h"
+#include "aclnnop/aclnn_moe_add_rms_norm_quant.h"
 #include "aclnnop/aclnn_moe_finalize_routing_v2.h"
+#include "aclnnop/aclnn_moe_gating_top_k_grouped.h"
 #include "aclnnop/aclnn_moe_gating_top_k_softmax_v2.h"
 #include "aclnnop/aclnn_moe_init_routing_quant_v2.h"
 #include "aclnnop/aclnn_moe_init_routing_v2.h"
 #include "aclnnop/aclnn_moe_init_routing_v3.h"
+#include "aclnnop/aclnn_moe_router_logits.h"
 #include "opapi_common.h"
 
 namespace {
 
 // The operators by number, with how many scalars and tensors each takes.
-enum { kGating, kRoutingV2, kRoutingQuantV2, kRoutingV3, kSwigluQuant, kGroupedMatmulV4, kFinalizeV2, kOperators };
-constexpr int kScalars[kOperators] = {3, 6, 7, 8, 0, 4, 1};
-constexpr int kTensors[kOperators] = {5, 6, 9, 7, 9, 7, 8};
+enum { kGating, kRoutingV2, kRoutingQuantV2, kRoutingV3, kSwigluQuant, kGroupedMatmulV4, kFinalizeV2, kAddRmsNormQuant, kRouterLogits,
+       kGatingGrouped, kOperators };
+constexpr int kScalars[kOperators] = {3, 6, 7, 8, 0, 4, 1, 1, 0, 8};
+constexpr int kTensors[kOperators] = {5, 6, 9, 7, 9, 7, 8, 8, 3, 6};
 constexpr int kMaxTensors = 9;
 
 // Tensors from packed[at] on, count of them; absent ones (no dimensions, no address) stay null.  False when the array is not exactly theirs.
@@ -35,6 +39,9 @@ bool Unpack(const int64_t* packed, uint64_t at, uint64_t length, int count, aclT
     }
     return at == length;
 }
+
+// A scalar that is no whole number travels as its bits.
+double Real(int64_t bits) { return __builtin_bit_cast(double, bits); }
 
 }  // namespace
 
@@ -77,6 +84,13 @@ extern "C" aclnnStatus opapiPlanPacked(const int64_t* packed, uint64_t length, u
             return aclnnGroupedMatmulV4GetWorkspaceSize(l[0], l[1], l[2], l[3], nullptr, nullptr, nullptr, l[4], t[5], nullptr, nullptr, nullptr,
                                                         s[0], s[1], s[2], s[3], l[6], nullptr, nullptr, workspaceSize, executor);
         }
+        case kAddRmsNormQuant:
+            return aclnnMoeAddRmsNormQuantGetWorkspaceSize(t[0], t[1], t[2], t[3], Real(s[0]), t[4], t[5], t[6], t[7], workspaceSize, executor);
+        case kRouterLogits:
+            return aclnnMoeRouterLogitsGetWorkspaceSize(t[0], t[1], t[2], workspaceSize, executor);
+        case kGatingGrouped:
+            return aclnnMoeGatingTopKGroupedGetWorkspaceSize(t[0], t[1], t[2], s[0], s[1], s[2], s[3], s[4], s[5], Real(s[6]), Real(s[7]), t[3],
+                                                             t[4], t[5], workspaceSize, executor);
         default:
             return aclnnMoeFinalizeRoutingV2GetWorkspaceSize(t[0], t[1], t[2], t[3], t[4], t[5], t[6], s[0], t[7], workspaceSize, executor);
     }
