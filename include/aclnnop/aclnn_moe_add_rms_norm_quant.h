@@ -10,7 +10,7 @@
  *   v = n * smoothScale;  scale = max|v| / 127;  y = round_half_even(v / scale) in [-127, 127]     -> yOut, scaleOut
  * A row with scale 0 (zeros, or squares whose sum passes fp32) gives zeros; one with a NaN or an infinity gives scale NaN and zeros in y.
  *
- * x, residualOptional, sumOutOptional, normOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents;
+ * x, residualOptional, sumOutOptional, normOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents, at most 2^26 rows;
  * gamma [H] of x's type or FLOAT; smoothScaleOptional FLOAT [H]; yOutOptional INT8 of x's extents with scaleOutOptional FLOAT of x's
  * extents without the last (both or neither; without them the operator is a plain RMS norm); at least one of normOut and yOut.
  * Inputs may be strided views; outputs are contiguous.  sumOut may be x's or residual's own memory, entirely; no other output

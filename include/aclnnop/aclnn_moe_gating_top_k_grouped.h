@@ -13,7 +13,7 @@
  *   yOut = y * routedScalingFactor, rounded to nearest even
  * NaN counts as larger than every number.  Rows whose finishedOptional entry is true get expertIdxOut = E in every slot (the values are
  * still written).
- * x: FLOAT, FLOAT16 or BF16, rank 2 or 3; biasOptional FLOAT [E], finite; finishedOptional BOOL of x's extents without the last;
+ * x: FLOAT, FLOAT16 or BF16, rank 2 or 3, at most 2^26 rows; biasOptional FLOAT [E], finite; finishedOptional BOOL of x's extents without the last;
  * yOut of x's type or FLOAT and expertIdxOut INT32, x's extents with the last replaced by k; scoresOutOptional FLOAT of x's
  * extents.  This build: E <= 2048, k <= 64; k <= kGroup * E / groupCount; groupSelectMode 1 takes groups of two experts or more.
  * Inputs may be strided views; outputs are contiguous and share no memory with an input or with each other.

@@ -53,11 +53,19 @@ inline bool SameButLast(const aclTensor* t, const aclTensor* x, int64_t last) {
     return last < 0 || t->dims.back() == last;
 }
 
-// Rows of a tensor of rank 2 or 3 whose extents are at most 2^31 - 1 each; -1 where there are more than a grid holds.
+// Rows of a tensor of rank 2 or 3 whose extents are at most 2^31 - 1 each; -1 where there are more than kMaxRows.
+constexpr int64_t kMaxRows = 1 << 26;
 inline int64_t RowsOf(const aclTensor* x) {
     const int64_t rows = x->dims.size() == 2 ? x->dims[0] : x->dims[0] * x->dims[1];
-    return rows <= 2147483647ll ? rows : -1;
+    return rows <= kMaxRows ? rows : -1;
 }
+
+// A grid has fewer than 2^32 threads in its first direction: workgroups are numbered over two.
+inline dim3 GridOf(int64_t groups) {
+    constexpr int64_t kLine = 1 << 20;
+    return groups <= kLine ? dim3(static_cast<unsigned>(groups)) : dim3(static_cast<unsigned>(kLine), static_cast<unsigned>((groups + kLine - 1) / kLine));
+}
+__device__ __forceinline__ int64_t GroupIndex() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
 
 // Without elements any strides do.
 inline bool InOrder(const aclTensor* t) { return opapi::IsEmpty(t) || opapi::IsContiguous(t); }

@@ -77,7 +77,8 @@ __global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
     uint64_t* const keys = reinterpret_cast<uint64_t*>(ldsRaw);     // [experts]
     uint64_t* const groupKeys = keys + a.experts;                   // [groups]
     const int lane = threadIdx.x;
-    const int64_t row = blockIdx.x;
+    const int64_t row = GroupIndex();
+    if (row >= a.rows) return;
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
 
     double shift = 0.0, sum = 1.0;
@@ -178,7 +179,7 @@ class GatingExecutor : public aclOpExecutor {
     template <typename Codec, typename Out>
     void Launch(hipStream_t stream) const {
         const size_t lds = (static_cast<size_t>(args.experts) + args.groups) * 8;
-        hipLaunchKernelGGL((GatingAnyKernel<Codec, Out>), dim3(static_cast<unsigned>(args.rows)), dim3(kWave), lds, stream, args);
+        hipLaunchKernelGGL((GatingAnyKernel<Codec, Out>), GridOf(args.rows), dim3(kWave), lds, stream, args);
     }
 
     template <typename Codec>
@@ -226,7 +227,7 @@ extern "C" aclnnStatus aclnnMoeGatingTopKGroupedGetWorkspaceSize(
     OPAPI_CHECK(experts > 0 && experts <= kMaxExperts, kInvalid, "the last extent of x (=%lld) must be 1 to %lld experts", (long long)experts,
                 (long long)kMaxExperts);
     const int64_t rows = RowsOf(x);
-    OPAPI_CHECK(rows >= 0, kInvalid, "x has more than 2147483647 rows");
+    OPAPI_CHECK(rows >= 0, kInvalid, "x has more than %lld rows", (long long)kMaxRows);
     OPAPI_CHECK(groupCount >= 1 && groupCount <= experts && experts % groupCount == 0, kInvalid,
                 "groupCount (=%lld) must divide the %lld experts", (long long)groupCount, (long long)experts);
     OPAPI_CHECK(kGroup >= 1 && kGroup <= groupCount, kInvalid, "kGroup (=%lld) must be 1 to groupCount (=%lld)", (long long)kGroup,

@@ -59,7 +59,7 @@ def test_norm_valid(aclnn):
     (dict(shape=(2, 2, 2, 24)), "rank 2 or 3"),
     (dict(shape=(6, 0)), "last extent of x is zero"),
     (dict(shape=(-6, 24)), "negative extent"),
-    (dict(shape=(65536, 65536, 1)), "more than 2147483647 rows"),
+    (dict(shape=(65536, 1025, 1)), "more than 67108864 rows"),
     (dict(gamma=(23,)), "gamma must be [24]"),
     (dict(gamma_dtype=F16), "of x's type or FLOAT"),
     (dict(gamma=(24, 1)), "gamma must be [24]"),
