@@ -1,13 +1,15 @@
 // aclnnMoeGatingTopKGrouped for gfx950: softmax or sigmoid scores, a bias that moves the choice only, groups, top-k.
 //
 // Two experts change places when their t = p + bias do, and near the top of 256 sigmoid scores a pair within fp32's rounding of an exponential
-// comes up in one row of some thousands.  t is therefore computed and compared in 64 bits, as order-preserving 64-bit keys (the bits of a
-// double mapped so that unsigned comparison equals that of the numbers, NaN on top): the choice is that of the formula, whatever the
-// exponential's last bit.  Key 0 marks an expert that is taken or lies in a group that was left out; it is below every real value, -inf
-// (an expert of logit -inf) among them.
+// comes up in one row of some thousands.  The choice is defined in 64 bits, and every row is chosen as if it were made there: the
+// fast kernel works on fp32 scores whose error it can bound, and where two values that decide something are closer than that, the wave makes
+// that row again in 64 bits.  Without a bias t is a monotone function of the logit: logits are compared in its place, exactly.
+// Keys are order-preserving: the bits of a number mapped so that unsigned comparison equals that of the numbers, NaN on top.  Key 0 marks an
+// expert that is taken or lies in a group that was left out; it is below every real value, -inf (an expert of logit -inf) among them.
 #include "moe_front.h"
 
 #include <cmath>
+#include <cstdlib>
 
 #include "aclnnop/aclnn_moe_gating_top_k_grouped.h"
 
@@ -33,6 +35,8 @@ struct GatingArgs {
     int32_t topTwo;           // a group's value is the sum of its two largest t
     int32_t sigmoid;
     int32_t renorm;
+    int32_t packets;          // rows start on 16 bytes and fill their lanes
+    uint32_t groupMagic;      // (c * groupMagic) >> 21 = c / (experts / groups) for c < 512
     float factor;
     double eps;
 };
@@ -70,19 +74,21 @@ __device__ __forceinline__ double ScoreOf(float x, bool sigmoid, double shift, d
     return sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x))) : exp(static_cast<double>(x) - shift) / sum;
 }
 
-// One wave per row, the keys in LDS.
+// What one lane of the wave has written to LDS, the others read: the wave's accesses are carried out in order, the compiler must keep them so.
+__device__ __forceinline__ void WaveSync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// A row by one wave in 64 bits.  keys: [experts + groups] in LDS, the wave's own.
 template <typename Codec, typename Out>
-__global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
-    extern __shared__ __attribute__((aligned(16))) unsigned char ldsRaw[];
-    uint64_t* const keys = reinterpret_cast<uint64_t*>(ldsRaw);     // [experts]
-    uint64_t* const groupKeys = keys + a.experts;                   // [groups]
-    const int lane = threadIdx.x;
-    const int64_t row = GroupIndex();
-    if (row >= a.rows) return;
+__device__ void ExactRow(const GatingArgs& a, int64_t row, int lane, uint64_t* keys, bool writeScores) {
+    uint64_t* const groupKeys = keys + a.experts;
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
+    const bool sigmoid = a.sigmoid != 0;
 
     double shift = 0.0, sum = 1.0;
-    if (a.sigmoid == 0) {
+    if (!sigmoid) {
         float top = -INFINITY;
         bool nan = false;
         for (int c = lane; c < a.experts; c += kWave) {
@@ -98,11 +104,11 @@ __global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
     }
     for (int c = lane; c < a.experts; c += kWave) {
         const float v = Codec::Load(x[c]);
-        const double p = ScoreOf(v, a.sigmoid != 0, shift, sum);
-        if (a.scores != nullptr) a.scores[row * a.experts + c] = static_cast<float>(p);
-        keys[c] = KeyOf(v == -INFINITY ? -INFINITY : a.bias == nullptr ? p : p + static_cast<double>(a.bias[c]));
+        const double p = a.bias != nullptr || writeScores ? ScoreOf(v, sigmoid, shift, sum) : 0.0;
+        if (writeScores) a.scores[row * a.experts + c] = static_cast<float>(p);
+        keys[c] = KeyOf(v == -INFINITY ? -INFINITY : a.bias == nullptr ? static_cast<double>(v) : p + static_cast<double>(a.bias[c]));
     }
-    __syncthreads();
+    WaveSync();
 
     if (a.kGroup < a.groups) {
         const int size = a.experts / a.groups;
@@ -117,10 +123,19 @@ __global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
                     second = key;
                 }
             }
-            const double one = ValueOf(first), two = ValueOf(second);
-            groupKeys[g] = a.topTwo != 0 && two != -INFINITY ? KeyOf(one + two) : first;
+            double one = ValueOf(first), two = ValueOf(second);
+            if (a.topTwo != 0 && two != -INFINITY) {
+                if (a.bias == nullptr) {
+                    one = ScoreOf(static_cast<float>(one), sigmoid, shift, sum);
+                    two = ScoreOf(static_cast<float>(two), sigmoid, shift, sum);
+                }
+                first = KeyOf(one + two);
+            } else if (a.topTwo != 0 && a.bias == nullptr && one != -INFINITY) {
+                first = KeyOf(ScoreOf(static_cast<float>(one), sigmoid, shift, sum));
+            }
+            groupKeys[g] = first;
         }
-        __syncthreads();
+        WaveSync();
         for (int j = 0; j < a.kGroup; ++j) {
             uint64_t best = 0;
             int32_t at = INT32_MAX;
@@ -131,14 +146,14 @@ __global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
                 }
             }
             WaveArgMax(best, at);
-            __syncthreads();
+            WaveSync();
             if (lane == 0) groupKeys[at] = 0;  // stays
-            __syncthreads();
+            WaveSync();
         }
         for (int c = lane; c < a.experts; c += kWave) {
             if (groupKeys[c / size] != 0) keys[c] = 0;
         }
-        __syncthreads();
+        WaveSync();
     }
 
     int32_t pick = 0;  // of lane j: the j-th
@@ -153,12 +168,12 @@ __global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
         }
         WaveArgMax(best, at);
         if (lane == j) pick = at;
-        __syncthreads();
+        WaveSync();
         if (lane == 0) keys[at] = 0;
-        __syncthreads();
+        WaveSync();
     }
 
-    double y = lane < a.k ? ScoreOf(Codec::Load(x[pick]), a.sigmoid != 0, shift, sum) : 0.0;
+    double y = lane < a.k ? ScoreOf(Codec::Load(x[pick]), sigmoid, shift, sum) : 0.0;
     if (a.renorm != 0) {
         const double total = WaveSum64(y) + a.eps;
         y = total == 0.0 ? 0.0 : y / total;
@@ -170,16 +185,424 @@ __global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
     }
 }
 
+// Any row: one wave each.
+template <typename Codec, typename Out>
+__global__ __launch_bounds__(kWave) void GatingAnyKernel(GatingArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char ldsRaw[];
+    const int64_t row = GroupIndex();
+    if (row < a.rows) ExactRow<Codec, Out>(a, row, threadIdx.x, reinterpret_cast<uint64_t*>(ldsRaw), a.scores != nullptr);
+}
+
+// Reductions over the kLanes (16 or 64) neighbouring lanes that share a row; every one of them has the result.
+template <int kLanes, typename T, typename Op>
+__device__ __forceinline__ T RowReduce(T v, Op op) {
+    auto ror = [](T t, auto ctl) __attribute__((always_inline)) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, t), decltype(ctl)::value, 0xF, 0xF, true));
+    };
+    v = op(v, ror(v, std::integral_constant<int, 0x128>{}));  // row_ror:8
+    v = op(v, ror(v, std::integral_constant<int, 0x124>{}));
+    v = op(v, ror(v, std::integral_constant<int, 0x122>{}));
+    v = op(v, ror(v, std::integral_constant<int, 0x121>{}));
+    if constexpr (kLanes == 64) {
+        auto lane = [&](int l) { return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l)); };
+        v = op(op(lane(0), lane(16)), op(lane(32), lane(48)));
+    }
+    return v;
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t RowMax(uint32_t v) { return RowReduce<kLanes>(v, [](uint32_t p, uint32_t q) { return max(p, q); }); }
+template <int kLanes>
+__device__ __forceinline__ uint32_t RowMin(uint32_t v) { return RowReduce<kLanes>(v, [](uint32_t p, uint32_t q) { return min(p, q); }); }
+template <int kLanes>
+__device__ __forceinline__ double RowSum(double v) {
+    auto ror = [](double d, auto ctl) __attribute__((always_inline)) {
+        const long long u = __double_as_longlong(d);
+        const int lo = __builtin_amdgcn_mov_dpp(static_cast<int>(u), decltype(ctl)::value, 0xF, 0xF, true);
+        const int hi = __builtin_amdgcn_mov_dpp(static_cast<int>(u >> 32), decltype(ctl)::value, 0xF, 0xF, true);
+        return __longlong_as_double(static_cast<long long>(static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo)));
+    };
+    v += ror(v, std::integral_constant<int, 0x128>{});
+    v += ror(v, std::integral_constant<int, 0x124>{});
+    v += ror(v, std::integral_constant<int, 0x122>{});
+    v += ror(v, std::integral_constant<int, 0x121>{});
+    if constexpr (kLanes == 64) {
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+    }
+    return v;
+}
+
+// The lowest lane of the wave that holds the largest key; uniform.  The upper halves settle it nearly always.
+__device__ __forceinline__ int WaveHolder(uint64_t key) {
+    const uint32_t hi = static_cast<uint32_t>(key >> 32), lo = static_cast<uint32_t>(key);
+    const bool top = hi == RowMax<64>(hi);
+    uint64_t holders = __ballot(top);
+    if ((holders & (holders - 1)) != 0) {
+        const uint32_t low = RowMax<64>(top ? lo : 0u);
+        holders = __ballot(top && lo == low);
+    }
+    return __ffsll(static_cast<unsigned long long>(holders)) - 1;
+}
+
+__device__ __forceinline__ uint32_t Key32(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return f != f ? 0xffc00000u : (u & 0x80000000u) != 0 ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float Value32(uint32_t key) { return __uint_as_float((key & 0x80000000u) != 0 ? (key & 0x7fffffffu) : ~key); }
+
+// exp(d) for d <= 0 to an fp32 unit in the last place: the product with log2(e) to twice fp32's bits, its tail put back behind the instruction.
+__device__ __forceinline__ float ExpNotAbove1(float d) {
+    const float h = d * 0x1.715476p+0f;
+    const float tail = fmaf(d, 0x1.715476p+0f, -h) + d * 0x1.4ae0cp-26f;
+    const float e = __builtin_amdgcn_exp2f(h);
+    return h < -150.f ? 0.f : fmaf(e, tail * 0x1.62e43p-1f, e);
+}
+
+// The kPer values of a lane; absent ones are -inf.
+template <typename Codec, int kPer>
+__device__ __forceinline__ void LoadLane(const GatingArgs& a, const typename Codec::Storage* x, int l, float (&v)[kPer]) {
+    if (a.packets != 0) {
+        constexpr int kPiece = kPer * sizeof(typename Codec::Storage) >= 16 ? 16 / sizeof(typename Codec::Storage) : kPer;
+        struct alignas(kPiece * sizeof(typename Codec::Storage)) Piece {
+            typename Codec::Storage e[kPiece];
+        };
+#pragma unroll
+        for (int i = 0; i < kPer; i += kPiece) {
+            const Piece piece = *reinterpret_cast<const Piece*>(x + l * kPer + i);
+#pragma unroll
+            for (int j = 0; j < kPiece; ++j) v[i + j] = Codec::Load(piece.e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) v[i] = l * kPer + i < a.experts ? Codec::Load(x[l * kPer + i]) : -INFINITY;
+    }
+}
+
+// y and the index of a row's picks, the j-th of them in its lane j.
+template <typename Codec, typename Out, int kLanes>
+__device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int l, int32_t pick, double shift, double sum) {
+    const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
+    double y = l < a.k ? ScoreOf(Codec::Load(x[pick]), a.sigmoid != 0, shift, sum) : 0.0;
+    if (a.renorm != 0) {
+        const double total = RowSum<kLanes>(y) + a.eps;
+        y = total == 0.0 ? 0.0 : y / total;
+    }
+    if (l < a.k) {
+        const bool done = a.finished != nullptr && a.finished[row] != 0;
+        static_cast<typename Out::Storage*>(a.y)[row * a.k + l] = Out::Store(static_cast<float>(y * a.factor));
+        a.expertIdx[row * a.k + l] = done ? a.experts : pick;
+    }
+}
+
+// A row of up to 64 * kPer experts, at most 64 groups, by one wave in 64 bits: lane l holds experts l * kPer + i, the keys in registers.  lds: 8 bytes an
+// expert, the wave's own, for the groups.
+template <typename Codec, typename Out, int kPer>
+__device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int lane, uint64_t* lds, bool writeScores) {
+    const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
+    const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr, grouped = a.kGroup < a.groups;
+    float v[kPer];
+    LoadLane<Codec, kPer>(a, x, lane, v);
+    double shift = 0.0, sum = 1.0;
+    if (!sigmoid) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) most = max(most, Key32(v[i]));
+        shift = Value32(RowMax<64>(most));
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += ScoreOf(v[i], false, shift, 1.0);
+        sum = RowSum<64>(sum);
+    }
+    uint64_t keys[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int c = lane * kPer + i;
+        double t = v[i];
+        if (biased || writeScores) {
+            const double p = ScoreOf(v[i], sigmoid, shift, sum);
+            if (writeScores && c < a.experts) a.scores[row * a.experts + c] = static_cast<float>(p);
+            if (biased && v[i] != -INFINITY) t = p + static_cast<double>(a.bias[c < a.experts ? c : 0]);
+        }
+        keys[i] = c < a.experts ? KeyOf(t) : 0;
+    }
+    if (grouped) {
+        // the lanes are shared out among the groups, a power of two each
+        const int size = a.experts / a.groups;
+        const int share = kWave >> (32 - __builtin_clz(a.groups * 2 - 1) - 1);
+        WaveSync();
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (lane * kPer + i < a.experts) lds[lane * kPer + i] = keys[i];
+        }
+        WaveSync();
+        const int group = lane / share;
+        uint64_t one = 0, two = 0;
+        if (group < a.groups) {
+            for (int c = lane % share; c < size; c += share) {
+                const uint64_t key = lds[group * size + c];
+                two = key > one ? one : key > two ? key : two;
+                one = key > one ? key : one;
+            }
+        }
+        for (int d = 1; d < share; d <<= 1) {
+            const uint64_t otherOne = __shfl_xor(static_cast<unsigned long long>(one), d), otherTwo = __shfl_xor(static_cast<unsigned long long>(two), d);
+            const uint64_t less = one > otherOne ? otherOne : one, second = two > otherTwo ? two : otherTwo;
+            two = less > second ? less : second;
+            one = one > otherOne ? one : otherOne;
+        }
+        if (a.topTwo != 0 && one != 0) {
+            double first = ValueOf(one), second = two == 0 ? -INFINITY : ValueOf(two);
+            if (!biased) {
+                if (first != -INFINITY) first = ScoreOf(static_cast<float>(first), sigmoid, shift, sum);
+                if (second != -INFINITY) second = ScoreOf(static_cast<float>(second), sigmoid, shift, sum);
+            }
+            one = KeyOf(second == -INFINITY ? first : first + second);
+        }
+        if (lane % share != 0) one = 0;
+        uint64_t kept = 0;
+        for (int j = 0; j < a.kGroup; ++j) {
+            const int holder = WaveHolder(one);
+            kept |= 1ull << (holder / share);
+            if (lane == holder) one = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t c = lane * kPer + i;
+            if ((kept >> ((c * a.groupMagic >> 21) & 63) & 1) == 0) keys[i] = 0;
+        }
+    }
+    int32_t pick = 0;
+    for (int j = 0; j < a.k; ++j) {
+        uint64_t best = keys[0];
+        int at = 0;
+#pragma unroll
+        for (int i = 1; i < kPer; ++i) {
+            if (keys[i] > best) {  // equal keys: the lower expert stays
+                best = keys[i];
+                at = i;
+            }
+        }
+        const int holder = WaveHolder(best);
+        const int taken = __builtin_amdgcn_readlane(at, holder);
+        if (lane == j) pick = holder * kPer + taken;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (lane == holder && i == taken) keys[i] = 0;
+        }
+    }
+    WritePicks<Codec, Out, 64>(a, row, lane, pick, shift, sum);
+}
+
+constexpr int kRowWaves = 4;  // of a workgroup
+
+template <typename Codec, typename Out, int kPer>
+__global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs a) {
+    extern __shared__ __attribute__((aligned(16))) unsigned char ldsRaw[];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t row = GroupIndex() * kRowWaves + wave;
+    if (row < a.rows) WaveRow<Codec, Out, kPer>(a, row, lane, reinterpret_cast<uint64_t*>(ldsRaw) + wave * a.experts, a.scores != nullptr);
+}
+
+// LDS of a wave: an fp32 value per expert of its four rows, or a row's keys in 64 bits.
+constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts) * 16; }
+
+// Rows of up to 16 * kPer experts, at most 16 picks and groups: four rows a wave, sixteen lanes each, fp32 keys in registers.  Lane l of a row holds experts
+// l * kPer + i, so that among equal values the lower lane has the lower index; within a lane the number i goes into the lowest b bits of the key, which
+// costs fp32 keys as many bits and 16-bit logits nothing, and makes a lane's keys different.  `bound` is the last key that a lane gave away: of the
+// differences key - bound modulo 2^32 the largest is that of the next smaller key.
+// Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once, b bits cut off
+// a key are 2^(b+1) u.  Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
+template <typename Codec, typename Out, int kPer>
+__global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs a) {
+    constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : 4;
+    constexpr uint32_t kLow = (1u << kBits) - 1;
+    constexpr float kU = 0x1p-24f;
+    extern __shared__ __attribute__((aligned(16))) unsigned char ldsRaw[];
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const int l = lane % kLanes, first = lane - l;  // place in the row, the row's first lane
+    const int64_t rowsFrom = (GroupIndex() * kRowWaves + wave) * 4;
+    if (rowsFrom >= a.rows) return;
+    const int64_t row = min(rowsFrom + lane / kLanes, a.rows - 1);
+    const bool mine = rowsFrom + lane / kLanes < a.rows;
+    unsigned char* const own = ldsRaw + wave * QuadBytes(a.experts);
+    float* const values = reinterpret_cast<float*>(own) + lane / kLanes * a.experts;  // of the row, while groups are chosen
+
+    const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
+    const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr, grouped = a.kGroup < a.groups;
+    float v[kPer];
+    LoadLane<Codec, kPer>(a, x, l, v);
+
+    float shift = 0.f, top = 1.f;  // top: no p of the row is larger
+    double sum = 1.0;
+    if (!sigmoid) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) most = max(most, Key32(v[i]));
+        shift = Value32(RowMax<kLanes>(most));
+        sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) sum += v[i] == -INFINITY ? 0.f : ExpNotAbove1(v[i] - shift);
+        sum = RowSum<kLanes>(sum);
+        top = 1.f / static_cast<float>(sum);
+    }
+    float t[kPer];
+    if (biased || (grouped && a.topTwo != 0)) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            t[i] = v[i] == -INFINITY ? 0.f
+                   : sigmoid         ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v[i] * -0x1.715476p+0f))
+                                     : __builtin_amdgcn_exp2f((v[i] - shift) * 0x1.715476p+0f) * top;
+        }
+    }
+    if (a.scores != nullptr && mine) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            if (l * kPer + i < a.experts) a.scores[row * a.experts + l * kPer + i] = static_cast<float>(ScoreOf(v[i], sigmoid, shift, sum));
+        }
+    }
+    float largest = top;  // of |t|
+    if (biased) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            t[i] += a.bias[l * kPer + i < a.experts ? l * kPer + i : 0];
+            if (v[i] == -INFINITY) t[i] = -INFINITY;
+            else most = max(most, __float_as_uint(fabsf(t[i])));
+        }
+        largest = __uint_as_float(RowMax<kLanes>(most));
+    }
+
+    bool close = false;  // uniform over the row
+    uint64_t kept = ~0ull;
+    if (grouped) {
+        const int size = a.experts / a.groups;
+        const int share = kLanes >> (32 - __builtin_clz(a.groups * 2 - 1) - 1);  // lanes of a group, a power of two
+        const int group = l / share;
+        uint32_t one = 0, two = 0;
+        auto take = [&](float value) {
+            const uint32_t key = Key32(value);
+            two = max(two, min(one, key));
+            one = max(one, key);
+        };
+        auto valueOf = [&](int i) { return v[i] == -INFINITY ? -INFINITY : biased || a.topTwo != 0 ? t[i] : v[i]; };
+        if (share * kPer == size) {  // a group's experts are those of its lanes
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) take(valueOf(i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (l * kPer + i < a.experts) values[l * kPer + i] = valueOf(i);
+            }
+            WaveSync();
+            if (group < a.groups) {
+                for (int c = l % share; c < size; c += share) take(values[group * size + c]);
+            }
+            WaveSync();
+        }
+        for (int d = 1; d < share; d <<= 1) {
+            const uint32_t otherOne = __shfl_xor(one, d), otherTwo = __shfl_xor(two, d);
+            two = max(min(one, otherOne), max(two, otherTwo));
+            one = max(one, otherOne);
+        }
+        uint32_t value = 0;
+        if (l % share == 0 && group < a.groups) {
+            value = a.topTwo != 0 && two != 0 && Value32(two) != -INFINITY ? Key32(Value32(one) + Value32(two)) : one;
+        }
+        kept = 0;
+        uint32_t last = 0;
+        for (int j = 0; j < a.kGroup; ++j) {
+            last = RowMax<kLanes>(value);
+            const uint32_t at = RowMin<kLanes>(value == last ? l : kLanes - 1);
+            kept |= 1ull << (at / share);
+            if (l == static_cast<int>(at)) value = 0;
+        }
+        const uint32_t next = RowMax<kLanes>(value);
+        if (biased || a.topTwo != 0) close = Value32(last) - Value32(next) <= kU * (32.f * top + 16.f * largest);
+    }
+
+    uint32_t keys[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const uint32_t c = l * kPer + i;
+        keys[i] = c < static_cast<uint32_t>(a.experts) ? (Key32(biased ? t[i] : v[i]) & ~kLow) | (kLow - i) : 0u;
+        if (grouped && (kept >> ((c * a.groupMagic >> 21) & 63) & 1) == 0) keys[i] = 0u;
+    }
+    // logits of 16 bits are compared exactly, fp32 ones up to the bits that a key lacks
+    const float tolerance = biased ? kU * (16.f * top + 2.f * (1 + (2 << kBits)) * largest) : sizeof(typename Codec::Storage) == 4 && kBits > 0 ? 0.f : -1.f;
+    int32_t pick = 0;
+    float before = INFINITY;
+    uint32_t bound = 0;
+    for (int j = 0; j <= a.k; ++j) {
+        uint32_t best = 0u - bound;  // none left
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) best = max(best, keys[i] - bound);
+        best += bound;
+        const uint32_t most = RowMax<kLanes>(best & ~kLow);
+        const float now = Value32(most);
+        close |= before - now <= tolerance;
+        before = now;
+        if (j == a.k) break;
+        const uint32_t at = RowMin<kLanes>((best & ~kLow) == most ? l : kLanes - 1);
+        const uint32_t holder = __shfl(best, first + static_cast<int>(at));
+        if (l == j) pick = static_cast<int32_t>(at) * kPer + static_cast<int32_t>(kLow - (holder & kLow));
+        if (l == static_cast<int>(at)) bound = best;
+    }
+    if (!close && mine) WritePicks<Codec, Out, kLanes>(a, row, l, pick, shift, sum);
+    for (uint64_t again = __ballot(close && mine && l == 0); again != 0; again &= again - 1) {
+        const int64_t which = rowsFrom + (__ffsll(static_cast<unsigned long long>(again)) - 1) / kLanes;
+        GatingArgs whole = a;
+        whole.packets = 0;
+        WaveRow<Codec, Out, (kPer + 3) / 4>(whole, which, lane, reinterpret_cast<uint64_t*>(own), false);
+    }
+}
+
 class GatingExecutor : public aclOpExecutor {
    public:
     GatingArgs args{};
     aclDataType dtype = ACL_FLOAT;
     aclDataType outType = ACL_FLOAT;
 
+    // The arguments of a kernel whose rows are lanes of kPer experts.
+    template <typename Codec>
+    GatingArgs ForLanes(int lanes, int per) const {
+        GatingArgs g = args;
+        const size_t bytes = per * sizeof(typename Codec::Storage), piece = bytes < 16 ? bytes : 16;
+        g.packets = g.experts == lanes * per && reinterpret_cast<uintptr_t>(g.x) % piece == 0 ? 1 : 0;
+        return g;
+    }
+
+    template <typename Codec, typename Out, int kPer>
+    void LaunchWaves(hipStream_t stream) const {
+        hipLaunchKernelGGL((GatingWaveKernel<Codec, Out, kPer>), GridOf((args.rows + kRowWaves - 1) / kRowWaves), dim3(kWave * kRowWaves),
+                           static_cast<size_t>(kRowWaves) * args.experts * 8, stream, ForLanes<Codec>(kWave, kPer));
+    }
+
+    template <typename Codec, typename Out, int kPer>
+    void LaunchQuads(hipStream_t stream) const {
+        hipLaunchKernelGGL((GatingQuadKernel<Codec, Out, kPer>), GridOf((args.rows + 4 * kRowWaves - 1) / (4 * kRowWaves)), dim3(kWave * kRowWaves),
+                           kRowWaves * QuadBytes(args.experts), stream, ForLanes<Codec>(16, kPer));
+    }
+
     template <typename Codec, typename Out>
     void Launch(hipStream_t stream) const {
-        const size_t lds = (static_cast<size_t>(args.experts) + args.groups) * 8;
-        hipLaunchKernelGGL((GatingAnyKernel<Codec, Out>), GridOf(args.rows), dim3(kWave), lds, stream, args);
+        const char* env = std::getenv("GT_LANES");
+        const int lanes = env != nullptr ? atoi(env) : args.rows > 2048 ? 16 : 64;
+        const int E = args.experts;
+        if (lanes == 16 && E <= 256 && args.k <= 16 && args.groups <= 16) {
+            if (E <= 16) LaunchQuads<Codec, Out, 1>(stream);
+            else if (E <= 32) LaunchQuads<Codec, Out, 2>(stream);
+            else if (E <= 64) LaunchQuads<Codec, Out, 4>(stream);
+            else if (E <= 128) LaunchQuads<Codec, Out, 8>(stream);
+            else LaunchQuads<Codec, Out, 16>(stream);
+        } else if (lanes != 1 && E <= 512 && args.groups <= kWave) {
+            if (E <= 64) LaunchWaves<Codec, Out, 1>(stream);
+            else if (E <= 128) LaunchWaves<Codec, Out, 2>(stream);
+            else if (E <= 256) LaunchWaves<Codec, Out, 4>(stream);
+            else LaunchWaves<Codec, Out, 8>(stream);
+        } else {
+            const size_t lds = (static_cast<size_t>(E) + args.groups) * 8;
+            hipLaunchKernelGGL((GatingAnyKernel<Codec, Out>), GridOf(args.rows), dim3(kWave), lds, stream, args);
+        }
     }
 
     template <typename Codec>
@@ -288,6 +711,8 @@ extern "C" aclnnStatus aclnnMoeGatingTopKGroupedGetWorkspaceSize(
     ex->args.renorm = static_cast<int32_t>(renorm);
     ex->args.factor = static_cast<float>(routedScalingFactor);
     ex->args.eps = eps;
+    const int64_t size = experts / groupCount;
+    ex->args.groupMagic = static_cast<uint32_t>(((1ll << 21) + size - 1) / size);
     ex->SealWorkspace(0);
     *workspaceSize = ex->workspaceBytes;
     *executor = ex;

@@ -1,5 +1,13 @@
 // aclnnMoeRouterLogits for gfx950: fp32 logits = x @ weight^T, x of 16 or 32 bits, weight of x's type or fp32.
+//
+// The matrix instructions take 16-bit operands, and an operand of more bits is a sum of bf16 parts, cut off eight significant bits at a time:
+// fp32 = three parts and fp16 (next to fp32 weights) = two, both without a remainder.  A product of parts a_i and b_j (i, j from 0) is below
+// 2^-8(i+j) of |x w|, so those with i + j <= 2 are summed, and what is left out is below fp32's rounding of each product.  bf16 rows on
+// fp32 weights take three instructions in place of one, fp16 rows five, fp32 rows six: with every bit of both sides, at several times the rate
+// of the fp32 matrix instructions.  Sums are fp32, in an order that only sizes decide.
 #include "moe_front.h"
+
+#include <cstdlib>
 
 #include "aclnnop/aclnn_moe_router_logits.h"
 
@@ -12,39 +20,336 @@ constexpr int64_t kMaxExperts = 4096;
 struct LogitsArgs {
     const void* x;
     const void* weight;
-    float* logits;
+    float* logits;    // [splits, rows, experts] where the columns are split, the operator's output otherwise
     int64_t rows;
     int64_t cols;
+    int64_t splitCols;  // columns of a split (blockIdx.z)
     int32_t experts;
 };
 
-// A workgroup per 16 rows and 16 experts, one product per thread, the columns 32 at a time through LDS.
-constexpr int kTile = 16;
-constexpr int kStep = 32;
+typedef __bf16 Bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 F16x8 __attribute__((ext_vector_type(8)));
+typedef float F32x4 __attribute__((ext_vector_type(4)));
+typedef float F32x16 __attribute__((ext_vector_type(16)));
 
-template <typename Codec, typename Weight>
-__global__ __launch_bounds__(kTile * kTile) void RouterLogitsAnyKernel(LogitsArgs a) {
-    __shared__ float xs[kTile][kStep + 1];
-    __shared__ float ws[kTile][kStep + 1];
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kTile;
-    const int expert0 = blockIdx.y * kTile;
-    const int r = threadIdx.x / kTile, e = threadIdx.x % kTile;
-    float acc = 0.f;
-    for (int64_t c0 = 0; c0 < a.cols; c0 += kStep) {
-        for (int i = threadIdx.x; i < kTile * kStep; i += kTile * kTile) {
-            const int line = i / kStep;
-            const int64_t c = c0 + i % kStep;
-            xs[line][i % kStep] = row0 + line < a.rows && c < a.cols
-                                      ? Codec::Load(static_cast<const typename Codec::Storage*>(a.x)[(row0 + line) * a.cols + c]) : 0.f;
-            ws[line][i % kStep] = expert0 + line < a.experts && c < a.cols
-                                      ? Weight::Load(static_cast<const typename Weight::Storage*>(a.weight)[(expert0 + line) * a.cols + c]) : 0.f;
-        }
-        __syncthreads();
+// Eight neighbouring values of one row as they lie in memory.
+template <typename Codec>
+struct Raw {
+    uint4 q[sizeof(typename Codec::Storage) / 2];
+};
+
+// Values from column c on of a row of `cols`; those behind `end` (at most cols) are zeros.  kAligned: rows start on 16 bytes and are whole numbers of
+// them, and so are the ranges.
+template <typename Codec, bool kAligned>
+__device__ __forceinline__ Raw<Codec> LoadRaw(const typename Codec::Storage* row, int64_t c, int64_t end) {
+    constexpr int kPieces = sizeof(typename Codec::Storage) / 2, kPer = 8 / kPieces;
+    Raw<Codec> r;
+    if constexpr (kAligned) {
 #pragma unroll
-        for (int i = 0; i < kStep; ++i) acc = fmaf(xs[r][i], ws[e][i], acc);
+        for (int i = 0; i < kPieces; ++i) {
+            r.q[i] = c + i * kPer < end ? *reinterpret_cast<const uint4*>(row + c + i * kPer) : uint4{0, 0, 0, 0};
+        }
+    } else {
+        typename Codec::Storage v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < end ? row[c + i] : typename Codec::Storage{};
+        __builtin_memcpy(&r, v, sizeof(r));
+    }
+    return r;
+}
+
+// Operands of the matrix instructions: one of the type itself, or kParts of bf16.
+template <typename Codec, int kParts>
+struct Parts {
+    uint4 p[kParts];
+};
+
+__device__ __forceinline__ uint32_t UpperHalves(float even, float odd) {
+    return __builtin_amdgcn_perm(__float_as_uint(odd), __float_as_uint(even), 0x07060302u);
+}
+__device__ __forceinline__ float Cut(float f) { return __uint_as_float(__float_as_uint(f) & 0xffff0000u); }
+
+template <typename Codec, int kParts>
+__device__ __forceinline__ Parts<Codec, kParts> PartsOf(const Raw<Codec>& r) {
+    Parts<Codec, kParts> out;
+    if constexpr (kParts == 1) {
+        static_assert(sizeof(typename Codec::Storage) == 2);
+        out.p[0] = r.q[0];
+    } else {
+        uint32_t words[kParts][4];
+#pragma unroll
+        for (int pair = 0; pair < 4; ++pair) {
+            float v[2];
+            if constexpr (std::is_same_v<Codec, F32>) {
+                const uint4 q = r.q[pair / 2];
+                v[0] = __uint_as_float(pair % 2 == 0 ? q.x : q.z);
+                v[1] = __uint_as_float(pair % 2 == 0 ? q.y : q.w);
+            } else {
+                const uint4 q = r.q[0];
+                const uint32_t two = pair == 0 ? q.x : pair == 1 ? q.y : pair == 2 ? q.z : q.w;
+                v[0] = Codec::Load(static_cast<uint16_t>(two));
+                v[1] = Codec::Load(static_cast<uint16_t>(two >> 16));
+            }
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                words[part][pair] = UpperHalves(v[0], v[1]);
+                v[0] -= Cut(v[0]);
+                v[1] -= Cut(v[1]);
+            }
+        }
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) out.p[part] = uint4{words[part][0], words[part][1], words[part][2], words[part][3]};
+    }
+    return out;
+}
+
+// Element types of the two sides and the number of parts of each.
+template <typename X, typename W>
+struct Sides {
+    using XType = X;
+    using WType = W;
+    static constexpr bool kSame16 = std::is_same_v<X, W> && sizeof(typename X::Storage) == 2;
+    static constexpr int kX = kSame16 || std::is_same_v<X, Bf16> ? 1 : std::is_same_v<X, F16> ? 2 : 3;
+    static constexpr int kW = kSame16 ? 1 : 3;
+    static constexpr bool kHalf = kSame16 && std::is_same_v<X, F16>;  // fp16 instructions; bf16 otherwise
+};
+
+template <bool kHalf>
+__device__ __forceinline__ F32x4 Multiply(const uint4& a, const uint4& b, F32x4 c) {  // 16 x 16 x 32
+    if constexpr (kHalf) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(F16x8, a), __builtin_bit_cast(F16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
+}
+template <bool kHalf>
+__device__ __forceinline__ F32x16 Multiply(const uint4& a, const uint4& b, F32x16 c) {  // 32 x 32 x 16
+    if constexpr (kHalf) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(F16x8, a), __builtin_bit_cast(F16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Bf16x8, a), __builtin_bit_cast(Bf16x8, b), c, 0, 0, 0);
+}
+
+// Few rows: operands go from memory to registers, the waves of a workgroup share its columns, 32 at a time in turn, and add up through LDS.  A workgroup makes
+// kM x kN tiles of 16 rows and 16 experts.  With kSub > 1 (kM = kN = 1) the sixteen lines of either operand are 16 / kSub rows or experts times kSub
+// neighbouring runs of 32 columns: the products of a run with itself, one in kSub, are what is added up, and a workgroup streams fewer experts' weights.
+template <typename S, int kM, int kN, int kSub, int kWaves, bool kAligned>
+__global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsArgs a) {
+    using X = typename S::XType;
+    using W = typename S::WType;
+        constexpr int kLines = 16 / kSub;
+    __shared__ F32x4 sums[kWaves * kM * kN][kWave];
+    constexpr int kDepth = kAligned ? (kM * kN > 1 ? 2 : 4) : 1;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int line = lane % 16 / kSub, sub = lane % 16 % kSub;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kLines * kM);
+    const int expert0 = blockIdx.y * (kLines * kN);
+    const int64_t begin = blockIdx.z * a.splitCols, end = min(a.cols, begin + a.splitCols);
+    const typename X::Storage* x[kM];
+    const typename W::Storage* w[kN];
+#pragma unroll
+    for (int m = 0; m < kM; ++m) x[m] = static_cast<const typename X::Storage*>(a.x) + min(row0 + m * kLines + line, a.rows - 1) * a.cols;
+#pragma unroll
+    for (int n = 0; n < kN; ++n) {
+        w[n] = static_cast<const typename W::Storage*>(a.weight) + static_cast<int64_t>(min(expert0 + n * kLines + line, a.experts - 1)) * a.cols;
+    }
+    F32x4 acc[kM][kN] = {};
+    const int at = (lane / 16 * kSub + sub) * 8;
+    for (int64_t base = begin + wave * (kSub * 32); base < end; base += kDepth * kWaves * kSub * 32) {
+        Raw<X> xr[kDepth][kM];
+        Raw<W> wr[kDepth][kN];
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            const int64_t c = base + d * (kWaves * kSub * 32) + at;
+#pragma unroll
+            for (int n = 0; n < kN; ++n) wr[d][n] = LoadRaw<W, kAligned>(w[n], c, end);
+#pragma unroll
+            for (int m = 0; m < kM; ++m) xr[d][m] = LoadRaw<X, kAligned>(x[m], c, end);
+        }
+#pragma unroll
+        for (int d = 0; d < kDepth; ++d) {
+            Parts<X, S::kX> xp[kM];
+#pragma unroll
+            for (int m = 0; m < kM; ++m) xp[m] = PartsOf<X, S::kX>(xr[d][m]);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) {
+                const Parts<W, S::kW> wp = PartsOf<W, S::kW>(wr[d][n]);
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+#pragma unroll
+                    for (int i = S::kX - 1; i >= 0; --i) {
+#pragma unroll
+                        for (int j = S::kW - 1; j >= 0; --j) {
+                            if (i + j <= 2) acc[m][n] = Multiply<S::kHalf>(xp[m].p[i], wp.p[j], acc[m][n]);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    // of a tile, lane l holds the columns l % 16 of the lines l / 16 * 4 + 0 .. 3
+#pragma unroll
+    for (int m = 0; m < kM; ++m) {
+#pragma unroll
+        for (int n = 0; n < kN; ++n) sums[wave * kM * kN + m * kN + n][lane] = acc[m][n];
+    }
+    __syncthreads();
+    const float* const all = reinterpret_cast<const float*>(sums);
+    float* const out = a.logits + static_cast<int64_t>(blockIdx.z) * a.rows * a.experts;
+    for (int i = threadIdx.x; i < kLines * kM * kLines * kN; i += kWave * kWaves) {
+        const int r = i / (kLines * kN), e = i % (kLines * kN);
+        const int64_t row = row0 + r;
+        const int expert = expert0 + e;
+        const int tile = r / kLines * kN + e / kLines;
+        float sum = 0.f;
+        for (int v = 0; v < kWaves; ++v) {
+#pragma unroll
+            for (int t = 0; t < kSub; ++t) {
+                const int i16 = r % kLines * kSub + t, j16 = e % kLines * kSub + t;
+                sum += all[((v * kM * kN + tile) * kWave + i16 / 4 * 16 + j16) * 4 + i16 % 4];
+            }
+        }
+        if (row < a.rows && expert < a.experts) out[row * a.experts + expert] = sum;
+    }
+}
+
+// Many rows: tiles of 128 rows and kBn experts through LDS, cut into parts on the way, two buffers deep, eight waves of 32 x 32 x 16 products.
+// Lines in LDS are 16 bytes longer than their columns, so that eight lanes of a fragment read meet eight different sets of banks.
+constexpr int kBm = 128;
+constexpr int kTileThreads = 512;
+
+template <typename S, int kBn>
+struct TileShape {
+    static constexpr int kBk = S::kX == 1 && S::kW == 1 ? 64 : 32;
+    static constexpr int kPitch = kBk * 2 + 16;
+    static constexpr int kXBytes = S::kX * kBm * kPitch;
+    static constexpr int kStage = kXBytes + S::kW * kBn * kPitch;
+    static constexpr int kWavesM = kBn == 64 ? 4 : 2, kWavesN = 8 / kWavesM;
+    static constexpr int kMt = kBm / kWavesM / 32, kNt = kBn / kWavesN / 32;
+};
+
+template <typename S, int kBn, bool kAligned>
+__global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArgs a) {
+    using X = typename S::XType;
+    using W = typename S::WType;
+    using Shape = TileShape<S, kBn>;
+    constexpr int kBk = Shape::kBk, kPitch = Shape::kPitch, kChunks = kBk / 8;
+    constexpr int kXLoads = kBm * kChunks / kTileThreads, kWLoads = (kBn * kChunks + kTileThreads - 1) / kTileThreads;
+    constexpr bool kWHalf = kBn * kChunks < kTileThreads;  // the first threads alone load weights
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBm;
+    const int expert0 = blockIdx.y * kBn;
+    const int64_t begin = blockIdx.z * a.splitCols, end = min(a.cols, begin + a.splitCols);
+    const int steps = static_cast<int>((end - begin + kBk - 1) / kBk);
+
+    const int chunk = tid % kChunks, lineOf = tid / kChunks;
+    constexpr int kLineStep = kTileThreads / kChunks;
+    const bool loadsW = !kWHalf || lineOf < kBn;
+    const typename X::Storage* x[kXLoads];
+    const typename W::Storage* w[kWLoads];
+#pragma unroll
+    for (int i = 0; i < kXLoads; ++i) {
+        x[i] = static_cast<const typename X::Storage*>(a.x) + min(row0 + lineOf + i * kLineStep, a.rows - 1) * a.cols;
+    }
+#pragma unroll
+    for (int i = 0; i < kWLoads; ++i) {
+        w[i] = static_cast<const typename W::Storage*>(a.weight) + static_cast<int64_t>(min(expert0 + lineOf + i * kLineStep, a.experts - 1)) * a.cols;
+    }
+    Raw<X> xr[kXLoads];
+    Raw<W> wr[kWLoads];
+    auto load = [&](int step) {
+        const int64_t c = begin + step * kBk + chunk * 8;
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) xr[i] = LoadRaw<X, kAligned>(x[i], c, end);
+        if (loadsW) {
+#pragma unroll
+            for (int i = 0; i < kWLoads; ++i) wr[i] = LoadRaw<W, kAligned>(w[i], c, end);
+        }
+    };
+    auto store = [&](unsigned char* stage) {
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) {
+            const Parts<X, S::kX> parts = PartsOf<X, S::kX>(xr[i]);
+#pragma unroll
+            for (int p = 0; p < S::kX; ++p) {
+                *reinterpret_cast<uint4*>(stage + (p * kBm + lineOf + i * kLineStep) * kPitch + chunk * 16) = parts.p[p];
+            }
+        }
+        if (loadsW) {
+#pragma unroll
+            for (int i = 0; i < kWLoads; ++i) {
+                const Parts<W, S::kW> parts = PartsOf<W, S::kW>(wr[i]);
+#pragma unroll
+                for (int p = 0; p < S::kW; ++p) {
+                    *reinterpret_cast<uint4*>(stage + Shape::kXBytes + (p * kBn + lineOf + i * kLineStep) * kPitch + chunk * 16) = parts.p[p];
+                }
+            }
+        }
+    };
+
+    F32x16 acc[Shape::kMt][Shape::kNt] = {};
+    const int waveRow = wave / Shape::kWavesN * (Shape::kMt * 32), waveExpert = wave % Shape::kWavesN * (Shape::kNt * 32);
+    const int fragment = lane % 32 * kPitch + lane / 32 * 16;
+    load(0);
+    store(lds);
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        if (step + 1 < steps) load(step + 1);
+        const unsigned char* const xs = lds + step % 2 * Shape::kStage + waveRow * kPitch + fragment;
+        const unsigned char* const ws = lds + step % 2 * Shape::kStage + Shape::kXBytes + waveExpert * kPitch + fragment;
+#pragma unroll
+        for (int k = 0; k < kBk / 16; ++k) {
+            uint4 xf[S::kX][Shape::kMt], wf[S::kW][Shape::kNt];
+#pragma unroll
+            for (int p = 0; p < S::kX; ++p) {
+#pragma unroll
+                for (int m = 0; m < Shape::kMt; ++m) xf[p][m] = *reinterpret_cast<const uint4*>(xs + (p * kBm + m * 32) * kPitch + k * 32);
+            }
+#pragma unroll
+            for (int p = 0; p < S::kW; ++p) {
+#pragma unroll
+                for (int n = 0; n < Shape::kNt; ++n) wf[p][n] = *reinterpret_cast<const uint4*>(ws + (p * kBn + n * 32) * kPitch + k * 32);
+            }
+#pragma unroll
+            for (int i = S::kX - 1; i >= 0; --i) {
+#pragma unroll
+                for (int j = S::kW - 1; j >= 0; --j) {
+                    if (i + j > 2) continue;
+#pragma unroll
+                    for (int m = 0; m < Shape::kMt; ++m) {
+#pragma unroll
+                        for (int n = 0; n < Shape::kNt; ++n) acc[m][n] = Multiply<S::kHalf>(xf[i][m], wf[j][n], acc[m][n]);
+                    }
+                }
+            }
+        }
+        if (step + 1 < steps) store(lds + (step + 1) % 2 * Shape::kStage);
         __syncthreads();
     }
-    if (row0 + r < a.rows && expert0 + e < a.experts) a.logits[(row0 + r) * a.experts + expert0 + e] = acc;
+    // of a tile, lane l holds column l % 32 of the lines 8 (i / 4) + 4 (l / 32) + i % 4, i = 0 .. 15
+    float* const out = a.logits + static_cast<int64_t>(blockIdx.z) * a.rows * a.experts;
+#pragma unroll
+    for (int m = 0; m < Shape::kMt; ++m) {
+#pragma unroll
+        for (int n = 0; n < Shape::kNt; ++n) {
+            const int expert = expert0 + waveExpert + n * 32 + lane % 32;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int64_t row = row0 + waveRow + m * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+                if (row < a.rows && expert < a.experts) out[row * a.experts + expert] = acc[m][n][i];
+            }
+        }
+    }
+}
+
+// Adds the splits up, in their order.
+constexpr int kAddThreads = 256;
+
+template <int kVec>
+__global__ __launch_bounds__(kAddThreads) void AddSplitsKernel(const float* partial, float* logits, int64_t count, int splits) {
+    typedef float Vec __attribute__((ext_vector_type(kVec)));
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kAddThreads + threadIdx.x;
+    if (i * kVec >= count) return;
+    Vec sum = reinterpret_cast<const Vec*>(partial)[i];
+#pragma unroll 4
+    for (int s = 1; s < splits; ++s) sum += reinterpret_cast<const Vec*>(partial + s * count)[i];
+    reinterpret_cast<Vec*>(logits)[i] = sum;
 }
 
 class LogitsExecutor : public aclOpExecutor {
@@ -52,26 +357,135 @@ class LogitsExecutor : public aclOpExecutor {
     LogitsArgs args{};
     aclDataType dtype = ACL_FLOAT;
     aclDataType weightType = ACL_FLOAT;
+    // The plan, made from sizes alone.
+    int tile = 0;      // experts of a tile of 128 rows, or 0: slim
+    int slimM = 1, slimN = 1, slimSub = 1, slimWaves = 8;
+    int splits = 1;
 
-    template <typename Codec, typename Weight>
-    void Launch(hipStream_t stream) const {
-        const dim3 grid(static_cast<unsigned>((args.rows + kTile - 1) / kTile), static_cast<unsigned>((args.experts + kTile - 1) / kTile));
-        hipLaunchKernelGGL((RouterLogitsAnyKernel<Codec, Weight>), grid, dim3(kTile * kTile), 0, stream, args);
+    void Plan() {
+        const int64_t T = args.rows, K = args.cols, E = args.experts;
+        const char* env = std::getenv("RL_PLAN");  // tuning
+        int v[6] = {0, 0, 0, 0, 0, 0};
+        if (env != nullptr) sscanf(env, "%d,%d,%d,%d,%d,%d", &v[0], &v[1], &v[2], &v[3], &v[4], &v[5]);
+        if (env != nullptr) {
+            tile = v[0]; slimM = v[1]; slimN = v[2]; slimSub = v[3]; slimWaves = v[4]; splits = v[5];
+        } else if (T > 512 && E > 16) {
+            tile = E <= 64 ? 64 : E <= 128 || dtype != ACL_BF16 ? 128 : 256;
+            const int64_t groups = (T + kBm - 1) / kBm * ((E + tile - 1) / tile);
+            while (groups * splits < 256 && splits < 32) splits *= 2;
+        } else {
+            slimSub = T <= 1 ? 16 : T <= 2 ? 8 : T <= 4 ? 4 : T <= 8 ? 2 : 1;
+        }
+        const int64_t grain = 64 * slimSub;
+        args.splitCols = ((K + splits - 1) / splits + grain - 1) / grain * grain;
+        splits = static_cast<int>((K + args.splitCols - 1) / args.splitCols);
     }
 
-    template <typename Codec>
-    void LaunchFor(hipStream_t stream) const {
-        if (weightType == Codec::kType) Launch<Codec, Codec>(stream);
-        else Launch<Codec, F32>(stream);
+    uint64_t OwnBytes() const { return splits > 1 ? static_cast<uint64_t>(splits) * args.rows * args.experts * sizeof(float) : 0; }
+
+    template <typename S, int kM, int kN, int kSub, int kWaves, bool kAligned>
+    hipError_t LaunchSlim(const LogitsArgs& a, hipStream_t stream) const {
+        constexpr int kLines = 16 / kSub;
+        const dim3 grid(static_cast<unsigned>((a.rows + kLines * kM - 1) / (kLines * kM)), static_cast<unsigned>((a.experts + kLines * kN - 1) / (kLines * kN)),
+                        splits);
+        hipLaunchKernelGGL((RouterLogitsSlimKernel<S, kM, kN, kSub, kWaves, kAligned>), grid, dim3(kWave * kWaves), 0, stream, a);
+        return hipGetLastError();
     }
 
-    aclnnStatus Run(void*, hipStream_t stream) override {
+    template <typename S, int kBn, bool kAligned>
+    hipError_t LaunchTile(const LogitsArgs& a, hipStream_t stream) const {
+        auto kernel = RouterLogitsTileKernel<S, kBn, kAligned>;
+        constexpr int kBytes = 2 * TileShape<S, kBn>::kStage;
+        static_assert(kBytes <= 160 * 1024);
+        static std::atomic<uint64_t> optedIn{0};
+        const hipError_t attr = opapi::EnsureDynamicLds(reinterpret_cast<const void*>(kernel), kBytes, optedIn);
+        if (attr != hipSuccess) return attr;
+        const dim3 grid(static_cast<unsigned>((a.rows + kBm - 1) / kBm), static_cast<unsigned>((a.experts + kBn - 1) / kBn), splits);
+        hipLaunchKernelGGL(kernel, grid, dim3(kTileThreads), kBytes, stream, a);
+        return hipGetLastError();
+    }
+
+    template <typename S, bool kAligned>
+    hipError_t LaunchPlan(const LogitsArgs& a, hipStream_t stream) const {
+        if (tile == 64) return LaunchTile<S, 64, kAligned>(a, stream);
+        if (tile == 128) return LaunchTile<S, 128, kAligned>(a, stream);
+        if constexpr (S::kX == 1) {
+            if (tile == 256) return LaunchTile<S, 256, kAligned>(a, stream);
+        }
+        if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 16, 4, kAligned>(a, stream);
+        if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 16, 8, kAligned>(a, stream);
+        if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 16, 16, kAligned>(a, stream);
+        if (slimSub == 8 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 8, 4, kAligned>(a, stream);
+        if (slimSub == 8 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 8, 8, kAligned>(a, stream);
+        if (slimSub == 8 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 8, 16, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 4, 4, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 4, 8, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 4, 16, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 2 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 2, 1, 4, 8, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 2 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 2, 1, 4, 16, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 1 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 1, 2, 4, 8, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 1 && slimN == 2 && slimWaves == 16) return LaunchSlim<S, 1, 2, 4, 16, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 2 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 2, 2, 4, 8, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 4 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 4, 1, 4, 8, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 4 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 4, 2, 4, 8, kAligned>(a, stream);
+        if (slimSub == 4 && slimM == 4 && slimN == 4 && slimWaves == 8) return LaunchSlim<S, 4, 4, 4, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 2, 4, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 2, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 2, 16, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 2 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 2, 1, 2, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 2 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 2, 1, 2, 16, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 1 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 1, 2, 2, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 1 && slimN == 2 && slimWaves == 16) return LaunchSlim<S, 1, 2, 2, 16, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 2 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 2, 2, 2, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 4 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 4, 1, 2, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 4 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 4, 2, 2, 8, kAligned>(a, stream);
+        if (slimSub == 2 && slimM == 4 && slimN == 4 && slimWaves == 8) return LaunchSlim<S, 4, 4, 2, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 1, 4, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 1, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 1, 16, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 2 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 2, 1, 1, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 2 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 2, 1, 1, 16, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 1 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 1, 2, 1, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 1 && slimN == 2 && slimWaves == 16) return LaunchSlim<S, 1, 2, 1, 16, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 2 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 2, 2, 1, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 4 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 4, 1, 1, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 4 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 4, 2, 1, 8, kAligned>(a, stream);
+        if (slimSub == 1 && slimM == 4 && slimN == 4 && slimWaves == 8) return LaunchSlim<S, 4, 4, 1, 8, kAligned>(a, stream);
+        return hipErrorInvalidValue;
+    }
+
+    template <typename X, typename W>
+    hipError_t Launch(const LogitsArgs& a, hipStream_t stream) const {
+        auto onGrid = [&](const void* p, size_t size) {
+            return reinterpret_cast<uintptr_t>(p) % 16 == 0 && static_cast<uint64_t>(a.cols) * size % 16 == 0;
+        };
+        const bool aligned = onGrid(a.x, sizeof(typename X::Storage)) && onGrid(a.weight, sizeof(typename W::Storage));
+        return aligned ? LaunchPlan<Sides<X, W>, true>(a, stream) : LaunchPlan<Sides<X, W>, false>(a, stream);
+    }
+
+    aclnnStatus Run(void* workspace, hipStream_t stream) override {
         if (args.rows == 0) return ACLNN_SUCCESS;
-        opapi::KernelTimer timer("router_logits", stream);
-        if (dtype == ACL_FLOAT) Launch<F32, F32>(stream);
-        else if (dtype == ACL_FLOAT16) LaunchFor<F16>(stream);
-        else LaunchFor<Bf16>(stream);
-        const hipError_t err = hipGetLastError();
+        OPAPI_CHECK(splits == 1 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, ACLNN_ERR_PARAM_INVALID,
+                    "aclnnMoeRouterLogits: the workspace must be 16-byte aligned");
+        hipError_t err;
+        {
+            opapi::KernelTimer timer("router_logits", stream);
+            LogitsArgs a = args;
+            if (splits > 1) a.logits = static_cast<float*>(workspace);
+            if (dtype == ACL_FLOAT) err = Launch<F32, F32>(a, stream);
+            else if (dtype == ACL_FLOAT16) err = weightType == ACL_FLOAT ? Launch<F16, F32>(a, stream) : Launch<F16, F16>(a, stream);
+            else err = weightType == ACL_FLOAT ? Launch<Bf16, F32>(a, stream) : Launch<Bf16, Bf16>(a, stream);
+        }
+        if (err == hipSuccess && splits > 1) {
+            opapi::KernelTimer timer("router_logits_add", stream);
+            const int64_t count = args.rows * args.experts;
+            const float* const partial = static_cast<const float*>(workspace);
+            const int vec = count % 4 == 0 && reinterpret_cast<uintptr_t>(args.logits) % 16 == 0 ? 4 : 1;
+            const unsigned blocks = static_cast<unsigned>((count / vec + kAddThreads - 1) / kAddThreads);
+            if (vec == 4) hipLaunchKernelGGL(AddSplitsKernel<4>, dim3(blocks), dim3(kAddThreads), 0, stream, partial, args.logits, count, splits);
+            else hipLaunchKernelGGL(AddSplitsKernel<1>, dim3(blocks), dim3(kAddThreads), 0, stream, partial, args.logits, count, splits);
+            err = hipGetLastError();
+        }
         if (err != hipSuccess) {
             opapi::SetError("aclnnMoeRouterLogits: launch failed: %s", hipGetErrorString(err));
             return ACLNN_ERR_RUNTIME_ERROR;
@@ -100,7 +514,7 @@ extern "C" aclnnStatus aclnnMoeRouterLogitsGetWorkspaceSize(const aclTensor* x, 
     const int64_t cols = x->dims.back();
     OPAPI_CHECK(cols > 0, kInvalid, "the last extent of x is zero");
     const int64_t rows = RowsOf(x);
-    OPAPI_CHECK(rows >= 0, kInvalid, "x has more than 2147483647 rows");
+    OPAPI_CHECK(rows >= 0, kInvalid, "x has more than %lld rows", (long long)kMaxRows);
     OPAPI_CHECK(weight->dtype == x->dtype || weight->dtype == ACL_FLOAT, kInvalid, "weight must be of x's type or FLOAT");
     OPAPI_CHECK(weight->dims.size() == 2 && weight->dims[1] == cols, kInvalid, "weight %s must be [experts, %lld]", ShapeStr(weight).c_str(),
                 (long long)cols);
@@ -126,7 +540,8 @@ extern "C" aclnnStatus aclnnMoeRouterLogitsGetWorkspaceSize(const aclTensor* x, 
     ex->args.rows = rows;
     ex->args.cols = cols;
     ex->args.experts = static_cast<int32_t>(experts);
-    ex->SealWorkspace(0);
+    if (rows > 0) ex->Plan();
+    ex->SealWorkspace(ex->OwnBytes());
     *workspaceSize = ex->workspaceBytes;
     *executor = ex;
     return ACLNN_SUCCESS;

@@ -256,10 +256,11 @@ def _gating_reference(x, k, bias=None, k_group=1, group_count=1, group_select_mo
             e = np.where(masked, 0, np.exp(x - top))
             p = np.where(masked, 0, e / e.sum(-1, keepdims=True))
         t = np.where(masked, -np.inf, p if bias is None else p + bias.double().numpy())
+    key = x if bias is None else t               # p is a monotone function of the logit: without a bias logits are compared
     order_of = lambda v: np.argsort(-np.nan_to_num(v, nan=np.inf, neginf=-np.inf), axis=-1, kind="stable")  # NaN ahead of all
     out = np.zeros((rows, E), dtype=bool)
     if k_group < group_count:
-        g = t.reshape(rows, group_count, -1)
+        g = (t if group_select_mode == 1 else key).reshape(rows, group_count, -1)
         desc = -np.sort(-np.nan_to_num(g, nan=np.inf, neginf=-np.inf), axis=-1)
         best = desc[:, :, 0]
         if group_select_mode == 1:
@@ -271,7 +272,7 @@ def _gating_reference(x, k, bias=None, k_group=1, group_count=1, group_select_mo
     idx = np.empty((rows, k), dtype=np.int64)
     for r in range(rows):
         kept = np.flatnonzero(~out[r])
-        idx[r] = kept[order_of(t[r:r + 1, kept])[0][:k]]
+        idx[r] = kept[order_of(key[r:r + 1, kept])[0][:k]]
     y = np.take_along_axis(p, idx, -1)
     if renorm:
         total = y.sum(-1, keepdims=True) + eps
