@@ -35,7 +35,8 @@ struct GatingArgs {
     int32_t topTwo;           // a group's value is the sum of its two largest t
     int32_t sigmoid;
     int32_t renorm;
-    int32_t packets;          // rows start on 16 bytes and fill their lanes
+    int32_t packets;          // rows fill their lanes and start on the lanes' boundaries
+    int32_t biasPackets;      // so does the bias
     uint32_t groupMagic;      // (c * groupMagic) >> 21 = c / (experts / groups) for c < 512
     float factor;
     double eps;
@@ -250,12 +251,20 @@ __device__ __forceinline__ uint32_t Key32(float f) {
 }
 __device__ __forceinline__ float Value32(uint32_t key) { return __uint_as_float((key & 0x80000000u) != 0 ? (key & 0x7fffffffu) : ~key); }
 
-// exp(d) for d <= 0 to an fp32 unit in the last place: the product with log2(e) to twice fp32's bits, its tail put back behind the instruction.
+// Key32 of a number that is no NaN.
+__device__ __forceinline__ uint32_t NumberKey(float f) {
+    const int32_t u = __builtin_bit_cast(int32_t, f);
+    return static_cast<uint32_t>(u) ^ (static_cast<uint32_t>(u >> 31) | 0x80000000u);
+}
+
+// exp(d) for d <= 0 to an fp32 unit in the last place (0 below e^-110): the product with log2(e) to twice fp32's bits, its tail put back behind the
+// instruction.
 __device__ __forceinline__ float ExpNotAbove1(float d) {
+    d = d < -110.f ? -110.f : d;
     const float h = d * 0x1.715476p+0f;
     const float tail = fmaf(d, 0x1.715476p+0f, -h) + d * 0x1.4ae0cp-26f;
     const float e = __builtin_amdgcn_exp2f(h);
-    return h < -150.f ? 0.f : fmaf(e, tail * 0x1.62e43p-1f, e);
+    return fmaf(e, tail * 0x1.62e43p-1f, e);
 }
 
 // The kPer values of a lane; absent ones are -inf.
@@ -429,29 +438,53 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
 
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
     const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr, grouped = a.kGroup < a.groups;
-    float v[kPer];
+    float v[kPer], b[kPer];
     LoadLane<Codec, kPer>(a, x, l, v);
+    if (biased) {
+        if (a.biasPackets != 0) {
+            constexpr int kPiece = kPer < 4 ? kPer : 4;
+            struct alignas(kPiece * 4) Piece {
+                float e[kPiece];
+            };
+#pragma unroll
+            for (int i = 0; i < kPer; i += kPiece) {
+                const Piece piece = *reinterpret_cast<const Piece*>(a.bias + l * kPer + i);
+#pragma unroll
+                for (int j = 0; j < kPiece; ++j) b[i + j] = piece.e[j];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) b[i] = a.bias[min(l * kPer + i, a.experts - 1)];
+        }
+    }
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) nan |= v[i] != v[i];
+    // uniform over the row: it is made again, for values too close to be told apart here, or a NaN
+    bool close = __any(nan) && RowMax<kLanes>(nan ? 1u : 0u) != 0;
 
     float shift = 0.f, top = 1.f;  // top: no p of the row is larger
     double sum = 1.0;
     if (!sigmoid) {
-        uint32_t most = 0;
+        float most = v[0];
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) most = max(most, Key32(v[i]));
-        shift = Value32(RowMax<kLanes>(most));
+        for (int i = 1; i < kPer; ++i) most = fmaxf(most, v[i]);
+        shift = RowReduce<kLanes>(most, [](float p, float q) { return fmaxf(p, q); });
+        if (shift == -INFINITY) shift = 0.f;  // nothing but -inf
         sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += v[i] == -INFINITY ? 0.f : ExpNotAbove1(v[i] - shift);
+        for (int i = 0; i < kPer; ++i) sum += static_cast<double>(ExpNotAbove1(v[i] - shift));
         sum = RowSum<kLanes>(sum);
         top = 1.f / static_cast<float>(sum);
     }
-    float t[kPer];
+    float t[kPer];  // what is compared
     if (biased || (grouped && a.topTwo != 0)) {
+        if (sigmoid) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            t[i] = v[i] == -INFINITY ? 0.f
-                   : sigmoid         ? __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v[i] * -0x1.715476p+0f))
-                                     : __builtin_amdgcn_exp2f((v[i] - shift) * 0x1.715476p+0f) * top;
+            for (int i = 0; i < kPer; ++i) t[i] = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v[i] * -0x1.715476p+0f));
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) t[i] = __builtin_amdgcn_exp2f((v[i] - shift) * 0x1.715476p+0f) * top;
         }
     }
     if (a.scores != nullptr && mine) {
@@ -460,42 +493,49 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             if (l * kPer + i < a.experts) a.scores[row * a.experts + l * kPer + i] = static_cast<float>(ScoreOf(v[i], sigmoid, shift, sum));
         }
     }
-    float largest = top;  // of |t|
+    float largest = top;  // |t| and what it is the sum of
     if (biased) {
-        uint32_t most = 0;
+        float most = 0.f;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            t[i] += a.bias[l * kPer + i < a.experts ? l * kPer + i : 0];
-            if (v[i] == -INFINITY) t[i] = -INFINITY;
-            else most = max(most, __float_as_uint(fabsf(t[i])));
+            most = fmaxf(most, fabsf(b[i]));
+            t[i] += b[i];
         }
-        largest = __uint_as_float(RowMax<kLanes>(most));
+        largest += RowReduce<kLanes>(most, [](float p, float q) { return fmaxf(p, q); });
+    }
+    if (biased || (grouped && a.topTwo != 0)) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) t[i] = v[i] == -INFINITY ? -INFINITY : t[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) t[i] = v[i];
     }
 
-    bool close = false;  // uniform over the row
-    uint64_t kept = ~0ull;
+    uint32_t kept = ~0u;  // groups, a bit each
+    int group = 0;
+    bool whole = false;   // a group's experts are those of its lanes
     if (grouped) {
         const int size = a.experts / a.groups;
-        const int share = kLanes >> (32 - __builtin_clz(a.groups * 2 - 1) - 1);  // lanes of a group, a power of two
-        const int group = l / share;
+        const int logShare = 4 - (32 - __builtin_clz(a.groups * 2 - 1) - 1), share = 1 << logShare;  // lanes of a group, a power of two
+        group = l >> logShare;
+        whole = share * kPer == size;
         uint32_t one = 0, two = 0;
         auto take = [&](float value) {
-            const uint32_t key = Key32(value);
+            const uint32_t key = NumberKey(value);
             two = max(two, min(one, key));
             one = max(one, key);
         };
-        auto valueOf = [&](int i) { return v[i] == -INFINITY ? -INFINITY : biased || a.topTwo != 0 ? t[i] : v[i]; };
-        if (share * kPer == size) {  // a group's experts are those of its lanes
+        if (whole) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) take(valueOf(i));
+            for (int i = 0; i < kPer; ++i) take(t[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
-                if (l * kPer + i < a.experts) values[l * kPer + i] = valueOf(i);
+                if (l * kPer + i < a.experts) values[l * kPer + i] = t[i];
             }
             WaveSync();
             if (group < a.groups) {
-                for (int c = l % share; c < size; c += share) take(values[group * size + c]);
+                for (int c = l & (share - 1); c < size; c += share) take(values[group * size + c]);
             }
             WaveSync();
         }
@@ -505,28 +545,42 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             one = max(one, otherOne);
         }
         uint32_t value = 0;
-        if (l % share == 0 && group < a.groups) {
-            value = a.topTwo != 0 && two != 0 && Value32(two) != -INFINITY ? Key32(Value32(one) + Value32(two)) : one;
+        if ((l & (share - 1)) == 0 && group < a.groups) {
+            value = a.topTwo != 0 && two != 0 && Value32(two) != -INFINITY ? NumberKey(Value32(one) + Value32(two)) : one;
         }
         kept = 0;
         uint32_t last = 0;
         for (int j = 0; j < a.kGroup; ++j) {
             last = RowMax<kLanes>(value);
             const uint32_t at = RowMin<kLanes>(value == last ? l : kLanes - 1);
-            kept |= 1ull << (at / share);
+            kept |= 1u << (at >> logShare);
             if (l == static_cast<int>(at)) value = 0;
         }
         const uint32_t next = RowMax<kLanes>(value);
-        if (biased || a.topTwo != 0) close = Value32(last) - Value32(next) <= kU * (32.f * top + 16.f * largest);
+        if (biased || a.topTwo != 0) close |= Value32(last) - Value32(next) <= kU * (32.f * top + 16.f * largest);
+        if (!biased && a.topTwo != 0) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) t[i] = v[i];
+        }
     }
 
+    // a bit for every value that is looked at: there, and in a group that stays
+    uint32_t present = 0;
+    if (!grouped) {
+        const int count = a.experts - l * kPer;
+        present = count >= kPer ? ~0u : count > 0 ? (1u << count) - 1 : 0u;
+    } else if (whole) {
+        present = (kept >> group & 1) != 0 ? ~0u : 0u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t c = l * kPer + i;
+            present |= (c < static_cast<uint32_t>(a.experts) ? kept >> ((c * a.groupMagic >> 21) & 31) & 1 : 0u) << i;
+        }
+    }
     uint32_t keys[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const uint32_t c = l * kPer + i;
-        keys[i] = c < static_cast<uint32_t>(a.experts) ? (Key32(biased ? t[i] : v[i]) & ~kLow) | (kLow - i) : 0u;
-        if (grouped && (kept >> ((c * a.groupMagic >> 21) & 63) & 1) == 0) keys[i] = 0u;
-    }
+    for (int i = 0; i < kPer; ++i) keys[i] = (present >> i & 1) != 0 ? (NumberKey(t[i]) & ~kLow) | (kLow - i) : 0u;
     // logits of 16 bits are compared exactly, fp32 ones up to the bits that a key lacks
     const float tolerance = biased ? kU * (16.f * top + 2.f * (1 + (2 << kBits)) * largest) : sizeof(typename Codec::Storage) == 4 && kBits > 0 ? 0.f : -1.f;
     int32_t pick = 0;
@@ -568,6 +622,7 @@ class GatingExecutor : public aclOpExecutor {
         GatingArgs g = args;
         const size_t bytes = per * sizeof(typename Codec::Storage), piece = bytes < 16 ? bytes : 16;
         g.packets = g.experts == lanes * per && reinterpret_cast<uintptr_t>(g.x) % piece == 0 ? 1 : 0;
+        g.biasPackets = g.experts == lanes * per && reinterpret_cast<uintptr_t>(g.bias) % 16 == 0 ? 1 : 0;
         return g;
     }
 
