@@ -9,7 +9,6 @@
 #include "moe_front.h"
 
 #include <cmath>
-#include <cstdlib>
 
 #include "aclnnop/aclnn_moe_gating_top_k_grouped.h"
 
@@ -304,7 +303,9 @@ __device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int
 }
 
 // A row of up to 64 * kPer experts, at most 64 groups, by one wave in 64 bits: lane l holds experts l * kPer + i, the keys in registers.  lds: 8 bytes an
-// expert, the wave's own, for the groups.
+// expert, the wave's own, for groups whose experts are not those of whole lanes.  What bounds it is latency: a pick is a maximum over four rotations inside
+// a row of sixteen lanes, four lane reads and a ballot (256 experts, 8 picks: 4.7 us, with sigmoid, bias and groups 6.0; with the keys in LDS and the
+// arg-max over twelve shuffles 10.9 and 15.8).
 template <typename Codec, typename Out, int kPer>
 __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int lane, uint64_t* lds, bool writeScores) {
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
@@ -338,19 +339,24 @@ __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int la
         // the lanes are shared out among the groups, a power of two each
         const int size = a.experts / a.groups;
         const int share = kWave >> (32 - __builtin_clz(a.groups * 2 - 1) - 1);
-        WaveSync();
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            if (lane * kPer + i < a.experts) lds[lane * kPer + i] = keys[i];
-        }
-        WaveSync();
         const int group = lane / share;
         uint64_t one = 0, two = 0;
-        if (group < a.groups) {
-            for (int c = lane % share; c < size; c += share) {
-                const uint64_t key = lds[group * size + c];
-                two = key > one ? one : key > two ? key : two;
-                one = key > one ? key : one;
+        auto take = [&](uint64_t key) {
+            two = key > one ? one : key > two ? key : two;
+            one = key > one ? key : one;
+        };
+        if (share * kPer == size) {  // a group's experts are those of its lanes
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) take(keys[i]);
+        } else {
+            WaveSync();
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                if (lane * kPer + i < a.experts) lds[lane * kPer + i] = keys[i];
+            }
+            WaveSync();
+            if (group < a.groups) {
+                for (int c = lane % share; c < size; c += share) take(lds[group * size + c]);
             }
         }
         for (int d = 1; d < share; d <<= 1) {
@@ -416,14 +422,16 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs
 constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts) * 16; }
 
 // Rows of up to 16 * kPer experts, at most 16 picks and groups: four rows a wave, sixteen lanes each, fp32 keys in registers.  Lane l of a row holds experts
-// l * kPer + i, so that among equal values the lower lane has the lower index; within a lane the number i goes into the lowest b bits of the key, which
-// costs fp32 keys as many bits and 16-bit logits nothing, and makes a lane's keys different.  `bound` is the last key that a lane gave away: of the
+// l * kPer + i, so that among equal values the lower lane has the lower index; within a lane the number i goes into the lowest bits of the key, which
+// makes a lane's keys different.  `bound` is the last key that a lane gave away: of the
 // differences key - bound modulo 2^32 the largest is that of the next smaller key.
-// Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once, b bits cut off
-// a key are 2^(b+1) u.  Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
+// Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once.  Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
+// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.8 us (16.8 MB of logits are 3.3), of which a row that
+// is made twice is 3; softmax without bias or groups, bf16 9.0.
 template <typename Codec, typename Out, int kPer>
 __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs a) {
-    constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : 4;
+    constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : kPer == 16 ? 4 : 5;
+    constexpr int kPlaceBits = 27;
     constexpr uint32_t kLow = (1u << kBits) - 1;
     constexpr float kU = 0x1p-24f;
     extern __shared__ __attribute__((aligned(16))) unsigned char ldsRaw[];
@@ -493,16 +501,19 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             if (l * kPer + i < a.experts) a.scores[row * a.experts + l * kPer + i] = static_cast<float>(ScoreOf(v[i], sigmoid, shift, sum));
         }
     }
-    float largest = top;  // |t| and what it is the sum of
+    float low = 0.f, high = top;  // low <= t <= high
     if (biased) {
-        float most = 0.f;
+        float least = b[0], most = b[0];
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            most = fmaxf(most, fabsf(b[i]));
+            least = fminf(least, b[i]);
+            most = fmaxf(most, b[i]);
             t[i] += b[i];
         }
-        largest += RowReduce<kLanes>(most, [](float p, float q) { return fmaxf(p, q); });
+        low = RowReduce<kLanes>(least, [](float p, float q) { return fminf(p, q); });
+        high = top + RowReduce<kLanes>(most, [](float p, float q) { return fmaxf(p, q); });
     }
+    const float largest = fmaxf(fabsf(low), fabsf(high));
     if (biased || (grouped && a.topTwo != 0)) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) t[i] = v[i] == -INFINITY ? -INFINITY : t[i];
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         }
     }
 
-    // a bit for every value that is looked at: there, and in a group that stays
+    // a bit for every value that is looked at: there, and in a group that stays (without branches for each: a third of the kernel's time)
     uint32_t present = 0;
     if (!grouped) {
         const int count = a.experts - l * kPer;
@@ -578,25 +589,40 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             present |= (c < static_cast<uint32_t>(a.experts) ? kept >> ((c * a.groupMagic >> 21) & 31) & 1 : 0u) << i;
         }
     }
+    // Without a bias a key is the logit's, cut: exact for 16 bits, and fp32 ones that agree in what is left are too close.  With one it is t's place
+    // between low and high in 2^27ths, from 32 on, and 1 for -inf.
     uint32_t keys[kPer];
+    uint32_t tooClose;  // a difference of two keys
+    if (biased) {
+        const float scale = 0x0.ffffp27f / (high - low);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) keys[i] = (present >> i & 1) != 0 ? (NumberKey(t[i]) & ~kLow) | (kLow - i) : 0u;
-    // logits of 16 bits are compared exactly, fp32 ones up to the bits that a key lacks
-    const float tolerance = biased ? kU * (16.f * top + 2.f * (1 + (2 << kBits)) * largest) : sizeof(typename Codec::Storage) == 4 && kBits > 0 ? 0.f : -1.f;
+        for (int i = 0; i < kPer; ++i) {
+            keys[i] = static_cast<uint32_t>(__builtin_amdgcn_fmed3f(fmaf(t[i] - low, scale, 32.f), 1.f, 0x0.fffffp27f)) << (32 - kPlaceBits) | (kLow - i);
+        }
+        // the difference to low, the product and the whole number round once each: 8, 8 and 1 units at most
+        const float units = (16.f * top + 2.f * largest) * kU * scale * 1.01f + 36.f;
+        tooClose = units < 0x1p26f ? static_cast<uint32_t>(units) << (32 - kPlaceBits) : ~0u;
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) keys[i] = (NumberKey(t[i]) & ~kLow) | (kLow - i);
+        tooClose = 0;
+    }
+    const bool exact = !biased && (sizeof(typename Codec::Storage) == 2 || kBits == 0);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) keys[i] = (present >> i & 1) != 0 ? keys[i] : 0u;
+    const uint32_t upper = biased ? ~31u : ~kLow, lowest = biased ? 2u << (32 - kPlaceBits) : 0x00800000u;  // below: -inf, or none left
     int32_t pick = 0;
-    float before = INFINITY;
-    uint32_t bound = 0;
+    uint32_t before = ~0u, bound = 0;
     for (int j = 0; j <= a.k; ++j) {
         uint32_t best = 0u - bound;  // none left
 #pragma unroll
         for (int i = 0; i < kPer; ++i) best = max(best, keys[i] - bound);
         best += bound;
-        const uint32_t most = RowMax<kLanes>(best & ~kLow);
-        const float now = Value32(most);
-        close |= before - now <= tolerance;
-        before = now;
+        const uint32_t most = RowMax<kLanes>(best & upper);
+        close |= !exact && j > 0 && most >= lowest && before - most <= tooClose;
+        before = most;
         if (j == a.k) break;
-        const uint32_t at = RowMin<kLanes>((best & ~kLow) == most ? l : kLanes - 1);
+        const uint32_t at = RowMin<kLanes>((best & upper) == most ? l : kLanes - 1);
         const uint32_t holder = __shfl(best, first + static_cast<int>(at));
         if (l == j) pick = static_cast<int32_t>(at) * kPer + static_cast<int32_t>(kLow - (holder & kLow));
         if (l == static_cast<int>(at)) bound = best;
@@ -640,16 +666,19 @@ class GatingExecutor : public aclOpExecutor {
 
     template <typename Codec, typename Out>
     void Launch(hipStream_t stream) const {
-        const char* env = std::getenv("GT_LANES");
-        const int lanes = env != nullptr ? atoi(env) : args.rows > 2048 ? 16 : 64;
         const int E = args.experts;
-        if (lanes == 16 && E <= 256 && args.k <= 16 && args.groups <= 16) {
+        // Sixteen lanes a row make more rows at a time and take longer for one, most of all with a bias, where one row in a thousand is
+        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 9.2 and 10.1 at 4096, 15.8 and
+        // 27.5 at 16384; softmax without a bias 5.2 and 5.3, 5.3 and 8.0, 9.0 and 20.7.
+        const bool many = args.rows > (args.bias != nullptr ? 4000 : 1024);
+        if (many && E <= 512 && args.k <= 16 && args.groups <= 16) {
             if (E <= 16) LaunchQuads<Codec, Out, 1>(stream);
             else if (E <= 32) LaunchQuads<Codec, Out, 2>(stream);
             else if (E <= 64) LaunchQuads<Codec, Out, 4>(stream);
             else if (E <= 128) LaunchQuads<Codec, Out, 8>(stream);
-            else LaunchQuads<Codec, Out, 16>(stream);
-        } else if (lanes != 1 && E <= 512 && args.groups <= kWave) {
+            else if (E <= 256) LaunchQuads<Codec, Out, 16>(stream);
+            else LaunchQuads<Codec, Out, 32>(stream);
+        } else if (E <= 512 && args.groups <= kWave) {
             if (E <= 64) LaunchWaves<Codec, Out, 1>(stream);
             else if (E <= 128) LaunchWaves<Codec, Out, 2>(stream);
             else if (E <= 256) LaunchWaves<Codec, Out, 4>(stream);
