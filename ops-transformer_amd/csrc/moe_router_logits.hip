@@ -58,6 +58,28 @@ __device__ __forceinline__ Raw<Codec> LoadRaw(const typename Codec::Storage* row
     return r;
 }
 
+// The same in two steps, for loads that are under way while others are used: the pieces, those from `end` on replaced by the row's last ones, and zeros in
+// their place once they are there.
+template <typename Codec, bool kAligned>
+__device__ __forceinline__ Raw<Codec> LoadClamped(const typename Codec::Storage* row, int64_t c, int64_t end) {
+    constexpr int kPieces = sizeof(typename Codec::Storage) / 2, kPer = 8 / kPieces;
+    if constexpr (!kAligned) return LoadRaw<Codec, false>(row, c, end);
+    Raw<Codec> r;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) r.q[i] = *reinterpret_cast<const uint4*>(row + min(c + i * kPer, end - kPer));
+    return r;
+}
+template <typename Codec, bool kAligned>
+__device__ __forceinline__ void ClearBehind(Raw<Codec>& r, int64_t c, int64_t end) {
+    constexpr int kPieces = sizeof(typename Codec::Storage) / 2, kPer = 8 / kPieces;
+    if constexpr (kAligned) {
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+            if (c + i * kPer >= end) r.q[i] = uint4{0, 0, 0, 0};
+        }
+    }
+}
+
 // Operands of the matrix instructions: one of the type itself, or kParts of bf16.
 template <typename Codec, int kParts>
 struct Parts {
@@ -208,39 +230,46 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
     }
 }
 
-// Many rows: tiles of 128 rows and kBn experts through LDS, cut into parts on the way, two buffers deep, eight waves of 32 x 32 x 16 products.
-// Lines in LDS are 16 bytes longer than their columns, so that eight lanes of a fragment read meet eight different sets of banks.
-constexpr int kBm = 128;
+// Many rows: eight waves, kWavesM x kWavesN of them with kMt tiles of 32 x 32 products each, one below the other.  Rows and weights come through LDS, two buffers
+// deep.  Rows are cut into parts on the way in, since every wave of a line reads them; weights of fp32 stay whole and are cut by the one wave (kWavesM of
+// them) that has those experts: four bytes of theirs are moved in place of six.  Lines in LDS are 16 bytes longer than their columns, so that eight
+// lanes of a fragment read meet eight different sets of banks.
 constexpr int kTileThreads = 512;
 
-template <typename S, int kBn>
+template <typename S, int kWavesM, int kWavesN, int kMt>
 struct TileShape {
+    static constexpr int kBm = kWavesM * kMt * 32, kBn = kWavesN * 32;
+    static constexpr int kWSize = sizeof(typename S::WType::Storage);
     static constexpr int kBk = S::kX == 1 && S::kW == 1 ? 64 : 32;
-    static constexpr int kPitch = kBk * 2 + 16;
-    static constexpr int kXBytes = S::kX * kBm * kPitch;
-    static constexpr int kStage = kXBytes + S::kW * kBn * kPitch;
-    static constexpr int kWavesM = kBn == 64 ? 4 : 2, kWavesN = 8 / kWavesM;
-    static constexpr int kMt = kBm / kWavesM / 32, kNt = kBn / kWavesN / 32;
+    static constexpr int kXPitch = kBk * 2 + 16, kWPitch = kBk * kWSize + 16;
+    static constexpr int kXBytes = S::kX * kBm * kXPitch;
+    static constexpr int kStage = kXBytes + kBn * kWPitch;
+    static constexpr int kBytes = 2 * kStage;
 };
 
-template <typename S, int kBn, bool kAligned>
-__global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArgs a) {
+template <typename S, int kWavesM, int kWavesN, int kMt, bool kAligned>
+__global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArgs a, int tilesN, int groups) {
+    static_assert(kWavesM * kWavesN == kTileThreads / kWave);
     using X = typename S::XType;
     using W = typename S::WType;
-    using Shape = TileShape<S, kBn>;
-    constexpr int kBk = Shape::kBk, kPitch = Shape::kPitch, kChunks = kBk / 8;
-    constexpr int kXLoads = kBm * kChunks / kTileThreads, kWLoads = (kBn * kChunks + kTileThreads - 1) / kTileThreads;
-    constexpr bool kWHalf = kBn * kChunks < kTileThreads;  // the first threads alone load weights
+    using Shape = TileShape<S, kWavesM, kWavesN, kMt>;
+    constexpr int kBm = Shape::kBm, kBn = Shape::kBn, kBk = Shape::kBk, kChunks = kBk / 8;
+    constexpr int kLineStep = kTileThreads / kChunks;
+    constexpr int kXLoads = (kBm + kLineStep - 1) / kLineStep, kWLoads = (kBn + kLineStep - 1) / kLineStep;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
-    const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kBm;
-    const int expert0 = blockIdx.y * kBn;
-    const int64_t begin = blockIdx.z * a.splitCols, end = min(a.cols, begin + a.splitCols);
+    const int tid = threadIdx.x, lane = tid % kWave, wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+    // Workgroups go round robin over the eight XCDs; those of one XCD take neighbouring rows of the same columns, whose weights their L2 holds.
+    const int linear = blockIdx.x, perXcd = groups / 8;
+    const int id = linear < perXcd * 8 ? linear % 8 * perXcd + linear / 8 : linear;
+    const int tileN = id % tilesN, rest = id / tilesN;
+    const int tilesM = static_cast<int>((a.rows + kBm - 1) / kBm);
+    const int64_t row0 = static_cast<int64_t>(rest % tilesM) * kBm;
+    const int split = rest / tilesM;
+    const int expert0 = tileN * kBn;
+    const int64_t begin = split * a.splitCols, end = min(a.cols, begin + a.splitCols);
     const int steps = static_cast<int>((end - begin + kBk - 1) / kBk);
 
     const int chunk = tid % kChunks, lineOf = tid / kChunks;
-    constexpr int kLineStep = kTileThreads / kChunks;
-    const bool loadsW = !kWHalf || lineOf < kBn;
     const typename X::Storage* x[kXLoads];
     const typename W::Storage* w[kWLoads];
 #pragma unroll
@@ -253,87 +282,105 @@ __global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArg
     }
     Raw<X> xr[kXLoads];
     Raw<W> wr[kWLoads];
-    auto load = [&](int step) {
-        const int64_t c = begin + step * kBk + chunk * 8;
-#pragma unroll
-        for (int i = 0; i < kXLoads; ++i) xr[i] = LoadRaw<X, kAligned>(x[i], c, end);
-        if (loadsW) {
-#pragma unroll
-            for (int i = 0; i < kWLoads; ++i) wr[i] = LoadRaw<W, kAligned>(w[i], c, end);
-        }
-    };
-    auto store = [&](unsigned char* stage) {
+    // Rows and weights are asked for half a step apart, each a whole step ahead of the store into LDS: there is always half a stage under way.
+    auto columnOf = [&](int step) { return begin + static_cast<int64_t>(step) * kBk + chunk * 8; };
+    auto loadX = [&](int step) {
 #pragma unroll
         for (int i = 0; i < kXLoads; ++i) {
+            if (kBm % kLineStep == 0 || lineOf + i * kLineStep < kBm) xr[i] = LoadClamped<X, kAligned>(x[i], columnOf(step), end);
+        }
+    };
+    auto loadW = [&](int step) {
+#pragma unroll
+        for (int i = 0; i < kWLoads; ++i) {
+            if (kBn % kLineStep == 0 || lineOf + i * kLineStep < kBn) wr[i] = LoadClamped<W, kAligned>(w[i], columnOf(step), end);
+        }
+    };
+    auto isTail = [&](int step) { return begin + static_cast<int64_t>(step + 1) * kBk > end; };
+    auto storeW = [&](int step) {
+        unsigned char* const stage = lds + step % 2 * Shape::kStage;
+        if (isTail(step)) {
+#pragma unroll
+            for (int i = 0; i < kWLoads; ++i) ClearBehind<W, kAligned>(wr[i], columnOf(step), end);
+        }
+#pragma unroll
+        for (int i = 0; i < kWLoads; ++i) {
+            if (kBn % kLineStep != 0 && lineOf + i * kLineStep >= kBn) continue;
+            uint4* const to = reinterpret_cast<uint4*>(stage + Shape::kXBytes + (lineOf + i * kLineStep) * Shape::kWPitch + chunk * (8 * Shape::kWSize));
+#pragma unroll
+            for (int q = 0; q < Shape::kWSize / 2; ++q) to[q] = wr[i].q[q];
+        }
+    };
+    auto storeX = [&](int step) {
+        unsigned char* const stage = lds + step % 2 * Shape::kStage;
+        if (isTail(step)) {
+#pragma unroll
+            for (int i = 0; i < kXLoads; ++i) ClearBehind<X, kAligned>(xr[i], columnOf(step), end);
+        }
+#pragma unroll
+        for (int i = 0; i < kXLoads; ++i) {
+            if (kBm % kLineStep != 0 && lineOf + i * kLineStep >= kBm) continue;
             const Parts<X, S::kX> parts = PartsOf<X, S::kX>(xr[i]);
 #pragma unroll
             for (int p = 0; p < S::kX; ++p) {
-                *reinterpret_cast<uint4*>(stage + (p * kBm + lineOf + i * kLineStep) * kPitch + chunk * 16) = parts.p[p];
-            }
-        }
-        if (loadsW) {
-#pragma unroll
-            for (int i = 0; i < kWLoads; ++i) {
-                const Parts<W, S::kW> parts = PartsOf<W, S::kW>(wr[i]);
-#pragma unroll
-                for (int p = 0; p < S::kW; ++p) {
-                    *reinterpret_cast<uint4*>(stage + Shape::kXBytes + (p * kBn + lineOf + i * kLineStep) * kPitch + chunk * 16) = parts.p[p];
-                }
+                *reinterpret_cast<uint4*>(stage + (p * kBm + lineOf + i * kLineStep) * Shape::kXPitch + chunk * 16) = parts.p[p];
             }
         }
     };
 
-    F32x16 acc[Shape::kMt][Shape::kNt] = {};
-    const int waveRow = wave / Shape::kWavesN * (Shape::kMt * 32), waveExpert = wave % Shape::kWavesN * (Shape::kNt * 32);
-    const int fragment = lane % 32 * kPitch + lane / 32 * 16;
-    load(0);
-    store(lds);
-    __syncthreads();
-    for (int step = 0; step < steps; ++step) {
-        if (step + 1 < steps) load(step + 1);
-        const unsigned char* const xs = lds + step % 2 * Shape::kStage + waveRow * kPitch + fragment;
-        const unsigned char* const ws = lds + step % 2 * Shape::kStage + Shape::kXBytes + waveExpert * kPitch + fragment;
+    F32x16 acc[kMt] = {};
+    const int waveN = wave % kWavesN, waveM = wave / kWavesN;
+    const int xAt = (waveM * (kMt * 32) + lane % 32) * Shape::kXPitch + lane / 32 * 16;
+    const int wAt = Shape::kXBytes + (waveN * 32 + lane % 32) * Shape::kWPitch + lane / 32 * (8 * Shape::kWSize);
+    auto multiply = [&](const unsigned char* stage, int k) {
+        Raw<W> raw;
 #pragma unroll
-        for (int k = 0; k < kBk / 16; ++k) {
-            uint4 xf[S::kX][Shape::kMt], wf[S::kW][Shape::kNt];
+        for (int q = 0; q < Shape::kWSize / 2; ++q) raw.q[q] = reinterpret_cast<const uint4*>(stage + wAt + k * (16 * Shape::kWSize))[q];
+        uint4 xf[S::kX][kMt];
 #pragma unroll
-            for (int p = 0; p < S::kX; ++p) {
+        for (int p = 0; p < S::kX; ++p) {
 #pragma unroll
-                for (int m = 0; m < Shape::kMt; ++m) xf[p][m] = *reinterpret_cast<const uint4*>(xs + (p * kBm + m * 32) * kPitch + k * 32);
-            }
+            for (int m = 0; m < kMt; ++m) xf[p][m] = *reinterpret_cast<const uint4*>(stage + xAt + (p * kBm + m * 32) * Shape::kXPitch + k * 32);
+        }
+        const Parts<W, S::kW> wf = PartsOf<W, S::kW>(raw);
 #pragma unroll
-            for (int p = 0; p < S::kW; ++p) {
+        for (int i = S::kX - 1; i >= 0; --i) {
 #pragma unroll
-                for (int n = 0; n < Shape::kNt; ++n) wf[p][n] = *reinterpret_cast<const uint4*>(ws + (p * kBn + n * 32) * kPitch + k * 32);
-            }
+            for (int j = S::kW - 1; j >= 0; --j) {
+                if (i + j > 2) continue;
 #pragma unroll
-            for (int i = S::kX - 1; i >= 0; --i) {
-#pragma unroll
-                for (int j = S::kW - 1; j >= 0; --j) {
-                    if (i + j > 2) continue;
-#pragma unroll
-                    for (int m = 0; m < Shape::kMt; ++m) {
-#pragma unroll
-                        for (int n = 0; n < Shape::kNt; ++n) acc[m][n] = Multiply<S::kHalf>(xf[i][m], wf[j][n], acc[m][n]);
-                    }
-                }
+                for (int m = 0; m < kMt; ++m) acc[m] = Multiply<S::kHalf>(xf[i][m], wf.p[j], acc[m]);
             }
         }
-        if (step + 1 < steps) store(lds + (step + 1) % 2 * Shape::kStage);
+    };
+    loadX(0);
+    loadW(0);
+    storeX(0);
+    loadX(1);
+    storeW(0);
+    loadW(1);
+    __syncthreads();
+    for (int step = 0; step < steps; ++step) {
+        const unsigned char* const stage = lds + step % 2 * Shape::kStage;
+        storeX(step + 1);
+        loadX(step + 2);
+#pragma unroll
+        for (int k = 0; k < kBk / 32; ++k) multiply(stage, k);
+        storeW(step + 1);
+        loadW(step + 2);
+#pragma unroll
+        for (int k = kBk / 32; k < kBk / 16; ++k) multiply(stage, k);
         __syncthreads();
     }
     // of a tile, lane l holds column l % 32 of the lines 8 (i / 4) + 4 (l / 32) + i % 4, i = 0 .. 15
-    float* const out = a.logits + static_cast<int64_t>(blockIdx.z) * a.rows * a.experts;
+    float* const out = a.logits + static_cast<int64_t>(split) * a.rows * a.experts;
+    const int expert = expert0 + waveN * 32 + lane % 32;
 #pragma unroll
-    for (int m = 0; m < Shape::kMt; ++m) {
+    for (int m = 0; m < kMt; ++m) {
 #pragma unroll
-        for (int n = 0; n < Shape::kNt; ++n) {
-            const int expert = expert0 + waveExpert + n * 32 + lane % 32;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int64_t row = row0 + waveRow + m * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
-                if (row < a.rows && expert < a.experts) out[row * a.experts + expert] = acc[m][n][i];
-            }
+        for (int i = 0; i < 16; ++i) {
+            const int64_t row = row0 + (waveM * kMt + m) * 32 + 8 * (i / 4) + 4 * (lane / 32) + i % 4;
+            if (row < a.rows && expert < a.experts) out[row * a.experts + expert] = acc[m][i];
         }
     }
 }
@@ -361,6 +408,7 @@ class LogitsExecutor : public aclOpExecutor {
     int tile = 0;      // experts of a tile of 128 rows, or 0: slim
     int slimM = 1, slimN = 1, slimSub = 1, slimWaves = 8;
     int splits = 1;
+    int tileN = 0;
 
     void Plan() {
         const int64_t T = args.rows, K = args.cols, E = args.experts;
@@ -368,10 +416,11 @@ class LogitsExecutor : public aclOpExecutor {
         int v[6] = {0, 0, 0, 0, 0, 0};
         if (env != nullptr) sscanf(env, "%d,%d,%d,%d,%d,%d", &v[0], &v[1], &v[2], &v[3], &v[4], &v[5]);
         if (env != nullptr) {
-            tile = v[0]; slimM = v[1]; slimN = v[2]; slimSub = v[3]; slimWaves = v[4]; splits = v[5];
+            tile = v[0]; tileN = v[1]; slimM = v[1]; slimN = v[2]; slimSub = v[3]; slimWaves = v[4]; splits = v[5];
         } else if (T > 512 && E > 16) {
-            tile = E <= 64 ? 64 : E <= 128 || dtype != ACL_BF16 ? 128 : 256;
-            const int64_t groups = (T + kBm - 1) / kBm * ((E + tile - 1) / tile);
+            tileN = E <= 64 ? 64 : E <= 128 ? 128 : 256;
+            tile = 128;
+            const int64_t groups = (T + tile - 1) / tile * ((E + tileN - 1) / tileN);
             while (groups * splits < 256 && splits < 32) splits *= 2;
         } else {
             slimSub = T <= 1 ? 16 : T <= 2 ? 8 : T <= 4 ? 4 : T <= 8 ? 2 : 1;
@@ -392,25 +441,31 @@ class LogitsExecutor : public aclOpExecutor {
         return hipGetLastError();
     }
 
-    template <typename S, int kBn, bool kAligned>
+    template <typename S, int kWavesM, int kWavesN, int kMt, bool kAligned>
     hipError_t LaunchTile(const LogitsArgs& a, hipStream_t stream) const {
-        auto kernel = RouterLogitsTileKernel<S, kBn, kAligned>;
-        constexpr int kBytes = 2 * TileShape<S, kBn>::kStage;
-        static_assert(kBytes <= 160 * 1024);
+        using Shape = TileShape<S, kWavesM, kWavesN, kMt>;
+        auto kernel = RouterLogitsTileKernel<S, kWavesM, kWavesN, kMt, kAligned>;
+        static_assert(Shape::kBytes <= 160 * 1024);
         static std::atomic<uint64_t> optedIn{0};
-        const hipError_t attr = opapi::EnsureDynamicLds(reinterpret_cast<const void*>(kernel), kBytes, optedIn);
+        const hipError_t attr = opapi::EnsureDynamicLds(reinterpret_cast<const void*>(kernel), Shape::kBytes, optedIn);
         if (attr != hipSuccess) return attr;
-        const dim3 grid(static_cast<unsigned>((a.rows + kBm - 1) / kBm), static_cast<unsigned>((a.experts + kBn - 1) / kBn), splits);
-        hipLaunchKernelGGL(kernel, grid, dim3(kTileThreads), kBytes, stream, a);
+        const int tilesN = static_cast<int>((a.experts + Shape::kBn - 1) / Shape::kBn);
+        const int64_t groups = (a.rows + Shape::kBm - 1) / Shape::kBm * tilesN * splits;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(kTileThreads), Shape::kBytes, stream, a, tilesN, static_cast<int>(groups));
         return hipGetLastError();
     }
 
     template <typename S, bool kAligned>
     hipError_t LaunchPlan(const LogitsArgs& a, hipStream_t stream) const {
-        if (tile == 64) return LaunchTile<S, 64, kAligned>(a, stream);
-        if (tile == 128) return LaunchTile<S, 128, kAligned>(a, stream);
-        if constexpr (S::kX == 1) {
-            if (tile == 256) return LaunchTile<S, 256, kAligned>(a, stream);
+        if (tile != 0) {  // rows of a tile, experts of a tile
+            if constexpr (S::kX == 1) {
+                if (tile == 256 && tileN == 256) return LaunchTile<S, 1, 8, 8, kAligned>(a, stream);
+                if (tile == 256 && tileN == 128) return LaunchTile<S, 2, 4, 4, kAligned>(a, stream);
+                if (tile == 256 && tileN == 64) return LaunchTile<S, 4, 2, 2, kAligned>(a, stream);
+            }
+            if (tileN == 256) return LaunchTile<S, 1, 8, 4, kAligned>(a, stream);
+            if (tileN == 128) return LaunchTile<S, 2, 4, 2, kAligned>(a, stream);
+            return LaunchTile<S, 4, 2, 1, kAligned>(a, stream);
         }
         if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 16, 4, kAligned>(a, stream);
         if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 16, 8, kAligned>(a, stream);
@@ -460,26 +515,24 @@ class LogitsExecutor : public aclOpExecutor {
             return reinterpret_cast<uintptr_t>(p) % 16 == 0 && static_cast<uint64_t>(a.cols) * size % 16 == 0;
         };
         const bool aligned = onGrid(a.x, sizeof(typename X::Storage)) && onGrid(a.weight, sizeof(typename W::Storage));
+        opapi::KernelTimer timer("router_logits", stream);
         return aligned ? LaunchPlan<Sides<X, W>, true>(a, stream) : LaunchPlan<Sides<X, W>, false>(a, stream);
     }
 
     aclnnStatus Run(void* workspace, hipStream_t stream) override {
         if (args.rows == 0) return ACLNN_SUCCESS;
-        OPAPI_CHECK(splits == 1 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, ACLNN_ERR_PARAM_INVALID,
+        OPAPI_CHECK(OwnBytes() == 0 || reinterpret_cast<uintptr_t>(workspace) % 16 == 0, ACLNN_ERR_PARAM_INVALID,
                     "aclnnMoeRouterLogits: the workspace must be 16-byte aligned");
         hipError_t err;
-        {
-            opapi::KernelTimer timer("router_logits", stream);
-            LogitsArgs a = args;
-            if (splits > 1) a.logits = static_cast<float*>(workspace);
-            if (dtype == ACL_FLOAT) err = Launch<F32, F32>(a, stream);
-            else if (dtype == ACL_FLOAT16) err = weightType == ACL_FLOAT ? Launch<F16, F32>(a, stream) : Launch<F16, F16>(a, stream);
-            else err = weightType == ACL_FLOAT ? Launch<Bf16, F32>(a, stream) : Launch<Bf16, Bf16>(a, stream);
-        }
+        LogitsArgs a = args;
+        float* const partial = static_cast<float*>(workspace);
+        if (splits > 1) a.logits = partial;
+        if (dtype == ACL_FLOAT) err = Launch<F32, F32>(a, stream);
+        else if (dtype == ACL_FLOAT16) err = weightType == ACL_FLOAT ? Launch<F16, F32>(a, stream) : Launch<F16, F16>(a, stream);
+        else err = weightType == ACL_FLOAT ? Launch<Bf16, F32>(a, stream) : Launch<Bf16, Bf16>(a, stream);
         if (err == hipSuccess && splits > 1) {
             opapi::KernelTimer timer("router_logits_add", stream);
             const int64_t count = args.rows * args.experts;
-            const float* const partial = static_cast<const float*>(workspace);
             const int vec = count % 4 == 0 && reinterpret_cast<uintptr_t>(args.logits) % 16 == 0 ? 4 : 1;
             const unsigned blocks = static_cast<unsigned>((count / vec + kAddThreads - 1) / kAddThreads);
             if (vec == 4) hipLaunchKernelGGL(AddSplitsKernel<4>, dim3(blocks), dim3(kAddThreads), 0, stream, partial, args.logits, count, splits);
