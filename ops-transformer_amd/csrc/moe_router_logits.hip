@@ -7,7 +7,7 @@
 // of the fp32 matrix instructions.  Sums are fp32, in an order that only sizes decide.
 #include "moe_front.h"
 
-#include <cstdlib>
+#include <cmath>
 
 #include "aclnnop/aclnn_moe_router_logits.h"
 
@@ -399,35 +399,71 @@ __global__ __launch_bounds__(kAddThreads) void AddSplitsKernel(const float* part
     reinterpret_cast<Vec*>(logits)[i] = sum;
 }
 
+// What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 147 000 measurements over the operator's range (1 to
+// 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types; 275 000 with the shapes that were dropped).  Nine in ten are within a quarter of the fit; the choice by it costs 3 % more
+// than the best of all shapes in the mean and a tenth more in one call of ten.
+struct Slim {
+    int m, n, sub, waves;
+};
+struct Tile {
+    int rows, experts;
+};
+constexpr int kSlims = 6, kTiles = 5;
+constexpr Slim kSlim[kSlims] = {{1, 1, 16, 4}, {1, 1, 4, 8}, {2, 1, 4, 8}, {1, 1, 2, 8}, {2, 1, 2, 8}, {2, 2, 2, 8}};
+constexpr Tile kTile[kTiles] = {{128, 64}, {128, 128}, {128, 256}, {256, 64}, {256, 128}};
+// us: of a launch; of 100 KB that come to a CU, eight waves that start and the cutting into parts, for each workgroup that a CU gets in turn
+constexpr double kSlimUs[] = {3.03, 1.19, 0.235, 1.12};
+// us: of a launch; a step of one part and of several; 100 KB, and the products at 2.5 PFLOP/s over all CUs; adding splits up, and a megabyte of them; a workgroup
+constexpr double kTileUs[] = {4.46, 0.077, 0.249, 0.886, 1.163, 2.44, 0.370, 1.43};
+
 class LogitsExecutor : public aclOpExecutor {
    public:
     LogitsArgs args{};
     aclDataType dtype = ACL_FLOAT;
     aclDataType weightType = ACL_FLOAT;
-    // The plan, made from sizes alone.
-    int tile = 0;      // experts of a tile of 128 rows, or 0: slim
-    int slimM = 1, slimN = 1, slimSub = 1, slimWaves = 8;
+    // The plan, made from sizes and types alone.
+    int kernel = 0;  // of kSlim, then of kTile
     int splits = 1;
-    int tileN = 0;
 
     void Plan() {
-        const int64_t T = args.rows, K = args.cols, E = args.experts;
-        const char* env = std::getenv("RL_PLAN");  // tuning
-        int v[6] = {0, 0, 0, 0, 0, 0};
-        if (env != nullptr) sscanf(env, "%d,%d,%d,%d,%d,%d", &v[0], &v[1], &v[2], &v[3], &v[4], &v[5]);
-        if (env != nullptr) {
-            tile = v[0]; tileN = v[1]; slimM = v[1]; slimN = v[2]; slimSub = v[3]; slimWaves = v[4]; splits = v[5];
-        } else if (T > 512 && E > 16) {
-            tileN = E <= 64 ? 64 : E <= 128 ? 128 : 256;
-            tile = 128;
-            const int64_t groups = (T + tile - 1) / tile * ((E + tileN - 1) / tileN);
-            while (groups * splits < 256 && splits < 32) splits *= 2;
-        } else {
-            slimSub = T <= 1 ? 16 : T <= 2 ? 8 : T <= 4 ? 4 : T <= 8 ? 2 : 1;
+        const double T = static_cast<double>(args.rows), K = static_cast<double>(args.cols), E = args.experts;
+        const double xSize = static_cast<double>(opapi::ElemSize(dtype)), wSize = static_cast<double>(opapi::ElemSize(weightType));
+        const bool same16 = dtype == weightType && dtype != ACL_FLOAT;
+        const int xParts = same16 || dtype == ACL_BF16 ? 1 : dtype == ACL_FLOAT16 ? 2 : 3;
+        const double products = same16 ? 1 : xParts == 1 ? 3 : xParts == 2 ? 5 : 6;
+        auto over = [](double n, double d) { return std::ceil(n / d); };
+        double best = 0;
+        auto offer = [&](double us, int which, int split) {
+            if (best != 0 && us >= best) return;
+            best = us;
+            kernel = which;
+            splits = split;
+        };
+        for (int i = 0; i < kSlims; ++i) {
+            const Slim& v = kSlim[i];
+            const double rows = 16 / v.sub * v.m, experts = 16 / v.sub * v.n;
+            const double rounds = over(over(T, rows) * over(E, experts), 256), steps = over(K, 32 * v.sub * v.waves) * v.waves / 4;
+            const double cuts = ((same16 ? 0 : 3) * v.n + (xParts > 1 ? 3 : 0) * v.m) * steps * 32 / 2400;
+            offer(kSlimUs[0] + rounds * (kSlimUs[1] * K * (rows * xSize + experts * wSize) * 1e-5 + kSlimUs[2] * v.waves / 8 + kSlimUs[3] * cuts), i, 1);
         }
-        const int64_t grain = 64 * slimSub;
-        args.splitCols = ((K + splits - 1) / splits + grain - 1) / grain * grain;
-        splits = static_cast<int>((K + args.splitCols - 1) / args.splitCols);
+        for (int i = 0; i < kTiles; ++i) {
+            const Tile& v = kTile[i];
+            if (v.rows > 128 && xParts > 1) continue;
+            const double tiles = over(T, v.rows) * over(E, v.experts), bk = same16 ? 64 : 32;
+            const double perCu = 2 * (xParts * v.rows * (2 * bk + 16) + v.experts * (wSize * bk + 16)) > 80 * 1024 ? 1 : 2;
+            for (const int target : {128, 256, 512}) {
+                int split = static_cast<int>(target / tiles);
+                if (split < 1) split = 1;
+                if (K / split < 128) continue;
+                const double cols = over(K / split, 64) * 64, used = over(K, cols), rounds = over(tiles * used, 256);
+                const double turns = over(rounds, perCu), bytes = cols * (v.rows * xSize + v.experts * wSize);
+                const double flops = v.rows * v.experts * cols * products * 2;
+                double us = kTileUs[0] + turns * (kTileUs[same16 ? 1 : 2] * cols / bk + kTileUs[7]) + rounds * (kTileUs[3] * bytes * 1e-5 + kTileUs[4] * flops * 256 / 2.5e9);
+                if (used > 1) us += kTileUs[5] + kTileUs[6] * used * T * E * 4e-6;
+                offer(us, kSlims + i, static_cast<int>(used));
+            }
+        }
+        args.splitCols = static_cast<int64_t>(over(K / splits, 64)) * 64;
     }
 
     uint64_t OwnBytes() const { return splits > 1 ? static_cast<uint64_t>(splits) * args.rows * args.experts * sizeof(float) : 0; }
@@ -457,56 +493,20 @@ class LogitsExecutor : public aclOpExecutor {
 
     template <typename S, bool kAligned>
     hipError_t LaunchPlan(const LogitsArgs& a, hipStream_t stream) const {
-        if (tile != 0) {  // rows of a tile, experts of a tile
-            if constexpr (S::kX == 1) {
-                if (tile == 256 && tileN == 256) return LaunchTile<S, 1, 8, 8, kAligned>(a, stream);
-                if (tile == 256 && tileN == 128) return LaunchTile<S, 2, 4, 4, kAligned>(a, stream);
-                if (tile == 256 && tileN == 64) return LaunchTile<S, 4, 2, 2, kAligned>(a, stream);
-            }
-            if (tileN == 256) return LaunchTile<S, 1, 8, 4, kAligned>(a, stream);
-            if (tileN == 128) return LaunchTile<S, 2, 4, 2, kAligned>(a, stream);
-            return LaunchTile<S, 4, 2, 1, kAligned>(a, stream);
+        switch (kernel) {
+            case 0: return LaunchSlim<S, 1, 1, 16, 4, kAligned>(a, stream);
+            case 1: return LaunchSlim<S, 1, 1, 4, 8, kAligned>(a, stream);
+            case 2: return LaunchSlim<S, 2, 1, 4, 8, kAligned>(a, stream);
+            case 3: return LaunchSlim<S, 1, 1, 2, 8, kAligned>(a, stream);
+            case 4: return LaunchSlim<S, 2, 1, 2, 8, kAligned>(a, stream);
+            case 5: return LaunchSlim<S, 2, 2, 2, 8, kAligned>(a, stream);
+            case 6: return LaunchTile<S, 4, 2, 1, kAligned>(a, stream);
+            case 7: return LaunchTile<S, 2, 4, 2, kAligned>(a, stream);
+            case 8: return LaunchTile<S, 1, 8, 4, kAligned>(a, stream);
+            default: break;
         }
-        if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 16, 4, kAligned>(a, stream);
-        if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 16, 8, kAligned>(a, stream);
-        if (slimSub == 16 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 16, 16, kAligned>(a, stream);
-        if (slimSub == 8 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 8, 4, kAligned>(a, stream);
-        if (slimSub == 8 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 8, 8, kAligned>(a, stream);
-        if (slimSub == 8 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 8, 16, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 4, 4, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 4, 8, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 4, 16, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 2 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 2, 1, 4, 8, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 2 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 2, 1, 4, 16, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 1 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 1, 2, 4, 8, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 1 && slimN == 2 && slimWaves == 16) return LaunchSlim<S, 1, 2, 4, 16, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 2 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 2, 2, 4, 8, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 4 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 4, 1, 4, 8, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 4 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 4, 2, 4, 8, kAligned>(a, stream);
-        if (slimSub == 4 && slimM == 4 && slimN == 4 && slimWaves == 8) return LaunchSlim<S, 4, 4, 4, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 2, 4, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 2, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 2, 16, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 2 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 2, 1, 2, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 2 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 2, 1, 2, 16, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 1 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 1, 2, 2, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 1 && slimN == 2 && slimWaves == 16) return LaunchSlim<S, 1, 2, 2, 16, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 2 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 2, 2, 2, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 4 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 4, 1, 2, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 4 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 4, 2, 2, 8, kAligned>(a, stream);
-        if (slimSub == 2 && slimM == 4 && slimN == 4 && slimWaves == 8) return LaunchSlim<S, 4, 4, 2, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 1 && slimN == 1 && slimWaves == 4) return LaunchSlim<S, 1, 1, 1, 4, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 1 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 1, 1, 1, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 1 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 1, 1, 1, 16, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 2 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 2, 1, 1, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 2 && slimN == 1 && slimWaves == 16) return LaunchSlim<S, 2, 1, 1, 16, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 1 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 1, 2, 1, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 1 && slimN == 2 && slimWaves == 16) return LaunchSlim<S, 1, 2, 1, 16, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 2 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 2, 2, 1, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 4 && slimN == 1 && slimWaves == 8) return LaunchSlim<S, 4, 1, 1, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 4 && slimN == 2 && slimWaves == 8) return LaunchSlim<S, 4, 2, 1, 8, kAligned>(a, stream);
-        if (slimSub == 1 && slimM == 4 && slimN == 4 && slimWaves == 8) return LaunchSlim<S, 4, 4, 1, 8, kAligned>(a, stream);
-        return hipErrorInvalidValue;
+        if constexpr (S::kX == 1) return kernel == 9 ? LaunchTile<S, 4, 2, 2, kAligned>(a, stream) : LaunchTile<S, 2, 4, 4, kAligned>(a, stream);
+        return hipErrorInvalidValue;  // not planned for rows of several parts
     }
 
     template <typename X, typename W>

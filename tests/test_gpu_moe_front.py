@@ -182,6 +182,18 @@ def test_logits_sizes(aclnn, dev, xt, wt, T, K, E):
     _check_logits(x, w, aclnn.moe_router_logits(*_on(dev, x, w)))
 
 
+@pytest.mark.parametrize("T,K,E,types", [(16, 200, 300, TYPES), (16, 520, 300, TYPES), (1500, 200, 20, TYPES), (16000, 200, 33, TYPES), (16000, 203, 300, TYPES),
+                                         (10000, 200, 200, TYPES), (10000, 1001, 33, TYPES), (3000, 7168, 20, TYPES[:1]), (3000, 6001, 20, TYPES[2:3]),
+                                         (6500, 2049, 200, TYPES[1:2]), (6500, 2056, 200, TYPES), (13000, 4096, 100, TYPES[:1])])
+def test_logits_of_many_rows(aclnn, dev, T, K, E, types):
+    """Sizes that every tile is chosen for, on and off the 16-byte grid, with and without the columns split."""
+    for xt, wt in types:
+        g = torch.Generator().manual_seed(T + K + E)
+        x = torch.randn((T, K), generator=g).to(TORCH[xt])
+        w = (torch.randn((E, K), generator=g) / K ** 0.5).to(TORCH[wt])
+        _check_logits(x, w, aclnn.moe_router_logits(*_on(dev, x, w)))
+
+
 @pytest.mark.parametrize("xt,wt", TYPES)
 @pytest.mark.parametrize("T", [1, 3, 16, 70, 300, 1100])
 def test_logits_keep_every_bit(aclnn, dev, xt, wt, T):
