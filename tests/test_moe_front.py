@@ -1,6 +1,7 @@
 """What the operators in front of the expert FFN refuse, and what they ask for, without a GPU: aclnnMoeAddRmsNormQuant,
 aclnnMoeRouterLogits, aclnnMoeGatingTopKGrouped.  First phases never touch device memory, so fake addresses suffice."""
 import ctypes
+import struct
 
 import pytest
 import torch
@@ -225,6 +226,32 @@ def test_second_phases_check_their_workspace(aclnn):
             assert getattr(lib, api + "GetWorkspaceSize")(*args, ctypes.byref(ws), ctypes.byref(ex)) == 0 and ws.value > 0
             assert getattr(lib, api)(workspace, ws.value - short, ex, None) == (NULLPTR if workspace is None else INVALID), api
         assert getattr(lib, api)(None, 0, None, None) == NULLPTR
+
+
+def _packed_logits(T, K, E, address=0x100000000):
+    shapes = [(T, K), (E, K), (T, E)]
+    packed = [8]
+    for i, (rows, cols) in enumerate(shapes):
+        packed += [2, BF16 if i < 2 else F32, address * (i + 1), rows, cols, cols, 1]
+    return packed
+
+
+def test_one_call_of_both_phases_enqueues_nothing_without_its_workspace(aclnn):
+    packed = _packed_logits(8192, 7168, 256)
+    data, needed = struct.pack("%dq" % len(packed), *packed), ctypes.c_uint64(0)
+    run = aclnn.lib().opapiRunPacked
+    for size in (0, 1 << 20):
+        assert run(data, len(packed), 0x1000, size, None, ctypes.byref(needed)) == 0
+        assert needed.value >= 2 * 8192 * 256 * 4 and needed.value > size
+    assert run(data, len(packed), None, 0, None, None) == NULLPTR
+    assert run(None, 0, None, 0, None, ctypes.byref(needed)) == NULLPTR
+    assert run(data, len(packed) - 1, None, 0, None, ctypes.byref(needed)) == INVALID
+    # the workspace's own second phase: what it asks for has to be there, and on 16 bytes
+    ws, ex = ctypes.c_uint64(0), ctypes.c_void_p(None)
+    lib = aclnn.lib()
+    args = _logits(aclnn, shape=(8192, 7168), experts=256)
+    assert lib.aclnnMoeRouterLogitsGetWorkspaceSize(*args, ctypes.byref(ws), ctypes.byref(ex)) == 0
+    assert lib.aclnnMoeRouterLogits(0x1008, ws.value, ex, None) == INVALID and "16-byte" in aclnn.last_error()
 
 
 def test_host_tensors_are_refused(aclnn):
