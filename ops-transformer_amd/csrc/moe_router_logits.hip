@@ -159,9 +159,11 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
     constexpr int kDepth = kAligned ? (kM * kN > 1 ? 2 : 4) : 1;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int line = lane % 16 / kSub, sub = lane % 16 % kSub;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kLines * kM);
-    const int expert0 = blockIdx.y * (kLines * kN);
-    const int64_t begin = blockIdx.z * a.splitCols, end = min(a.cols, begin + a.splitCols);
+    // Workgroups go round robin over the eight XCDs: neighbours take different experts, whose weights then come to one L2 each.
+    const int tilesN = (a.experts + kLines * kN - 1) / (kLines * kN);
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x / tilesN) * (kLines * kM);
+    const int expert0 = static_cast<int>(blockIdx.x % tilesN) * (kLines * kN);
+    const int64_t begin = 0, end = a.cols;
     const typename X::Storage* x[kM];
     const typename W::Storage* w[kN];
 #pragma unroll
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
     }
     __syncthreads();
     const float* const all = reinterpret_cast<const float*>(sums);
-    float* const out = a.logits + static_cast<int64_t>(blockIdx.z) * a.rows * a.experts;
+    float* const out = a.logits;
     for (int i = threadIdx.x; i < kLines * kM * kLines * kN; i += kWave * kWaves) {
         const int r = i / (kLines * kN), e = i % (kLines * kN);
         const int64_t row = row0 + r;
@@ -471,9 +473,8 @@ class LogitsExecutor : public aclOpExecutor {
     template <typename S, int kM, int kN, int kSub, int kWaves, bool kAligned>
     hipError_t LaunchSlim(const LogitsArgs& a, hipStream_t stream) const {
         constexpr int kLines = 16 / kSub;
-        const dim3 grid(static_cast<unsigned>((a.rows + kLines * kM - 1) / (kLines * kM)), static_cast<unsigned>((a.experts + kLines * kN - 1) / (kLines * kN)),
-                        splits);
-        hipLaunchKernelGGL((RouterLogitsSlimKernel<S, kM, kN, kSub, kWaves, kAligned>), grid, dim3(kWave * kWaves), 0, stream, a);
+        const int64_t groups = (a.rows + kLines * kM - 1) / (kLines * kM) * ((a.experts + kLines * kN - 1) / (kLines * kN));
+        hipLaunchKernelGGL((RouterLogitsSlimKernel<S, kM, kN, kSub, kWaves, kAligned>), dim3(static_cast<unsigned>(groups)), dim3(kWave * kWaves), 0, stream, a);
         return hipGetLastError();
     }
 
