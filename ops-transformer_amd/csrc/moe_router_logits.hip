@@ -401,9 +401,10 @@ __global__ __launch_bounds__(kAddThreads) void AddSplitsKernel(const float* part
     reinterpret_cast<Vec*>(logits)[i] = sum;
 }
 
-// What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 147 000 measurements over the operator's range (1 to
-// 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types; 275 000 with the shapes that were dropped).  Nine in ten are within a quarter of the fit; the choice by it costs 3 % more
-// than the best of all shapes in the mean and a tenth more in one call of ten.
+// What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 136 000 measurements of 21 600 calls over the operator's
+// range (1 to 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types).  Nine in ten are between 0.77 and 1.17 of the fit; the choice by it costs
+// 1.8 % more than the best shape in the mean, 6 % in one call of ten.  A shape each kind of call needs: without the slim kernels decode takes up to twice as
+// long (64 x 7168 x 256: 12.7 against 8.4 us, one row 7.4 against 2.9), without the tiles a prompt does (8192 x 7168 x 256, fp32 weights: 333 against 96 us).
 struct Slim {
     int m, n, sub, waves;
 };
@@ -413,10 +414,11 @@ struct Tile {
 constexpr int kSlims = 6, kTiles = 5;
 constexpr Slim kSlim[kSlims] = {{1, 1, 16, 4}, {1, 1, 4, 8}, {2, 1, 4, 8}, {1, 1, 2, 8}, {2, 1, 2, 8}, {2, 2, 2, 8}};
 constexpr Tile kTile[kTiles] = {{128, 64}, {128, 128}, {128, 256}, {256, 64}, {256, 128}};
-// us: of a launch; of 100 KB that come to a CU, eight waves that start and the cutting into parts, for each workgroup that a CU gets in turn
-constexpr double kSlimUs[] = {3.03, 1.19, 0.235, 1.12};
+// us: of a launch; of 100 KB that come to a CU, eight waves that start and the cutting into parts, for each workgroup that a CU gets in turn; of a megabyte of
+// operands
+constexpr double kSlimUs[] = {3.10, 1.00, 0.235, 1.136, 0.091};
 // us: of a launch; a step of one part and of several; 100 KB, and the products at 2.5 PFLOP/s over all CUs; adding splits up, and a megabyte of them; a workgroup
-constexpr double kTileUs[] = {4.46, 0.077, 0.249, 0.886, 1.163, 2.44, 0.370, 1.43};
+constexpr double kTileUs[] = {3.58, 0.058, 0.238, 0.975, 1.162, 2.50, 0.356, 2.33};
 
 class LogitsExecutor : public aclOpExecutor {
    public:
@@ -435,7 +437,9 @@ class LogitsExecutor : public aclOpExecutor {
         const double products = same16 ? 1 : xParts == 1 ? 3 : xParts == 2 ? 5 : 6;
         auto over = [](double n, double d) { return std::ceil(n / d); };
         double best = 0;
+        const double operands = (T * K * xSize + E * K * wSize) * 1e-6, streamed = kSlimUs[0] + 0.19 * operands;  // at a copy's 5.2 TB/s
         auto offer = [&](double us, int which, int split) {
+            if (us < streamed) us = streamed;
             if (best != 0 && us >= best) return;
             best = us;
             kernel = which;
@@ -446,7 +450,7 @@ class LogitsExecutor : public aclOpExecutor {
             const double rows = 16 / v.sub * v.m, experts = 16 / v.sub * v.n;
             const double rounds = over(over(T, rows) * over(E, experts), 256), steps = over(K, 32 * v.sub * v.waves) * v.waves / 4;
             const double cuts = ((same16 ? 0 : 3) * v.n + (xParts > 1 ? 3 : 0) * v.m) * steps * 32 / 2400;
-            offer(kSlimUs[0] + rounds * (kSlimUs[1] * K * (rows * xSize + experts * wSize) * 1e-5 + kSlimUs[2] * v.waves / 8 + kSlimUs[3] * cuts), i, 1);
+            offer(kSlimUs[0] + kSlimUs[4] * operands + rounds * (kSlimUs[1] * K * (rows * xSize + experts * wSize) * 1e-5 + kSlimUs[2] * v.waves / 8 + kSlimUs[3] * cuts), i, 1);
         }
         for (int i = 0; i < kTiles; ++i) {
             const Tile& v = kTile[i];

@@ -184,7 +184,7 @@ def test_logits_sizes(aclnn, dev, xt, wt, T, K, E):
 
 @pytest.mark.parametrize("T,K,E,types", [(16, 200, 300, TYPES), (16, 520, 300, TYPES), (1500, 200, 20, TYPES), (16000, 200, 33, TYPES), (16000, 203, 300, TYPES),
                                          (10000, 200, 200, TYPES), (10000, 1001, 33, TYPES), (3000, 7168, 20, TYPES[:1]), (3000, 6001, 20, TYPES[2:3]),
-                                         (6500, 2049, 200, TYPES[1:2]), (6500, 2056, 200, TYPES), (13000, 4096, 100, TYPES[:1])])
+                                         (6500, 2049, 200, TYPES[1:2]), (6500, 2056, 200, TYPES), (13000, 4096, 100, TYPES[:3:2]), (5000, 7168, 8, TYPES[2:3])])
 def test_logits_of_many_rows(aclnn, dev, T, K, E, types):
     """Sizes that every tile is chosen for, on and off the 16-byte grid, with and without the columns split."""
     for xt, wt in types:
