@@ -6,16 +6,16 @@
  * Per row of E logits:
  *   p = softmax(x) (scoreType 0) or sigmoid(x) (scoreType 1)                                  -> scoresOutOptional
  *   t = p + bias, compared in 64 bits; without a bias t = p, and experts are compared by their logits, of which p is a monotone
- *   function; a logit of -inf has p = 0 and comes behind every other expert
+ *   function; a logit of -inf has p = 0 and t = -inf, so that it comes behind every expert but those of a bias of -inf
  *   groups of E / groupCount neighbouring experts; a group's value is its largest t (groupSelectMode 0) or the sum of its two
- *   largest (1; experts of logit -inf add nothing, a group of nothing else comes last); the kGroup groups of the largest values stay
+ *   largest (1; experts of t = -inf add nothing, a group of nothing else comes last); the kGroup groups of the largest values stay
  *   expertIdxOut = the k experts of the largest t in them, descending;  equal values, here and among groups: the lower index first
  *   y = p at those (without the bias);  renorm 1: y = y / (sum of the k + eps), zeros where that sum is zero
  *   yOut = y * routedScalingFactor, rounded to nearest even
  * NaN counts as larger than every number; under softmax a row with a NaN or +inf has NaN for p and unspecified experts (k different
  * ones).  Rows whose finishedOptional entry is true get expertIdxOut = E in every slot (the values are
  * still written).
- * x: FLOAT, FLOAT16 or BF16, rank 2 or 3, at most 2^26 rows; biasOptional FLOAT [E], finite; finishedOptional BOOL of x's extents without the last;
+ * x: FLOAT, FLOAT16 or BF16, rank 2 or 3, at most 2^26 rows; biasOptional FLOAT [E] without NaN; finishedOptional BOOL of x's extents without the last;
  * yOut of x's type or FLOAT and expertIdxOut INT32, x's extents with the last replaced by k; scoresOutOptional FLOAT of x's
  * extents.  This build: E <= 2048, k <= 64; k <= kGroup * E / groupCount; groupSelectMode 1 takes groups of two experts or more.
  * Inputs may be strided views; outputs are contiguous and share no memory with an input or with each other.

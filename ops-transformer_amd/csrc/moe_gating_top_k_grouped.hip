@@ -51,6 +51,9 @@ __device__ __forceinline__ double ValueOf(uint64_t key) {
     return __longlong_as_double(static_cast<long long>((key >> 63) != 0 ? key & 0x7fffffffffffffffull : ~key));
 }
 
+// -0 as 0, whose key is another's.
+__device__ __forceinline__ float Unsigned0(float f) { return f + 0.f; }
+
 __device__ __forceinline__ double WaveSum64(double v) {
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     return v;
@@ -106,7 +109,7 @@ __device__ void ExactRow(const GatingArgs& a, int64_t row, int lane, uint64_t* k
         const float v = Codec::Load(x[c]);
         const double p = a.bias != nullptr || writeScores ? ScoreOf(v, sigmoid, shift, sum) : 0.0;
         if (writeScores) a.scores[row * a.experts + c] = static_cast<float>(p);
-        keys[c] = KeyOf(v == -INFINITY ? -INFINITY : a.bias == nullptr ? static_cast<double>(v) : p + static_cast<double>(a.bias[c]));
+        keys[c] = KeyOf(v == -INFINITY ? -INFINITY : a.bias == nullptr ? static_cast<double>(Unsigned0(v)) : p + static_cast<double>(a.bias[c]));
     }
     WaveSync();
 
@@ -327,7 +330,7 @@ __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int la
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c = lane * kPer + i;
-        double t = v[i];
+        double t = Unsigned0(v[i]);
         if (biased || writeScores) {
             const double p = ScoreOf(v[i], sigmoid, shift, sum);
             if (writeScores && c < a.experts) a.scores[row * a.experts + c] = static_cast<float>(p);
@@ -512,6 +515,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         }
         low = RowReduce<kLanes>(least, [](float p, float q) { return fminf(p, q); });
         high = top + RowReduce<kLanes>(most, [](float p, float q) { return fmaxf(p, q); });
+        close |= !(high - low < INFINITY);  // a bias of an infinity
     }
     const float largest = fmaxf(fabsf(low), fabsf(high));
     if (biased || (grouped && a.topTwo != 0)) {
@@ -519,7 +523,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         for (int i = 0; i < kPer; ++i) t[i] = v[i] == -INFINITY ? -INFINITY : t[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) t[i] = v[i];
+        for (int i = 0; i < kPer; ++i) t[i] = Unsigned0(v[i]);
     }
 
     uint32_t kept = ~0u;  // groups, a bit each
@@ -568,10 +572,10 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             if (l == static_cast<int>(at)) value = 0;
         }
         const uint32_t next = RowMax<kLanes>(value);
-        if (biased || a.topTwo != 0) close |= Value32(last) - Value32(next) <= kU * (32.f * top + 16.f * largest);
+        if (biased || a.topTwo != 0) close |= !(Value32(last) - Value32(next) > kU * (32.f * top + 16.f * largest));
         if (!biased && a.topTwo != 0) {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) t[i] = v[i];
+            for (int i = 0; i < kPer; ++i) t[i] = Unsigned0(v[i]);
         }
     }
 

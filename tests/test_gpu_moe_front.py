@@ -429,6 +429,83 @@ def test_gating_finished_strided_and_ranked_inputs(aclnn, dev):
     assert aclnn.moe_gating_top_k_grouped(torch.empty((0, 96), device=dev), 5, **kw)[1].shape == (0, 5)
 
 
+# Rows by the thousand are chosen sixteen lanes each: the cases above again at such lengths.
+LONG = 4003
+
+
+def _long_rows(E, seed):
+    """Twelve rows, of which ten are where a choice can go wrong, and the order they are repeated in."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((12, E), generator=g)
+    x[0, ::3] = -float("inf")
+    x[1] = -float("inf")
+    x[2, :E // 4] = -float("inf")
+    x[3, E // 4 + 1:E // 2] = -float("inf")
+    x[4, 1:] = -float("inf")
+    x[5, ::2] = torch.finfo(torch.float32).min
+    x[6] = torch.finfo(torch.float32).min
+    x[7, E // 2] = 1e4
+    x[8] *= 200
+    x[9] = torch.randint(0, 5, (E,), generator=g).float()
+    return x, torch.randint(0, 12, (LONG,), generator=g)
+
+
+def _check_long(aclnn, dev, x, order, k, **kw):
+    bias = kw.get("bias")
+    yr, ir, pr = _gating_reference(x, k, **kw)
+    y, idx, scores = aclnn.moe_gating_top_k_grouped(x[order].to(dev), k, output_scores=True, **dict(kw, bias=None if bias is None else bias.to(dev)))
+    assert np.array_equal(idx.cpu().numpy(), ir[order])
+    tol = 4 * U + (_half(y.dtype) if y.dtype != torch.float32 else 0)
+    np.testing.assert_allclose(y.cpu().double().numpy(), yr[order], rtol=tol, atol=float(_tiny(y.dtype)))
+    np.testing.assert_allclose(scores.cpu().double().numpy(), pr[order], rtol=4 * U, atol=1e-44)
+
+
+@pytest.mark.parametrize("E,groups", [(8, 4), (16, 4), (20, 4), (48, 3), (96, 4), (128, 16), (255, 5), (256, 8), (500, 10), (512, 16)])
+@pytest.mark.parametrize("score_type", [0, 1])
+def test_gating_long_batches(aclnn, dev, E, groups, score_type):
+    x, order = _long_rows(E, E + groups)
+    bias = torch.randn(E, generator=torch.Generator().manual_seed(E))
+    for k_group in sorted({1, (groups + 1) // 2, groups}):
+        k = min(16, E // groups * k_group)
+        for mode in (0, 1):
+            for b in (None, bias, 1e-3 * bias):
+                _check_long(aclnn, dev, x, order, k, bias=b, k_group=k_group, group_count=groups, group_select_mode=mode, score_type=score_type, renorm=mode)
+    for dtype in (torch.float16, torch.bfloat16):
+        short = x.clamp(min=torch.finfo(dtype).min).to(dtype)
+        short[x == -float("inf")] = -float("inf")
+        _check_long(aclnn, dev, short, order, min(8, E // groups), bias=bias, k_group=1, group_count=groups, score_type=score_type)
+        _check_long(aclnn, dev, short, order, min(8, E), score_type=score_type)
+
+
+@pytest.mark.parametrize("T", [3, LONG])
+@pytest.mark.parametrize("E,groups", [(16, 4), (96, 4), (640, 4)])
+def test_gating_zeros_of_either_sign_are_equal(aclnn, dev, T, E, groups):
+    x = torch.full((1, E), -1.0)
+    x[0, 1::2] = 0.0
+    x[0, 3::4] = -0.0
+    order = torch.zeros(T, dtype=torch.int64)
+    for score_type in (0, 1):
+        for mode in (0, 1):
+            _check_long(aclnn, dev, x, order, 4, score_type=score_type, k_group=2, group_count=groups, group_select_mode=mode)
+    x[0, ::2] = torch.finfo(torch.float32).min    # first in their lanes: what is compared is zeros of one lane and of others
+    _check_long(aclnn, dev, x, order, min(8, E // 2), score_type=1)
+
+
+@pytest.mark.parametrize("T", [12, LONG])
+@pytest.mark.parametrize("E", [16, 96, 256, 640])
+@pytest.mark.parametrize("low", [-float("inf"), torch.finfo(torch.float32).min])
+def test_gating_biases_that_mask_experts(aclnn, dev, T, E, low):
+    """A bias of -inf, or of the lowest value, puts an expert behind those that have none; its score stays what it is."""
+    x, order = _long_rows(E, E)
+    g = torch.Generator().manual_seed(E + 1)
+    for share in (0.25, 0.9):
+        bias = 0.1 * torch.randn(E, generator=g)
+        bias[torch.rand(E, generator=g) < share] = low
+        for score_type in (0, 1):
+            for kw in [dict(), dict(k_group=2, group_count=4), dict(k_group=2, group_count=4, group_select_mode=1)]:
+                _check_long(aclnn, dev, x, order[:T], min(8, E // 4), bias=bias, score_type=score_type, **kw)
+
+
 # ------------------------------------------------------------------------------------------------ together
 def _block(pkg, dev, tokens, H=1024, I=512, E=16, seed=3, weight32=True):
     g = torch.Generator().manual_seed(seed)
