@@ -16,6 +16,7 @@ namespace {
 using namespace moe_front;
 
 constexpr int64_t kMaxExperts = 4096;
+constexpr double kMaxThreads = 4294967040.0;  // of a launch: fewer than 2^32, in whole workgroups
 
 struct LogitsArgs {
     const void* x;
@@ -448,6 +449,7 @@ class LogitsExecutor : public aclOpExecutor {
         for (int i = 0; i < kSlims; ++i) {
             const Slim& v = kSlim[i];
             const double rows = 16 / v.sub * v.m, experts = 16 / v.sub * v.n;
+            if (over(T, rows) * over(E, experts) * v.waves * kWave > kMaxThreads) continue;
             const double rounds = over(over(T, rows) * over(E, experts), 256), steps = over(K, 32 * v.sub * v.waves) * v.waves / 4;
             const double cuts = ((same16 ? 0 : 3) * v.n + (xParts > 1 ? 3 : 0) * v.m) * steps * 32 / 2400;
             offer(kSlimUs[0] + kSlimUs[4] * operands + rounds * (kSlimUs[1] * K * (rows * xSize + experts * wSize) * 1e-5 + kSlimUs[2] * v.waves / 8 + kSlimUs[3] * cuts), i, 1);
@@ -456,11 +458,12 @@ class LogitsExecutor : public aclOpExecutor {
             const Tile& v = kTile[i];
             if (v.rows > 128 && xParts > 1) continue;
             const double tiles = over(T, v.rows) * over(E, v.experts), bk = same16 ? 64 : 32;
+            if (tiles * kTileThreads > kMaxThreads) continue;
             const double perCu = 2 * (xParts * v.rows * (2 * bk + 16) + v.experts * (wSize * bk + 16)) > 80 * 1024 ? 1 : 2;
             for (const int target : {128, 256, 512}) {
                 int split = static_cast<int>(target / tiles);
                 if (split < 1) split = 1;
-                if (K / split < 128) continue;
+                if (split > 1 && K / split < 128) continue;
                 const double cols = over(K / split, 64) * 64, used = over(K, cols), rounds = over(tiles * used, 256);
                 const double turns = over(rounds, perCu), bytes = cols * (v.rows * xSize + v.experts * wSize);
                 const double flops = v.rows * v.experts * cols * products * 2;

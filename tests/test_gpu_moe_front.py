@@ -255,6 +255,51 @@ def test_logits_rows_apart(aclnn, dev):
             assert torch.equal(room[T * E:], torch.full((4096,), 7.0, device=dev))
 
 
+def test_logits_of_few_columns_and_very_many_rows(aclnn, dev):
+    """2^26 rows of four columns: offsets behind 2^31 in the logits, and launches of fewer than 2^32 threads."""
+    T, K, E = 1 << 26, 4, 36
+    x = torch.randn((T, K), device=dev, generator=torch.Generator(device=dev).manual_seed(5)).bfloat16()
+    w = torch.randn((E, K), generator=torch.Generator().manual_seed(6)).bfloat16()
+    out = aclnn.moe_router_logits(x, w.to(dev))
+    for at in (0, T // 2 - 500, (1 << 31) // E - 500, (1 << 31) // E + 500, T - 1000):
+        _check_logits(x[at:at + 1000].cpu(), w, out[at:at + 1000])
+
+
+@pytest.mark.parametrize("dtype_name", ["f16", "bf16"])
+@pytest.mark.parametrize("T", [2, 40, 2000])
+def test_logits_of_subnormal_values(aclnn, dev, dtype_name, T):
+    """Values below the type's normal range are values like others; for bf16 those are fp32's own, so the weights are large."""
+    dtype = TORCH[dtype_name]
+    g = torch.Generator().manual_seed(T)
+    x = (torch.randn((T, 256), generator=g) * (torch.finfo(dtype).smallest_normal / 8)).to(dtype)
+    w = (torch.randn((40, 256), generator=g) * (1.0 if dtype_name == "f16" else 1e20)).to(dtype)
+    assert int((x != 0).sum()) > x.numel() // 2
+    _check_logits(x, w, aclnn.moe_router_logits(*_on(dev, x, w)))
+
+
+@pytest.mark.parametrize("K", [2048, 7168])
+def test_logits_of_prompts_in_graphs(aclnn, dev, K):
+    """Two captured calls over a workspace each (the longer columns are split), replayed in turn with eager calls between them."""
+    g = torch.Generator().manual_seed(7)
+    w = (torch.randn((256, K), generator=g) / 45).to(dev)
+    graphs = []
+    for T in (600, 700):
+        x, out, space = torch.randn((T, K), generator=g).bfloat16().to(dev), torch.empty((T, 256), device=dev), aclnn.Workspace()
+        aclnn.moe_router_logits(x, w, out=out, workspace=space)
+        assert K == 2048 or space.tensor is not None
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            aclnn.moe_router_logits(x, w, out=out, workspace=space)
+        graphs.append((x, out, space, graph))
+    for step in range(4):
+        for x, out, _, graph in graphs:
+            x.copy_(torch.randn(x.shape, generator=g).bfloat16())
+            graph.replay()
+            got = out.clone()
+            assert torch.equal(got, aclnn.moe_router_logits(x, w))
+
+
 # ------------------------------------------------------------------------------------------------ gating
 def _gating_reference(x, k, bias=None, k_group=1, group_count=1, group_select_mode=0, score_type=0, renorm=0, routed_scaling_factor=1.0, eps=1e-20):
     x = x.double().numpy()
