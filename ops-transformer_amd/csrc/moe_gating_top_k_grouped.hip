@@ -426,11 +426,13 @@ constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts
 
 // Rows of up to 16 * kPer experts, at most 16 picks and groups: four rows a wave, sixteen lanes each, fp32 keys in registers.  Lane l of a row holds experts
 // l * kPer + i, so that among equal values the lower lane has the lower index; within a lane the number i goes into the lowest bits of the key, which
-// makes a lane's keys different.  `bound` is the last key that a lane gave away: of the
-// differences key - bound modulo 2^32 the largest is that of the next smaller key.
-// Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once.  Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
-// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.8 us (16.8 MB of logits are 3.3), of which a row that
-// is made twice is 3; softmax without bias or groups, bf16 9.0.
+// makes a lane's keys different.  `bound` is the last key that a lane gave away: of the differences key - bound modulo 2^32 the largest is that of the next
+// smaller key.
+// Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once.
+// Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
+// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.9 us (16.8 MB of logits are 3.3), of which a row that
+// is made twice is 3: 1050 vector instructions a wave, more than half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
+// softmax without bias or groups, bf16 9.0.
 template <typename Codec, typename Out, int kPer>
 __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs a) {
     constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : kPer == 16 ? 4 : 5;
@@ -672,7 +674,7 @@ class GatingExecutor : public aclOpExecutor {
     void Launch(hipStream_t stream) const {
         const int E = args.experts;
         // Sixteen lanes a row make more rows at a time and take longer for one, most of all with a bias, where one row in a thousand is
-        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 9.2 and 10.1 at 4096, 15.8 and
+        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 9.1 and 10.1 at 4096, 15.9 and
         // 27.5 at 16384; softmax without a bias 5.2 and 5.3, 5.3 and 8.0, 9.0 and 20.7.
         const bool many = args.rows > (args.bias != nullptr ? 4000 : 1024);
         if (many && E <= 512 && args.k <= 16 && args.groups <= 16) {

@@ -151,11 +151,14 @@ __device__ __forceinline__ F32x16 Multiply(const uint4& a, const uint4& b, F32x1
 // Few rows: operands go from memory to registers, the waves of a workgroup share its columns, 32 at a time in turn, and add up through LDS.  A workgroup makes
 // kM x kN tiles of 16 rows and 16 experts.  With kSub > 1 (kM = kN = 1) the sixteen lines of either operand are 16 / kSub rows or experts times kSub
 // neighbouring runs of 32 columns: the products of a run with itself, one in kSub, are what is added up, and a workgroup streams fewer experts' weights.
+// What bounds it: one round trip to memory and the launch for a row (1 x 4096 x 128, bf16 2.9 us), the time a CU takes to bring in its share for a decode step
+// (64 x 7168 x 256, fp32 weights 8.3: 256 workgroups of 350 KB, of which the L2 serves all but 14.4 MB), memory for prompts of few experts
+// (16384 x 4096 x 8 22 to 25 us, 5.4 TB/s and more: a copy's rate).
 template <typename S, int kM, int kN, int kSub, int kWaves, bool kAligned>
 __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsArgs a) {
     using X = typename S::XType;
     using W = typename S::WType;
-        constexpr int kLines = 16 / kSub;
+    constexpr int kLines = 16 / kSub;
     __shared__ F32x4 sums[kWaves * kM * kN][kWave];
     constexpr int kDepth = kAligned ? (kM * kN > 1 ? 2 : 4) : 1;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -237,13 +240,17 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
 // deep.  Rows are cut into parts on the way in, since every wave of a line reads them; weights of fp32 stay whole and are cut by the one wave (kWavesM of
 // them) that has those experts: four bytes of theirs are moved in place of six.  Lines in LDS are 16 bytes longer than their columns, so that eight
 // lanes of a fragment read meet eight different sets of banks.
+// What bounds it: 8192 x 7168 x 256, fp32 weights 84 us and 7 for adding the splits up; 64 are the three parts' products at the rate of a large matrix product
+// (1409 TFLOP/s).  The matrix instructions are under way for 59 % of the time that CUs work, cutting weights into parts takes another 45 % of the vector
+// unit's, at 1.7 GHz.  With bf16 weights 43 and 7: instructions 34 %, then what a CU brings in, 41 GB/s.  Products a fragment ahead
+// and 64 columns a step took 600 x 7168 x 256 from 22.7 to 20.9 us, 16384 x 2880 x 60 from 38.7 to 34.0, 8192 x 7168 x 256, bf16 from 52 to 50.
 constexpr int kTileThreads = 512;
 
 template <typename S, int kWavesM, int kWavesN, int kMt>
 struct TileShape {
     static constexpr int kBm = kWavesM * kMt * 32, kBn = kWavesN * 32;
     static constexpr int kWSize = sizeof(typename S::WType::Storage);
-    static constexpr int kBk = S::kX == 1 && S::kW == 1 ? 64 : 32;
+    static constexpr int kBk = S::kX == 1 && (S::kW == 1 || kBn < 256) ? 64 : 32;
     static constexpr int kXPitch = kBk * 2 + 16, kWPitch = kBk * kWSize + 16;
     static constexpr int kXBytes = S::kX * kBm * kXPitch;
     static constexpr int kStage = kXBytes + kBn * kWPitch;
@@ -251,7 +258,8 @@ struct TileShape {
 };
 
 template <typename S, int kWavesM, int kWavesN, int kMt, bool kAligned>
-__global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArgs a, int tilesN, int groups) {
+__global__ __attribute__((amdgpu_flat_work_group_size(kTileThreads, kTileThreads), amdgpu_waves_per_eu(2))) void
+RouterLogitsTileKernel(LogitsArgs a, int tilesN, int groups) {
     static_assert(kWavesM * kWavesN == kTileThreads / kWave);
     using X = typename S::XType;
     using W = typename S::WType;
@@ -335,24 +343,29 @@ __global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArg
     const int waveN = wave % kWavesN, waveM = wave / kWavesN;
     const int xAt = (waveM * (kMt * 32) + lane % 32) * Shape::kXPitch + lane / 32 * 16;
     const int wAt = Shape::kXBytes + (waveN * 32 + lane % 32) * Shape::kWPitch + lane / 32 * (8 * Shape::kWSize);
-    auto multiply = [&](const unsigned char* stage, int k) {
-        Raw<W> raw;
+    // Fragments are read one product of 16 columns ahead, or every product waits for its own; the scheduling barriers keep the compiler to that.
+    struct Fragments {
+        uint4 x[S::kX][kMt];
+        Raw<W> w;
+    };
+    auto read = [&](const unsigned char* stage, int k, Fragments& f) {
 #pragma unroll
-        for (int q = 0; q < Shape::kWSize / 2; ++q) raw.q[q] = reinterpret_cast<const uint4*>(stage + wAt + k * (16 * Shape::kWSize))[q];
-        uint4 xf[S::kX][kMt];
+        for (int q = 0; q < Shape::kWSize / 2; ++q) f.w.q[q] = reinterpret_cast<const uint4*>(stage + wAt + k * (16 * Shape::kWSize))[q];
 #pragma unroll
         for (int p = 0; p < S::kX; ++p) {
 #pragma unroll
-            for (int m = 0; m < kMt; ++m) xf[p][m] = *reinterpret_cast<const uint4*>(stage + xAt + (p * kBm + m * 32) * Shape::kXPitch + k * 32);
+            for (int m = 0; m < kMt; ++m) f.x[p][m] = *reinterpret_cast<const uint4*>(stage + xAt + (p * kBm + m * 32) * Shape::kXPitch + k * 32);
         }
-        const Parts<W, S::kW> wf = PartsOf<W, S::kW>(raw);
+    };
+    auto multiply = [&](const Fragments& f) {
+        const Parts<W, S::kW> wf = PartsOf<W, S::kW>(f.w);
 #pragma unroll
         for (int i = S::kX - 1; i >= 0; --i) {
 #pragma unroll
             for (int j = S::kW - 1; j >= 0; --j) {
                 if (i + j > 2) continue;
 #pragma unroll
-                for (int m = 0; m < kMt; ++m) acc[m] = Multiply<S::kHalf>(xf[i][m], wf.p[j], acc[m]);
+                for (int m = 0; m < kMt; ++m) acc[m] = Multiply<S::kHalf>(f.x[i][m], wf.p[j], acc[m]);
             }
         }
     };
@@ -365,14 +378,24 @@ __global__ __launch_bounds__(kTileThreads) void RouterLogitsTileKernel(LogitsArg
     __syncthreads();
     for (int step = 0; step < steps; ++step) {
         const unsigned char* const stage = lds + step % 2 * Shape::kStage;
-        storeX(step + 1);
-        loadX(step + 2);
+        constexpr int kProducts = kBk / 16;
+        Fragments f[2];
+        read(stage, 0, f[0]);
 #pragma unroll
-        for (int k = 0; k < kBk / 32; ++k) multiply(stage, k);
-        storeW(step + 1);
-        loadW(step + 2);
-#pragma unroll
-        for (int k = kBk / 32; k < kBk / 16; ++k) multiply(stage, k);
+        for (int k = 0; k < kProducts; ++k) {
+            if (k + 1 < kProducts) read(stage, k + 1, f[(k + 1) % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(f[k % 2]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (k == 0) {
+                storeX(step + 1);
+                loadX(step + 2);
+            }
+            if (k == kProducts / 2) {
+                storeW(step + 1);
+                loadW(step + 2);
+            }
+        }
         __syncthreads();
     }
     // of a tile, lane l holds column l % 32 of the lines 8 (i / 4) + 4 (l / 32) + i % 4, i = 0 .. 15
@@ -402,10 +425,10 @@ __global__ __launch_bounds__(kAddThreads) void AddSplitsKernel(const float* part
     reinterpret_cast<Vec*>(logits)[i] = sum;
 }
 
-// What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 136 000 measurements of 21 600 calls over the operator's
-// range (1 to 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types).  Nine in ten are between 0.77 and 1.17 of the fit; the choice by it costs
-// 1.8 % more than the best shape in the mean, 6 % in one call of ten.  A shape each kind of call needs: without the slim kernels decode takes up to twice as
-// long (64 x 7168 x 256: 12.7 against 8.4 us, one row 7.4 against 2.9), without the tiles a prompt does (8192 x 7168 x 256, fp32 weights: 333 against 96 us).
+// What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 320 000 measurements of 50 900 calls over the operator's
+// range (1 to 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types).  Nine in ten are between 0.76 and 1.17 of the fit; the choice by it costs
+// 1.8 % more than the best shape in the mean, 7 % in one call of ten.  A shape each kind of call needs: without the slim kernels decode takes up to twice as
+// long (64 x 7168 x 256: 12.7 against 8.4 us, one row 7.4 against 2.9), without the tiles a prompt does (8192 x 7168 x 256, fp32 weights: 333 against 97 us).
 struct Slim {
     int m, n, sub, waves;
 };
@@ -419,7 +442,7 @@ constexpr Tile kTile[kTiles] = {{128, 64}, {128, 128}, {128, 256}, {256, 64}, {2
 // operands
 constexpr double kSlimUs[] = {3.10, 1.00, 0.235, 1.136, 0.091};
 // us: of a launch; a step of one part and of several; 100 KB, and the products at 2.5 PFLOP/s over all CUs; adding splits up, and a megabyte of them; a workgroup
-constexpr double kTileUs[] = {3.58, 0.058, 0.238, 0.975, 1.162, 2.50, 0.356, 2.33};
+constexpr double kTileUs[] = {4.01, 0.0135, 0.301, 0.930, 1.058, 2.48, 0.376, 1.84};
 
 class LogitsExecutor : public aclOpExecutor {
    public:
@@ -457,7 +480,7 @@ class LogitsExecutor : public aclOpExecutor {
         for (int i = 0; i < kTiles; ++i) {
             const Tile& v = kTile[i];
             if (v.rows > 128 && xParts > 1) continue;
-            const double tiles = over(T, v.rows) * over(E, v.experts), bk = same16 ? 64 : 32;
+            const double tiles = over(T, v.rows) * over(E, v.experts), bk = same16 || (xParts == 1 && v.experts < 256) ? 64 : 32;
             if (tiles * kTileThreads > kMaxThreads) continue;
             const double perCu = 2 * (xParts * v.rows * (2 * bk + 16) + v.experts * (wSize * bk + 16)) > 80 * 1024 ? 1 : 2;
             for (const int target : {128, 256, 512}) {
