@@ -9,6 +9,6 @@ The directory name contains a hyphen, so it is loaded by path (``__graft_entry__
 ``ops_transformer_amd``.  torch is used for device memory and streams only.
 """
 from . import aclnn, moe_ffn, synth  # noqa: F401
-from .aclnn import (AclnnError, grouped_matmul_swiglu_quant, grouped_matmul_v4, library_path, moe_finalize_routing_v2,  # noqa: F401
-                    moe_init_routing_v2)
+from .aclnn import (AclnnError, grouped_matmul_swiglu_quant, grouped_matmul_v4, library_path, moe_add_rms_norm_quant,  # noqa: F401
+                    moe_finalize_routing_v2, moe_gating_top_k_grouped, moe_init_routing_v2, moe_router_logits)
 from .moe_ffn import MoeFfnW8A8  # noqa: F401

@@ -446,7 +446,7 @@ def _run_whole(op, scalars, tensors, workspace):
     One array is packed for all tensors: gating of one token 8.8 -> 7.0 us."""
     api = _PLANNED[op]
     device = tensors[0].get_device()
-    if device < 0 or device != torch.cuda.current_device():
+    if device < 0 or device != torch._C._cuda_getDevice():
         raise AclnnError(api, ACLNN_ERR_PARAM_INVALID, "the tensors are on %s, not on the current GPU" % tensors[0].device)
     values = [op, *scalars]
     for t in tensors:
