@@ -5,7 +5,8 @@
  *
  *   logitsOut[..., e] = sum over h of x[..., h] * weight[e, h], products and sums in fp32
  * Router weights are often kept in 32 bits next to 16-bit hidden states: neither side is rounded to fewer bits than it has.
- * Results are the same bits on every launch.  A row with a NaN or an infinity gives NaN or infinities.
+ * Results are the same bits on every launch.  A row with a NaN or an infinity gives NaN or infinities; so does, where x is FLOAT or
+ * FLOAT16 next to FLOAT weights, a FLOAT value of 2^128 (1 - 2^-9) or more.
  *
  * x: FLOAT, FLOAT16 or BF16, rank 2 or 3, at most 2^26 rows, last extent H; weight: of x's type or FLOAT, [E, H], 1 <= E <= 4096;
  * logitsOut: FLOAT of x's extents with the last replaced by E, contiguous, apart from the inputs' memory.  Inputs may be

@@ -1,10 +1,12 @@
 // aclnnMoeRouterLogits for gfx950: fp32 logits = x @ weight^T, x of 16 or 32 bits, weight of x's type or fp32.
 //
-// The matrix instructions take 16-bit operands, and an operand of more bits is a sum of bf16 parts, cut off eight significant bits at a time:
-// fp32 = three parts and fp16 (next to fp32 weights) = two, both without a remainder.  A product of parts a_i and b_j (i, j from 0) is below
-// 2^-8(i+j) of |x w|, so those with i + j <= 2 are summed, and what is left out is below fp32's rounding of each product.  bf16 rows on
-// fp32 weights take three instructions in place of one, fp16 rows five, fp32 rows six: with every bit of both sides, at several times the rate
-// of the fp32 matrix instructions.  Sums are fp32, in an order that only sizes decide.
+// The matrix instructions take 16-bit operands, and an operand of more bits is a sum of bf16 parts of eight significant bits each: fp32 = three parts
+// and fp16 (next to fp32 weights) = two, both without a remainder.  Where both sides have several, each part is the nearest to what those before it
+// leave: a part a_i (i from 0) is at most 2^-8i of |x|, a product a_i b_j at most 2^-8(i+j) of |x w|, so those with i + j <= 2 are summed; of the rest
+// two are at most 2^-24 of |x w|, fp32's rounding of a product, and one 2^-32.  (Parts that are cut off are up to twice as large each and have one
+// sign: 2^-21 of |x w| in all, which in sums of few products showed.)  bf16 rows on fp32 weights leave nothing out, and their weights are cut off:
+// 600 x 7168 x 256 21.0 us, 22.6 with the nearest.  They take three instructions in place of one, fp16 rows five, fp32 rows six: with every bit
+// of both sides, at several times the rate of the fp32 matrix instructions.  Sums are fp32, in an order that only sizes decide.
 #include "moe_front.h"
 
 #include <cmath>
@@ -87,12 +89,17 @@ struct Parts {
     uint4 p[kParts];
 };
 
-__device__ __forceinline__ uint32_t UpperHalves(float even, float odd) {
+// The upper halves of two values, cut off; and the nearest bf16 to each.
+__device__ __forceinline__ uint32_t CutTwo(float even, float odd) {
     return __builtin_amdgcn_perm(__float_as_uint(odd), __float_as_uint(even), 0x07060302u);
 }
-__device__ __forceinline__ float Cut(float f) { return __uint_as_float(__float_as_uint(f) & 0xffff0000u); }
+__device__ __forceinline__ uint32_t NearestTwo(float even, float odd) {
+    typedef __bf16 Bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float F32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(F32x2{even, odd}, Bf16x2));
+}
 
-template <typename Codec, int kParts>
+template <typename Codec, int kParts, bool kNearest>
 __device__ __forceinline__ Parts<Codec, kParts> PartsOf(const Raw<Codec>& r) {
     Parts<Codec, kParts> out;
     if constexpr (kParts == 1) {
@@ -115,9 +122,15 @@ __device__ __forceinline__ Parts<Codec, kParts> PartsOf(const Raw<Codec>& r) {
             }
 #pragma unroll
             for (int part = 0; part < kParts; ++part) {
-                words[part][pair] = UpperHalves(v[0], v[1]);
-                v[0] -= Cut(v[0]);
-                v[1] -= Cut(v[1]);
+                if constexpr (kNearest) {
+                    words[part][pair] = NearestTwo(v[0], v[1]);
+                    v[0] -= __uint_as_float(words[part][pair] << 16);
+                    v[1] -= __uint_as_float(words[part][pair] & 0xffff0000u);
+                } else {
+                    words[part][pair] = CutTwo(v[0], v[1]);
+                    v[0] -= __uint_as_float(__float_as_uint(v[0]) & 0xffff0000u);
+                    v[1] -= __uint_as_float(__float_as_uint(v[1]) & 0xffff0000u);
+                }
             }
         }
 #pragma unroll
@@ -134,6 +147,7 @@ struct Sides {
     static constexpr bool kSame16 = std::is_same_v<X, W> && sizeof(typename X::Storage) == 2;
     static constexpr int kX = kSame16 || std::is_same_v<X, Bf16> ? 1 : std::is_same_v<X, F16> ? 2 : 3;
     static constexpr int kW = kSame16 ? 1 : 3;
+    static constexpr bool kNearest = kX > 1;  // parts that leave the least to the products that are left out
     static constexpr bool kHalf = kSame16 && std::is_same_v<X, F16>;  // fp16 instructions; bf16 otherwise
 };
 
@@ -193,10 +207,10 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
         for (int d = 0; d < kDepth; ++d) {
             Parts<X, S::kX> xp[kM];
 #pragma unroll
-            for (int m = 0; m < kM; ++m) xp[m] = PartsOf<X, S::kX>(xr[d][m]);
+            for (int m = 0; m < kM; ++m) xp[m] = PartsOf<X, S::kX, S::kNearest>(xr[d][m]);
 #pragma unroll
             for (int n = 0; n < kN; ++n) {
-                const Parts<W, S::kW> wp = PartsOf<W, S::kW>(wr[d][n]);
+                const Parts<W, S::kW> wp = PartsOf<W, S::kW, S::kNearest>(wr[d][n]);
 #pragma unroll
                 for (int m = 0; m < kM; ++m) {
 #pragma unroll
@@ -331,7 +345,7 @@ RouterLogitsTileKernel(LogitsArgs a, int tilesN, int groups) {
 #pragma unroll
         for (int i = 0; i < kXLoads; ++i) {
             if (kBm % kLineStep != 0 && lineOf + i * kLineStep >= kBm) continue;
-            const Parts<X, S::kX> parts = PartsOf<X, S::kX>(xr[i]);
+            const Parts<X, S::kX> parts = PartsOf<X, S::kX, S::kNearest>(xr[i]);
 #pragma unroll
             for (int p = 0; p < S::kX; ++p) {
                 *reinterpret_cast<uint4*>(stage + (p * kBm + lineOf + i * kLineStep) * Shape::kXPitch + chunk * 16) = parts.p[p];
@@ -358,7 +372,7 @@ RouterLogitsTileKernel(LogitsArgs a, int tilesN, int groups) {
         }
     };
     auto multiply = [&](const Fragments& f) {
-        const Parts<W, S::kW> wf = PartsOf<W, S::kW>(f.w);
+        const Parts<W, S::kW> wf = PartsOf<W, S::kW, S::kNearest>(f.w);
 #pragma unroll
         for (int i = S::kX - 1; i >= 0; --i) {
 #pragma unroll

@@ -213,6 +213,19 @@ def test_logits_keep_every_bit(aclnn, dev, xt, wt, T):
     assert torch.equal(aclnn.moe_router_logits(*_on(dev, x, w)).cpu(), x.float()[:, pick])
 
 
+@pytest.mark.parametrize("xt,wt", TYPES)
+@pytest.mark.parametrize("T", [30, 3000])
+@pytest.mark.parametrize("K", [1, 2, 3, 4, 9])
+def test_logits_of_few_columns(aclnn, dev, xt, wt, T, K):
+    """Of a few products each one's own rounding shows, and what is left out of those of parts."""
+    g = torch.Generator().manual_seed(T + K)
+    x, w = torch.randn((T, K), generator=g), torch.randn((393, K), generator=g)
+    x[::2] = torch.sign(x[::2]) * (1 + 2.0 ** -8 - 2.0 ** -16 - 2.0 ** -23)    # remainders as large as they get
+    w[::3] = torch.sign(w[::3]) * (1 + 2.0 ** -7 - 2.0 ** -16 - 2.0 ** -22)
+    x, w = x.to(TORCH[xt]), w.to(TORCH[wt])
+    _check_logits(x, w, aclnn.moe_router_logits(*_on(dev, x, w)))
+
+
 def test_logits_strides_offsets_and_extents(aclnn, dev):
     g = torch.Generator().manual_seed(2)
     for T, K, E in [(1, 1024, 60), (7, 1000, 16), (130, 1024, 60), (600, 513, 32)]:
