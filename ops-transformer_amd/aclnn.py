@@ -432,6 +432,7 @@ def moe_gating_top_k_softmax_v2(x, k, renorm=0, finished=None, output_softmax=Fa
 
 
 _REAL, _REAL_AS_WHOLE = struct.Struct("d"), struct.Struct("q")
+_WORDS = [struct.Struct("%dq" % n).pack for n in range(1 + 8 + 9 * (3 + 2 * 8) + 1)]  # by length: a number, scalars, tensors of eight dimensions
 
 
 def _bits(value):
@@ -443,7 +444,7 @@ def _run_whole(op, scalars, tensors, workspace):
     """Both phases of an operator in one foreign call (opapiRunPacked), in a second one where a workspace has to be made first.  The kernels run on
     the current device, on its current stream: tensors of another device, or of the host, are refused.
 
-    One array is packed for all tensors: gating of one token 8.8 -> 7.0 us."""
+    One array is packed for all tensors: gating of one token 8.8 -> 7.4 us."""
     api = _PLANNED[op]
     device = tensors[0].get_device()
     if device < 0 or device != torch._C._cuda_getDevice():
@@ -461,7 +462,7 @@ def _run_whole(op, scalars, tensors, workspace):
         values += (len(shape), _DTYPE_CODE[t.dtype], t.data_ptr(), *shape, *t.stride())
     l = lib()
     count = len(values)
-    packed = struct.pack("%dq" % count, *values)
+    packed = _WORDS[count](*values)
     stream = torch._C._cuda_getCurrentRawStream(device)
     needed = ctypes.c_uint64()
     ws = None if workspace is None or workspace.tensor is None or workspace.tensor.get_device() != device else workspace.tensor
