@@ -565,6 +565,25 @@ def test_gating_biases_that_mask_experts(aclnn, dev, T, E, low):
 
 
 # ------------------------------------------------------------------------------------------------ together
+@pytest.mark.parametrize("H", [37, 40])
+def test_elements_behind_2_to_the_31(aclnn, dev, H):
+    """The most rows there may be, of 2.5 and 2.7 thousand million elements: norm and choice of experts at the start, the middle and the end."""
+    T = 1 << 26
+    g = torch.Generator(device=dev).manual_seed(H)
+    x = torch.empty((T, H), dtype=torch.bfloat16, device=dev).normal_(generator=g)
+    gamma = torch.ones(H, dtype=torch.bfloat16)
+    y, scale, norm, total = aclnn.moe_add_rms_norm_quant(x, gamma.to(dev))
+    bias = 0.1 * torch.randn(H, generator=torch.Generator().manual_seed(H))
+    weight, idx, _ = aclnn.moe_gating_top_k_grouped(x, 2, bias=bias.to(dev), score_type=1, renorm=1, y_dtype=torch.float32)
+    assert total is None
+    for at in (0, T // 2, (1 << 31) // H - 500, T - 1000):
+        rows = x[at:at + 1000].cpu()
+        _check_norm(rows, None, gamma, None, 1e-6, (y[at:at + 1000], scale[at:at + 1000], norm[at:at + 1000], None))
+        yr, ir, _ = _gating_reference(rows, 2, bias, score_type=1, renorm=1)
+        assert np.array_equal(idx[at:at + 1000].cpu().numpy(), ir)
+        np.testing.assert_allclose(weight[at:at + 1000].cpu().numpy(), yr, rtol=4 * U)
+
+
 def _block(pkg, dev, tokens, H=1024, I=512, E=16, seed=3, weight32=True):
     g = torch.Generator().manual_seed(seed)
     x, res, gamma, _ = _norm_inputs(tokens, H, torch.bfloat16, seed)
