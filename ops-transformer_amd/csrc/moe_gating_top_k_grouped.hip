@@ -421,8 +421,8 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs
     if (row < a.rows) WaveRow<Codec, Out, kPer>(a, row, lane, reinterpret_cast<uint64_t*>(ldsRaw) + wave * a.experts, a.scores != nullptr);
 }
 
-// LDS of a wave: an fp32 value per expert of its four rows, or a row's keys in 64 bits.
-constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts) * 16; }
+// LDS of a wave: an fp32 value per expert of its four rows, then their picks, or a row's keys in 64 bits.
+constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts < 16 ? 16 : experts) * 16; }
 
 // Rows of up to 16 * kPer experts, at most 16 picks and groups: four rows a wave, sixteen lanes each, fp32 keys in registers.  Lane l of a row holds experts
 // l * kPer + i, so that among equal values the lower lane has the lower index; within a lane the number i goes into the lowest bits of the key, which
@@ -430,9 +430,9 @@ constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts
 // smaller key.
 // Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once.
 // Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
-// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.9 us (16.8 MB of logits are 3.3), of which a row that
-// is made twice is 3: 1050 vector instructions a wave, more than half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
-// softmax without bias or groups, bf16 9.0.
+// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.4 us (16.8 MB of logits are 3.3), of which a row that
+// is made twice is 3: 950 vector instructions a wave, near half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
+// softmax without bias or groups, bf16 8.4.  Rows without an infinity or a NaN are spared what those need: 16.0 and 9.0 without.
 template <typename Codec, typename Out, int kPer>
 __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs a) {
     constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : kPer == 16 ? 4 : 5;
@@ -470,11 +470,17 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             for (int i = 0; i < kPer; ++i) b[i] = a.bias[min(l * kPer + i, a.experts - 1)];
         }
     }
-    bool nan = false;
+    float all = v[0];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) nan |= v[i] != v[i];
-    // uniform over the row: it is made again, for values too close to be told apart here, or a NaN
-    bool close = __any(nan) && RowMax<kLanes>(nan ? 1u : 0u) != 0;
+    for (int i = 1; i < kPer; ++i) all += v[i];
+    const bool plain = __all(fabsf(all) < INFINITY);  // no NaN and no infinity in any of the wave's rows
+    bool close = false;  // uniform over the row: it is made again, for values too close to be told apart here, or a NaN
+    if (!plain) {
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) nan |= v[i] != v[i];
+        close = RowMax<kLanes>(nan ? 1u : 0u) != 0;
+    }
 
     float shift = 0.f, top = 1.f;  // top: no p of the row is larger
     double sum = 1.0;
@@ -521,8 +527,10 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     }
     const float largest = fmaxf(fabsf(low), fabsf(high));
     if (biased || (grouped && a.topTwo != 0)) {
+        if (!plain) {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) t[i] = v[i] == -INFINITY ? -INFINITY : t[i];
+            for (int i = 0; i < kPer; ++i) t[i] = v[i] == -INFINITY ? -INFINITY : t[i];
+        }
     } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) t[i] = Unsigned0(v[i]);
@@ -581,20 +589,6 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         }
     }
 
-    // a bit for every value that is looked at: there, and in a group that stays (without branches for each: a third of the kernel's time)
-    uint32_t present = 0;
-    if (!grouped) {
-        const int count = a.experts - l * kPer;
-        present = count >= kPer ? ~0u : count > 0 ? (1u << count) - 1 : 0u;
-    } else if (whole) {
-        present = (kept >> group & 1) != 0 ? ~0u : 0u;
-    } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const uint32_t c = l * kPer + i;
-            present |= (c < static_cast<uint32_t>(a.experts) ? kept >> ((c * a.groupMagic >> 21) & 31) & 1 : 0u) << i;
-        }
-    }
     // Without a bias a key is the logit's, cut: exact for 16 bits, and fp32 ones that agree in what is left are too close.  With one it is t's place
     // between low and high in 2^27ths, from 32 on, and 1 for -inf.
     uint32_t keys[kPer];
@@ -602,9 +596,13 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     if (biased) {
         const float scale = 0x0.ffffp27f / (high - low);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            keys[i] = static_cast<uint32_t>(__builtin_amdgcn_fmed3f(fmaf(t[i] - low, scale, 32.f), 1.f, 0x0.fffffp27f)) << (32 - kPlaceBits) | (kLow - i);
+        for (int i = 0; i < kPer; ++i) t[i] = fmaf(t[i] - low, scale, 32.f);
+        if (!plain) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) t[i] = __builtin_amdgcn_fmed3f(t[i], 1.f, 0x0.fffffp27f);
         }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) keys[i] = static_cast<uint32_t>(t[i]) << (32 - kPlaceBits) | (kLow - i);
         // the difference to low, the product and the whole number round once each: 8, 8 and 1 units at most
         const float units = (16.f * top + 2.f * largest) * kU * scale * 1.01f + 36.f;
         tooClose = units < 0x1p26f ? static_cast<uint32_t>(units) << (32 - kPlaceBits) : ~0u;
@@ -614,10 +612,20 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         tooClose = 0;
     }
     const bool exact = !biased && (sizeof(typename Codec::Storage) == 2 || kBits == 0);
+    // what is not looked at: experts that are not there, or in a group that was left out (no branches for each: a third of the kernel's time)
+    if (grouped && whole) {
+        const uint32_t stays = 0u - (kept >> group & 1);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) keys[i] = (present >> i & 1) != 0 ? keys[i] : 0u;
+        for (int i = 0; i < kPer; ++i) keys[i] &= stays;
+    } else if (grouped || a.experts != kLanes * kPer) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const uint32_t c = l * kPer + i, stays = grouped ? kept >> ((c * a.groupMagic >> 21) & 31) & 1 : 1u;
+            keys[i] &= 0u - (c < static_cast<uint32_t>(a.experts) ? stays : 0u);
+        }
+    }
     const uint32_t upper = biased ? ~31u : ~kLow, lowest = biased ? 2u << (32 - kPlaceBits) : 0x00800000u;  // below: -inf, or none left
-    int32_t pick = 0;
+    int32_t* const picks = reinterpret_cast<int32_t*>(own) + lane / kLanes * kLanes;
     uint32_t before = ~0u, bound = 0;
     for (int j = 0; j <= a.k; ++j) {
         uint32_t best = 0u - bound;  // none left
@@ -628,11 +636,15 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         close |= !exact && j > 0 && most >= lowest && before - most <= tooClose;
         before = most;
         if (j == a.k) break;
-        const uint32_t at = RowMin<kLanes>((best & upper) == most ? l : kLanes - 1);
-        const uint32_t holder = __shfl(best, first + static_cast<int>(at));
-        if (l == j) pick = static_cast<int32_t>(at) * kPer + static_cast<int32_t>(kLow - (holder & kLow));
-        if (l == static_cast<int>(at)) bound = best;
+        const uint64_t holders = __ballot((best & upper) == most) >> first;  // from the row's first lane on
+        if (l == __builtin_ctz(static_cast<uint32_t>(holders))) {
+            picks[j] = l * kPer + static_cast<int32_t>(kLow - (best & kLow));
+            bound = best;
+        }
     }
+    WaveSync();
+    const int32_t pick = l < a.k ? picks[l] : 0;
+    WaveSync();
     if (!close && mine) WritePicks<Codec, Out, kLanes>(a, row, l, pick, shift, sum);
     for (uint64_t again = __ballot(close && mine && l == 0); again != 0; again &= again - 1) {
         const int64_t which = rowsFrom + (__ffsll(static_cast<unsigned long long>(again)) - 1) / kLanes;
@@ -674,8 +686,8 @@ class GatingExecutor : public aclOpExecutor {
     void Launch(hipStream_t stream) const {
         const int E = args.experts;
         // Sixteen lanes a row make more rows at a time and take longer for one, most of all with a bias, where one row in a thousand is
-        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 9.1 and 10.1 at 4096, 15.9 and
-        // 27.5 at 16384; softmax without a bias 5.2 and 5.3, 5.3 and 8.0, 9.0 and 20.7.
+        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 8.8 and 10.1 at 4096, 15.4 and
+        // 27.5 at 16384; softmax without a bias 5.2 and 5.3, 5.0 and 8.0, 8.4 and 20.7.
         const bool many = args.rows > (args.bias != nullptr ? 4000 : 1024);
         if (many && E <= 512 && args.k <= 16 && args.groups <= 16) {
             if (E <= 16) LaunchQuads<Codec, Out, 1>(stream);
