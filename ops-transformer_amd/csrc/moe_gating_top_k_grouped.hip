@@ -289,11 +289,10 @@ __device__ __forceinline__ void LoadLane(const GatingArgs& a, const typename Cod
     }
 }
 
-// y and the index of a row's picks, the j-th of them in its lane j.
-template <typename Codec, typename Out, int kLanes>
-__device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int l, int32_t pick, double shift, double sum) {
-    const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
-    double y = l < a.k ? ScoreOf(Codec::Load(x[pick]), a.sigmoid != 0, shift, sum) : 0.0;
+// y and the index of a row's picks, the j-th of them, whose logit is x, in its lane j.
+template <typename Out, int kLanes>
+__device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int l, int32_t pick, float x, double shift, double sum) {
+    double y = l < a.k ? ScoreOf(x, a.sigmoid != 0, shift, sum) : 0.0;
     if (a.renorm != 0) {
         const double total = RowSum<kLanes>(y) + a.eps;
         y = total == 0.0 ? 0.0 : y / total;
@@ -305,8 +304,8 @@ __device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int
     }
 }
 
-// A row of up to 64 * kPer experts, at most 64 groups, by one wave in 64 bits: lane l holds experts l * kPer + i, the keys in registers.  lds: 8 bytes an
-// expert, the wave's own, for groups whose experts are not those of whole lanes.  What bounds it is latency: a pick is a maximum over four rotations inside
+// A row of up to 64 * kPer experts, at most 64 groups, by one wave in 64 bits: lane l holds experts l * kPer + i, the keys in registers.  lds: 12 bytes an
+// expert, the wave's own, for groups whose experts are not those of whole lanes and for the logits of the picks.  What bounds it is latency: a pick is a maximum over four rotations inside
 // a row of sixteen lanes, four lane reads and a ballot (256 experts, 8 picks: 4.7 us, with sigmoid, bias and groups 6.0; with the keys in LDS and the
 // arg-max over twelve shuffles 10.9 and 15.8).
 template <typename Codec, typename Out, int kPer>
@@ -315,27 +314,43 @@ __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int la
     const bool sigmoid = a.sigmoid != 0, biased = a.bias != nullptr, grouped = a.kGroup < a.groups;
     float v[kPer];
     LoadLane<Codec, kPer>(a, x, lane, v);
-    double shift = 0.0, sum = 1.0;
-    if (!sigmoid) {
+    float* const values = reinterpret_cast<float*>(lds + a.experts);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        if (lane * kPer + i < a.experts) values[lane * kPer + i] = v[i];
+    }
+    // p as ScoreOf has it, without branches for each: exponentials in 64 bits are long chains, which run side by side
+    double shift = 0.0, sum = 1.0, p[kPer] = {};
+    if (sigmoid) {
+        if (biased || writeScores) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) p[i] = 1.0 / (1.0 + exp(-static_cast<double>(v[i])));  // 0 of -inf
+        }
+    } else {
         uint32_t most = 0;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) most = max(most, Key32(v[i]));
         shift = Value32(RowMax<64>(most));
         sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) sum += ScoreOf(v[i], false, shift, 1.0);
+        for (int i = 0; i < kPer; ++i) {
+            p[i] = exp(static_cast<double>(v[i]) - shift);
+            p[i] = v[i] == -INFINITY ? 0.0 : p[i];
+            sum += p[i];
+        }
         sum = RowSum<64>(sum);
+        if (biased || writeScores) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) p[i] = v[i] == -INFINITY ? 0.0 : p[i] / sum;
+        }
     }
     uint64_t keys[kPer];
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
         const int c = lane * kPer + i;
+        if (writeScores && c < a.experts) a.scores[row * a.experts + c] = static_cast<float>(p[i]);
         double t = Unsigned0(v[i]);
-        if (biased || writeScores) {
-            const double p = ScoreOf(v[i], sigmoid, shift, sum);
-            if (writeScores && c < a.experts) a.scores[row * a.experts + c] = static_cast<float>(p);
-            if (biased && v[i] != -INFINITY) t = p + static_cast<double>(a.bias[c < a.experts ? c : 0]);
-        }
+        if (biased) t = v[i] == -INFINITY ? t : p[i] + static_cast<double>(a.bias[c < a.experts ? c : 0]);
         keys[i] = c < a.experts ? KeyOf(t) : 0;
     }
     if (grouped) {
@@ -408,21 +423,22 @@ __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int la
             if (lane == holder && i == taken) keys[i] = 0;
         }
     }
-    WritePicks<Codec, Out, 64>(a, row, lane, pick, shift, sum);
+    WaveSync();
+    WritePicks<Out, 64>(a, row, lane, pick, values[pick], shift, sum);
 }
 
 constexpr int kRowWaves = 4;  // of a workgroup
+
+// LDS of a wave: a row's keys in 64 bits and its logits; or an fp32 value per expert of its four rows, then their picks.
+constexpr uint32_t WaveBytes(int experts) { return static_cast<uint32_t>(experts < 16 ? 16 : experts) * 16; }
 
 template <typename Codec, typename Out, int kPer>
 __global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs a) {
     extern __shared__ __attribute__((aligned(16))) unsigned char ldsRaw[];
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t row = GroupIndex() * kRowWaves + wave;
-    if (row < a.rows) WaveRow<Codec, Out, kPer>(a, row, lane, reinterpret_cast<uint64_t*>(ldsRaw) + wave * a.experts, a.scores != nullptr);
+    if (row < a.rows) WaveRow<Codec, Out, kPer>(a, row, lane, reinterpret_cast<uint64_t*>(ldsRaw + wave * WaveBytes(a.experts)), a.scores != nullptr);
 }
-
-// LDS of a wave: an fp32 value per expert of its four rows, then their picks, or a row's keys in 64 bits.
-constexpr uint32_t QuadBytes(int experts) { return static_cast<uint32_t>(experts < 16 ? 16 : experts) * 16; }
 
 // Rows of up to 16 * kPer experts, at most 16 picks and groups: four rows a wave, sixteen lanes each, fp32 keys in registers.  Lane l of a row holds experts
 // l * kPer + i, so that among equal values the lower lane has the lower index; within a lane the number i goes into the lowest bits of the key, which
@@ -446,7 +462,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     if (rowsFrom >= a.rows) return;
     const int64_t row = min(rowsFrom + lane / kLanes, a.rows - 1);
     const bool mine = rowsFrom + lane / kLanes < a.rows;
-    unsigned char* const own = ldsRaw + wave * QuadBytes(a.experts);
+    unsigned char* const own = ldsRaw + wave * WaveBytes(a.experts);
     float* const values = reinterpret_cast<float*>(own) + lane / kLanes * a.experts;  // of the row, while groups are chosen
 
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
@@ -645,7 +661,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     WaveSync();
     const int32_t pick = l < a.k ? picks[l] : 0;
     WaveSync();
-    if (!close && mine) WritePicks<Codec, Out, kLanes>(a, row, l, pick, shift, sum);
+    if (!close && mine) WritePicks<Out, kLanes>(a, row, l, pick, Codec::Load(x[pick]), shift, sum);
     for (uint64_t again = __ballot(close && mine && l == 0); again != 0; again &= again - 1) {
         const int64_t which = rowsFrom + (__ffsll(static_cast<unsigned long long>(again)) - 1) / kLanes;
         GatingArgs whole = a;
@@ -673,13 +689,13 @@ class GatingExecutor : public aclOpExecutor {
     template <typename Codec, typename Out, int kPer>
     void LaunchWaves(hipStream_t stream) const {
         hipLaunchKernelGGL((GatingWaveKernel<Codec, Out, kPer>), GridOf((args.rows + kRowWaves - 1) / kRowWaves), dim3(kWave * kRowWaves),
-                           static_cast<size_t>(kRowWaves) * args.experts * 8, stream, ForLanes<Codec>(kWave, kPer));
+                           kRowWaves * WaveBytes(args.experts), stream, ForLanes<Codec>(kWave, kPer));
     }
 
     template <typename Codec, typename Out, int kPer>
     void LaunchQuads(hipStream_t stream) const {
         hipLaunchKernelGGL((GatingQuadKernel<Codec, Out, kPer>), GridOf((args.rows + 4 * kRowWaves - 1) / (4 * kRowWaves)), dim3(kWave * kRowWaves),
-                           kRowWaves * QuadBytes(args.experts), stream, ForLanes<Codec>(16, kPer));
+                           kRowWaves * WaveBytes(args.experts), stream, ForLanes<Codec>(16, kPer));
     }
 
     template <typename Codec, typename Out>
