@@ -34,7 +34,7 @@ struct GatingArgs {
     int32_t topTwo;           // a group's value is the sum of its two largest t
     int32_t sigmoid;
     int32_t renorm;
-    int32_t packets;          // rows fill their lanes and start on the lanes' boundaries
+    int32_t packets;          // lanes have all of their experts or none (1), or all of them have (2), and rows start on the lanes' boundaries
     int32_t biasPackets;      // so does the bias
     uint32_t groupMagic;      // (c * groupMagic) >> 21 = c / (experts / groups) for c < 512
     float factor;
@@ -277,11 +277,20 @@ __device__ __forceinline__ void LoadLane(const GatingArgs& a, const typename Cod
         struct alignas(kPiece * sizeof(typename Codec::Storage)) Piece {
             typename Codec::Storage e[kPiece];
         };
+        auto read = [&] {
 #pragma unroll
-        for (int i = 0; i < kPer; i += kPiece) {
-            const Piece piece = *reinterpret_cast<const Piece*>(x + l * kPer + i);
+            for (int i = 0; i < kPer; i += kPiece) {
+                const Piece piece = *reinterpret_cast<const Piece*>(x + l * kPer + i);
 #pragma unroll
-            for (int j = 0; j < kPiece; ++j) v[i + j] = Codec::Load(piece.e[j]);
+                for (int j = 0; j < kPiece; ++j) v[i + j] = Codec::Load(piece.e[j]);
+            }
+        };
+        if (a.packets == 2) {
+            read();
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) v[i] = -INFINITY;
+            if (l * kPer < a.experts) read();
         }
     } else {
 #pragma unroll
@@ -305,9 +314,10 @@ __device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int
 }
 
 // A row of up to 64 * kPer experts, at most 64 groups, by one wave in 64 bits: lane l holds experts l * kPer + i, the keys in registers.  lds: 12 bytes an
-// expert, the wave's own, for groups whose experts are not those of whole lanes and for the logits of the picks.  What bounds it is latency: a pick is a maximum over four rotations inside
-// a row of sixteen lanes, four lane reads and a ballot (256 experts, 8 picks: 4.7 us, with sigmoid, bias and groups 6.0; with the keys in LDS and the
-// arg-max over twelve shuffles 10.9 and 15.8).
+// expert, the wave's own, for groups whose experts are not those of whole lanes and for the logits of the picks.  What bounds it is latency: a pick is a
+// maximum over four rotations inside a row of sixteen lanes, four lane reads and a ballot (256 experts, 8 picks: 4.7 us, with sigmoid, bias and groups
+// 5.8; with the keys in LDS and the arg-max over twelve shuffles 10.9 and 15.8), a value's exponential in 64 bits a chain of fifty instructions
+// (301 x 160, softmax with the scores 6.1 us; with a branch for each value 7.3).
 template <typename Codec, typename Out, int kPer>
 __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int lane, uint64_t* lds, bool writeScores) {
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
@@ -446,9 +456,10 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs
 // smaller key.
 // Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once.
 // Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
-// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.4 us (16.8 MB of logits are 3.3), of which a row that
+// What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.6 us (16.8 MB of logits are 3.3), of which a row that
 // is made twice is 3: 950 vector instructions a wave, near half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
-// softmax without bias or groups, bf16 8.4.  Rows without an infinity or a NaN are spared what those need: 16.0 and 9.0 without.
+// softmax without bias or groups, bf16 8.4.  Rows without an infinity or a NaN are spared what those need: 16.0 and 9.0 without.  Rows that end
+// between two lanes are read in packets too: 384 experts, bf16, sigmoid, bias 18.4 us, an element at a time 36.
 template <typename Codec, typename Out, int kPer>
 __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs a) {
     constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : kPer == 16 ? 4 : 5;
@@ -475,9 +486,10 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
             struct alignas(kPiece * 4) Piece {
                 float e[kPiece];
             };
+            const float* const own = a.bias + min(l * kPer, a.experts - kPer);
 #pragma unroll
             for (int i = 0; i < kPer; i += kPiece) {
-                const Piece piece = *reinterpret_cast<const Piece*>(a.bias + l * kPer + i);
+                const Piece piece = *reinterpret_cast<const Piece*>(own + i);
 #pragma unroll
                 for (int j = 0; j < kPiece; ++j) b[i + j] = piece.e[j];
             }
@@ -489,7 +501,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     float all = v[0];
 #pragma unroll
     for (int i = 1; i < kPer; ++i) all += v[i];
-    const bool plain = __all(fabsf(all) < INFINITY);  // no NaN and no infinity in any of the wave's rows
+    const bool plain = __all(fabsf(all) < INFINITY || l * kPer >= a.experts);  // no NaN and no infinity in any of the wave's rows
     bool close = false;  // uniform over the row: it is made again, for values too close to be told apart here, or a NaN
     if (!plain) {
         bool nan = false;
@@ -629,15 +641,18 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     }
     const bool exact = !biased && (sizeof(typename Codec::Storage) == 2 || kBits == 0);
     // what is not looked at: experts that are not there, or in a group that was left out (no branches for each: a third of the kernel's time)
-    if (grouped && whole) {
-        const uint32_t stays = 0u - (kept >> group & 1);
+    if (grouped || a.experts != kLanes * kPer) {
+        auto mask = [&](uint32_t c) {
+            const uint32_t stays = grouped ? kept >> ((c * a.groupMagic >> 21) & 31) & 1 : 1u;
+            return 0u - (c < static_cast<uint32_t>(a.experts) ? stays : 0u);
+        };
+        if ((grouped ? a.experts / a.groups : a.experts) % kPer == 0) {
+            const uint32_t stays = mask(l * kPer);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) keys[i] &= stays;
-    } else if (grouped || a.experts != kLanes * kPer) {
+            for (int i = 0; i < kPer; ++i) keys[i] &= stays;
+        } else {
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            const uint32_t c = l * kPer + i, stays = grouped ? kept >> ((c * a.groupMagic >> 21) & 31) & 1 : 1u;
-            keys[i] &= 0u - (c < static_cast<uint32_t>(a.experts) ? stays : 0u);
+            for (int i = 0; i < kPer; ++i) keys[i] &= mask(l * kPer + i);
         }
     }
     const uint32_t upper = biased ? ~31u : ~kLow, lowest = biased ? 2u << (32 - kPlaceBits) : 0x00800000u;  // below: -inf, or none left
@@ -681,8 +696,8 @@ class GatingExecutor : public aclOpExecutor {
     GatingArgs ForLanes(int lanes, int per) const {
         GatingArgs g = args;
         const size_t bytes = per * sizeof(typename Codec::Storage), piece = bytes < 16 ? bytes : 16;
-        g.packets = g.experts == lanes * per && reinterpret_cast<uintptr_t>(g.x) % piece == 0 ? 1 : 0;
-        g.biasPackets = g.experts == lanes * per && reinterpret_cast<uintptr_t>(g.bias) % 16 == 0 ? 1 : 0;
+        g.packets = g.experts % per == 0 && reinterpret_cast<uintptr_t>(g.x) % piece == 0 ? (g.experts == lanes * per ? 2 : 1) : 0;
+        g.biasPackets = g.experts % per == 0 && reinterpret_cast<uintptr_t>(g.bias) % 16 == 0 ? 1 : 0;
         return g;
     }
 
@@ -702,7 +717,7 @@ class GatingExecutor : public aclOpExecutor {
     void Launch(hipStream_t stream) const {
         const int E = args.experts;
         // Sixteen lanes a row make more rows at a time and take longer for one, most of all with a bias, where one row in a thousand is
-        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 8.8 and 10.1 at 4096, 15.4 and
+        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 8.8 and 10.1 at 4096, 15.6 and
         // 27.5 at 16384; softmax without a bias 5.2 and 5.3, 5.0 and 8.0, 8.4 and 20.7.
         const bool many = args.rows > (args.bias != nullptr ? 4000 : 1024);
         if (many && E <= 512 && args.k <= 16 && args.groups <= 16) {

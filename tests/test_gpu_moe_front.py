@@ -535,6 +535,25 @@ def test_gating_long_batches(aclnn, dev, E, groups, score_type):
         _check_long(aclnn, dev, short, order, min(8, E), score_type=score_type)
 
 
+@pytest.mark.parametrize("T", [7, LONG])
+@pytest.mark.parametrize("E", [16, 24, 60, 100, 160, 256, 384])
+def test_gating_rows_off_the_grid(aclnn, dev, T, E):
+    """Rows and a bias that start between the boundaries of the lanes' packets: the same bits as those on them."""
+    g = torch.Generator().manual_seed(E)
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.randn((T, E), generator=g).to(dtype).to(dev)
+        bias = (0.1 * torch.randn(E, generator=g)).to(dev)
+        odd = torch.zeros(T * E + 1, dtype=dtype, device=dev)[1:].view(T, E)
+        odd.copy_(x)
+        shifted = torch.zeros(E + 1, device=dev)[1:]
+        shifted.copy_(bias)
+        for kw in [dict(), dict(k_group=2, group_count=4, group_select_mode=1)]:
+            for b, o in [(None, None), (bias, shifted)]:
+                want = aclnn.moe_gating_top_k_grouped(x, 4, bias=b, score_type=1, renorm=1, output_scores=True, **kw)
+                got = aclnn.moe_gating_top_k_grouped(odd, 4, bias=o, score_type=1, renorm=1, output_scores=True, **kw)
+                assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
 @pytest.mark.parametrize("T", [3, LONG])
 @pytest.mark.parametrize("E,groups", [(16, 4), (96, 4), (640, 4)])
 def test_gating_zeros_of_either_sign_are_equal(aclnn, dev, T, E, groups):
