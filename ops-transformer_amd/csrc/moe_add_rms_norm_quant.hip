@@ -74,7 +74,7 @@ __device__ __forceinline__ void ReduceRow(float& sumSquares, uint32_t& maxBits) 
     }
 }
 
-// Rows of any length and alignment: a workgroup per row, one element at a time, the row read again for the outputs (from the sum where that
+// Rows of any length: a workgroup per row, one element at a time, the row read again for the outputs (from the sum where that
 // was written, by the same lane: it may lie in x's memory).
 constexpr int kAnyThreads = 256;
 
@@ -110,12 +110,15 @@ __global__ __launch_bounds__(kAnyThreads) void NormQuantAnyKernel(NormArgs a) {
     }
 }
 
-// Rows in pieces of eight elements on the 16-byte grid, up to kPackets of them per lane, read once and kept in registers from the reduction to the
+// Rows in pieces of eight elements, up to kPackets of them per lane, read once and kept in registers from the reduction to the
 // outputs.  A workgroup takes every gridDim.x-th row: gamma and smooth stay with it, and the next row is asked for before the present one is
 // reduced.  What bounds it is HBM: 8192 x 7168 bf16 with a residual, all outputs, 100 us at 5.3 TB/s, where a plain copy of 1 GiB reaches 5.2 (the
 // kernel that reads rows twice, an element at a time: 350 us); one row of 4096 3.6 us, a launch and one round trip.  As few packets a lane as
 // 512 threads allow: the same row on one, two and four takes 3.6, 3.9 and 5.2 us, 4096 x 4096 fp32 55, 56 and 60.  Workgroups: 4096 at most, for the
 // widest rows 100 us against 103 to 104 for 512 to 2048; narrow rows 2048 (16384 x 1024: 31.5 us, with 4096 33.3, with 1024 37.8).
+// Off the 16-byte grid (kGrid false) pieces are read and written where they lie, which the vector memory instructions do at any address, and a row's last
+// one by its elements: 8192 x 7167 bf16 174 us (246 twice and an element at a time), 64 x 7167 6.7 (19).  Pieces on the grid whose first and last are another
+// row's in part: 148 to 157, but rows of 3001 42 instead of 33.
 constexpr int kMaxPacketThreads = 512;
 constexpr int kMaxPackets = 4;
 
@@ -150,30 +153,68 @@ __device__ __forceinline__ Packet<Codec> Pack(const float (&v)[8]) {
     return p;
 }
 
-template <typename Codec, typename Gamma, int kPackets, bool kSmooth>
+// `count` (1 to 8) elements from `at` on, zeros behind them, and back.
+template <bool kGrid, typename Codec>
+__device__ __forceinline__ Packet<Codec> LoadPacket(const void* base, int64_t at, int count) {
+    const typename Codec::Storage* const from = static_cast<const typename Codec::Storage*>(base) + at;
+    Packet<Codec> p;
+    if constexpr (kGrid) {
+        p = *reinterpret_cast<const Packet<Codec>*>(from);
+    } else if (count == 8) {
+        __builtin_memcpy(&p, from, sizeof(p));
+    } else {
+        typename Codec::Storage raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) raw[i] = i < count ? from[i] : typename Codec::Storage{};
+        __builtin_memcpy(&p, raw, sizeof(p));
+    }
+    return p;
+}
+template <bool kGrid, typename Storage, typename P>
+__device__ __forceinline__ void StorePacket(void* base, int64_t at, int count, const P& p) {
+    static_assert(sizeof(P) == 8 * sizeof(Storage));
+    Storage* const to = static_cast<Storage*>(base) + at;
+    if constexpr (kGrid) {
+        *reinterpret_cast<P*>(to) = p;
+    } else if (count == 8) {
+        __builtin_memcpy(to, &p, sizeof(p));
+    } else {
+        Storage raw[8];
+        __builtin_memcpy(raw, &p, sizeof(p));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i < count) to[i] = raw[i];
+        }
+    }
+}
+
+template <typename Codec, typename Gamma, int kPackets, bool kSmooth, bool kGrid>
 __global__ __launch_bounds__(kMaxPacketThreads) void NormQuantPacketsKernel(NormArgs a) {
     using P = Packet<Codec>;
+    using Storage = typename Codec::Storage;
     __shared__ float2 partial[2][kMaxPacketThreads / kWave];
     const int threads = blockDim.x, waves = threads / kWave, tid = threadIdx.x;
-    const int64_t packets = a.cols / 8;  // of a row
+    const int cols = static_cast<int>(a.cols);
     P x[kPackets], r[kPackets];
     Packet<Gamma> gamma[kPackets];
     Packet<F32> smooth[kSmooth ? kPackets : 1];
     bool here[kPackets];
+    auto at = [&](int p) { return (p * threads + tid) * 8; };
+    auto count = [&](int p) { return min(cols - at(p), 8); };
 #pragma unroll
     for (int p = 0; p < kPackets; ++p) {
-        here[p] = p * threads + tid < packets;
+        here[p] = at(p) < cols;
         if (here[p]) {
-            gamma[p] = static_cast<const Packet<Gamma>*>(a.gamma)[p * threads + tid];
-            if constexpr (kSmooth) smooth[p] = reinterpret_cast<const Packet<F32>*>(a.smooth)[p * threads + tid];
+            gamma[p] = LoadPacket<kGrid, Gamma>(a.gamma, at(p), count(p));
+            if constexpr (kSmooth) smooth[p] = LoadPacket<kGrid, F32>(a.smooth, at(p), count(p));
         }
     }
     auto load = [&](int64_t row) {
 #pragma unroll
         for (int p = 0; p < kPackets; ++p) {
             if (!here[p]) continue;
-            x[p] = static_cast<const P*>(a.x)[row * packets + p * threads + tid];
-            if (a.residual != nullptr) r[p] = static_cast<const P*>(a.residual)[row * packets + p * threads + tid];
+            x[p] = LoadPacket<kGrid, Codec>(a.x, row * cols + at(p), count(p));
+            if (a.residual != nullptr) r[p] = LoadPacket<kGrid, Codec>(a.residual, row * cols + at(p), count(p));
         }
     };
     int64_t row = blockIdx.x;
@@ -196,7 +237,7 @@ __global__ __launch_bounds__(kMaxPacketThreads) void NormQuantPacketsKernel(Norm
                 s[p] = Pack<Codec>(v);
                 Unpack<Codec>(s[p], v);
             }
-            if (a.sum != nullptr) static_cast<P*>(a.sum)[row * packets + p * threads + tid] = s[p];
+            if (a.sum != nullptr) StorePacket<kGrid, Storage>(a.sum, row * cols + at(p), count(p), s[p]);
             float g[8];
             Unpack<Gamma>(gamma[p], g);
 #pragma unroll
@@ -233,7 +274,7 @@ __global__ __launch_bounds__(kMaxPacketThreads) void NormQuantPacketsKernel(Norm
                 float n[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) n[i] = v[i] * scales.r * g[i];
-                static_cast<P*>(a.norm)[row * packets + p * threads + tid] = Pack<Codec>(n);
+                StorePacket<kGrid, Storage>(a.norm, row * cols + at(p), count(p), Pack<Codec>(n));
             }
             if (a.y != nullptr) {
                 uint32_t q[2] = {0, 0};
@@ -243,7 +284,7 @@ __global__ __launch_bounds__(kMaxPacketThreads) void NormQuantPacketsKernel(Norm
                     if constexpr (kSmooth) w *= reinterpret_cast<const float*>(&smooth[p])[i];
                     q[i / 4] |= (static_cast<uint32_t>(Quantised(w, scales)) & 0xffu) << (i % 4 * 8);
                 }
-                reinterpret_cast<uint2*>(a.y)[row * packets + p * threads + tid] = uint2{q[0], q[1]};
+                StorePacket<kGrid, int8_t>(a.y, row * cols + at(p), count(p), uint2{q[0], q[1]});
             }
         }
         row = next;
@@ -257,37 +298,43 @@ class NormQuantExecutor : public aclOpExecutor {
     aclDataType gammaType = ACL_FLOAT;
 
     // Every tensor starts on the boundaries that packets are read and written at, row after row.
-    template <typename Codec, typename Gamma>
     bool OnGrid() const {
         auto on = [](const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
-        return args.cols % 8 == 0 && args.cols <= 8 * kMaxPacketThreads * kMaxPackets && on(args.x, 16) && on(args.residual, 16) &&
+        return args.cols % 8 == 0 && on(args.x, 16) && on(args.residual, 16) &&
                on(args.gamma, 16) && on(args.smooth, 16) && on(args.norm, 16) && on(args.sum, 16) && on(args.y, 8);
     }
 
-    template <typename Codec, typename Gamma, int kPackets>
+    template <typename Codec, typename Gamma, int kPackets, bool kGrid>
     void LaunchPackets(hipStream_t stream) const {
-        const int64_t lanes = (args.cols / 8 + kPackets - 1) / kPackets;
+        const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
         const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
         int64_t groups = args.rows;
         const int64_t most = threads >= 256 ? 4096 : 2048;
         if (groups > most) groups = most;
         if (args.smooth != nullptr) {
-            hipLaunchKernelGGL((NormQuantPacketsKernel<Codec, Gamma, kPackets, true>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, args);
+            hipLaunchKernelGGL((NormQuantPacketsKernel<Codec, Gamma, kPackets, true, kGrid>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, args);
         } else {
-            hipLaunchKernelGGL((NormQuantPacketsKernel<Codec, Gamma, kPackets, false>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, args);
+            hipLaunchKernelGGL((NormQuantPacketsKernel<Codec, Gamma, kPackets, false, kGrid>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, args);
         }
     }
 
     template <typename Codec, typename Gamma>
     void Launch(hipStream_t stream) const {
-        if (!OnGrid<Codec, Gamma>()) {
+        if (args.cols > 8 * kMaxPacketThreads * kMaxPackets) {
             hipLaunchKernelGGL((NormQuantAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
-            return;
+        } else if (OnGrid()) {
+            ChoosePackets<Codec, Gamma, true>(stream);
+        } else {
+            ChoosePackets<Codec, Gamma, false>(stream);
         }
-        const int64_t lanes = args.cols / 8;
-        if (lanes <= kMaxPacketThreads) LaunchPackets<Codec, Gamma, 1>(stream);
-        else if (lanes <= 2 * kMaxPacketThreads) LaunchPackets<Codec, Gamma, 2>(stream);
-        else LaunchPackets<Codec, Gamma, 4>(stream);
+    }
+
+    template <typename Codec, typename Gamma, bool kGrid>
+    void ChoosePackets(hipStream_t stream) const {
+        const int64_t lanes = (args.cols + 7) / 8;
+        if (lanes <= kMaxPacketThreads) LaunchPackets<Codec, Gamma, 1, kGrid>(stream);
+        else if (lanes <= 2 * kMaxPacketThreads) LaunchPackets<Codec, Gamma, 2, kGrid>(stream);
+        else LaunchPackets<Codec, Gamma, 4, kGrid>(stream);
     }
 
     template <typename Codec>
