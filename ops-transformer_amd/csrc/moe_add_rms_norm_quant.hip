@@ -112,7 +112,7 @@ __global__ __launch_bounds__(kAnyThreads) void NormQuantAnyKernel(NormArgs a) {
 
 // Rows in pieces of eight elements, up to kPackets of them per lane, read once and kept in registers from the reduction to the
 // outputs.  A workgroup takes every gridDim.x-th row: gamma and smooth stay with it, and the next row is asked for before the present one is
-// reduced.  What bounds it is HBM: 8192 x 7168 bf16 with a residual, all outputs, 100 us at 5.3 TB/s, where a plain copy of 1 GiB reaches 5.2 (the
+// reduced.  What bounds it is HBM: 8192 x 7168 bf16 with a residual, all outputs, 97 to 100 us at 5.3 TB/s and more, where a plain copy of 1 GiB reaches 5.2 (the
 // kernel that reads rows twice, an element at a time: 350 us); one row of 4096 3.6 us, a launch and one round trip.  As few packets a lane as
 // 512 threads allow: the same row on one, two and four takes 3.6, 3.9 and 5.2 us, 4096 x 4096 fp32 55, 56 and 60.  Workgroups: 4096 at most, for the
 // widest rows 100 us against 103 to 104 for 512 to 2048; narrow rows 2048 (16384 x 1024: 31.5 us, with 4096 33.3, with 1024 37.8).

@@ -457,7 +457,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs
 // Errors, u = 2^-24: p is within 8 u top of itself (an exponential and its argument, the sum in 64 bits, a reciprocal), t = p + bias rounds once.
 // Values that decide something and lie closer: the row is made again by the whole wave, in 64 bits.
 // What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.6 us (16.8 MB of logits are 3.3), of which a row that
-// is made twice is 3: 950 vector instructions a wave, near half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
+// is made twice is 3: 980 vector instructions a wave, near half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
 // softmax without bias or groups, bf16 8.4.  Rows without an infinity or a NaN are spared what those need: 16.0 and 9.0 without.  Rows that end
 // between two lanes are read in packets too: 384 experts, bf16, sigmoid, bias 18.4 us, an element at a time 36.
 template <typename Codec, typename Out, int kPer>
