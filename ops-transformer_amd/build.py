@@ -17,6 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libcust_opapi.so")
+BINDING_PATH = os.path.join(LIB_DIR, "opapi_torch.so")  # the Python module that reads torch's tensors; the library itself knows nothing of torch
 EXPORTS = os.path.join(CSRC, "exports.map")  # linker version script: only the C entry points leave the library
 
 SOURCES = [
@@ -286,14 +287,34 @@ def build_sanitized(jobs=None):
     return SANITIZED_LIB_PATH
 
 
+def build_binding(force=False):
+    """Compiles the Python module (host code only) against the installed torch's headers.  Returns its path."""
+    import sysconfig
+
+    import torch
+    src = os.path.join(CSRC, "torch_binding.cpp")
+    deps = [src, os.path.abspath(__file__), torch.version.__file__] + _headers()
+    if not force and os.path.exists(BINDING_PATH) and all(os.path.getmtime(BINDING_PATH) >= os.path.getmtime(d) for d in deps):
+        return BINDING_PATH
+    base = os.path.dirname(torch.__file__)
+    include = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"],
+               os.path.join(ROOT, "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch.compiled_with_cxx11_abi())]
+    cmd += ["-isystem" + d for d in include[:3]] + ["-I" + include[3], src, "-o", BINDING_PATH, "-L" + os.path.join(base, "lib")]
+    subprocess.check_call(cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10"])
+    return BINDING_PATH
+
+
 def build(force=False, jobs=None):
-    """Compile every source for gfx950 and link the shared library.  Returns its path."""
+    """Compile every source for gfx950 and link the shared library, and the Python module over it.  Returns the library's path."""
     check_compiler()
     os.makedirs(OBJ_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     jobs = jobs or min(len(SOURCES), os.cpu_count() or 1)
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
+        binding = pool.submit(build_binding, force)
         results = list(pool.map(lambda s: _compile(s, force), SOURCES))
+        binding.result()
     objs = [o for o, _ in results]
     rebuilt = any(r for _, r in results)
     if rebuilt or not os.path.exists(LIB_PATH) or os.path.getmtime(LIB_PATH) < os.path.getmtime(EXPORTS):

@@ -681,6 +681,20 @@ def test_block_in_a_graph_and_on_another_stream(pkg, aclnn, dev, tokens):
         assert torch.equal(a, b)
 
 
+def test_tensors_that_do_not_fit_are_refused(aclnn, dev):
+    x, gamma = torch.ones((2, 64), dtype=torch.bfloat16, device=dev), torch.ones(64, dtype=torch.bfloat16)
+    with pytest.raises(aclnn.AclnnError, match="on cuda:0 and cpu"):
+        aclnn.moe_add_rms_norm_quant(x, gamma)
+    with pytest.raises(TypeError, match="not one the operators know"):
+        aclnn.moe_router_logits(x, torch.ones((3, 64), dtype=torch.float64, device=dev))
+    with pytest.raises(aclnn.AclnnError, match="must be"):
+        aclnn.moe_router_logits(x, torch.ones((3, 63), dtype=torch.bfloat16, device=dev))
+    with pytest.raises(TypeError):
+        aclnn.moe_router_logits(x, torch.ones((1,) * 9, device=dev), out=torch.ones((2, 1), device=dev))
+    y, scale, norm, _ = aclnn.moe_add_rms_norm_quant(x, gamma.to(dev), epsilon=0)  # a whole number for a double
+    assert torch.equal(norm, x) and int(y.min()) == 127
+
+
 def test_calls_at_once_on_two_streams(aclnn, dev):
     """Calls of the same sizes side by side: without a workspace of the caller's every call has its own."""
     g = torch.Generator().manual_seed(8)

@@ -261,3 +261,17 @@ def test_host_tensors_are_refused(aclnn):
         with pytest.raises(aclnn.AclnnError, match="not on the current GPU") as e:
             call()
         assert e.value.code == INVALID
+
+
+def test_the_module_that_reads_tensors_checks_what_it_is_given(aclnn):
+    run, function = aclnn._binding()
+    x = torch.zeros((2, 4))
+    assert run(function, 0, 0, 0, 0, (8,), (x, x, x)) is x                       # not on the device
+    assert run(function, 0, 0, 0, 0, (8,), (None, None, None)) == -NULLPTR
+    assert run(function, 0, 0, 0, 0, (99,), ()) == -INVALID
+    for args in [(function, 0, 0, 0, 0, (8,), (1, x, x)), (function, 0, 0, 0, 0, ("8",), (x,)), (function, 0, 0, 0, 0, [8], (x,)), (function,),
+                 (function, 0, 0, 0, 0, (8,) * 17, ()), (function, 0, 0, 0, 0, (8,), (None,) * 17), ("f", 0, 0, 0, 0, (8,), ())]:
+        with pytest.raises(TypeError):
+            run(*args)
+    with pytest.raises(OverflowError):
+        run(function, 0, 0, 0, 0, (1 << 64,), ())
