@@ -490,7 +490,8 @@ __global__ __launch_bounds__(kAddThreads) void AddSplitsKernel(const float* part
 
 // What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 320 000 measurements of 50 900 calls over the operator's
 // range (1 to 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types).  Nine in ten are between 0.76 and 1.17 of the fit; the choice by it costs
-// 1.8 % more than the best shape in the mean, 7 % in one call of ten.  A shape each kind of call needs: without the slim kernels decode takes up to twice as
+// 1.8 % more than the best shape in the mean, 7 % in one call of ten (columns off the 16-byte grid 1.4 %, odd ones of 16 bits 2.8 %, and without their own
+// weights 1.8 and 6.5).  A shape each kind of call needs: without the slim kernels decode takes up to twice as
 // long (64 x 7168 x 256: 12.7 against 8.4 us, one row 7.4 against 2.9), without the tiles a prompt does (8192 x 7168 x 256, fp32 weights: 333 against 97 us).
 struct Slim {
     int m, n, sub, waves;
@@ -521,6 +522,9 @@ class LogitsExecutor : public aclOpExecutor {
         const double xSize = static_cast<double>(opapi::ElemSize(dtype)), wSize = static_cast<double>(opapi::ElemSize(weightType));
         const bool same16 = dtype == weightType && dtype != ACL_FLOAT;
         const int xParts = same16 || dtype == ACL_BF16 ? 1 : dtype == ACL_FLOAT16 ? 2 : 3;
+        // bytes off the 16-byte grid take longer to come, most of all where rows start between two words and each is read by many
+        const int64_t rowBytes[] = {args.cols * opapi::ElemSize(dtype), args.cols * opapi::ElemSize(weightType)};
+        const double slimBytes = rowBytes[0] % 4 != 0 ? 3 : rowBytes[0] % 16 != 0 || rowBytes[1] % 16 != 0 ? 1.5 : 1, tileBytes = slimBytes > 1 ? 1.5 : 1;
         const double products = same16 ? 1 : xParts == 1 ? 3 : xParts == 2 ? 5 : 6;
         auto over = [](double n, double d) { return std::ceil(n / d); };
         double best = 0;
@@ -538,7 +542,7 @@ class LogitsExecutor : public aclOpExecutor {
             if (over(T, rows) * over(E, experts) * v.waves * kWave > kMaxThreads) continue;
             const double rounds = over(over(T, rows) * over(E, experts), 256), steps = over(K, 32 * v.sub * v.waves) * v.waves / 4;
             const double cuts = ((same16 ? 0 : 3) * v.n + (xParts > 1 ? 3 : 0) * v.m) * steps * 32 / 2400;
-            offer(kSlimUs[0] + kSlimUs[4] * operands + rounds * (kSlimUs[1] * K * (rows * xSize + experts * wSize) * 1e-5 + kSlimUs[2] * v.waves / 8 + kSlimUs[3] * cuts), i, 1);
+            offer(kSlimUs[0] + kSlimUs[4] * operands + rounds * (kSlimUs[1] * slimBytes * K * (rows * xSize + experts * wSize) * 1e-5 + kSlimUs[2] * v.waves / 8 + kSlimUs[3] * cuts), i, 1);
         }
         for (int i = 0; i < kTiles; ++i) {
             const Tile& v = kTile[i];
@@ -553,7 +557,7 @@ class LogitsExecutor : public aclOpExecutor {
                 const double cols = over(K / split, 64) * 64, used = over(K, cols), rounds = over(tiles * used, 256);
                 const double turns = over(rounds, perCu), bytes = cols * (v.rows * xSize + v.experts * wSize);
                 const double flops = v.rows * v.experts * cols * products * 2;
-                double us = kTileUs[0] + turns * (kTileUs[same16 ? 1 : 2] * cols / bk + kTileUs[7]) + rounds * (kTileUs[3] * bytes * 1e-5 + kTileUs[4] * flops * 256 / 2.5e9);
+                double us = kTileUs[0] + turns * (kTileUs[same16 ? 1 : 2] * cols / bk + kTileUs[7]) + rounds * (kTileUs[3] * tileBytes * bytes * 1e-5 + kTileUs[4] * flops * 256 / 2.5e9);
                 if (used > 1) us += kTileUs[5] + kTileUs[6] * used * T * E * 4e-6;
                 offer(us, kSlims + i, static_cast<int>(used));
             }
