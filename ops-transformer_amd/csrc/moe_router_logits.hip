@@ -41,8 +41,8 @@ struct Raw {
     uint4 q[sizeof(typename Codec::Storage) / 2];
 };
 
-// They need no alignment but their own, the vector memory instructions take any: 8192 x 7167 x 256 with fp32 weights 104 us, bf16 75 (312 and 368 an element at a
-// time), 64 x 7167 x 256 12.3 and 14.7 (38 and 37), where 7168 columns take 96, 52, 8.2 and 5.5.
+// They need no alignment but their own, the vector memory instructions take any: 8192 x 7167 x 256 with fp32 weights 103 us, bf16 64 (312 and 368 an element at a
+// time), 64 x 7167 x 256 13.5 and 14.7 (38 and 37), where 7168 columns take 98, 52, 8.2 and 5.5.
 template <typename Codec>
 __device__ __forceinline__ Raw<Codec> LoadWhole(const typename Codec::Storage* at) {
     Raw<Codec> r;
