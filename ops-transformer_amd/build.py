@@ -288,10 +288,15 @@ def build_sanitized(jobs=None):
 
 
 def build_binding(force=False):
-    """Compiles the Python module (host code only) against the installed torch's headers.  Returns its path."""
+    """Compiles the Python module (host code only) against the installed torch's headers.  Returns its path, None where there is no torch: callers of
+    the C interface need neither."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        sys.stderr.write("torch is not installed: opapi_torch.so is not built\n")
+        return None
     src = os.path.join(CSRC, "torch_binding.cpp")
     deps = [src, os.path.abspath(__file__), torch.version.__file__] + _headers()
     if not force and os.path.exists(BINDING_PATH) and all(os.path.getmtime(BINDING_PATH) >= os.path.getmtime(d) for d in deps):
