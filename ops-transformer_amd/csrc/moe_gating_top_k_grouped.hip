@@ -541,6 +541,7 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         }
     }
     float low = 0.f, high = top;  // low <= t <= high
+    bool spread = true;           // they have a distance that places can be taken of
     if (biased) {
         float least = b[0], most = b[0];
 #pragma unroll
@@ -551,7 +552,9 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
         }
         low = RowReduce<kLanes>(least, [](float p, float q) { return fminf(p, q); });
         high = top + RowReduce<kLanes>(most, [](float p, float q) { return fmaxf(p, q); });
-        close |= !(high - low < INFINITY);  // a bias of an infinity
+        // not where a bias is an infinity, nor where all are equal and so large that no p shows beside them (16 experts of 2^24)
+        spread = high - low > 0.f && high - low < INFINITY;
+        close |= !spread;
     }
     const float largest = fmaxf(fabsf(low), fabsf(high));
     if (biased || (grouped && a.topTwo != 0)) {
@@ -622,10 +625,10 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs
     uint32_t keys[kPer];
     uint32_t tooClose;  // a difference of two keys
     if (biased) {
-        const float scale = 0x0.ffffp27f / (high - low);
+        const float scale = spread ? 0x0.ffffp27f / (high - low) : 0.f;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) t[i] = fmaf(t[i] - low, scale, 32.f);
-        if (!plain) {
+        if (!plain || !spread) {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) t[i] = __builtin_amdgcn_fmed3f(t[i], 1.f, 0x0.fffffp27f);
         }

@@ -583,6 +583,22 @@ def test_gating_biases_that_mask_experts(aclnn, dev, T, E, low):
                 _check_long(aclnn, dev, x, order[:T], min(8, E // 4), bias=bias, score_type=score_type, **kw)
 
 
+@pytest.mark.parametrize("T", [12, LONG])
+@pytest.mark.parametrize("E", [8, 16, 60, 96, 256, 384, 640])
+def test_gating_biases_that_are_all_equal(aclnn, dev, T, E):
+    """One bias for all, from zero to those beside which no score shows in 32 bits, and every expert masked: the choice is the one in 64 bits, however many
+    rows there are."""
+    x, order = _long_rows(E, E)
+    for value in (0.0, -3.0, 2.0 ** 18, 2.0 ** 24, -2.0 ** 24, 2.0 ** 25, 1e9, -1e9, torch.finfo(torch.float32).max, torch.finfo(torch.float32).min, -float("inf")):
+        bias = torch.full((E,), value)
+        for score_type in (0, 1):
+            for kw in [dict(), dict(k_group=2, group_count=4), dict(k_group=2, group_count=4, group_select_mode=1)]:
+                _check_long(aclnn, dev, x, order[:T], min(8, E // 4), bias=bias, score_type=score_type, **kw)
+    flat = 1e-3 * torch.randn((12, E), generator=torch.Generator().manual_seed(E))   # softmax scores of 1 / E: 2^16 hides them
+    for value in (2.0 ** 14, 2.0 ** 16, -2.0 ** 17):
+        _check_long(aclnn, dev, flat, order[:T], min(8, E // 4), bias=torch.full((E,), value), score_type=0)
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("H", [37, 40])
 def test_elements_behind_2_to_the_31(aclnn, dev, H):
