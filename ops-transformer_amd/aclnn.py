@@ -238,7 +238,7 @@ class _Handles:
 
 
 class Workspace:
-    """A device scratch buffer reused across operator calls; grows to the largest size any call asked for."""
+    """A device scratch buffer reused across operator calls; grows to the largest size any call asked for, and is made anew on another device."""
 
     def __init__(self):
         self.tensor = None
@@ -247,7 +247,9 @@ class Workspace:
     def reserve(self, nbytes, device, api=None):
         if api is not None:
             self.requested[api] = max(self.requested.get(api, 0), int(nbytes))
-        if self.tensor is None or self.tensor.numel() < nbytes:
+        device = torch.device(device)
+        at = None if self.tensor is None else self.tensor.device
+        if at is None or self.tensor.numel() < nbytes or at.type != device.type or device.index not in (None, at.index):
             self.tensor = torch.empty(nbytes, dtype=torch.uint8, device=device)
         return self.tensor
 

@@ -275,3 +275,14 @@ def test_the_module_that_reads_tensors_checks_what_it_is_given(aclnn):
             run(*args)
     with pytest.raises(OverflowError):
         run(function, 0, 0, 0, 0, (1 << 64,), ())
+
+
+def test_a_workspace_follows_the_device(aclnn):
+    """What was reserved on one device is no memory for a call on another one, however large it is."""
+    space = aclnn.Workspace()
+    first = space.reserve(64, torch.device("cpu"))
+    assert space.reserve(16, "cpu") is first and space.reserve(64, first.device) is first
+    moved = space.reserve(16, torch.device("meta"))
+    assert moved.device.type == "meta" and space.tensor is moved
+    assert space.reserve(32, "meta").numel() == 32
+    assert space.reserve(16, "cpu").device.type == "cpu"
