@@ -32,7 +32,8 @@ struct Bf16 {
     __device__ static Storage Store(float f) { return __builtin_bit_cast(uint16_t, static_cast<__bf16>(f)); }
 };
 
-__device__ __forceinline__ float WaveSum(float v) {
+template <typename T>
+__device__ __forceinline__ T WaveSum(T v) {
     for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
     return v;
 }

@@ -150,6 +150,24 @@ def test_norm_rows_of_unusual_values(aclnn, dev, H):
     assert not z.any() and not zs.any() and not zn.any()
 
 
+@pytest.mark.parametrize("dtype_name", ["f32", "bf16"])
+@pytest.mark.parametrize("H", [1 << 20, (1 << 22) + 3])
+def test_norm_of_very_long_rows(aclnn, dev, H, dtype_name):
+    """The error does not grow with the row.  Of squares that are added up in 64 bits the sum's rounding to fp32 is what is left: that, the division by H
+    and the addition of epsilon under the root, 3/2 u; the root, its reciprocal and two products 4 u."""
+    dtype = TORCH[dtype_name]
+    tol = 5.5 * U
+    g = torch.Generator().manual_seed(H)
+    x = (torch.tensor([[0.7], [1.1]]) * (1 + 2.0 ** -10 * torch.rand((2, H), generator=g))).to(dtype)   # nearly equal: roundings of one sign in long runs
+    gamma = (1 + 0.3 * torch.randn(H, generator=g)).to(dtype)
+    y, scale, norm, _ = [t if t is None else t.cpu() for t in aclnn.moe_add_rms_norm_quant(*_on(dev, x, gamma), epsilon=1e-6)]
+    n = x.double() / torch.sqrt(x.double().square().mean(-1, keepdim=True) + 1e-6) * gamma.double()
+    assert torch.all((norm.double() - n).abs() <= (tol + _half(dtype) * (1 + tol)) * n.abs())
+    want = n.abs().amax(-1) / 127
+    assert torch.all((scale.double() - want).abs() <= (tol + U) * want)     # a division more
+    assert torch.all((y.double() - n / want[:, None]).abs() <= 0.5 + 127 * 8 * U)
+
+
 def test_norm_long_batches_and_empty_ones(aclnn, dev):
     x, res, gamma, _ = _norm_inputs(70000, 64, torch.bfloat16, 3)     # more rows than a grid of one dimension had in 16 bits
     _check_norm(x, res, gamma, None, 1e-6, aclnn.moe_add_rms_norm_quant(*_on(dev, x, gamma, res)))
