@@ -37,7 +37,7 @@ struct GatingArgs {
     int32_t packets;          // lanes have all of their experts or none (1), or all of them have (2), and rows start on the lanes' boundaries
     int32_t biasPackets;      // so does the bias
     uint32_t groupMagic;      // (c * groupMagic) >> 21 = c / (experts / groups) for c < 512
-    float factor;
+    double factor;
     double eps;
 };
 
@@ -845,7 +845,7 @@ extern "C" aclnnStatus aclnnMoeGatingTopKGroupedGetWorkspaceSize(
     ex->args.topTwo = static_cast<int32_t>(groupSelectMode);
     ex->args.sigmoid = static_cast<int32_t>(scoreType);
     ex->args.renorm = static_cast<int32_t>(renorm);
-    ex->args.factor = static_cast<float>(routedScalingFactor);
+    ex->args.factor = routedScalingFactor;
     ex->args.eps = eps;
     const int64_t size = experts / groupCount;
     ex->args.groupMagic = static_cast<uint32_t>(((1ll << 21) + size - 1) / size);

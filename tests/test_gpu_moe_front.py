@@ -617,6 +617,17 @@ def test_gating_biases_that_are_all_equal(aclnn, dev, T, E):
         _check_long(aclnn, dev, flat, order[:T], min(8, E // 4), bias=torch.full((E,), value), score_type=0)
 
 
+@pytest.mark.parametrize("T", [12, LONG])
+@pytest.mark.parametrize("E", [16, 640])
+def test_gating_factors_that_only_64_bits_hold(aclnn, dev, T, E):
+    """The factor is a double, and what counts is whether the weights fit: 2^130 passes fp32, times a weight below 1/4 it does not."""
+    g = torch.Generator().manual_seed(E)
+    x, order = 0.01 * torch.randn((12, E), generator=g), torch.randint(0, 12, (T,), generator=g)
+    for factor in (2.0 ** 130, -2.0 ** 130, 0.1, 2.0 ** -160):
+        _check_long(aclnn, dev, x, order, 4, routed_scaling_factor=factor)
+        _check_long(aclnn, dev, x, order, 4, bias=torch.randn(E, generator=g), routed_scaling_factor=factor)
+
+
 # ------------------------------------------------------------------------------------------------ together
 @pytest.mark.parametrize("H", [37, 40])
 def test_elements_behind_2_to_the_31(aclnn, dev, H):
