@@ -13,6 +13,7 @@
 #define OPS_TRANSFORMER_AMD_OPAPI_PROFILE_H_
 
 #include <stddef.h>
+#include <stdint.h>
 
 #ifdef __cplusplus
 extern "C" {
@@ -67,6 +68,14 @@ __attribute__((visibility("default"))) void opapiGemmWorkgroupSpansEnable(int en
  * Returns the number of lines, or -1 on an error.
  */
 __attribute__((visibility("default"))) int opapiGemmWorkgroupSpansReport(char* buf, size_t cap);
+
+/*
+ * What aclnnMoeRouterLogits runs for rows x cols hidden states of type xType (an aclDataType) and experts x cols weights of type weightType: the
+ * number of the kernel's shape (0 to 5 without LDS tiles, 6 to 10 with) and over how many workgroups the columns are split.  The choice
+ * depends on these alone, not on addresses; nothing is launched.  Returns 0, or an aclnn status code for sizes or types that the operator refuses.
+ */
+__attribute__((visibility("default"))) int opapiRouterLogitsPlan(int xType, int weightType, int64_t rows, int64_t cols, int64_t experts,
+                                                                 int* shape, int* splits);
 
 #ifdef __cplusplus
 }

@@ -737,6 +737,20 @@ def moe_ffn_forward(routing, tensors, workspace, device):
         workspace.requested[api] = max(workspace.requested.get(api, 0), nbytes)
 
 
+def router_logits_plan(x_dtype, weight_dtype, rows, cols, experts):
+    """(shape, splits): which kernel moe_router_logits runs for such tensors, and over how many workgroups their columns are split
+    (include/opapi_profile.h)."""
+    l = lib()
+    l.opapiRouterLogitsPlan.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.POINTER(ctypes.c_int),
+                                        ctypes.POINTER(ctypes.c_int)]
+    l.opapiRouterLogitsPlan.restype = ctypes.c_int
+    shape, splits = ctypes.c_int(-1), ctypes.c_int(-1)
+    st = l.opapiRouterLogitsPlan(_DTYPE_CODE[x_dtype], _DTYPE_CODE[weight_dtype], rows, cols, experts, ctypes.byref(shape), ctypes.byref(splits))
+    if st != ACLNN_SUCCESS:
+        raise AclnnError("opapiRouterLogitsPlan", st, last_error())
+    return shape.value, splits.value
+
+
 # ------------------------------------------------------------------------------------------------ kernel timing
 def kernel_timer_enable(enable=True):
     """Turns per-kernel HIP-event timing inside the library on or off (include/opapi_profile.h)."""

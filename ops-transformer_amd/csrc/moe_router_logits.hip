@@ -12,6 +12,7 @@
 #include <cmath>
 
 #include "aclnnop/aclnn_moe_router_logits.h"
+#include "opapi_profile.h"
 
 namespace {
 
@@ -703,4 +704,25 @@ extern "C" aclnnStatus aclnnMoeRouterLogitsGetWorkspaceSize(const aclTensor* x, 
 
 extern "C" aclnnStatus aclnnMoeRouterLogits(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream) {
     return opapi::RunAndRelease(workspace, workspaceSize, executor, stream);
+}
+
+extern "C" int opapiRouterLogitsPlan(int xType, int weightType, int64_t rows, int64_t cols, int64_t experts, int* shape, int* splits) {
+    using namespace opapi;
+    ClearError();
+    OPAPI_CHECK(shape != nullptr && splits != nullptr, ACLNN_ERR_PARAM_NULLPTR, "shape or splits is null");
+    const auto floating = [](int type) { return type == ACL_FLOAT || type == ACL_FLOAT16 || type == ACL_BF16; };
+    OPAPI_CHECK(floating(xType) && (weightType == xType || weightType == ACL_FLOAT), ACLNN_ERR_PARAM_INVALID,
+                "x must be FLOAT, FLOAT16 or BF16, weight of x's type or FLOAT");
+    OPAPI_CHECK(rows > 0 && rows <= kMaxRows && cols > 0 && cols <= 2147483647ll && experts > 0 && experts <= kMaxExperts, ACLNN_ERR_PARAM_INVALID,
+                "rows, cols or experts are out of range");
+    LogitsExecutor ex;
+    ex.dtype = static_cast<aclDataType>(xType);
+    ex.weightType = static_cast<aclDataType>(weightType);
+    ex.args.rows = rows;
+    ex.args.cols = cols;
+    ex.args.experts = static_cast<int32_t>(experts);
+    ex.Plan();
+    *shape = ex.kernel;
+    *splits = ex.splits;
+    return ACLNN_SUCCESS;
 }

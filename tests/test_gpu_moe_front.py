@@ -13,6 +13,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_moe_front import ROUTER_SIZES
+
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
@@ -242,6 +244,22 @@ def test_logits_of_few_columns(aclnn, dev, xt, wt, T, K):
     w[::3] = torch.sign(w[::3]) * (1 + 2.0 ** -7 - 2.0 ** -16 - 2.0 ** -22)
     x, w = x.to(TORCH[xt]), w.to(TORCH[wt])
     _check_logits(x, w, aclnn.moe_router_logits(*_on(dev, x, w)))
+
+
+@pytest.mark.parametrize("T,K,E", ROUTER_SIZES)
+def test_logits_of_every_kernel(aclnn, dev, T, K, E):
+    """Every shape there is, as planned and, with rows and weights an element further on, by the kernel for those off the 16-byte grid."""
+    g = torch.Generator().manual_seed(T + K + E)
+    x, w = torch.randn((T, K), generator=g), torch.randn((E, K), generator=g) / K ** 0.5
+    for xt, wt in TYPES:
+        xs, ws = x.to(TORCH[xt]), w.to(TORCH[wt])
+        room = torch.full((T * E + 4096,), 7.0, device=dev)
+        _check_logits(xs, ws, aclnn.moe_router_logits(*_on(dev, xs, ws), out=room[:T * E].view(T, E)))
+        assert torch.all(room[T * E:] == 7.0)
+        if K * xs.element_size() % 16 == 0 and K * ws.element_size() % 16 == 0:
+            odd = [torch.zeros(t.numel() + 1, dtype=t.dtype, device=dev)[1:].view(t.shape) for t in (xs, ws)]
+            _check_logits(xs, ws, aclnn.moe_router_logits(odd[0].copy_(xs), odd[1].copy_(ws), out=room[:T * E].view(T, E)))
+            assert torch.all(room[T * E:] == 7.0)
 
 
 def test_logits_strides_offsets_and_extents(aclnn, dev):

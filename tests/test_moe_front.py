@@ -1,6 +1,8 @@
 """What the operators in front of the expert FFN refuse, and what they ask for, without a GPU: aclnnMoeAddRmsNormQuant,
 aclnnMoeRouterLogits, aclnnMoeGatingTopKGrouped.  First phases never touch device memory, so fake addresses suffice."""
 import ctypes
+import math
+import random
 import struct
 
 import pytest
@@ -286,3 +288,56 @@ def test_a_workspace_follows_the_device(aclnn):
     assert moved.device.type == "meta" and space.tensor is moved
     assert space.reserve(32, "meta").numel() == 32
     assert space.reserve(16, "cpu").device.type == "cpu"
+
+
+# ------------------------------------------------------------------------------------------------ which kernel a router product takes
+ROUTER_DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+ROUTER_TYPES = [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32"), ("f32", "f32")]
+ROUTER_SHAPES = 11        # 0 to 5 without LDS tiles, 6 to 10 with; 9 and 10 take rows of one part only
+
+# Rows, columns and experts that between them take every kernel there is, with the columns split and whole.  Which size takes which goes by fitted costs:
+# the tests below fail when a change of theirs leaves a kernel out, and the sizes are then chosen again.
+ROUTER_SIZES = [(1, 130, 1), (1, 134, 2524), (1, 136, 1), (1, 136, 2127), (1, 162, 1069), (1, 184, 1033), (3, 130, 171), (3, 136, 173), (3, 24259, 505),
+                (7, 22789, 131), (9, 30808, 359), (10, 26456, 77), (12, 135, 1032), (17, 7216, 2739), (20, 552, 209), (25, 152, 569), (28, 438, 154),
+                (41, 17808, 432), (43, 22197, 12), (1195, 14928, 10), (2018, 503, 517), (2181, 4561, 1), (2336, 544, 3205), (2879, 820, 2724), (3286, 518, 1179),
+                (5725, 512, 141), (8440, 3497, 68), (11041, 544, 272), (11180, 504, 332), (11429, 507, 133), (11753, 3536, 66), (11783, 504, 138),
+                (11928, 512, 593), (12326, 530, 530), (13226, 519, 274)]
+
+
+def _router_kernel(aclnn, xt, wt, rows, cols, experts):
+    """(types, shape, whether rows and weights lie on 16 bytes, whether columns are split)."""
+    x, w = ROUTER_DTYPES[xt], ROUTER_DTYPES[wt]
+    shape, splits = aclnn.router_logits_plan(x, w, rows, cols, experts)
+    return xt, wt, shape, cols * x.itemsize % 16 == 0 and cols * w.itemsize % 16 == 0, splits > 1
+
+
+def test_the_router_sizes_take_every_kernel(aclnn):
+    ran = {_router_kernel(aclnn, xt, wt, *size)[:4] for size in ROUTER_SIZES for xt, wt in ROUTER_TYPES}
+    there = {(xt, wt, shape, grid) for xt, wt in ROUTER_TYPES for shape in range(ROUTER_SHAPES) for grid in (False, True)
+             if shape < 9 or xt == "bf16" or (xt, wt) == ("f16", "f16")}
+    assert ran == there
+
+
+def test_the_router_sizes_take_what_other_sizes_take(aclnn):
+    ran = {_router_kernel(aclnn, xt, wt, *size) for size in ROUTER_SIZES for xt, wt in ROUTER_TYPES}
+    rng = random.Random(11)
+    spread = lambda least, most: int(round(math.exp(rng.uniform(math.log(least), math.log(most)))))
+    for _ in range(20000):
+        size = [spread(1, 16384), spread(1, 32768), spread(1, 4096 if rng.random() < 0.1 else 512)]
+        if rng.random() < 0.5:
+            size[1] = max(8, size[1] // 8 * 8)
+        kernel = _router_kernel(aclnn, *rng.choice(ROUTER_TYPES), *size)
+        assert kernel in ran, (size, kernel)
+
+
+def test_router_plan_refuses_what_the_operator_refuses(aclnn):
+    f32, f16, bf16 = torch.float32, torch.float16, torch.bfloat16
+    for args, fragment in [((torch.int8, f32, 1, 1, 1), "x must be"), ((f16, bf16, 1, 1, 1), "weight of x's type"), ((f32, f16, 1, 1, 1), "weight of x's type"),
+                           ((f32, f32, 0, 1, 1), "out of range"), ((f32, f32, (1 << 26) + 1, 1, 1), "out of range"), ((f32, f32, 1, 0, 1), "out of range"),
+                           ((f32, f32, 1, 1 << 31, 1), "out of range"), ((f32, f32, 1, 1, 4097), "out of range")]:
+        with pytest.raises(aclnn.AclnnError, match=fragment) as e:
+            aclnn.router_logits_plan(*args)
+        assert e.value.code == INVALID
+    null = ctypes.POINTER(ctypes.c_int)()
+    assert aclnn.lib().opapiRouterLogitsPlan(F32, F32, 1, 1, 1, null, null) == NULLPTR
+    assert aclnn.router_logits_plan(f32, f32, 1, 1, 1)[1] == 1
