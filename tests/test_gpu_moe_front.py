@@ -775,3 +775,31 @@ def test_calls_at_once_on_two_streams(aclnn, dev):
     for i in range(2):
         for t in got[i]:
             assert torch.equal(t, want[i])
+
+
+@pytest.mark.parametrize("kept", [False, True])
+def test_split_products_at_once_on_two_streams(aclnn, dev, kept):
+    """Products whose columns are split over workgroups, and so need room for their parts, side by side: each call has room of its own, or each stream has
+    (kept)."""
+    T, K, E = 600, 7168, 256
+    assert aclnn.router_logits_plan(torch.bfloat16, torch.float32, T, K, E)[1] > 1
+    g = torch.Generator().manual_seed(9)
+    w = (torch.randn((E, K), generator=g) / K ** 0.5).to(dev)
+    xs = [torch.randn((T, K), generator=g).bfloat16().to(dev) for _ in range(2)]
+    spaces = [aclnn.Workspace() for _ in xs]
+    want = [aclnn.moe_router_logits(x, w, workspace=space) for x, space in zip(xs, spaces)]
+    for x, space, t in zip(xs, spaces, want):
+        assert space.requested["aclnnMoeRouterLogits"] >= 2 * T * E * 4
+        _check_logits(x.cpu(), w.cpu(), t)
+    assert spaces[0].tensor.data_ptr() != spaces[1].tensor.data_ptr()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in xs]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(aclnn.moe_router_logits(xs[i], w, workspace=spaces[i] if kept else None))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for t in got[i]:
+            assert torch.equal(t, want[i])
