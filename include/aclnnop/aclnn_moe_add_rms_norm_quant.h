@@ -8,6 +8,7 @@
  *   s = x + residual, rounded to x's type (s = x without a residual)                              -> sumOutOptional
  *   n = s * (1 / sqrt(mean(s^2) + epsilon)) * gamma, in fp32                                       -> normOutOptional (rounded)
  *   v = n * smoothScale;  scale = max|v| / 127;  y = round_half_even(v / scale) in [-127, 127]     -> yOut, scaleOut
+ *   (v / scale is 127 w / max|w| of w = s * gamma * smoothScale: y is the nearest whole number to that of the fp32 products w)
  * A row with scale 0 (zeros, squares whose sum passes fp32 or, with epsilon 0, is lost in it) gives zeros; one with a NaN or an infinity gives scale NaN and zeros in y.
  *
  * x, residualOptional, sumOutOptional, normOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents, at most 2^26 rows;

@@ -33,8 +33,9 @@ struct NormArgs {
 struct RowScales {
     float r;      // of the norm
     float scale;  // of the int8 row
-    float up;     // w is taken times `up` before `inv`, so that 127 / max|w| stays finite for rows of tiny values
-    float inv;    // 0 where the row's int8 values are zeros
+    float up;     // w is taken times `up`, so that the quotient below stays a normal number in both parts for rows of tiny and of huge values
+    float inv;    // 127 / (max|w| up), and what is left of it behind its rounding; 0 where the row's int8 values are zeros
+    float rest;
 };
 
 // sumSquares and maxBits (the bits of max|w|, whose order as unsigned numbers is that of the values, NaN last) are the row's.
@@ -44,13 +45,18 @@ __device__ __forceinline__ RowScales ScalesOf(float sumSquares, uint32_t maxBits
     s.r = mean == 0.f ? 0.f : 1.f / sqrtf(mean);
     const float m = __uint_as_float(maxBits);
     s.scale = m * s.r / 127.f;
-    s.up = m < 0x1p-100f ? 0x1p100f : 1.f;
+    s.up = m < 0x1p-100f ? 0x1p100f : m > 0x1p100f ? 0x1p-100f : 1.f;
     s.inv = s.scale > 0.f && s.scale < INFINITY ? 127.f / (m * s.up) : 0.f;
+    s.rest = fmaf(-s.inv, m * s.up, 127.f) * s.inv * (1.f / 127.f);
     return s;
 }
 
+// 127 w / max to the nearest whole number, half to even.  The factor has twice fp32's bits: a value in the middle between two whole numbers, as one in
+// 25 000 of 16-bit rows is, is seen to be there (rounded to fp32 the factor took one in six of those to the odd number).  No |w| passes the maximum, so
+// nothing passes 127.
 __device__ __forceinline__ int32_t Quantised(float w, const RowScales& s) {
-    return s.inv == 0.f ? 0 : static_cast<int32_t>(fminf(fmaxf(rintf(w * s.up * s.inv), -127.f), 127.f));
+    const float v = w * s.up;
+    return s.inv == 0.f ? 0 : static_cast<int32_t>(rintf(fmaf(v, s.inv, v * s.rest)));
 }
 
 template <int kWaves>

@@ -170,6 +170,22 @@ def test_norm_of_very_long_rows(aclnn, dev, H, dtype_name):
     assert torch.all((y.double() - n / want[:, None]).abs() <= 0.5 + 127 * 8 * U)
 
 
+@pytest.mark.parametrize("dtype_name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H", [1000, 1001, 4096, 20001])
+def test_norm_values_in_the_middle_go_to_the_even_step(aclnn, dev, H, dtype_name):
+    """Rows of whole numbers up to 254 times one gamma: 127 w / max w is half the number whatever gamma is, and every odd one lies in the middle."""
+    dtype = TORCH[dtype_name]
+    g = torch.Generator().manual_seed(H)
+    s = torch.randint(-253, 254, (34, H), generator=g)
+    s[:, 0] = torch.where(torch.arange(34) % 2 == 0, 254, -254)
+    s[:, -1] = -s[:, 0]
+    want = torch.round(s.double() / 2).to(torch.int8)                      # half to even
+    x = (s.double() * torch.exp2(torch.arange(34) % 17 - 10.0)[:, None]).to(dtype)
+    for value in (7, 13, 51, 253, 201):
+        y, _, _, _ = aclnn.moe_add_rms_norm_quant(*_on(dev, x, torch.full((H,), float(value), dtype=dtype)))
+        assert torch.equal(y.cpu(), want)
+
+
 def test_norm_long_batches_and_empty_ones(aclnn, dev):
     x, res, gamma, _ = _norm_inputs(70000, 64, torch.bfloat16, 3)     # more rows than a grid of one dimension had in 16 bits
     _check_norm(x, res, gamma, None, 1e-6, aclnn.moe_add_rms_norm_quant(*_on(dev, x, gamma, res)))
