@@ -288,8 +288,9 @@ def build_sanitized(jobs=None):
 
 
 def build_binding(force=False):
-    """Compiles the Python module (host code only) against the installed torch's headers.  Returns its path, None where there is no torch: callers of
-    the C interface need neither."""
+    """Compiles the Python module (host code only) against the installed torch's headers.  Returns its path, None where there is no torch, no g++ or
+    no Python headers: callers of the C interface need none of them, and the operators that the module serves say that it is missing."""
+    import shutil
     import sysconfig
 
     try:
@@ -297,6 +298,10 @@ def build_binding(force=False):
     except ImportError:
         sys.stderr.write("torch is not installed: opapi_torch.so is not built\n")
         return None
+    for there, what in [(shutil.which("g++"), "g++"), (os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")), "Python.h")]:
+        if not there:
+            sys.stderr.write("%s is not installed: opapi_torch.so is not built\n" % what)
+            return None
     src = os.path.join(CSRC, "torch_binding.cpp")
     deps = [src, os.path.abspath(__file__), torch.version.__file__] + _headers()
     if not force and os.path.exists(BINDING_PATH) and all(os.path.getmtime(BINDING_PATH) >= os.path.getmtime(d) for d in deps):
@@ -319,12 +324,11 @@ def build(force=False, jobs=None):
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as pool:
         binding = pool.submit(build_binding, force)
         results = list(pool.map(lambda s: _compile(s, force), SOURCES))
-        binding.result()
     objs = [o for o, _ in results]
-    rebuilt = any(r for _, r in results)
-    if rebuilt or not os.path.exists(LIB_PATH) or os.path.getmtime(LIB_PATH) < os.path.getmtime(EXPORTS):
+    if any(r for _, r in results) or not os.path.exists(LIB_PATH) or any(os.path.getmtime(LIB_PATH) < os.path.getmtime(f) for f in objs + [EXPORTS]):
         cmd = [HIPCC, "-shared", "-fPIC", "--offload-arch=gfx950", "-Wl,--version-script=" + EXPORTS, "-o", LIB_PATH] + objs
         subprocess.check_call(cmd)
+    binding.result()  # the library does not wait for it
     return LIB_PATH
 
 

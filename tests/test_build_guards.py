@@ -144,3 +144,63 @@ def test_barrier_guard_refuses_a_wait_for_all_requests_among_products(build, tmp
 def test_barrier_guard_accepts_a_wait_for_all_requests_elsewhere(build, tmp_path):
     for kept in ("\ts_endpgm", ".LBB0_1:"):  # behind the loop and in front of it
         assert build.check_ring_barrier_waits(_write(tmp_path, BARRIER_GOOD.replace(kept, "\ts_waitcnt vmcnt(0)\n" + kept))) == 1
+
+
+def _build_without_compiling(build, monkeypatch, tmp_path):
+    """build.build() on empty objects; returns the commands it starts."""
+    def compiled(src, force):
+        obj = tmp_path / (src + ".o")
+        obj.write_text("")
+        return str(obj), False
+
+    commands = []
+
+    def call(cmd, **_):
+        commands.append(cmd)
+        open(cmd[cmd.index("-o") + 1], "w").close()
+
+    monkeypatch.setattr(build, "check_compiler", lambda: "")
+    monkeypatch.setattr(build, "_compile", compiled)
+    monkeypatch.setattr(build, "LIB_PATH", str(tmp_path / "libcust_opapi.so"))
+    monkeypatch.setattr(build, "BINDING_PATH", str(tmp_path / "opapi_torch.so"))
+    monkeypatch.setattr(build.subprocess, "check_call", call)
+    return commands
+
+
+def test_the_library_is_linked_where_the_python_module_cannot_be_built(build, monkeypatch, tmp_path):
+    commands = _build_without_compiling(build, monkeypatch, tmp_path)
+    monkeypatch.setattr(build, "build_binding", lambda force=False: (_ for _ in ()).throw(OSError("no module")))
+    with pytest.raises(OSError, match="no module"):
+        build.build()
+    assert [c[0] for c in commands] == [build.HIPCC] and os.path.exists(build.LIB_PATH)
+
+
+@pytest.mark.parametrize("missing", ["g++", "Python.h"])
+def test_without_its_tools_the_python_module_is_left_out(build, monkeypatch, tmp_path, capsys, missing):
+    import shutil
+    import sysconfig
+    commands = _build_without_compiling(build, monkeypatch, tmp_path)
+    if missing == "g++":
+        monkeypatch.setattr(shutil, "which", lambda name: None)
+    else:
+        monkeypatch.setattr(sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    assert build.build() == build.LIB_PATH
+    assert [c[0] for c in commands] == [build.HIPCC] and missing + " is not installed" in capsys.readouterr().err
+
+
+def test_objects_newer_than_the_library_are_linked(build, monkeypatch, tmp_path):
+    """A build that ended between compiling and linking is made up for by the next one."""
+    commands = _build_without_compiling(build, monkeypatch, tmp_path)
+    monkeypatch.setattr(build, "build_binding", lambda force=False: None)
+    open(build.LIB_PATH, "w").close()
+    os.utime(build.LIB_PATH, (1, 1))
+    monkeypatch.setattr(build, "EXPORTS", str(tmp_path / "exports.map"))
+    open(build.EXPORTS, "w").close()
+    os.utime(build.EXPORTS, (1, 1))
+    build.build()
+    assert len(commands) == 1
+    for obj in tmp_path.glob("*.o"):
+        os.utime(obj, (1, 1))
+    monkeypatch.setattr(build, "_compile", lambda src, force: (str(tmp_path / (src + ".o")), False))
+    build.build()
+    assert len(commands) == 1
