@@ -27,7 +27,7 @@ struct LogitsArgs {
     float* logits;    // [splits, rows, experts] where the columns are split, the operator's output otherwise
     int64_t rows;
     int64_t cols;
-    int64_t splitCols;  // columns of a split (blockIdx.z)
+    int64_t splitCols;  // columns of a split
     int32_t experts;
 };
 
@@ -201,7 +201,7 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
     const int tilesN = (a.experts + kLines * kN - 1) / (kLines * kN);
     const int64_t row0 = static_cast<int64_t>(blockIdx.x / tilesN) * (kLines * kM);
     const int expert0 = static_cast<int>(blockIdx.x % tilesN) * (kLines * kN);
-    const int64_t begin = 0, end = a.cols;
+    const int64_t end = a.cols;
     const typename X::Storage* x[kM];
     const typename W::Storage* w[kN];
 #pragma unroll
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
     };
     using One = std::integral_constant<int, 1>;
     using Depth = std::integral_constant<int, kDepth>;
-    int64_t base = begin + wave * (kSub * 32);
+    int64_t base = wave * (kSub * 32);
     if constexpr (kAligned) {
         for (; base < end; base += kDepth * kRound) pass(base, Depth{}, std::false_type{});
     } else {
@@ -275,7 +275,6 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
     }
     __syncthreads();
     const float* const all = reinterpret_cast<const float*>(sums);
-    float* const out = a.logits;
     for (int i = threadIdx.x; i < kLines * kM * kLines * kN; i += kWave * kWaves) {
         const int r = i / (kLines * kN), e = i % (kLines * kN);
         const int64_t row = row0 + r;
@@ -289,7 +288,7 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
                 sum += all[((v * kM * kN + tile) * kWave + i16 / 4 * 16 + j16) * 4 + i16 % 4];
             }
         }
-        if (row < a.rows && expert < a.experts) out[row * a.experts + expert] = sum;
+        if (row < a.rows && expert < a.experts) a.logits[row * a.experts + expert] = sum;
     }
 }
 
@@ -514,7 +513,8 @@ class LogitsExecutor : public aclOpExecutor {
     LogitsArgs args{};
     aclDataType dtype = ACL_FLOAT;
     aclDataType weightType = ACL_FLOAT;
-    // The plan, made from sizes and types alone.
+    // The plan, made from sizes and types alone: the workspace that is asked for does not hang on addresses.  Tensors whose extents are on the 16-byte grid and
+    // whose addresses are not run the shape chosen for the grid, by its kernel for rows off it.
     int kernel = 0;  // of kSlim, then of kTile
     int splits = 1;
 
