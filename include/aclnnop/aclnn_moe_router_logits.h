@@ -5,6 +5,7 @@
  *
  *   logitsOut[..., e] = sum over h of x[..., h] * weight[e, h], products and sums in fp32
  * Router weights are often kept in 32 bits next to 16-bit hidden states: neither side is rounded to fewer bits than it has.
+ * (Where x is FLOAT or FLOAT16 next to FLOAT weights both are sums of bf16 parts, and products of parts that are left out come to at most 2^-23 of |x w|.)
  * Results are the same bits on every launch.  A row with a NaN or an infinity gives NaN or infinities; so does, where x is FLOAT or
  * FLOAT16 next to FLOAT weights, a FLOAT value of 2^128 (1 - 2^-9) or more.
  *

@@ -82,7 +82,8 @@ __device__ __forceinline__ void ReduceRow(double& sumSquares, uint32_t& maxBits)
 
 // Rows of any length: a workgroup per row, one element at a time, the row read again for the outputs (from the sum where that
 // was written, by the same lane: it may lie in x's memory).  A lane adds up a 256th of the row, one square behind the other: in 64 bits, since
-// in 32 the error grows with the row (2^22 equal values: 1800 units of 2^-24 in the sum, which is 1 / 18000 of the norm).
+// in 32 the error grows with the row (2^22 equal values: 1800 units of 2^-24 in the sum, which is 1 / 18000 of the norm).  An element at a time twice
+// is what bounds it: 4096 x 16392 bf16 271 us, where 16384 columns take 125 in packets; a single row has one CU to itself (65536 columns 143).
 constexpr int kAnyThreads = 256;
 
 template <typename Codec, typename Gamma>
@@ -119,12 +120,12 @@ __global__ __launch_bounds__(kAnyThreads) void NormQuantAnyKernel(NormArgs a) {
 
 // Rows in pieces of eight elements, up to kPackets of them per lane, read once and kept in registers from the reduction to the
 // outputs.  A workgroup takes every gridDim.x-th row: gamma and smooth stay with it, and the next row is asked for before the present one is
-// reduced.  What bounds it is HBM: 8192 x 7168 bf16 with a residual, all outputs, 97 to 100 us at 5.3 TB/s and more, where a plain copy of 1 GiB reaches 5.2 (the
-// kernel that reads rows twice, an element at a time: 350 us); one row of 4096 3.6 us, a launch and one round trip.  As few packets a lane as
-// 512 threads allow: the same row on one, two and four takes 3.6, 3.9 and 5.2 us, 4096 x 4096 fp32 55, 56 and 60.  Workgroups: 4096 at most, for the
+// reduced.  What bounds it is HBM: 8192 x 7168 bf16 with a residual, all outputs, 94 us alone, 96 to 99 in a row of calls: 5.3 to 5.6 TB/s, with what the
+// memory-side cache still holds (a copy of 1 GiB moves 5.2; the kernel that reads rows twice, an element at a time: 350 us); one row of 4096 3.4 us, a launch and one round trip.  As few packets a lane as
+// 512 threads allow: on two and four the same row takes 0.3 and 1.6 us longer, 4096 x 4096 fp32 (54 us) 1 and 5.  Workgroups: 4096 at most, for the
 // widest rows 100 us against 103 to 104 for 512 to 2048; narrow rows 2048 (16384 x 1024: 31.5 us, with 4096 33.3, with 1024 37.8).
 // Off the 16-byte grid (kGrid false) pieces are read and written where they lie, which the vector memory instructions do at any address, and a row's last
-// one by its elements: 8192 x 7167 bf16 174 us (246 twice and an element at a time), 64 x 7167 6.7 (19).  Pieces on the grid whose first and last are another
+// one by its elements: 8192 x 7167 bf16 172 us (246 twice and an element at a time), 64 x 7167 6.5 (19).  Pieces on the grid whose first and last are another
 // row's in part: 148 to 157, but rows of 3001 42 instead of 33.
 constexpr int kMaxPacketThreads = 512;
 constexpr int kMaxPackets = 4;

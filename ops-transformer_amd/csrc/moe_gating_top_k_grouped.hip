@@ -317,7 +317,7 @@ __device__ __forceinline__ void WritePicks(const GatingArgs& a, int64_t row, int
 // expert, the wave's own, for groups whose experts are not those of whole lanes and for the logits of the picks.  What bounds it is latency: a pick is a
 // maximum over four rotations inside a row of sixteen lanes, four lane reads and a ballot (256 experts, 8 picks: 4.7 us, with sigmoid, bias and groups
 // 5.8; with the keys in LDS and the arg-max over twelve shuffles 10.9 and 15.8), a value's exponential in 64 bits a chain of fifty instructions
-// (301 x 160, softmax with the scores 6.1 us; with a branch for each value 7.3).
+// (301 x 160, softmax, with and without the scores 6.0 and 5.9 us; with a branch for each value 7.3).
 template <typename Codec, typename Out, int kPer>
 __device__ __forceinline__ void WaveRow(const GatingArgs& a, int64_t row, int lane, uint64_t* lds, bool writeScores) {
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
@@ -459,7 +459,8 @@ __global__ __launch_bounds__(kWave * kRowWaves) void GatingWaveKernel(GatingArgs
 // What bounds it is the number of instructions: 16384 x 256, sigmoid, bias, 4 of 8 groups, 8 picks 15.6 us (16.8 MB of logits are 3.3), of which a row that
 // is made twice is 3: 980 vector instructions a wave, near half of them in the nine rounds of picking, and a wave waits for 39 % of its time;
 // softmax without bias or groups, bf16 8.4.  Rows without an infinity or a NaN are spared what those need: 16.0 and 9.0 without.  Rows that end
-// between two lanes are read in packets too: 384 experts, bf16, sigmoid, bias 18.4 us, an element at a time 36.
+// between two lanes are read in packets too: 384 experts, bf16, sigmoid, bias 18.6 us, an element at a time 36.  A bias of -inf or the lowest value, on
+// one expert or on many, leaves the others' places no bits: every row is made again then, 40 to 45 us in place of 15.6 (by 64 lanes alone 27).
 template <typename Codec, typename Out, int kPer>
 __global__ __launch_bounds__(kWave * kRowWaves) void GatingQuadKernel(GatingArgs a) {
     constexpr int kLanes = 16, kBits = kPer == 1 ? 0 : kPer == 2 ? 1 : kPer == 4 ? 2 : kPer == 8 ? 3 : kPer == 16 ? 4 : 5;
@@ -720,8 +721,8 @@ class GatingExecutor : public aclOpExecutor {
     void Launch(hipStream_t stream) const {
         const int E = args.experts;
         // Sixteen lanes a row make more rows at a time and take longer for one, most of all with a bias, where one row in a thousand is
-        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 7.9 and 6.9 at 1024 rows, 8.8 and 10.1 at 4096, 15.6 and
-        // 27.5 at 16384; softmax without a bias 5.2 and 5.3, 5.0 and 8.0, 8.4 and 20.7.
+        // made twice.  us by sixteen and by 64 lanes: 256 experts, sigmoid, bias, 4 of 8 groups 9.6 and 6.6 at 1024 rows, 9.7 and 9.9 at 4096, 15.0 and
+        // 27.0 at 16384; softmax without a bias 4.9 and 5.3, 5.0 and 7.9, 8.3 and 20.6.
         const bool many = args.rows > (args.bias != nullptr ? 4000 : 1024);
         if (many && E <= 512 && args.k <= 16 && args.groups <= 16) {
             if (E <= 16) LaunchQuads<Codec, Out, 1>(stream);

@@ -42,8 +42,8 @@ struct Raw {
     uint4 q[sizeof(typename Codec::Storage) / 2];
 };
 
-// They need no alignment but their own, the vector memory instructions take any: 8192 x 7167 x 256 with fp32 weights 103 us, bf16 64 (312 and 368 an element at a
-// time), 64 x 7167 x 256 13.5 and 14.7 (38 and 37), where 7168 columns take 98, 52, 8.2 and 5.5.
+// They need no alignment but their own, the vector memory instructions take any: 8192 x 7167 x 256 with fp32 weights 102 us, bf16 64 (312 and 368 an element at a
+// time), 64 x 7167 x 256 13.0 and 14.7 (38 and 37), where 7168 columns take 93, 54, 8.2 and 5.5.
 template <typename Codec>
 __device__ __forceinline__ Raw<Codec> LoadWhole(const typename Codec::Storage* at) {
     Raw<Codec> r;
@@ -186,8 +186,8 @@ __device__ __forceinline__ F32x16 Multiply(const uint4& a, const uint4& b, F32x1
 // kM x kN tiles of 16 rows and 16 experts.  With kSub > 1 (kM = kN = 1) the sixteen lines of either operand are 16 / kSub rows or experts times kSub
 // neighbouring runs of 32 columns: the products of a run with itself, one in kSub, are what is added up, and a workgroup streams fewer experts' weights.
 // What bounds it: one round trip to memory and the launch for a row (1 x 4096 x 128, bf16 2.9 us), the time a CU takes to bring in its share for a decode step
-// (64 x 7168 x 256, fp32 weights 8.3: 256 workgroups of 350 KB, of which the L2 serves all but 14.4 MB), memory for prompts of few experts
-// (16384 x 4096 x 8 22 to 25 us, 5.4 TB/s and more: a copy's rate).
+// (64 x 7168 x 256, fp32 weights 8.2, fp16 and fp32 rows on them 10.0 and 11.4: 256 workgroups of 350 KB, of which the L2 serves all but 14.4 MB; that is the
+// shape's doing, whose workgroups take all columns), memory for prompts of few experts (16384 x 4096 x 8 22 us alone, 26 in a row of calls: a copy's rate).
 template <typename S, int kM, int kN, int kSub, int kWaves, bool kAligned>
 __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsArgs a) {
     using X = typename S::XType;
@@ -296,10 +296,11 @@ __global__ __launch_bounds__(kWave * kWaves) void RouterLogitsSlimKernel(LogitsA
 // deep.  Rows are cut into parts on the way in, since every wave of a line reads them; weights of fp32 stay whole and are cut by the one wave (kWavesM of
 // them) that has those experts: four bytes of theirs are moved in place of six.  Lines in LDS are 16 bytes longer than their columns, so that eight
 // lanes of a fragment read meet eight different sets of banks.
-// What bounds it: 8192 x 7168 x 256, fp32 weights 84 us and 7 for adding the splits up; 64 are the three parts' products at the rate of a large matrix product
+// What bounds it: 8192 x 7168 x 256, fp32 weights 85 us and 7 for adding the splits up; 64 are the three parts' products at the rate of a large matrix product
 // (1409 TFLOP/s).  The matrix instructions are under way for 59 % of the time that CUs work, cutting weights into parts takes another 45 % of the vector
-// unit's, at 1.7 GHz.  With bf16 weights 43 and 7: instructions 34 %, then what a CU brings in, 41 GB/s.  Products a fragment ahead
-// and 64 columns a step took 600 x 7168 x 256 from 22.7 to 20.9 us, 16384 x 2880 x 60 from 38.7 to 34.0, 8192 x 7168 x 256, bf16 from 52 to 50.
+// unit's, at 1.7 GHz.  fp16 and fp32 rows on fp32 weights 136 and 169 us, 107 and 128 of them five and six parts' products.  With bf16 weights
+// 48 in 128 x 256 tiles and four splits, for which the costs below take 128 x 128 in two (53 to 56); 25 are the bytes.  Products a fragment ahead and 64 columns
+// a step took 600 x 7168 x 256 from 22.7 to 20.0 us, 16384 x 2880 x 60 from 38.7 to 28.4.
 constexpr int kTileThreads = 512;
 
 template <typename S, int kWavesM, int kWavesN, int kMt>
@@ -489,10 +490,10 @@ __global__ __launch_bounds__(kAddThreads) void AddSplitsKernel(const float* part
 }
 
 // What there is to choose from, in the order of LaunchPlan, and what a call is taken to cost: fitted to 320 000 measurements of 50 900 calls over the operator's
-// range (1 to 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types).  Nine in ten are between 0.76 and 1.17 of the fit; the choice by it costs
-// 1.8 % more than the best shape in the mean, 7 % in one call of ten (columns off the 16-byte grid 1.4 %, odd ones of 16 bits 2.8 %, and without their own
-// weights 1.8 and 6.5).  A shape each kind of call needs: without the slim kernels decode takes up to twice as
-// long (64 x 7168 x 256: 12.7 against 8.4 us, one row 7.4 against 2.9), without the tiles a prompt does (8192 x 7168 x 256, fp32 weights: 333 against 97 us).
+// range (1 to 16384 rows, 4 to 512 experts, 512 to 8192 columns, all types).  In nine of ten the fit is 0.77 to 1.18 of what was measured; the choice by it costs
+// 1.8 % more than the best shape in the mean, 7 % in one call of ten, 50 % at worst (columns off the 16-byte grid 1.4 % in the mean, odd ones of 16 bits 2.8).
+// A shape each kind of call needs: without the slim kernels decode takes longer (64 x 7168 x 256, fp32 weights: 12.3 against 8.3 us, one row 10.8 against
+// 3.5), without the tiles a prompt does (8192 x 7168 x 256, fp32 weights: 332 against 94 us).
 struct Slim {
     int m, n, sub, waves;
 };
