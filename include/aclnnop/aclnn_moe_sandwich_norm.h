@@ -1,0 +1,43 @@
+/*
+ * aclnnMoeSandwichNorm — what closes a block and opens the next one, in one pass over its rows: the norm behind the block, its gate, the scales of residual
+ * and branch, the addition, the next block's norm and its int8 rows.
+ * An operator of this library beside aclnnMoeAddRmsNormQuant, which has the addition, one norm and the int8 rows.
+ *
+ * Per row of H values, in fp32:
+ *   u = x * (1 / sqrt(mean(x^2) + epsilon)) * postGamma  (x without postGamma);  the factor 1 / sqrt(...)      -> postRstdOutOptional
+ *   g = gate (gateType 0) or sigmoid(gate) (gateType 1); 1 without a gate
+ *   s = residualScale * residual + branchScale * (g * u), rounded to x's type                                   -> sumOut
+ *   n = s * (1 / sqrt(mean(s^2) + epsilon)) * preGamma                                                          -> normOutOptional (rounded)
+ *   the factor 1 / sqrt(...)                                                                                    -> preRstdOutOptional
+ *   v = n * smoothScale;  scale = max|v| / 127;  y = round_half_even(v / scale) in [-127, 127]                  -> yOutOptional, scaleOutOptional
+ * Rows of zeros, of a NaN or an infinity, and what epsilon 0 does to rows of nothing: as in aclnn_moe_add_rms_norm_quant.h (a factor of 0 stands for 1 / 0).
+ *
+ * x, residual, sumOut, normOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents, at most 2^26 rows.  postGammaOptional and preGammaOptional
+ * [H] of x's type or FLOAT, equal types; normOut, yOut, smoothScale and preRstdOut need preGamma, postRstdOut needs postGamma.  gateOptional, by its extents: [H] (a
+ * value per channel, of the gammas' type; of x's type or FLOAT without one), x's extents with the last one 1 (a value per row; x's type or FLOAT), or x's extents
+ * (a value each; x's type; where H is 1, a value per row).  smoothScaleOptional FLOAT [H]; yOutOptional INT8 of x's extents with scaleOutOptional; scaleOutOptional, postRstdOutOptional and
+ * preRstdOutOptional FLOAT of x's extents without the last.  Inputs may be strided views; outputs are contiguous.  sumOut may be x's or residual's own memory,
+ * entirely; no other output may share memory with an input or another output.
+ */
+#ifndef OPS_TRANSFORMER_AMD_ACLNN_MOE_SANDWICH_NORM_H_
+#define OPS_TRANSFORMER_AMD_ACLNN_MOE_SANDWICH_NORM_H_
+
+#include "acl/acl.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+ACLNN_API aclnnStatus aclnnMoeSandwichNormGetWorkspaceSize(
+    const aclTensor* x, const aclTensor* residual, const aclTensor* postGammaOptional, const aclTensor* gateOptional, const aclTensor* preGammaOptional,
+    const aclTensor* smoothScaleOptional, int64_t gateType, double residualScale, double branchScale, double epsilon, const aclTensor* sumOut,
+    const aclTensor* normOutOptional, const aclTensor* yOutOptional, const aclTensor* scaleOutOptional, const aclTensor* postRstdOutOptional,
+    const aclTensor* preRstdOutOptional, uint64_t* workspaceSize, aclOpExecutor** executor);
+
+ACLNN_API aclnnStatus aclnnMoeSandwichNorm(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif  /* OPS_TRANSFORMER_AMD_ACLNN_MOE_SANDWICH_NORM_H_ */

@@ -68,6 +68,14 @@ _PHASE1_SIGNATURES = {
         [_VP, _VP, _VP, _U64P, _VPP],
     "aclnnMoeGatingTopKGroupedGetWorkspaceSize":
         [_VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, _I64, ctypes.c_double, ctypes.c_double, _VP, _VP, _VP, _U64P, _VPP],
+    "aclnnMoeBalanceLossGetWorkspaceSize":
+        [_VP, _VP, _VP, _I64, _VP, _VP, _VP, _VP, _U64P, _VPP],
+    "aclnnMoeGatingTopKGroupedGradGetWorkspaceSize":
+        [_VP] * 7 + [_I64, _I64, ctypes.c_double, ctypes.c_double, _VP, _U64P, _VPP],
+    "aclnnMoeSandwichNormGetWorkspaceSize":
+        [_VP] * 6 + [_I64, ctypes.c_double, ctypes.c_double, ctypes.c_double] + [_VP] * 6 + [_U64P, _VPP],
+    "aclnnMoeSandwichNormGradGetWorkspaceSize":
+        [_VP] * 9 + [_I64, ctypes.c_double, ctypes.c_double] + [_VP] * 5 + [_U64P, _VPP],
     "aclnnMoeInitRoutingV3GetWorkspaceSize":
         [_VP, _VP, _VP, _VP, _I64, _I64, _I64, _I64, _I64, ctypes.c_bool, _I64, _VP, _I64, _VP, _VP, _VP, _VP, _U64P, _VPP],
     "aclnnGroupedMatmulSwigluQuantGetWorkspaceSize":
@@ -96,7 +104,8 @@ _PHASE1_SIGNATURES = {
 _PHASE2 = ["aclnnMoeInitRoutingQuantV2", "aclnnGroupedMatmulSwigluQuantWeightNZ", "aclnnGroupedMatmulWeightNz",
            "aclnnGroupedMatmulFinalizeRoutingWeightNz", "aclnnGroupedMatmulFinalizeRoutingWeightNzV2", "aclnnGroupedMatmulFinalizeRouting", "aclnnGroupedMatmulFinalizeRoutingV2", "aclnnGroupedMatmulFinalizeRoutingV3",
            "aclnnMoeGatingTopKSoftmaxV2", "aclnnMoeInitRoutingV2", "aclnnMoeInitRoutingV3", "aclnnGroupedMatmulSwigluQuant", "aclnnGroupedMatmulV4", "aclnnGroupedMatmulV5",
-           "aclnnMoeFinalizeRoutingV2", "aclnnMoeAddRmsNormQuant", "aclnnMoeRouterLogits", "aclnnMoeGatingTopKGrouped"]
+           "aclnnMoeFinalizeRoutingV2", "aclnnMoeAddRmsNormQuant", "aclnnMoeRouterLogits", "aclnnMoeGatingTopKGrouped",
+           "aclnnMoeBalanceLoss", "aclnnMoeGatingTopKGroupedGrad", "aclnnMoeSandwichNorm", "aclnnMoeSandwichNormGrad"]
 
 
 def lib():
@@ -294,9 +303,10 @@ def _run_two_phase(api, args, device, workspace=None, static_workspace_api=None)
 # Operators of opapiPlanPacked (include/opapi_descriptor.h), by number.
 _PLANNED = ("aclnnMoeGatingTopKSoftmaxV2", "aclnnMoeInitRoutingV2", "aclnnMoeInitRoutingQuantV2", "aclnnMoeInitRoutingV3",
             "aclnnGroupedMatmulSwigluQuant", "aclnnGroupedMatmulV4", "aclnnMoeFinalizeRoutingV2", "aclnnMoeAddRmsNormQuant",
-            "aclnnMoeRouterLogits", "aclnnMoeGatingTopKGrouped")
+            "aclnnMoeRouterLogits", "aclnnMoeGatingTopKGrouped", "aclnnMoeBalanceLoss", "aclnnMoeGatingTopKGroupedGrad",
+            "aclnnMoeSandwichNorm", "aclnnMoeSandwichNormGrad")
 (_GATING, _ROUTING_V2, _ROUTING_QUANT_V2, _ROUTING_V3, _SWIGLU_QUANT, _GROUPED_MATMUL_V4, _FINALIZE_V2, _ADD_RMS_NORM_QUANT, _ROUTER_LOGITS,
- _GATING_GROUPED) = range(10)
+ _GATING_GROUPED, _BALANCE_LOSS, _GATING_GROUPED_GRAD, _SANDWICH_NORM, _SANDWICH_NORM_GRAD) = range(14)
 
 
 def _packed(t):
@@ -517,6 +527,78 @@ def moe_gating_top_k_grouped(x, k, bias=None, finished=None, k_group=1, group_co
     _run_whole(_GATING_GROUPED, (_GATING_GROUPED, k, k_group, group_count, group_select_mode, score_type, renorm, float(routed_scaling_factor), float(eps)),
                (x, bias, finished, y, idx, scores), workspace)
     return y, idx, scores
+
+
+def moe_balance_loss(x, expert_idx, seq_offsets=None, score_type=0, output_prob=True, out=None, workspace=None):
+    """aclnnMoeBalanceLoss.  Returns (loss fp32 [S], counts int32 [S, E], rows int32 [S], prob fp32 [S, E] or None) of router logits x [..., E] and the
+    experts picked from them, int32 [..., k], over the S sequences that seq_offsets [S + 1] (int32 or int64) cut the rows into, or over all rows as
+    one.  Rows whose first id is no expert (finished ones) and rows in no sequence do not count.  score_type 0 softmax, 1 sigmoid."""
+    if out is not None:
+        loss, counts, rows, prob = out
+    else:
+        S, E = 1 if seq_offsets is None else seq_offsets.shape[0] - 1, x.shape[-1]
+        loss = torch.empty((S,), dtype=torch.float32, device=x.device)
+        counts = torch.empty((S, E), dtype=torch.int32, device=x.device)
+        rows = torch.empty((S,), dtype=torch.int32, device=x.device)
+        prob = torch.empty((S, E), dtype=torch.float32, device=x.device) if output_prob else None
+    _run_whole(_BALANCE_LOSS, (_BALANCE_LOSS, score_type), (x, expert_idx, seq_offsets, loss, counts, rows, prob), workspace)
+    return loss, counts, rows, prob
+
+
+def moe_gating_top_k_grouped_grad(x, expert_idx, y_grad=None, loss_grad=None, counts=None, rows=None, seq_offsets=None, score_type=0, renorm=0,
+                                  routed_scaling_factor=1.0, eps=1e-20, x_grad_dtype=None, out=None, workspace=None):
+    """aclnnMoeGatingTopKGroupedGrad.  Returns the gradient [..., E] in x_grad_dtype (x's or fp32; x's when not given) with respect to the logits x: of the
+    weights y that moe_gating_top_k_grouped gave for expert_idx (y_grad, with its score_type, renorm, routed_scaling_factor and eps), of
+    moe_balance_loss (loss_grad fp32 [S], with its counts, rows and seq_offsets), or of both."""
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype if x_grad_dtype is None else x_grad_dtype, device=x.device)
+    _run_whole(_GATING_GROUPED_GRAD, (_GATING_GROUPED_GRAD, score_type, renorm, float(routed_scaling_factor), float(eps)),
+               (x, expert_idx, y_grad, loss_grad, counts, rows, seq_offsets, out), workspace)
+    return out
+
+
+def moe_sandwich_norm(x, residual, post_gamma=None, gate=None, pre_gamma=None, smooth_scale=None, gate_type=0, residual_scale=1.0, branch_scale=1.0,
+                      epsilon=1e-6, quantise=False, output_norm=True, output_rstd=False, out=None, workspace=None):
+    """aclnnMoeSandwichNorm.  Returns (sum, norm, y int8, scale fp32, post_rstd fp32, pre_rstd fp32), None for those that are not there:
+    sum = residual_scale * residual + branch_scale * gate * rms_norm(x) * post_gamma in x's dtype, norm = rms_norm(sum) * pre_gamma, its int8 rows with
+    a scale each, and the factors 1 / sqrt(mean + epsilon) of both norms, which moe_sandwich_norm_grad takes.  gate is [H], [..., 1] or [..., H];
+    gate_type 1 takes its sigmoid.  ``out`` may carry the outputs in that order, None for those that are not wanted; its sum may be x or residual."""
+    if out is not None:
+        total, norm, y, scale, post_rstd, pre_rstd = out
+    else:
+        empty = lambda wanted, shape, dtype: torch.empty(shape, dtype=dtype, device=x.device) if wanted else None
+        pre, per_row = pre_gamma is not None, x.shape[:-1]
+        total = empty(True, x.shape, x.dtype)
+        norm = empty(pre and output_norm, x.shape, x.dtype)
+        y, scale = empty(pre and quantise, x.shape, torch.int8), empty(pre and quantise, per_row, torch.float32)
+        post_rstd = empty(post_gamma is not None and output_rstd, per_row, torch.float32)
+        pre_rstd = empty(pre and output_rstd, per_row, torch.float32)
+    _run_whole(_SANDWICH_NORM, (_SANDWICH_NORM, gate_type, float(residual_scale), float(branch_scale), float(epsilon)),
+               (x, residual, post_gamma, gate, pre_gamma, smooth_scale, total, norm, y, scale, post_rstd, pre_rstd), workspace)
+    return total, norm, y, scale, post_rstd, pre_rstd
+
+
+def moe_sandwich_norm_grad(x, sum=None, sum_grad=None, norm_grad=None, post_gamma=None, gate=None, pre_gamma=None, post_rstd=None, pre_rstd=None,
+                           gate_type=0, residual_scale=1.0, branch_scale=1.0, out=None, workspace=None):
+    """aclnnMoeSandwichNormGrad.  Returns (x_grad, residual_grad, post_gamma_grad fp32 [H], gate_grad, pre_gamma_grad fp32 [H]), None for those without
+    an input, from the gradients of moe_sandwich_norm's sum and norm (either may be None; without norm_grad leave pre_gamma and pre_rstd out, too).
+    gate_grad has the gate's shape, in fp32 where the gate is shared.  ``out`` may carry the outputs in that order, None for those that are
+    not wanted."""
+    if out is not None:
+        x_grad, residual_grad, post_grad, gate_grad, pre_grad = out
+    else:
+        H = x.shape[-1]
+        x_grad, residual_grad = torch.empty(x.shape, dtype=x.dtype, device=x.device), torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        post_grad = None if post_gamma is None else torch.empty((H,), dtype=torch.float32, device=x.device)
+        pre_grad = None if pre_gamma is None else torch.empty((H,), dtype=torch.float32, device=x.device)
+        gate_grad = None
+        if gate is not None:
+            shared = gate.dim() == 1 or gate.shape[-1] == 1
+            gate_grad = torch.empty(gate.shape, dtype=torch.float32 if shared else x.dtype, device=x.device)
+    _run_whole(_SANDWICH_NORM_GRAD, (_SANDWICH_NORM_GRAD, gate_type, float(residual_scale), float(branch_scale)),
+               (x, sum, sum_grad, norm_grad, post_gamma, gate, pre_gamma, post_rstd, pre_rstd, x_grad, residual_grad, post_grad, gate_grad, pre_grad),
+               workspace)
+    return x_grad, residual_grad, post_grad, gate_grad, pre_grad
 
 
 def moe_init_routing_v3(x, expert_idx, scale=None, expert_num=0, expert_tokens_num_type=1, quant_mode=-1,

@@ -26,6 +26,10 @@ SOURCES = [
     "moe_add_rms_norm_quant.hip",
     "moe_router_logits.hip",
     "moe_gating_top_k_grouped.hip",
+    "moe_gating_top_k_grouped_grad.hip",
+    "moe_balance_loss.hip",
+    "moe_sandwich_norm.hip",
+    "moe_sandwich_norm_grad.hip",
     "moe_init_routing.hip",
     "grouped_gemm_i8.hip",
     "grouped_gemm_i8_int32.hip",

@@ -1,0 +1,367 @@
+// aclnnMoeBalanceLoss for gfx950: picks and mean probabilities per expert and sequence, and the sum of their products.
+//
+// The batch is cut into chunks of rows, a workgroup each, and a chunk is cut where a sequence ends.  Walking along the rows, every step goes to the next
+// chunk or to the next sequence: the piece that chunk c has of sequence s is number c + s, and of s there are pieces from its first chunk to its
+// last.  So the pieces' sums lie in a table of chunks + sequences entries without a count or an offset made beforehand, and a second kernel adds up those
+// of each sequence in their order.  One chunk and one sequence: the first kernel finishes by itself.
+#include "router_rows.h"
+
+#include "aclnnop/aclnn_moe_balance_loss.h"
+
+namespace {
+
+using namespace moe_front;
+
+struct BalanceArgs {
+    const void* x;
+    const int32_t* expertIdx;
+    Sequences sequences;
+    int32_t experts;
+    int32_t k;
+    int32_t sigmoid;
+    int32_t chunkRows;
+    int32_t chunks;
+    int32_t alone;  // one workgroup makes everything
+    // outputs
+    float* loss;
+    int32_t* counts;
+    int32_t* rowsOut;
+    float* prob;  // optional
+    // workspace, by piece
+    float* pieceSums;       // [pieces, experts]
+    int32_t* pieceCounts;   // [pieces, experts]
+    int32_t* pieceRows;     // [pieces]
+    double* lossParts;      // [sequences, parts]
+    uint32_t* tickets;      // [sequences]
+};
+
+constexpr int kChunkThreads = 512;
+constexpr int kChunkWaves = kChunkThreads / kWave;
+// A lane's rows in flight: their loads and reductions overlap.
+constexpr int UnrollOf(int pieces) { return pieces == 1 ? 4 : pieces == 2 ? 2 : 1; }
+// Chunks: as many as there are CUs, of at least the rows that a workgroup has in flight at once, and of at most so many that a lane's fp32 sums stay short.
+constexpr int64_t kMostChunks = 256, kMaxChunkRows = 4096;
+// One sequence of up to so many such passes is one workgroup's: it spares the second launch.
+constexpr int64_t kAlonePasses = 4;
+constexpr int kFinishExperts = 64;
+constexpr int kFinishThreads = 1024;
+
+template <typename Codec, int kLanes, int kPieces, bool kSigmoid>
+__global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs a) {
+    using Row = RowOf<kLanes, kPieces>;
+    constexpr int kEach = Row::kEach;
+    constexpr int kRowsAtOnce = kWave / kLanes;
+    constexpr int kUnroll = UnrollOf(kPieces);
+    constexpr int kStride = kChunkWaves * kRowsAtOnce;
+    __shared__ float sums[kChunkWaves][Row::kWidth];
+    __shared__ int32_t picked[Row::kWidth];
+    __shared__ int32_t live;
+    __shared__ double finishing[kChunkWaves];
+    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, l = lane % kLanes, group = lane / kLanes;
+    const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x);
+    auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
+
+    // Leaves the sums of rows [begin, end) in `sums` by wave, their picks in `picked` and how many count in `live`.
+    auto sumUp = [&](int64_t begin, int64_t end) {
+        for (int e = tid; e < a.experts; e += kChunkThreads) picked[e] = 0;
+        if (tid == 0) live = 0;
+        __syncthreads();
+        float sum[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
+        int32_t counted = 0;
+        for (int64_t at = begin + wave * kRowsAtOnce + group; at < end; at += kUnroll * kStride) {
+            float v[kUnroll][kEach];
+            int32_t id[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const int64_t row = min(at + u * kStride, end - 1);
+                id[u] = a.expertIdx[row * a.k];
+                Row::template Load<Codec>(x + row * a.experts, a.experts, l, -INFINITY, v[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const bool counts = at + u * kStride < end && isExpert(id[u]);
+                float share[kEach];
+                if constexpr (kSigmoid) {
+                    float p[kEach];
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) p[i] = SigmoidOf(v[u][i]).p;
+                    SharesOf<kLanes>(v[u], p, share);
+                } else {
+                    SoftmaxOf<kLanes>(v[u]);
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) share[i] = v[u][i];
+                }
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) sum[i] += counts ? share[i] : 0.f;
+                counted += counts && l == 0 ? 1 : 0;
+            }
+        }
+        if (counted != 0) atomicAdd(&live, counted);
+        // the rows side by side in a wave; the waves are added up when they are read
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            for (int d = kLanes; d < kWave; d <<= 1) sum[i] += __shfl_xor(sum[i], d);
+        }
+        if (lane < kLanes) {
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sums[wave][Row::At(p, l) + i] = sum[4 * p + i];
+            }
+        }
+        const int32_t ids = static_cast<int32_t>(end - begin) * a.k;
+        const int32_t* const idx = a.expertIdx + begin * a.k;
+        for (int32_t i = tid; i < ids; i += kChunkThreads) {
+            const int32_t id = idx[i];
+            if (isExpert(idx[i / a.k * a.k]) && isExpert(id)) atomicAdd(&picked[id], 1);
+        }
+        __syncthreads();
+    };
+    auto totalOf = [&](int e) {
+        float total = 0.f;
+#pragma unroll
+        for (int w = 0; w < kChunkWaves; ++w) total += sums[w][e];
+        return total;
+    };
+
+    const Sequences& seqs = a.sequences;
+    if (a.alone) {
+        sumUp(seqs.Start(0), max(seqs.Start(0), seqs.Start(1)));
+        const double n = live > 0 ? live : 1;
+        double loss = 0.0;
+        for (int e = tid; e < a.experts; e += kChunkThreads) {
+            const double mean = totalOf(e) / n;
+            a.counts[e] = picked[e];
+            if (a.prob != nullptr) a.prob[e] = static_cast<float>(mean);
+            loss += mean * picked[e];
+        }
+        loss = WaveSum(loss);
+        if (lane == 0) finishing[wave] = loss;
+        __syncthreads();
+        if (tid == 0) {
+            loss = 0.0;
+            for (int w = 0; w < kChunkWaves; ++w) loss += finishing[w];
+            a.loss[0] = static_cast<float>(loss * a.experts / (a.k * n));
+            a.rowsOut[0] = live;
+        }
+        return;
+    }
+    if (blockIdx.x == 0) {  // for the second kernel
+        for (int s = tid; s < seqs.count; s += kChunkThreads) a.tickets[s] = 0;
+    }
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * a.chunkRows, last = min(first + a.chunkRows, seqs.rows);
+    int32_t s = -2;
+    for (int64_t at = first; at < last;) {
+        // `at` is in the next sequence, unless some have no rows; whatever the offsets are, s starts at or in front of it and ends behind it
+        s = s >= 0 && s + 1 < seqs.count && seqs.Start(s + 2) > at ? s + 1 : seqs.Of(at);
+        if (s >= seqs.count) break;
+        const int64_t end = min(last, seqs.Start(s + 1));
+        if (s >= 0) {
+            sumUp(at, end);
+            const int64_t piece = static_cast<int64_t>(blockIdx.x) + s;
+            for (int e = tid; e < a.experts; e += kChunkThreads) {
+                a.pieceSums[piece * a.experts + e] = totalOf(e);
+                a.pieceCounts[piece * a.experts + e] = picked[e];
+            }
+            if (tid == 0) a.pieceRows[piece] = live;
+            __syncthreads();  // the tables are cleared for the next sequence
+        }
+        at = end;
+    }
+}
+
+// A sequence and kFinishExperts of its experts: the pieces' sums in their order, in runs side by side.  The workgroup of a sequence that ends last adds up
+// the loss, part by part in their order.
+__global__ __launch_bounds__(kFinishThreads) void BalanceFinishKernel(BalanceArgs a) {
+    constexpr int kRuns = kFinishThreads / kFinishExperts;
+    __shared__ double sums[kRuns][kFinishExperts];
+    __shared__ int32_t picks[kRuns][kFinishExperts];
+    __shared__ int32_t rowsOf[kFinishThreads / kWave];
+    const int64_t group = GroupIndex();
+    const int32_t parts = (a.experts + kFinishExperts - 1) / kFinishExperts;
+    const int64_t s = group / parts;
+    if (s >= a.sequences.count) return;
+    const int part = static_cast<int>(group % parts);
+    const int tid = threadIdx.x, run = tid / kFinishExperts, lane = tid % kFinishExperts;
+    const int e = part * kFinishExperts + lane;
+    const int64_t begin = a.sequences.Start(s), end = a.sequences.Start(s + 1);
+    int64_t from = 0, to = 0;
+    if (begin < end) {
+        from = begin / a.chunkRows + s;
+        to = (end - 1) / a.chunkRows + 1 + s;
+    }
+    int32_t live = 0;
+    for (int64_t p = from + tid; p < to; p += kFinishThreads) live += a.pieceRows[p];
+    double sum = 0.0;
+    int32_t count = 0;
+    if (e < a.experts) {
+#pragma unroll 4
+        for (int64_t p = from + run; p < to; p += kRuns) {
+            sum += a.pieceSums[p * a.experts + e];
+            count += a.pieceCounts[p * a.experts + e];
+        }
+    }
+    for (int d = 32; d > 0; d >>= 1) live += __shfl_xor(live, d);
+    if (tid % kWave == 0) rowsOf[tid / kWave] = live;
+    sums[run][lane] = sum;
+    picks[run][lane] = count;
+    __syncthreads();
+    if (run != 0) return;
+    static_assert(kFinishExperts == kWave, "one wave is left");
+    live = 0;
+    for (int w = 0; w < kFinishThreads / kWave; ++w) live += rowsOf[w];
+    const double n = live > 0 ? live : 1;
+    sum = 0.0;
+    count = 0;
+    for (int r = 0; r < kRuns; ++r) {
+        sum += sums[r][lane];
+        count += picks[r][lane];
+    }
+    const double mean = sum / n;
+    if (e < a.experts) {
+        a.counts[s * a.experts + e] = count;
+        if (a.prob != nullptr) a.prob[s * a.experts + e] = static_cast<float>(mean);
+    }
+    double loss = WaveSum(mean * count);
+    if (lane != 0) return;
+    if (parts > 1) {
+        double* const all = a.lossParts + s * parts;
+        __hip_atomic_store(all + part, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__hip_atomic_fetch_add(a.tickets + s, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) != static_cast<uint32_t>(parts - 1)) return;
+        loss = 0.0;
+        for (int i = 0; i < parts; ++i) loss += __hip_atomic_load(all + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    a.loss[s] = static_cast<float>(loss * a.experts / (a.k * n));
+    a.rowsOut[s] = live;
+}
+
+class BalanceExecutor : public aclOpExecutor {
+   public:
+    BalanceArgs args{};
+    aclDataType dtype = ACL_FLOAT;
+    uint64_t offRows = 0, offCounts = 0, offLoss = 0, offTickets = 0, offSums = 0;
+
+    template <typename Codec>
+    void Launch(hipStream_t stream) const {
+        ForRowLayout(args.experts, [&](auto lanes, auto pieces) {
+            constexpr int kLanes = decltype(lanes)::value, kPieces = decltype(pieces)::value;
+            const dim3 grid(static_cast<unsigned>(args.chunks));
+            if (args.sigmoid) hipLaunchKernelGGL((BalanceChunkKernel<Codec, kLanes, kPieces, true>), grid, dim3(kChunkThreads), 0, stream, args);
+            else hipLaunchKernelGGL((BalanceChunkKernel<Codec, kLanes, kPieces, false>), grid, dim3(kChunkThreads), 0, stream, args);
+        });
+    }
+
+    aclnnStatus Run(void* workspace, hipStream_t stream) override {
+        if (!args.alone) {
+            OPAPI_CHECK(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, ACLNN_ERR_PARAM_INVALID, "aclnnMoeBalanceLoss: the workspace must be 16-byte aligned");
+            char* const at = static_cast<char*>(workspace);
+            args.lossParts = reinterpret_cast<double*>(at + offLoss);
+            args.tickets = reinterpret_cast<uint32_t*>(at + offTickets);
+            args.pieceRows = reinterpret_cast<int32_t*>(at + offRows);
+            args.pieceCounts = reinterpret_cast<int32_t*>(at + offCounts);
+            args.pieceSums = reinterpret_cast<float*>(at + offSums);
+        }
+        {
+            opapi::KernelTimer timer("balance_chunks", stream);
+            if (dtype == ACL_FLOAT) Launch<F32>(stream);
+            else if (dtype == ACL_FLOAT16) Launch<F16>(stream);
+            else Launch<Bf16>(stream);
+        }
+        if (!args.alone) {
+            opapi::KernelTimer timer("balance_finish", stream);
+            const int64_t parts = (args.experts + kFinishExperts - 1) / kFinishExperts;
+            hipLaunchKernelGGL(BalanceFinishKernel, GridOf(parts * args.sequences.count), dim3(kFinishThreads), 0, stream, args);
+        }
+        const hipError_t err = hipGetLastError();
+        OPAPI_CHECK(err == hipSuccess, ACLNN_ERR_RUNTIME_ERROR, "aclnnMoeBalanceLoss: launch failed: %s", hipGetErrorString(err));
+        return ACLNN_SUCCESS;
+    }
+};
+
+}  // namespace
+
+extern "C" aclnnStatus aclnnMoeBalanceLossGetWorkspaceSize(const aclTensor* x, const aclTensor* expertIdx, const aclTensor* seqOffsetsOptional,
+                                                           int64_t scoreType, const aclTensor* lossOut, const aclTensor* countsOut,
+                                                           const aclTensor* rowsOut, const aclTensor* probOutOptional, uint64_t* workspaceSize,
+                                                           aclOpExecutor** executor) try {
+    using namespace opapi;
+    ClearError();
+    OPAPI_CHECK_NOTNULL(x, "x");
+    OPAPI_CHECK_NOTNULL(expertIdx, "expertIdx");
+    OPAPI_CHECK_NOTNULL(lossOut, "lossOut");
+    OPAPI_CHECK_NOTNULL(countsOut, "countsOut");
+    OPAPI_CHECK_NOTNULL(rowsOut, "rowsOut");
+    OPAPI_CHECK_NOTNULL(workspaceSize, "workspaceSize");
+    OPAPI_CHECK_NOTNULL(executor, "executor");
+    OPAPI_CHECK_EXTENTS(x, expertIdx, seqOffsetsOptional, lossOut, countsOut, rowsOut, probOutOptional);
+
+    constexpr aclnnStatus kInvalid = ACLNN_ERR_PARAM_INVALID;
+    int64_t rows = 0, experts = 0, k = 0, sequences = 0;
+    const aclnnStatus router = CheckRouterRows(x, expertIdx, seqOffsetsOptional, scoreType, &rows, &experts, &k, &sequences);
+    if (router != ACLNN_SUCCESS) return router;
+    OPAPI_CHECK(lossOut->dtype == ACL_FLOAT && HasExtents(lossOut, {sequences}), kInvalid, "lossOut %s must be FLOAT [%lld]", ShapeStr(lossOut).c_str(),
+                (long long)sequences);
+    OPAPI_CHECK(rowsOut->dtype == ACL_INT32 && HasExtents(rowsOut, {sequences}), kInvalid, "rowsOut %s must be INT32 [%lld]", ShapeStr(rowsOut).c_str(),
+                (long long)sequences);
+    OPAPI_CHECK(countsOut->dtype == ACL_INT32 && HasExtents(countsOut, {sequences, experts}), kInvalid, "countsOut %s must be INT32 [%lld,%lld]",
+                ShapeStr(countsOut).c_str(), (long long)sequences, (long long)experts);
+    OPAPI_CHECK(probOutOptional == nullptr || (probOutOptional->dtype == ACL_FLOAT && HasExtents(probOutOptional, {sequences, experts})), kInvalid,
+                "probOut %s must be FLOAT [%lld,%lld]", ShapeStr(probOutOptional).c_str(), (long long)sequences, (long long)experts);
+    const aclnnStatus memory = CheckMemory({x, expertIdx, seqOffsetsOptional}, {lossOut, countsOut, rowsOut, probOutOptional});
+    if (memory != ACLNN_SUCCESS) return memory;
+
+    auto* ex = new (std::nothrow) BalanceExecutor();
+    OPAPI_CHECK(ex != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "out of host memory");
+    BalanceArgs& a = ex->args;
+    ex->dtype = x->dtype;
+    OPAPI_BIND(ex, x, &a.x);
+    OPAPI_BIND(ex, expertIdx, &a.expertIdx);
+    OPAPI_BIND(ex, seqOffsetsOptional, &a.sequences.offsets);
+    a.sequences.isInt64 = seqOffsetsOptional != nullptr && seqOffsetsOptional->dtype == ACL_INT64;
+    a.sequences.count = static_cast<int32_t>(sequences);
+    a.sequences.rows = rows;
+    a.experts = static_cast<int32_t>(experts);
+    a.k = static_cast<int32_t>(k);
+    a.sigmoid = scoreType == 1;
+    a.loss = reinterpret_cast<float*>(DataPtr(lossOut));
+    a.counts = reinterpret_cast<int32_t*>(DataPtr(countsOut));
+    a.rowsOut = reinterpret_cast<int32_t*>(DataPtr(rowsOut));
+    a.prob = reinterpret_cast<float*>(DataPtr(probOutOptional));
+    int passRows = 1;
+    ForRowLayout(experts, [&](auto lanes, auto pieces) { passRows = kChunkWaves * (kWave / decltype(lanes)::value) * UnrollOf(decltype(pieces)::value); });
+    a.alone = sequences == 1 && rows <= kAlonePasses * passRows;
+    int64_t chunkRows = (rows + kMostChunks - 1) / kMostChunks;
+    if (chunkRows < passRows) chunkRows = passRows;
+    if (chunkRows > kMaxChunkRows) chunkRows = kMaxChunkRows;
+    a.chunkRows = static_cast<int32_t>(chunkRows);
+    a.chunks = a.alone ? 1 : static_cast<int32_t>((rows + chunkRows - 1) / chunkRows);
+    if (a.chunks < 1) a.chunks = 1;  // of no rows: the outputs are zeros all the same
+    uint64_t bytes = 0;
+    if (!a.alone) {
+        const uint64_t pieces = static_cast<uint64_t>(a.chunks) + static_cast<uint64_t>(sequences);
+        const uint64_t parts = static_cast<uint64_t>((experts + kFinishExperts - 1) / kFinishExperts);
+        auto take = [&](uint64_t size) {
+            const uint64_t at = bytes;
+            bytes = AlignUp(bytes + size, 16);
+            return at;
+        };
+        ex->offLoss = take(8 * parts * static_cast<uint64_t>(sequences));
+        ex->offTickets = take(4 * static_cast<uint64_t>(sequences));
+        ex->offRows = take(4 * pieces);
+        ex->offCounts = take(4 * pieces * static_cast<uint64_t>(experts));
+        ex->offSums = take(4 * pieces * static_cast<uint64_t>(experts));
+    }
+    ex->SealWorkspace(bytes);
+    *workspaceSize = ex->workspaceBytes;
+    *executor = ex;
+    return ACLNN_SUCCESS;
+} catch (...) {  // no exception may cross the C boundary
+    opapi::SetError("out of host memory");
+    return ACLNN_ERR_INNER;
+}
+
+extern "C" aclnnStatus aclnnMoeBalanceLoss(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream) {
+    return opapi::RunAndRelease(workspace, workspaceSize, executor, stream);
+}

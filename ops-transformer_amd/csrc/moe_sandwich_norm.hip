@@ -1,0 +1,416 @@
+// aclnnMoeSandwichNorm for gfx950: s = a residual + b gate * (rms_norm(x) * postGamma), n = rms_norm(s) * preGamma, int8 rows of n * smooth.
+//
+// Two reductions over a row, the second on what the first one settles: the row stays in registers from its load to its last output, so it crosses the
+// memory once.  Sums, factors, u, v and n are fp32; what is rounded is s (to the stream's type, and that rounded value is what is normalised), n where it
+// leaves, and y, which is made as aclnnMoeAddRmsNormQuant makes it (norm_rows.h).
+#include "sandwich_norm.h"
+
+#include "aclnnop/aclnn_moe_sandwich_norm.h"
+
+namespace {
+
+using namespace moe_front;
+
+struct SandwichArgs {
+    const void* x;
+    const void* residual;
+    const void* post;      // optional
+    const void* gate;      // optional
+    const void* pre;       // optional
+    const float* smooth;   // optional
+    void* sum;             // may be x's or residual's memory
+    void* norm;            // optional
+    int8_t* y;             // optional, with scale
+    float* scale;
+    float* postRstd;       // optional
+    float* preRstd;        // optional
+    int64_t rows;
+    int64_t cols;
+    int32_t gateKind;
+    int32_t sigmoid;
+    int32_t gateIsFloat;
+    float residualScale;
+    float branchScale;
+    float eps;
+};
+
+__device__ __forceinline__ float FactorOf(float sumSquares, int64_t cols, float eps) {
+    const float mean = sumSquares / static_cast<float>(cols) + eps;
+    return mean == 0.f ? 0.f : 1.f / sqrtf(mean);
+}
+
+template <typename Codec>
+__device__ __forceinline__ float RowGate(const SandwichArgs& a, int64_t row) {
+    if (a.gateKind != kGateRow) return 1.f;
+    const float raw = a.gateIsFloat ? static_cast<const float*>(a.gate)[row] : Codec::Load(static_cast<const typename Codec::Storage*>(a.gate)[row]);
+    return Gated(raw, a.sigmoid);
+}
+
+// Rows in pieces of eight elements, up to kPackets of them a lane; a workgroup takes every gridDim.x-th row and asks for the next one before the
+// present one is reduced.  Gammas and a gate per channel stay in registers.  Pieces are read and written where they lie (see norm_rows.h).
+constexpr int kMaxPacketThreads = 512;
+constexpr int kMaxPackets = 4;
+
+template <typename Codec, typename Gamma, int kPackets, int kGate>
+__global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(SandwichArgs a) {
+    using P = Packet<Codec>;
+    using Storage = typename Codec::Storage;
+    constexpr int kMaxWaves = kMaxPacketThreads / kWave;
+    __shared__ float postSums[2][kMaxWaves][1];
+    __shared__ float2 partial[2][kMaxWaves];
+    const int threads = blockDim.x, waves = threads / kWave, tid = threadIdx.x;
+    const int cols = static_cast<int>(a.cols);
+    const bool post = a.post != nullptr, pre = a.pre != nullptr;
+    P x[kPackets], r[kPackets], gateRow[kGate == kReadPackets ? kPackets : 1];
+    Packet<Gamma> postGamma[kPackets], preGamma[kPackets];
+    float gateHeld[kGate == kHeldPackets ? kPackets : 1][8];
+    float rowGate = 1.f;
+    bool here[kPackets];
+    auto at = [&](int p) { return (p * threads + tid) * 8; };
+    auto count = [&](int p) { return min(cols - at(p), 8); };
+#pragma unroll
+    for (int p = 0; p < kPackets; ++p) {
+        here[p] = at(p) < cols;
+        if (!here[p]) continue;
+        if (post) postGamma[p] = LoadPacket<false, Gamma>(a.post, at(p), count(p));
+        if (pre) preGamma[p] = LoadPacket<false, Gamma>(a.pre, at(p), count(p));
+        if constexpr (kGate == kHeldPackets) {
+            Unpack<Gamma>(LoadPacket<false, Gamma>(a.gate, at(p), count(p)), gateHeld[p]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) gateHeld[p][i] = Gated(gateHeld[p][i], a.sigmoid);
+        }
+    }
+    auto load = [&](int64_t row) {
+#pragma unroll
+        for (int p = 0; p < kPackets; ++p) {
+            if (!here[p]) continue;
+            x[p] = LoadPacket<false, Codec>(a.x, row * cols + at(p), count(p));
+            r[p] = LoadPacket<false, Codec>(a.residual, row * cols + at(p), count(p));
+            if constexpr (kGate == kReadPackets) gateRow[p] = LoadPacket<false, Codec>(a.gate, row * cols + at(p), count(p));
+        }
+        if constexpr (kGate == kNoPackets) rowGate = RowGate<Codec>(a, row);
+    };
+    int64_t row = blockIdx.x;
+    load(row);
+    for (int parity = 0; row < a.rows; parity ^= 1) {
+        float postRstd = 0.f;
+        if (post) {
+            float squares[1] = {0.f};
+#pragma unroll
+            for (int p = 0; p < kPackets; ++p) {
+                if (!here[p]) continue;
+                float v[8];
+                Unpack<Codec>(x[p], v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) squares[0] = fmaf(v[i], v[i], squares[0]);
+            }
+            SumsOverGroup<1, kMaxWaves>(squares, waves, parity, postSums);
+            postRstd = FactorOf(squares[0], a.cols, a.eps);
+            if (a.postRstd != nullptr && tid == 0) a.postRstd[row] = postRstd;
+        }
+        P s[kPackets];
+        float sumSquares = 0.f;
+        uint32_t maxBits = 0;
+#pragma unroll
+        for (int p = 0; p < kPackets; ++p) {
+            if (!here[p]) continue;
+            float v[8], w[8];
+            Unpack<Codec>(x[p], v);
+            Unpack<Codec>(r[p], w);
+            if (post) {
+                float g[8];
+                Unpack<Gamma>(postGamma[p], g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * postRstd * g[i];
+            }
+            if constexpr (kGate == kHeldPackets) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= gateHeld[p][i];
+            } else if constexpr (kGate == kReadPackets) {
+                float g[8];
+                Unpack<Codec>(gateRow[p], g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= Gated(g[i], a.sigmoid);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] *= rowGate;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fmaf(a.residualScale, w[i], a.branchScale * v[i]);
+            s[p] = Pack<Codec>(v);
+            StorePacket<false, Storage>(a.sum, row * cols + at(p), count(p), s[p]);
+            if (!pre) continue;
+            Unpack<Codec>(s[p], v);
+            float g[8];
+            Unpack<Gamma>(preGamma[p], g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sumSquares = fmaf(v[i], v[i], sumSquares);
+            if (a.y != nullptr) {
+                if (a.smooth != nullptr) {
+                    const Packet<F32> smooth = LoadPacket<false, F32>(a.smooth, at(p), count(p));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) maxBits = max(maxBits, __float_as_uint(fabsf(v[i] * g[i] * reinterpret_cast<const float*>(&smooth)[i])));
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) maxBits = max(maxBits, __float_as_uint(fabsf(v[i] * g[i])));
+                }
+            }
+        }
+        const int64_t next = row + gridDim.x;
+        if (next < a.rows) load(next);
+        if (pre) {
+            sumSquares = SumOver<kWave>(sumSquares);
+            if (a.y != nullptr) maxBits = WaveMax(maxBits);
+            if (waves > 1) {
+                if (tid % kWave == 0) partial[parity][tid / kWave] = float2{sumSquares, __uint_as_float(maxBits)};
+                __syncthreads();  // two buffers in turn: one barrier a reduction
+                sumSquares = partial[parity][0].x;
+                maxBits = __float_as_uint(partial[parity][0].y);
+                for (int w = 1; w < waves; ++w) {
+                    sumSquares += partial[parity][w].x;
+                    maxBits = max(maxBits, __float_as_uint(partial[parity][w].y));
+                }
+            }
+            const RowScales scales = ScalesOf(sumSquares, maxBits, a.cols, a.eps);
+            if (tid == 0) {
+                if (a.preRstd != nullptr) a.preRstd[row] = scales.r;
+                if (a.scale != nullptr) a.scale[row] = scales.scale;
+            }
+#pragma unroll
+            for (int p = 0; p < kPackets; ++p) {
+                if (!here[p]) continue;
+                float v[8], g[8];
+                Unpack<Codec>(s[p], v);
+                Unpack<Gamma>(preGamma[p], g);
+                if (a.norm != nullptr) {
+                    float n[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) n[i] = v[i] * scales.r * g[i];
+                    StorePacket<false, Storage>(a.norm, row * cols + at(p), count(p), Pack<Codec>(n));
+                }
+                if (a.y != nullptr) {
+                    float smooth[8];
+                    if (a.smooth != nullptr) {
+                        Unpack<F32>(LoadPacket<false, F32>(a.smooth, at(p), count(p)), smooth);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) smooth[i] = 1.f;
+                    }
+                    uint32_t q[2] = {0, 0};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        q[i / 4] |= (static_cast<uint32_t>(Quantised(v[i] * g[i] * smooth[i], scales)) & 0xffu) << (i % 4 * 8);
+                    }
+                    StorePacket<false, int8_t>(a.y, row * cols + at(p), count(p), uint2{q[0], q[1]});
+                }
+            }
+        }
+        row = next;
+    }
+}
+
+// Rows of any length: a workgroup per row, one element at a time, the row read again behind each reduction (from the sum once that is written, by the
+// same lane: it may lie in x's or the residual's memory), squares added up in 64 bits.
+constexpr int kAnyThreads = 256;
+
+__device__ __forceinline__ double SumOfGroup(double v, double (&lds)[kAnyThreads / kWave]) {
+    v = WaveSum(v);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < kAnyThreads / kWave; ++w) v += lds[w];
+    return v;
+}
+
+template <typename Codec, typename Gamma>
+__global__ __launch_bounds__(kAnyThreads) void SandwichAnyKernel(SandwichArgs a) {
+    using S = typename Codec::Storage;
+    __shared__ double sums[kAnyThreads / kWave];
+    __shared__ uint32_t maxima[kAnyThreads / kWave];
+    const int64_t row = GroupIndex();
+    if (row >= a.rows) return;
+    const int64_t at = row * a.cols;
+    const S* const x = static_cast<const S*>(a.x) + at;
+    const S* const residual = static_cast<const S*>(a.residual) + at;
+    S* const sum = static_cast<S*>(a.sum) + at;
+    auto weight = [&](const void* w, int64_t c) { return Gamma::Load(static_cast<const typename Gamma::Storage*>(w)[c]); };
+    float rstd = 0.f;
+    if (a.post != nullptr) {
+        double squares = 0.0;
+        for (int64_t c = threadIdx.x; c < a.cols; c += kAnyThreads) {
+            const double v = Codec::Load(x[c]);
+            squares = fma(v, v, squares);
+        }
+        rstd = FactorOf(static_cast<float>(SumOfGroup(squares, sums)), a.cols, a.eps);
+        if (a.postRstd != nullptr && threadIdx.x == 0) a.postRstd[row] = rstd;
+    }
+    const float rowGate = RowGate<Codec>(a, row);
+    double squares = 0.0;
+    uint32_t maxBits = 0;
+    auto scaled = [&](float s, int64_t c) { return s * weight(a.pre, c) * (a.smooth == nullptr ? 1.f : a.smooth[c]); };
+    for (int64_t c = threadIdx.x; c < a.cols; c += kAnyThreads) {
+        float v = Codec::Load(x[c]);
+        if (a.post != nullptr) v = v * rstd * weight(a.post, c);
+        if (a.gateKind == kGateChannel) v *= Gated(weight(a.gate, c), a.sigmoid);
+        else if (a.gateKind == kGateEach) v *= Gated(Codec::Load(static_cast<const S*>(a.gate)[at + c]), a.sigmoid);
+        else v *= rowGate;
+        const S raw = Codec::Store(fmaf(a.residualScale, Codec::Load(residual[c]), a.branchScale * v));
+        sum[c] = raw;
+        if (a.pre == nullptr) continue;
+        const float s = Codec::Load(raw);
+        squares = fma(static_cast<double>(s), static_cast<double>(s), squares);
+        if (a.y != nullptr) maxBits = max(maxBits, __float_as_uint(fabsf(scaled(s, c))));
+    }
+    if (a.pre == nullptr) return;
+    squares = SumOfGroup(squares, sums);
+    maxBits = WaveMax(maxBits);
+    if (threadIdx.x % kWave == 0) maxima[threadIdx.x / kWave] = maxBits;
+    __syncthreads();
+    for (int w = 0; w < kAnyThreads / kWave; ++w) maxBits = max(maxBits, maxima[w]);
+    const RowScales scales = ScalesOf(static_cast<float>(squares), maxBits, a.cols, a.eps);
+    if (threadIdx.x == 0) {
+        if (a.preRstd != nullptr) a.preRstd[row] = scales.r;
+        if (a.scale != nullptr) a.scale[row] = scales.scale;
+    }
+    for (int64_t c = threadIdx.x; c < a.cols; c += kAnyThreads) {
+        const float s = Codec::Load(sum[c]);
+        if (a.norm != nullptr) static_cast<S*>(a.norm)[at + c] = Codec::Store(s * scales.r * weight(a.pre, c));
+        if (a.y != nullptr) a.y[at + c] = static_cast<int8_t>(Quantised(scaled(s, c), scales));
+    }
+}
+
+class SandwichExecutor : public aclOpExecutor {
+   public:
+    SandwichArgs args{};
+    aclDataType dtype = ACL_FLOAT;
+    aclDataType weightType = ACL_FLOAT;
+
+    template <typename Codec, typename Gamma, int kPackets, int kGate>
+    void LaunchPackets(hipStream_t stream) const {
+        const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
+        const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
+        int64_t groups = args.rows;
+        const int64_t most = threads >= 256 ? 4096 : 2048;
+        if (groups > most) groups = most;
+        hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kGate>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, args);
+    }
+
+    template <typename Codec, typename Gamma, int kPackets>
+    void ForGate(hipStream_t stream) const {
+        const int packets = GatePackets(args.gateKind);
+        if (packets == kHeldPackets) LaunchPackets<Codec, Gamma, kPackets, kHeldPackets>(stream);
+        else if (packets == kReadPackets) LaunchPackets<Codec, Gamma, kPackets, kReadPackets>(stream);
+        else LaunchPackets<Codec, Gamma, kPackets, kNoPackets>(stream);
+    }
+
+    aclnnStatus Run(void*, hipStream_t stream) override {
+        if (args.rows == 0) return ACLNN_SUCCESS;
+        opapi::KernelTimer timer("sandwich_norm", stream);
+        ForTypes(dtype, weightType, [&](auto codec, auto gamma) {
+            using Codec = decltype(codec);
+            using Gamma = decltype(gamma);
+            const int64_t lanes = (args.cols + 7) / 8;
+            if (lanes <= kMaxPacketThreads) ForGate<Codec, Gamma, 1>(stream);
+            else if (lanes <= 2 * kMaxPacketThreads) ForGate<Codec, Gamma, 2>(stream);
+            else if (lanes <= kMaxPackets * kMaxPacketThreads) ForGate<Codec, Gamma, kMaxPackets>(stream);
+            else hipLaunchKernelGGL((SandwichAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
+        });
+        const hipError_t err = hipGetLastError();
+        OPAPI_CHECK(err == hipSuccess, ACLNN_ERR_RUNTIME_ERROR, "aclnnMoeSandwichNorm: launch failed: %s", hipGetErrorString(err));
+        return ACLNN_SUCCESS;
+    }
+};
+
+}  // namespace
+
+extern "C" aclnnStatus aclnnMoeSandwichNormGetWorkspaceSize(
+    const aclTensor* x, const aclTensor* residual, const aclTensor* postGammaOptional, const aclTensor* gateOptional, const aclTensor* preGammaOptional,
+    const aclTensor* smoothScaleOptional, int64_t gateType, double residualScale, double branchScale, double epsilon, const aclTensor* sumOut,
+    const aclTensor* normOutOptional, const aclTensor* yOutOptional, const aclTensor* scaleOutOptional, const aclTensor* postRstdOutOptional,
+    const aclTensor* preRstdOutOptional, uint64_t* workspaceSize, aclOpExecutor** executor) try {
+    using namespace opapi;
+    ClearError();
+    OPAPI_CHECK_NOTNULL(x, "x");
+    OPAPI_CHECK_NOTNULL(residual, "residual");
+    OPAPI_CHECK_NOTNULL(sumOut, "sumOut");
+    OPAPI_CHECK_NOTNULL(workspaceSize, "workspaceSize");
+    OPAPI_CHECK_NOTNULL(executor, "executor");
+    OPAPI_CHECK_EXTENTS(x, residual, postGammaOptional, gateOptional, preGammaOptional, smoothScaleOptional, sumOut, normOutOptional, yOutOptional,
+                        scaleOutOptional, postRstdOutOptional, preRstdOutOptional);
+
+    constexpr aclnnStatus kInvalid = ACLNN_ERR_PARAM_INVALID;
+    SandwichShape shape;
+    const aclnnStatus checked = CheckSandwich(x, postGammaOptional, gateOptional, preGammaOptional, gateType, residualScale, branchScale, &shape);
+    if (checked != ACLNN_SUCCESS) return checked;
+    OPAPI_CHECK(epsilon >= 0 && epsilon <= 1e30, kInvalid, "epsilon must be a number of at least 0");
+    OPAPI_CHECK(Like(residual, x), kInvalid, "residual %s must have x's type and extents %s", ShapeStr(residual).c_str(), ShapeStr(x).c_str());
+    OPAPI_CHECK(Like(sumOut, x), kInvalid, "sumOut %s must have x's type and extents %s", ShapeStr(sumOut).c_str(), ShapeStr(x).c_str());
+    OPAPI_CHECK(Like(normOutOptional, x), kInvalid, "normOut %s must have x's type and extents %s", ShapeStr(normOutOptional).c_str(), ShapeStr(x).c_str());
+    OPAPI_CHECK((yOutOptional == nullptr) == (scaleOutOptional == nullptr), ACLNN_ERR_PARAM_NULLPTR, "yOut and scaleOut belong together");
+    OPAPI_CHECK(yOutOptional == nullptr || (yOutOptional->dtype == ACL_INT8 && SameButLast(yOutOptional, x, shape.cols)), kInvalid,
+                "yOut %s must be INT8 of x's extents %s", ShapeStr(yOutOptional).c_str(), ShapeStr(x).c_str());
+    OPAPI_CHECK(PerRow(scaleOutOptional, x), kInvalid, "scaleOut %s must be FLOAT of x's extents %s without the last", ShapeStr(scaleOutOptional).c_str(),
+                ShapeStr(x).c_str());
+    OPAPI_CHECK(PerRow(postRstdOutOptional, x), kInvalid, "postRstdOut %s must be FLOAT of x's extents %s without the last",
+                ShapeStr(postRstdOutOptional).c_str(), ShapeStr(x).c_str());
+    OPAPI_CHECK(PerRow(preRstdOutOptional, x), kInvalid, "preRstdOut %s must be FLOAT of x's extents %s without the last",
+                ShapeStr(preRstdOutOptional).c_str(), ShapeStr(x).c_str());
+    OPAPI_CHECK(smoothScaleOptional == nullptr || (smoothScaleOptional->dtype == ACL_FLOAT && HasExtents(smoothScaleOptional, {shape.cols})), kInvalid,
+                "smoothScale must be FLOAT [%lld]", (long long)shape.cols);
+    OPAPI_CHECK(yOutOptional != nullptr || smoothScaleOptional == nullptr, kInvalid, "smoothScale goes into yOut, which is not given");
+    OPAPI_CHECK(preGammaOptional != nullptr || (normOutOptional == nullptr && yOutOptional == nullptr && preRstdOutOptional == nullptr), kInvalid,
+                "normOut, yOut and preRstdOut are of the norm with preGamma, which is not given");
+    OPAPI_CHECK(preGammaOptional == nullptr || normOutOptional != nullptr || yOutOptional != nullptr || preRstdOutOptional != nullptr, ACLNN_ERR_PARAM_NULLPTR,
+                "preGamma is given, but none of its norm's outputs");
+    OPAPI_CHECK(postGammaOptional != nullptr || postRstdOutOptional == nullptr, kInvalid, "postRstdOut is of the norm with postGamma, which is not given");
+    const aclTensor* const apart[] = {normOutOptional, yOutOptional, scaleOutOptional, postRstdOutOptional, preRstdOutOptional};
+    const aclnnStatus memory =
+        CheckMemory({x, residual, postGammaOptional, gateOptional, preGammaOptional, smoothScaleOptional}, {apart[0], apart[1], apart[2], apart[3], apart[4]});
+    if (memory != ACLNN_SUCCESS) return memory;
+    OPAPI_CHECK(InOrder(sumOut), kInvalid, "the outputs must be contiguous");
+    OPAPI_CHECK(IsEmpty(sumOut) || sumOut->data != nullptr, ACLNN_ERR_PARAM_NULLPTR, "an output carries no device memory");
+    for (const aclTensor* out : apart) OPAPI_CHECK(!Overlap(out, sumOut), kInvalid, "two outputs share memory");
+    for (const aclTensor* in : {x, residual, postGammaOptional, gateOptional, preGammaOptional, smoothScaleOptional}) {
+        if (in == nullptr || !IsContiguous(in)) continue;
+        const bool inPlace = (in == x || in == residual) && DataPtr(in) == DataPtr(sumOut);
+        OPAPI_CHECK(inPlace || !Overlap(sumOut, in), kInvalid, "an output shares memory with an input");
+    }
+
+    auto* ex = new (std::nothrow) SandwichExecutor();
+    OPAPI_CHECK(ex != nullptr, ACLNN_ERR_INNER_CREATE_EXECUTOR, "out of host memory");
+    SandwichArgs& a = ex->args;
+    ex->dtype = x->dtype;
+    ex->weightType = shape.weightType;
+    OPAPI_BIND(ex, x, &a.x);
+    OPAPI_BIND(ex, residual, &a.residual);
+    OPAPI_BIND(ex, postGammaOptional, &a.post);
+    OPAPI_BIND(ex, gateOptional, &a.gate);
+    OPAPI_BIND(ex, preGammaOptional, &a.pre);
+    OPAPI_BIND(ex, smoothScaleOptional, &a.smooth);
+    a.sum = DataPtr(sumOut);
+    a.norm = DataPtr(normOutOptional);
+    a.y = reinterpret_cast<int8_t*>(DataPtr(yOutOptional));
+    a.scale = reinterpret_cast<float*>(DataPtr(scaleOutOptional));
+    a.postRstd = reinterpret_cast<float*>(DataPtr(postRstdOutOptional));
+    a.preRstd = reinterpret_cast<float*>(DataPtr(preRstdOutOptional));
+    a.rows = shape.rows;
+    a.cols = shape.cols;
+    a.gateKind = shape.gateKind;
+    a.gateIsFloat = shape.gateIsFloat;
+    a.sigmoid = static_cast<int32_t>(gateType);
+    a.residualScale = static_cast<float>(residualScale);
+    a.branchScale = static_cast<float>(branchScale);
+    a.eps = static_cast<float>(epsilon);
+    ex->SealWorkspace(0);
+    *workspaceSize = ex->workspaceBytes;
+    *executor = ex;
+    return ACLNN_SUCCESS;
+} catch (...) {  // no exception may cross the C boundary
+    opapi::SetError("out of host memory");
+    return ACLNN_ERR_INNER;
+}
+
+extern "C" aclnnStatus aclnnMoeSandwichNorm(void* workspace, uint64_t workspaceSize, aclOpExecutor* executor, aclrtStream stream) {
+    return opapi::RunAndRelease(workspace, workspaceSize, executor, stream);
+}

@@ -4,23 +4,27 @@
 #include "aclnnop/aclnn_grouped_matmul_swiglu_quant.h"
 #include "aclnnop/aclnn_grouped_matmul_v4.h"
 #include "aclnnop/aclnn_moe_add_rms_norm_quant.h"
+#include "aclnnop/aclnn_moe_balance_loss.h"
 #include "aclnnop/aclnn_moe_finalize_routing_v2.h"
 #include "aclnnop/aclnn_moe_gating_top_k_grouped.h"
+#include "aclnnop/aclnn_moe_gating_top_k_grouped_grad.h"
 #include "aclnnop/aclnn_moe_gating_top_k_softmax_v2.h"
 #include "aclnnop/aclnn_moe_init_routing_quant_v2.h"
 #include "aclnnop/aclnn_moe_init_routing_v2.h"
 #include "aclnnop/aclnn_moe_init_routing_v3.h"
 #include "aclnnop/aclnn_moe_router_logits.h"
+#include "aclnnop/aclnn_moe_sandwich_norm.h"
+#include "aclnnop/aclnn_moe_sandwich_norm_grad.h"
 #include "opapi_common.h"
 
 namespace {
 
 // The operators by number, with how many scalars and tensors each takes.
 enum { kGating, kRoutingV2, kRoutingQuantV2, kRoutingV3, kSwigluQuant, kGroupedMatmulV4, kFinalizeV2, kAddRmsNormQuant, kRouterLogits,
-       kGatingGrouped, kOperators };
-constexpr int kScalars[kOperators] = {3, 6, 7, 8, 0, 4, 1, 1, 0, 8};
-constexpr int kTensors[kOperators] = {5, 6, 9, 7, 9, 7, 8, 8, 3, 6};
-constexpr int kMaxTensors = 9;
+       kGatingGrouped, kBalanceLoss, kGatingGroupedGrad, kSandwichNorm, kSandwichNormGrad, kOperators };
+constexpr int kScalars[kOperators] = {3, 6, 7, 8, 0, 4, 1, 1, 0, 8, 1, 4, 4, 3};
+constexpr int kTensors[kOperators] = {5, 6, 9, 7, 9, 7, 8, 8, 3, 6, 7, 8, 12, 14};
+constexpr int kMaxTensors = 14;
 
 // Tensors from packed[at] on, count of them; absent ones (no dimensions, no address) stay null.  False when the array is not exactly theirs.
 bool Unpack(const int64_t* packed, uint64_t at, uint64_t length, int count, aclTensor (&tensors)[kMaxTensors], aclTensor* (&given)[kMaxTensors]) {
@@ -91,6 +95,17 @@ extern "C" aclnnStatus opapiPlanPacked(const int64_t* packed, uint64_t length, u
         case kGatingGrouped:
             return aclnnMoeGatingTopKGroupedGetWorkspaceSize(t[0], t[1], t[2], s[0], s[1], s[2], s[3], s[4], s[5], Real(s[6]), Real(s[7]), t[3],
                                                              t[4], t[5], workspaceSize, executor);
+        case kBalanceLoss:
+            return aclnnMoeBalanceLossGetWorkspaceSize(t[0], t[1], t[2], s[0], t[3], t[4], t[5], t[6], workspaceSize, executor);
+        case kGatingGroupedGrad:
+            return aclnnMoeGatingTopKGroupedGradGetWorkspaceSize(t[0], t[1], t[2], t[3], t[4], t[5], t[6], s[0], s[1], Real(s[2]), Real(s[3]), t[7],
+                                                                 workspaceSize, executor);
+        case kSandwichNorm:
+            return aclnnMoeSandwichNormGetWorkspaceSize(t[0], t[1], t[2], t[3], t[4], t[5], s[0], Real(s[1]), Real(s[2]), Real(s[3]), t[6], t[7], t[8], t[9],
+                                                        t[10], t[11], workspaceSize, executor);
+        case kSandwichNormGrad:
+            return aclnnMoeSandwichNormGradGetWorkspaceSize(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], s[0], Real(s[1]), Real(s[2]), t[9], t[10],
+                                                            t[11], t[12], t[13], workspaceSize, executor);
         default:
             return aclnnMoeFinalizeRoutingV2GetWorkspaceSize(t[0], t[1], t[2], t[3], t[4], t[5], t[6], s[0], t[7], workspaceSize, executor);
     }

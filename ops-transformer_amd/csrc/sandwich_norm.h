@@ -1,0 +1,105 @@
+// What aclnnMoeSandwichNorm and its gradient share: the gate's forms, sums over a workgroup's waves, and the checks of their first phases.
+#pragma once
+
+#include <algorithm>
+#include <initializer_list>
+#include <new>
+
+#include "norm_rows.h"
+#include "router_rows.h"
+
+namespace moe_front {
+
+// How a gate is shared.  kGateRow is a factor of the row, kGateChannel lies in registers beside the gammas, kGateEach is read with the rows.
+enum GateKind { kGateNone = 0, kGateChannel = 1, kGateRow = 2, kGateEach = 3 };
+
+// The kernels are made for gates in registers, gates read with the rows, and neither.
+constexpr int kNoPackets = 0, kHeldPackets = 1, kReadPackets = 2;
+inline int GatePackets(int kind) { return kind == kGateChannel ? kHeldPackets : kind == kGateEach ? kReadPackets : kNoPackets; }
+
+__device__ __forceinline__ float Gated(float gate, int sigmoid) { return sigmoid ? SigmoidOf(gate).p : gate; }
+
+// kCount sums over a workgroup, the same bits in every lane.  `parity` alternates between calls that follow each other: one barrier a call.
+template <int kCount, int kMaxWaves>
+__device__ __forceinline__ void SumsOverGroup(float (&v)[kCount], int waves, int parity, float (&lds)[2][kMaxWaves][kCount]) {
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) v[i] = SumOver<kWave>(v[i]);
+    if (waves == 1) return;
+    if (threadIdx.x % kWave == 0) {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) lds[parity][threadIdx.x / kWave][i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) v[i] = lds[parity][0][i];
+    for (int w = 1; w < waves; ++w) {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) v[i] += lds[parity][w][i];
+    }
+}
+
+// The weights that go with the channels, gammas and a gate per channel, share a type: x's, or FLOAT.
+struct SandwichShape {
+    int64_t rows = 0, cols = 0;
+    int gateKind = kGateNone;
+    bool gateIsFloat = false;  // of a value per row
+    aclDataType weightType = ACL_FLOAT;
+};
+
+inline aclnnStatus CheckSandwich(const aclTensor* x, const aclTensor* postGamma, const aclTensor* gate, const aclTensor* preGamma, int64_t gateType,
+                                 double residualScale, double branchScale, SandwichShape* shape) {
+    using namespace opapi;
+    constexpr aclnnStatus kInvalid = ACLNN_ERR_PARAM_INVALID;
+    OPAPI_CHECK(IsFloating(x), kInvalid, "x must be FLOAT, FLOAT16 or BF16");
+    OPAPI_CHECK(x->dims.size() == 2 || x->dims.size() == 3, kInvalid, "x must have rank 2 or 3, not %zu", x->dims.size());
+    for (int64_t d : x->dims) OPAPI_CHECK(d <= 2147483647ll, kInvalid, "an extent of x is larger than 2147483647");
+    const int64_t cols = x->dims.back();
+    OPAPI_CHECK(cols > 0, kInvalid, "the last extent of x is zero");
+    shape->cols = cols;
+    shape->rows = RowsOf(x);
+    OPAPI_CHECK(shape->rows >= 0, kInvalid, "x has more than %lld rows", (long long)kMaxRows);
+    shape->weightType = x->dtype;
+    const aclTensor* const first = postGamma != nullptr ? postGamma : preGamma;
+    for (const aclTensor* gamma : {postGamma, preGamma}) {
+        OPAPI_CHECK(gamma == nullptr || ((gamma->dtype == x->dtype || gamma->dtype == ACL_FLOAT) && HasExtents(gamma, {cols})), kInvalid,
+                    "%s %s must be [%lld] of x's type or FLOAT", gamma == postGamma ? "postGamma" : "preGamma", ShapeStr(gamma).c_str(), (long long)cols);
+        OPAPI_CHECK(gamma == nullptr || gamma->dtype == first->dtype, kInvalid, "postGamma and preGamma must have one type");
+    }
+    if (first != nullptr) shape->weightType = first->dtype;
+    OPAPI_CHECK(gateType == 0 || gateType == 1, kInvalid, "gateType (=%lld) must be 0 or 1", (long long)gateType);
+    OPAPI_CHECK(std::isfinite(static_cast<float>(residualScale)) && std::isfinite(static_cast<float>(branchScale)), kInvalid,
+                "residualScale and branchScale must be finite numbers");
+    if (gate == nullptr) return ACLNN_SUCCESS;
+    const bool floating = gate->dtype == x->dtype || gate->dtype == ACL_FLOAT;
+    if (HasExtents(gate, {cols})) {
+        OPAPI_CHECK(floating && (first == nullptr || gate->dtype == first->dtype), kInvalid,
+                    "a gate [%lld] must be of x's type or FLOAT, and of the gammas' type", (long long)cols);
+        shape->gateKind = kGateChannel;
+        shape->weightType = gate->dtype;
+    } else if (SameButLast(gate, x, 1)) {
+        OPAPI_CHECK(floating, kInvalid, "a gate of a value per row must be of x's type or FLOAT");
+        shape->gateKind = kGateRow;
+        shape->gateIsFloat = gate->dtype == ACL_FLOAT;
+    } else {
+        OPAPI_CHECK(SameButLast(gate, x, cols) && gate->dtype == x->dtype, kInvalid,
+                    "gate %s must be [%lld], x's extents %s with the last one 1, or these and x's type", ShapeStr(gate).c_str(), (long long)cols,
+                    ShapeStr(x).c_str());
+        shape->gateKind = kGateEach;
+    }
+    return ACLNN_SUCCESS;
+}
+
+// A tensor of x's type and extents (absent ones pass).
+inline bool Like(const aclTensor* t, const aclTensor* x) { return t == nullptr || (t->dtype == x->dtype && SameButLast(t, x, x->dims.back())); }
+// A FLOAT of x's rows.
+inline bool PerRow(const aclTensor* t, const aclTensor* x) { return t == nullptr || (t->dtype == ACL_FLOAT && SameButLast(t, x, -1)); }
+
+// f(element type, weights' type) as tags.
+template <typename F>
+void ForTypes(aclDataType type, aclDataType weightType, F f) {
+    if (type == ACL_FLOAT) f(F32{}, F32{});
+    else if (type == ACL_FLOAT16) weightType == type ? f(F16{}, F16{}) : f(F16{}, F32{});
+    else weightType == type ? f(Bf16{}, Bf16{}) : f(Bf16{}, F32{});
+}
+
+}  // namespace moe_front
