@@ -38,13 +38,15 @@ struct BalanceArgs {
 constexpr int kChunkThreads = 512;
 constexpr int kChunkWaves = kChunkThreads / kWave;
 // A lane's rows in flight: their loads and reductions overlap.
-constexpr int UnrollOf(int pieces) { return pieces == 1 ? 4 : pieces == 2 ? 2 : 1; }
+constexpr int UnrollOf(int pieces) { return pieces <= 2 ? 2 : 1; }
 // Chunks: as many as there are CUs, of at least the rows that a workgroup has in flight at once, and of at most so many that a lane's fp32 sums stay short.
 constexpr int64_t kMostChunks = 256, kMaxChunkRows = 4096;
 // One sequence of up to so many such passes is one workgroup's: it spares the second launch.
-constexpr int64_t kAlonePasses = 4;
-constexpr int kFinishExperts = 64;
+constexpr int64_t kAlonePasses = 8;
+// A workgroup of the second kernel takes few experts in many runs of pieces, or, where a sequence has few pieces, many in few.
 constexpr int kFinishThreads = 1024;
+constexpr int kFinishFew = 64, kFinishMany = 256;
+constexpr int64_t kFewPieces = 64;
 
 template <typename Codec, int kLanes, int kPieces, bool kSigmoid>
 __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs a) {
@@ -53,7 +55,7 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
     constexpr int kRowsAtOnce = kWave / kLanes;
     constexpr int kUnroll = UnrollOf(kPieces);
     constexpr int kStride = kChunkWaves * kRowsAtOnce;
-    __shared__ float sums[kChunkWaves][Row::kWidth];
+    __shared__ alignas(16) float sums[kChunkWaves][Row::kWidth];
     __shared__ int32_t picked[Row::kWidth];
     __shared__ int32_t live;
     __shared__ double finishing[kChunkWaves];
@@ -61,143 +63,215 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x);
     auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
 
-    // Leaves the sums of rows [begin, end) in `sums` by wave, their picks in `picked` and how many count in `live`.
-    auto sumUp = [&](int64_t begin, int64_t end) {
-        for (int e = tid; e < a.experts; e += kChunkThreads) picked[e] = 0;
-        if (tid == 0) live = 0;
-        __syncthreads();
-        float sum[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
-        int32_t counted = 0;
-        for (int64_t at = begin + wave * kRowsAtOnce + group; at < end; at += kUnroll * kStride) {
-            float v[kUnroll][kEach];
-            int32_t id[kUnroll];
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const int64_t row = min(at + u * kStride, end - 1);
-                id[u] = a.expertIdx[row * a.k];
-                Row::template Load<Codec>(x + row * a.experts, a.experts, l, -INFINITY, v[u]);
-            }
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const bool counts = at + u * kStride < end && isExpert(id[u]);
-                float share[kEach];
-                if constexpr (kSigmoid) {
-                    float p[kEach];
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) p[i] = SigmoidOf(v[u][i]).p;
-                    SharesOf<kLanes>(v[u], p, share);
-                } else {
-                    SoftmaxOf<kLanes>(v[u]);
-#pragma unroll
-                    for (int i = 0; i < kEach; ++i) share[i] = v[u][i];
-                }
-#pragma unroll
-                for (int i = 0; i < kEach; ++i) sum[i] += counts ? share[i] : 0.f;
-                counted += counts && l == 0 ? 1 : 0;
-            }
-        }
-        if (counted != 0) atomicAdd(&live, counted);
-        // the rows side by side in a wave; the waves are added up when they are read
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            for (int d = kLanes; d < kWave; d <<= 1) sum[i] += __shfl_xor(sum[i], d);
-        }
-        if (lane < kLanes) {
-#pragma unroll
-            for (int p = 0; p < kPieces; ++p) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sums[wave][Row::At(p, l) + i] = sum[4 * p + i];
-            }
-        }
-        const int32_t ids = static_cast<int32_t>(end - begin) * a.k;
-        const int32_t* const idx = a.expertIdx + begin * a.k;
-        for (int32_t i = tid; i < ids; i += kChunkThreads) {
-            const int32_t id = idx[i];
-            if (isExpert(idx[i / a.k * a.k]) && isExpert(id)) atomicAdd(&picked[id], 1);
-        }
-        __syncthreads();
-    };
     auto totalOf = [&](int e) {
         float total = 0.f;
 #pragma unroll
         for (int w = 0; w < kChunkWaves; ++w) total += sums[w][e];
         return total;
     };
-
     const Sequences& seqs = a.sequences;
+    int64_t first = static_cast<int64_t>(blockIdx.x) * a.chunkRows, last = min(first + a.chunkRows, seqs.rows);
     if (a.alone) {
-        sumUp(seqs.Start(0), max(seqs.Start(0), seqs.Start(1)));
-        const double n = live > 0 ? live : 1;
-        double loss = 0.0;
-        for (int e = tid; e < a.experts; e += kChunkThreads) {
-            const double mean = totalOf(e) / n;
-            a.counts[e] = picked[e];
-            if (a.prob != nullptr) a.prob[e] = static_cast<float>(mean);
-            loss += mean * picked[e];
-        }
-        loss = WaveSum(loss);
-        if (lane == 0) finishing[wave] = loss;
-        __syncthreads();
-        if (tid == 0) {
-            loss = 0.0;
-            for (int w = 0; w < kChunkWaves; ++w) loss += finishing[w];
-            a.loss[0] = static_cast<float>(loss * a.experts / (a.k * n));
-            a.rowsOut[0] = live;
-        }
-        return;
+        first = seqs.Start(0);
+        last = max(first, seqs.Start(1));
     }
-    if (blockIdx.x == 0) {  // for the second kernel
+    // Rows that a lane has in flight: those of the next pass are asked for before the present one's scores are worked out, those of the first one, and
+    // each lane's first id, before the workgroup looks for their sequence.
+    typename Row::template Raw<typename Codec::Storage> raw[kUnroll];
+    int32_t rowIds[kUnroll], id = -1, rowId = -1;
+    auto load = [&](int64_t at, int64_t end) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t row = min(at + u * kStride, end - 1);
+            rowIds[u] = a.expertIdx[row * a.k];
+            raw[u] = Row::Ask(x + row * a.experts, a.experts, l);
+        }
+    };
+    auto loadFirst = [&](int64_t begin, int64_t end) {
+        if (begin + wave * kRowsAtOnce + group < end) load(begin + wave * kRowsAtOnce + group, end);
+        if (tid < (end - begin) * a.k) {
+            id = a.expertIdx[begin * a.k + tid];
+            rowId = a.expertIdx[(begin + tid / a.k) * a.k];
+        }
+    };
+    loadFirst(first, last);
+    for (int e = tid; e < a.experts; e += kChunkThreads) picked[e] = 0;
+    if (tid == 0) live = 0;
+    if (blockIdx.x == 0 && !a.alone) {  // for the second kernel
         for (int s = tid; s < seqs.count; s += kChunkThreads) a.tickets[s] = 0;
     }
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * a.chunkRows, last = min(first + a.chunkRows, seqs.rows);
-    int32_t s = -2;
-    for (int64_t at = first; at < last;) {
-        // `at` is in the next sequence, unless some have no rows; whatever the offsets are, s starts at or in front of it and ends behind it
-        s = s >= 0 && s + 1 < seqs.count && seqs.Start(s + 2) > at ? s + 1 : seqs.Of(at);
-        if (s >= seqs.count) break;
-        const int64_t end = min(last, seqs.Start(s + 1));
-        if (s >= 0) {
-            sumUp(at, end);
-            const int64_t piece = static_cast<int64_t>(blockIdx.x) + s;
-            for (int e = tid; e < a.experts; e += kChunkThreads) {
-                a.pieceSums[piece * a.experts + e] = totalOf(e);
-                a.pieceCounts[piece * a.experts + e] = picked[e];
+    __syncthreads();
+    int32_t s = -1;
+    int64_t following = first;  // where the sequence behind s ends
+    for (int64_t at = first;;) {
+        int64_t end = last;
+        if (!a.alone) {
+            if (at >= last) return;
+            if (seqs.offsets == nullptr) {
+                s = 0;
+            } else {
+                // `at` is in the next sequence, unless some have no rows; whatever the offsets are, s starts at or in front of it and ends behind it
+                if (following > at) {
+                    end = following;
+                    ++s;
+                } else {
+                    s = seqs.Of(at, end);
+                }
+                if (s >= seqs.count) return;
+                end = min(last, end);
             }
-            if (tid == 0) a.pieceRows[piece] = live;
-            __syncthreads();  // the tables are cleared for the next sequence
+            if (s < 0) {
+                at = end;
+                following = 0;
+                if (at < last) loadFirst(at, last);
+                continue;
+            }
+        }
+        float sum[kEach];
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
+        int32_t counted = 0;
+#pragma unroll 1
+        for (int64_t row = at + wave * kRowsAtOnce + group; row < end; row += kUnroll * kStride) {
+            // Scores, for softmax before their division by the sum.  Row by row without a branch: the rows' reductions overlap.
+            float p[kUnroll][kEach], total[kUnroll];
+            bool counts[kUnroll], lost = false;
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                counts[u] = row + u * kStride < end && isExpert(rowIds[u]);
+                Row::template Logits<Codec>(raw[u], a.experts, l, p[u]);
+            }
+            if (row + kUnroll * kStride < end) load(row + kUnroll * kStride, end);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if constexpr (kSigmoid) {
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) p[u][i] = SigmoidOf(p[u][i]).p;
+                } else {
+                    const ExpFrom e(TopOf<kLanes>(p[u]));
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) p[u][i] = e(p[u][i]);
+                }
+                total[u] = 0.f;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) total[u] += p[u][i];
+                total[u] = SumOver<kLanes>(total[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                counted += counts[u] && l == 0 ? 1 : 0;
+                if (kSigmoid && counts[u] && total[u] < kLostSum) {
+                    lost = true;
+                    counts[u] = false;
+                }
+                const float inverse = total[u] == 0.f ? 0.f : Reciprocal(total[u]);
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) sum[i] = counts[u] ? fmaf(p[u][i], inverse, sum[i]) : sum[i];
+            }
+            if (kSigmoid && lost) {  // rare, and made again (the lanes of a row agree)
+#pragma unroll 1
+                for (int64_t again = row; again < min(row + kUnroll * kStride, end); again += kStride) {
+                    float v[kEach], share[kEach], scores = 0.f;
+                    Row::template Logits<Codec>(Row::Ask(x + again * a.experts, a.experts, l), a.experts, l, v);
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) scores += SigmoidOf(v[i]).p;
+                    if (!(SumOver<kLanes>(scores) < kLostSum) || !isExpert(a.expertIdx[again * a.k])) continue;
+                    LostSharesOf<kLanes>(v, share);
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) sum[i] += share[i];
+                }
+            }
+        }
+        counted = WaveSum(counted);
+        if (lane == 0 && counted != 0) atomicAdd(&live, counted);
+        const int32_t ids = static_cast<int32_t>(end - at) * a.k;
+        if (tid < ids && isExpert(rowId) && isExpert(id)) atomicAdd(&picked[id], 1);
+#pragma unroll 1
+        for (int32_t i = tid + kChunkThreads; i < ids; i += kChunkThreads) {
+            const int32_t* const idx = a.expertIdx + at * a.k;
+            const int32_t more = idx[i];
+            if (isExpert(idx[i / a.k * a.k]) && isExpert(more)) atomicAdd(&picked[more], 1);
+        }
+        if (end < last) {  // what comes behind this sequence, on its way meanwhile
+            loadFirst(end, last);
+            following = s + 2 <= seqs.count ? seqs.Start(s + 2) : 0;
+        }
+        // the rows side by side in a wave; the waves are added up when they are read
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+#pragma unroll
+            for (int d = kLanes; d < kWave; d <<= 1) sum[i] += __shfl_xor(sum[i], d);
+        }
+        if (lane < kLanes) {
+#pragma unroll
+            for (int p = 0; p < kPieces; ++p) *reinterpret_cast<float4*>(&sums[wave][Row::At(p, l)]) = float4{sum[4 * p], sum[4 * p + 1], sum[4 * p + 2], sum[4 * p + 3]};
+        }
+        __syncthreads();
+        if (a.alone) break;
+        const int64_t piece = static_cast<int64_t>(blockIdx.x) + s;
+#pragma unroll 1
+        for (int e = tid; e < a.experts; e += kChunkThreads) {
+            a.pieceSums[piece * a.experts + e] = totalOf(e);
+            a.pieceCounts[piece * a.experts + e] = picked[e];
+            picked[e] = 0;  // for the next sequence
+        }
+        if (tid == 0) {
+            a.pieceRows[piece] = live;
+            live = 0;
         }
         at = end;
+        if (at >= last) return;
+        __syncthreads();
     }
+    const double n = live > 0 ? live : 1;
+    double loss = 0.0;
+#pragma unroll 1
+    for (int e = tid; e < a.experts; e += kChunkThreads) {
+        const double mean = totalOf(e) / n;
+        a.counts[e] = picked[e];
+        if (a.prob != nullptr) a.prob[e] = static_cast<float>(mean);
+        loss += mean * picked[e];
+    }
+    loss = WaveSum(loss);
+    if (lane == 0) finishing[wave] = loss;
+    __syncthreads();
+    if (tid != 0) return;
+    loss = 0.0;
+    for (int w = 0; w < kChunkWaves; ++w) loss += finishing[w];
+    a.loss[0] = static_cast<float>(loss * a.experts / (a.k * n));
+    a.rowsOut[0] = live;
 }
 
-// A sequence and kFinishExperts of its experts: the pieces' sums in their order, in runs side by side.  The workgroup of a sequence that ends last adds up
-// the loss, part by part in their order.
+// A sequence and kExperts of its experts: the pieces' sums in their order, in runs side by side.  Where one workgroup does not hold all experts, the one
+// of a sequence that ends last adds up the loss, part by part in their order.
+template <int kExperts>
 __global__ __launch_bounds__(kFinishThreads) void BalanceFinishKernel(BalanceArgs a) {
-    constexpr int kRuns = kFinishThreads / kFinishExperts;
-    __shared__ double sums[kRuns][kFinishExperts];
-    __shared__ int32_t picks[kRuns][kFinishExperts];
+    constexpr int kRuns = kFinishThreads / kExperts, kWaves = kExperts / kWave;
+    __shared__ double sums[kRuns][kExperts];
+    __shared__ int32_t picks[kRuns][kExperts];
     __shared__ int32_t rowsOf[kFinishThreads / kWave];
-    const int64_t group = GroupIndex();
-    const int32_t parts = (a.experts + kFinishExperts - 1) / kFinishExperts;
-    const int64_t s = group / parts;
-    if (s >= a.sequences.count) return;
-    const int part = static_cast<int>(group % parts);
-    const int tid = threadIdx.x, run = tid / kFinishExperts, lane = tid % kFinishExperts;
-    const int e = part * kFinishExperts + lane;
+    __shared__ double losses[kWaves];
+    // (32 bits hold every sequence's parts, and every row: divisions of 64 would be a good part of this kernel)
+    const uint32_t group = static_cast<uint32_t>(GroupIndex()), parts = static_cast<uint32_t>(a.experts + kExperts - 1) / kExperts;
+    const uint32_t whose = parts == 1 ? group : group / parts;
+    if (whose >= static_cast<uint32_t>(a.sequences.count)) return;
+    const int64_t s = whose;
+    const int part = static_cast<int>(group - whose * parts);
+    const int tid = threadIdx.x, run = tid / kExperts, lane = tid % kExperts;
+    const int e = part * kExperts + lane;
     const int64_t begin = a.sequences.Start(s), end = a.sequences.Start(s + 1);
     int64_t from = 0, to = 0;
     if (begin < end) {
-        from = begin / a.chunkRows + s;
-        to = (end - 1) / a.chunkRows + 1 + s;
+        const uint32_t chunkRows = static_cast<uint32_t>(a.chunkRows);
+        from = static_cast<uint32_t>(begin) / chunkRows + s;
+        to = static_cast<uint32_t>(end - 1) / chunkRows + 1 + s;
     }
     int32_t live = 0;
     for (int64_t p = from + tid; p < to; p += kFinishThreads) live += a.pieceRows[p];
     double sum = 0.0;
     int32_t count = 0;
     if (e < a.experts) {
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t p = from + run; p < to; p += kRuns) {
             sum += a.pieceSums[p * a.experts + e];
             count += a.pieceCounts[p * a.experts + e];
@@ -208,30 +282,34 @@ __global__ __launch_bounds__(kFinishThreads) void BalanceFinishKernel(BalanceArg
     sums[run][lane] = sum;
     picks[run][lane] = count;
     __syncthreads();
-    if (run != 0) return;
-    static_assert(kFinishExperts == kWave, "one wave is left");
     live = 0;
     for (int w = 0; w < kFinishThreads / kWave; ++w) live += rowsOf[w];
     const double n = live > 0 ? live : 1;
-    sum = 0.0;
-    count = 0;
-    for (int r = 0; r < kRuns; ++r) {
-        sum += sums[r][lane];
-        count += picks[r][lane];
+    double loss = 0.0;
+    if (run == 0) {
+        sum = 0.0;
+        count = 0;
+        for (int r = 0; r < kRuns; ++r) {
+            sum += sums[r][lane];
+            count += picks[r][lane];
+        }
+        const double mean = sum / n;
+        if (e < a.experts) {
+            a.counts[s * a.experts + e] = count;
+            if (a.prob != nullptr) a.prob[s * a.experts + e] = static_cast<float>(mean);
+        }
+        loss = WaveSum(mean * count);
+        if (tid % kWave == 0) losses[tid / kWave] = loss;
     }
-    const double mean = sum / n;
-    if (e < a.experts) {
-        a.counts[s * a.experts + e] = count;
-        if (a.prob != nullptr) a.prob[s * a.experts + e] = static_cast<float>(mean);
-    }
-    double loss = WaveSum(mean * count);
-    if (lane != 0) return;
+    if constexpr (kWaves > 1) __syncthreads();
+    if (tid != 0) return;
+    for (int w = 1; w < kWaves; ++w) loss += losses[w];
     if (parts > 1) {
         double* const all = a.lossParts + s * parts;
         __hip_atomic_store(all + part, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (__hip_atomic_fetch_add(a.tickets + s, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) != static_cast<uint32_t>(parts - 1)) return;
+        if (__hip_atomic_fetch_add(a.tickets + s, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) != parts - 1) return;
         loss = 0.0;
-        for (int i = 0; i < parts; ++i) loss += __hip_atomic_load(all + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (uint32_t i = 0; i < parts; ++i) loss += __hip_atomic_load(all + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     a.loss[s] = static_cast<float>(loss * a.experts / (a.k * n));
     a.rowsOut[s] = live;
@@ -241,6 +319,7 @@ class BalanceExecutor : public aclOpExecutor {
    public:
     BalanceArgs args{};
     aclDataType dtype = ACL_FLOAT;
+    int64_t finishExperts = 0;  // of a workgroup of the second kernel
     uint64_t offRows = 0, offCounts = 0, offLoss = 0, offTickets = 0, offSums = 0;
 
     template <typename Codec>
@@ -271,8 +350,10 @@ class BalanceExecutor : public aclOpExecutor {
         }
         if (!args.alone) {
             opapi::KernelTimer timer("balance_finish", stream);
-            const int64_t parts = (args.experts + kFinishExperts - 1) / kFinishExperts;
-            hipLaunchKernelGGL(BalanceFinishKernel, GridOf(parts * args.sequences.count), dim3(kFinishThreads), 0, stream, args);
+            const int64_t parts = (args.experts + finishExperts - 1) / finishExperts;
+            const dim3 grid = GridOf(parts * args.sequences.count);
+            if (finishExperts == kFinishFew) hipLaunchKernelGGL(BalanceFinishKernel<kFinishFew>, grid, dim3(kFinishThreads), 0, stream, args);
+            else hipLaunchKernelGGL(BalanceFinishKernel<kFinishMany>, grid, dim3(kFinishThreads), 0, stream, args);
         }
         const hipError_t err = hipGetLastError();
         OPAPI_CHECK(err == hipSuccess, ACLNN_ERR_RUNTIME_ERROR, "aclnnMoeBalanceLoss: launch failed: %s", hipGetErrorString(err));
@@ -333,7 +414,7 @@ extern "C" aclnnStatus aclnnMoeBalanceLossGetWorkspaceSize(const aclTensor* x, c
     ForRowLayout(experts, [&](auto lanes, auto pieces) { passRows = kChunkWaves * (kWave / decltype(lanes)::value) * UnrollOf(decltype(pieces)::value); });
     a.alone = sequences == 1 && rows <= kAlonePasses * passRows;
     int64_t chunkRows = (rows + kMostChunks - 1) / kMostChunks;
-    if (chunkRows < passRows) chunkRows = passRows;
+    if (chunkRows < 2 * passRows) chunkRows = 2 * passRows;
     if (chunkRows > kMaxChunkRows) chunkRows = kMaxChunkRows;
     a.chunkRows = static_cast<int32_t>(chunkRows);
     a.chunks = a.alone ? 1 : static_cast<int32_t>((rows + chunkRows - 1) / chunkRows);
@@ -341,7 +422,8 @@ extern "C" aclnnStatus aclnnMoeBalanceLossGetWorkspaceSize(const aclTensor* x, c
     uint64_t bytes = 0;
     if (!a.alone) {
         const uint64_t pieces = static_cast<uint64_t>(a.chunks) + static_cast<uint64_t>(sequences);
-        const uint64_t parts = static_cast<uint64_t>((experts + kFinishExperts - 1) / kFinishExperts);
+        ex->finishExperts = a.chunks / sequences <= kFewPieces && experts > kFinishFew ? kFinishMany : kFinishFew;
+        const uint64_t parts = static_cast<uint64_t>((experts + ex->finishExperts - 1) / ex->finishExperts);
         auto take = [&](uint64_t size) {
             const uint64_t at = bytes;
             bytes = AlignUp(bytes + size, 16);

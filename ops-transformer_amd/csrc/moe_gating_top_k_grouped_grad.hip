@@ -33,105 +33,153 @@ struct GradArgs {
 constexpr int kGradThreads = 256;
 constexpr int kGradWaves = kGradThreads / kWave;
 
+// What is asked for of a row before the one in front of it is done.
+template <typename Raw>
+struct RowInputs {
+    Raw x;
+    int32_t first;  // its first id
+    int32_t id;     // the lane's pick, the first of its own where a row has more picks than lanes, and its gradient
+    float y;
+};
+
+// What bounds it: the chain of a row's steps, and its arithmetic.  Scores are held unnormalised, so that their sum, that of the picked ones and both
+// means are reduced side by side.
 template <typename Codec, typename Out, int kLanes, int kPieces, bool kSigmoid>
 __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
     using Row = RowOf<kLanes, kPieces>;
     constexpr int kEach = Row::kEach;
     constexpr int kRowsAtOnce = kWave / kLanes;
-    __shared__ float4 picked[kGradWaves][kRowsAtOnce][Row::kWidth / 4];
+    __shared__ float4 scores[kGradWaves][kRowsAtOnce][Row::kWidth / 4];
+    __shared__ float4 picked[kGradWaves][kRowsAtOnce][Row::kWidth / 4];  // zero between rows
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, l = lane % kLanes, side = lane / kLanes;
-    float* const mine = reinterpret_cast<float*>(picked[wave][side]);
+    const float* const scoreOf = reinterpret_cast<const float*>(scores[wave][side]);
+    float* const pickedOf = reinterpret_cast<float*>(picked[wave][side]);
     const bool weights = a.yGrad != nullptr, balance = a.lossGrad != nullptr;
+    auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
+    auto yGradOf = [&](int64_t row, int j) {
+        const int64_t at = row * a.k + j;
+        return a.yGradIsFloat ? static_cast<const float*>(a.yGrad)[at] : Codec::Load(static_cast<const typename Codec::Storage*>(a.yGrad)[at]);
+    };
+    // The rows of a wave follow each other, `side` by side: their sequence changes seldom, and with it the counts in registers.
+    const int64_t first = (GroupIndex() * kGradWaves + wave) * a.waveRows, last = min(first + a.waveRows, a.sequences.rows);
+    if (first >= last) return;
+    using Inputs = RowInputs<typename Row::template Raw<typename Codec::Storage>>;
+    Inputs in;
+    auto load = [&](int64_t row) {
+        in.x = Row::Ask(static_cast<const typename Codec::Storage*>(a.x) + row * a.experts, a.experts, l);
+        in.first = a.expertIdx[row * a.k];
+        in.id = -1;
+        in.y = 0.f;
+        if (weights && l < a.k) {
+            in.id = a.expertIdx[row * a.k + l];
+            in.y = yGradOf(row, l);
+        }
+    };
+    if (first + side < last) load(first + side);
     if (weights) {
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) picked[wave][side][Row::At(p, l) / 4] = float4{0.f, 0.f, 0.f, 0.f};
     }
-    // The rows of a wave follow each other, `side` by side: their sequence changes seldom, and with it the counts in registers.
-    const int64_t first = (GroupIndex() * kGradWaves + wave) * a.waveRows, last = min(first + a.waveRows, a.sequences.rows);
-    int32_t sequence = -2;  // of this row, its end, and what its loss gives each share
+    int32_t sequence = -2;     // of the row, and where it ends
     int64_t sequenceEnd = -1;
-    float shareGrad[kEach];
+    bool inside = false;       // whether it is one
+    float shareGrad[kEach];    // what its loss gives each share
 #pragma unroll
     for (int i = 0; i < kEach; ++i) shareGrad[i] = 0.f;
+    // The loads of a sequence go out together, those of rows in none being of another one's.
+    auto enter = [&](int32_t s, int64_t end) {
+        sequenceEnd = end;
+        sequence = s;
+        inside = s >= 0 && s < a.sequences.count;
+        const int32_t at = s < 0 ? 0 : min(s, a.sequences.count - 1);
+        const int32_t rows = a.seqRows[at];
+        const float lossGrad = a.lossGrad[at];
+        const auto raw = Row::Ask(a.counts + static_cast<int64_t>(at) * a.experts, a.experts, l);
+        int32_t counts[kEach];
+        Row::Place(raw, a.experts, l, 0, counts);
+        const float n = static_cast<float>(rows);
+        const float each = rows > 0 ? lossGrad * (static_cast<float>(a.experts) / static_cast<float>(a.k)) / n / n : 0.f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) shareGrad[i] = rows > 0 ? each * static_cast<float>(counts[i]) : 0.f;
+    };
+    if (balance) {
+        int64_t end;
+        const int32_t s = a.sequences.Of(first, end);
+        enter(s, end);
+    }
     for (int64_t row = first + side; row < last; row += kRowsAtOnce) {
-        const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x) + row * a.experts;
-        const int32_t* const idx = a.expertIdx + row * a.k;
-        auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
-        float v[kEach];
-        Row::template Load<Codec>(x, a.experts, l, -INFINITY, v);
-        const bool live = isExpert(idx[0]);
-        if (balance && row >= sequenceEnd) {
-            sequence = a.sequences.Of(row);
-            const bool inside = sequence >= 0 && sequence < a.sequences.count;
-            sequenceEnd = inside ? a.sequences.Start(sequence + 1) : sequence < 0 ? a.sequences.Start(0) : a.sequences.rows;
-            const float n = inside ? static_cast<float>(a.seqRows[sequence]) : 0.f;
-            const float each = n > 0.f ? a.lossGrad[sequence] * (static_cast<float>(a.experts) / static_cast<float>(a.k)) / n / n : 0.f;
-#pragma unroll
-            for (int p = 0; p < kPieces; ++p) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int e = Row::At(p, l) + i;
-                    shareGrad[4 * p + i] = n > 0.f && e < a.experts ? each * static_cast<float>(a.counts[static_cast<int64_t>(sequence) * a.experts + e]) : 0.f;
-                }
-            }
+        if (balance && row >= sequenceEnd && sequence < a.sequences.count) {
+            int64_t end;
+            const int32_t s = SequenceBehind(a.sequences, sequence, row, end);
+            enter(s, end);
         }
-        // scores: p, and 1 - p of sigmoid ones
-        float p[kEach], rest[kEach];
-        Softmax softmax{};
+        const Inputs now = in;
+        if (row + kRowsAtOnce < last) load(row + kRowsAtOnce);
+        float x[kEach];
+        Row::template Logits<Codec>(now.x, a.experts, l, x);
+        // p: sigmoid's score, with rest = 1 - p, or softmax's before its division by the sum
+        float p[kEach], rest[kSigmoid ? kEach : 1];
         if constexpr (kSigmoid) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                const Sigmoid s = SigmoidOf(v[i]);
+                const Sigmoid s = SigmoidOf(x[i]);
                 p[i] = s.p;
                 rest[i] = s.rest;
             }
         } else {
+            const ExpFrom e(TopOf<kLanes>(x));
 #pragma unroll
-            for (int i = 0; i < kEach; ++i) p[i] = v[i];
-            softmax = SoftmaxOf<kLanes>(p);
+            for (int i = 0; i < kEach; ++i) p[i] = e(x[i]);
+        }
+        float sum = 0.f, shared = 0.f, pickedSum = 0.f, weighted = 0.f;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            sum += p[i];
+            shared = fmaf(shareGrad[i], p[i], shared);
+        }
+        if (weights) {
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q) scores[wave][side][Row::At(q, l) / 4] = float4{p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]};
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (isExpert(now.id)) {
+                pickedSum = scoreOf[now.id];
+                weighted = now.y * pickedSum;
+            }
+            for (int j = l + kLanes; j < a.k; j += kLanes) {
+                const int32_t id = a.expertIdx[row * a.k + j];
+                if (!isExpert(id)) continue;
+                pickedSum += scoreOf[id];
+                weighted = fmaf(yGradOf(row, j), scoreOf[id], weighted);
+            }
+        }
+        sum = SumOver<kLanes>(sum);
+        shared = SumOver<kLanes>(shared);
+        if (weights) {
+            pickedSum = SumOver<kLanes>(pickedSum);
+            weighted = SumOver<kLanes>(weighted);
+        }
+        const float inverse = sum == 0.f ? 0.f : Reciprocal(sum);
+        if constexpr (!kSigmoid) {
+            pickedSum *= inverse;
+            weighted *= inverse;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) p[i] *= inverse;
         }
         float grad[kEach];
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) grad[i] = 0.f;
         if (weights) {
-            auto yGradOf = [&](int j) {
-                const int64_t at = row * a.k + j;
-                return a.yGradIsFloat ? static_cast<const float*>(a.yGrad)[at] : Codec::Load(static_cast<const typename Codec::Storage*>(a.yGrad)[at]);
-            };
-            auto scoreOf = [&](int32_t id) {
-                const float logit = Codec::Load(x[id]);
-                if constexpr (kSigmoid) return SigmoidOf(logit).p;
-                else return softmax.Of(logit);
-            };
-            float sum = 0.f, weighted = 0.f;
-            int32_t id0 = -1;  // the lane's first pick, kept
-            float y0 = 0.f;
-            for (int j = l; j < a.k; j += kLanes) {
-                const int32_t id = idx[j];
-                const float y = yGradOf(j);
-                if (j == l) {
-                    id0 = id;
-                    y0 = y;
-                }
-                if (!isExpert(id)) continue;
-                const float score = scoreOf(id);
-                sum += score;
-                weighted += y * score;
-            }
-            sum = SumOver<kLanes>(sum);
-            weighted = SumOver<kLanes>(weighted);
             float mean = 0.f, scale = a.factor, all = a.factor * weighted;
             if (a.renorm) {
-                const float total = sum + a.eps;
-                scale = total == 0.f ? 0.f : a.factor / total;
-                mean = total == 0.f ? 0.f : weighted / total;
-                all = total == 0.f ? 0.f : a.factor * mean * (a.eps / total);
-                if (sum == 0.f) scale = mean = all = 0.f;
+                const float total = pickedSum + a.eps;
+                const bool none = pickedSum == 0.f;
+                scale = none ? 0.f : a.factor / total;
+                mean = none ? 0.f : weighted / total;
+                all = none ? 0.f : a.factor * mean * (a.eps / total);
             }
-            for (int j = l; j < a.k; j += kLanes) {
-                const int32_t id = j == l ? id0 : idx[j];
-                const float y = j == l ? y0 : yGradOf(j);
-                if (isExpert(id)) atomicAdd(mine + id, scale * (y - mean));
+            if (isExpert(now.id)) atomicAdd(pickedOf + now.id, scale * (now.y - mean));
+            for (int j = l + kLanes; j < a.k; j += kLanes) {
+                const int32_t id = a.expertIdx[row * a.k + j];
+                if (isExpert(id)) atomicAdd(pickedOf + id, scale * (yGradOf(row, j) - mean));
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -143,32 +191,35 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
                 const float d[4] = {dp.x, dp.y, dp.z, dp.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if constexpr (kSigmoid) grad[4 * q + i] = d[i] * p[4 * q + i] * rest[4 * q + i];
+                    if constexpr (kSigmoid) grad[4 * q + i] = d[i] * (p[4 * q + i] * rest[4 * q + i]);
                     else grad[4 * q + i] = p[4 * q + i] * (d[i] - all);
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+        } else {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) grad[i] = 0.f;
         }
-        if (balance) {
-            float share[kEach];
-            if constexpr (kSigmoid) {
-                SharesOf<kLanes>(v, p, share);
-            } else {
+        if (balance && inside) {
+            float share[kEach], mean = shared * inverse;
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) share[i] = p[i];
+            for (int i = 0; i < kEach; ++i) share[i] = kSigmoid ? p[i] * inverse : p[i];
+            if (kSigmoid && sum < kLostSum) {  // (the lanes of a row agree)
+                LostSharesOf<kLanes>(x, share);
+                mean = 0.f;
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) mean = fmaf(shareGrad[i], share[i], mean);
+                mean = SumOver<kLanes>(mean);
             }
-            float mean = 0.f;
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) mean = fmaf(shareGrad[i], share[i], mean);
-            mean = SumOver<kLanes>(mean);
 #pragma unroll
             for (int i = 0; i < kEach; ++i) {
-                float g = share[i] * (shareGrad[i] - mean);
-                if constexpr (kSigmoid) g *= rest[i];
-                grad[i] += sequence >= 0 && sequence < a.sequences.count ? g : 0.f;
+                const float d = shareGrad[i] - mean;
+                if constexpr (kSigmoid) grad[i] = fmaf(share[i] * rest[i], d, grad[i]);
+                else grad[i] = fmaf(share[i], d, grad[i]);
             }
         }
+        const bool live = isExpert(now.first);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) grad[i] = live ? grad[i] : 0.f;
         Row::template Store<Out>(static_cast<typename Out::Storage*>(a.xGrad) + row * a.experts, a.experts, l, grad);

@@ -26,17 +26,43 @@ struct Sequences {
         const int64_t at = isInt64 ? static_cast<const int64_t*>(offsets)[i] : static_cast<const int32_t*>(offsets)[i];
         return at < 0 ? 0 : at > rows ? rows : at;
     }
-    // The last sequence that starts at or in front of `row`: -1 in front of the first, `count` behind the last.
-    __device__ __forceinline__ int32_t Of(int64_t row) const {
-        int64_t lo = -1, hi = static_cast<int64_t>(count) + 1;
+    // The last sequence that starts at or in front of `row`, the same in all lanes of a whole wave: -1 in front of the first, `count` behind the last.  The
+    // lanes look at 64 places at a time, so that the round trips are one for up to 63 sequences and four for the most.  Whatever the offsets are, the
+    // sequence starts at or in front of the row, and the next one, at `end`, behind it (behind the last: all rows).
+    __device__ __forceinline__ int32_t Of(int64_t row, int64_t& end) const {
+        int32_t lo = -1, hi = count + 1;
+        end = rows;
         while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) / 2;
-            if (Start(mid) <= row) lo = mid;
-            else hi = mid;
+            const int32_t step = (hi - lo - 2) / kWave + 1;
+            const int32_t at = lo + (static_cast<int32_t>(threadIdx.x % kWave) + 1) * step;
+            const int32_t start = at < hi ? static_cast<int32_t>(Start(at)) : 0;
+            const uint64_t behind = __ballot(at >= hi || start > row);
+            const int32_t steps = behind == 0 ? kWave : __builtin_ctzll(behind);  // that do not lead behind the row
+            if (behind != 0 && lo + (steps + 1) * step < hi) {
+                hi = lo + (steps + 1) * step;
+                end = __shfl(start, steps);
+            }
+            lo += steps * step;
         }
-        return static_cast<int32_t>(lo);
+        return lo;
     }
 };
+
+// The sequence of a row in the lane's own place, from that of a row in front of it: the next one, if it is not further.
+__device__ __forceinline__ int32_t SequenceBehind(const Sequences& s, int32_t sequence, int64_t row, int64_t& end) {
+    end = s.rows;
+    if (sequence + 1 >= s.count) return sequence + 1;
+    end = s.Start(sequence + 2);
+    if (end > row) return sequence + 1;
+    int32_t lo = sequence + 1, hi = s.count + 1;
+    while (hi - lo > 1) {
+        const int32_t mid = (lo + hi) / 2;
+        if (s.Start(mid) <= row) lo = mid;
+        else hi = mid;
+    }
+    end = hi <= s.count ? s.Start(hi) : s.rows;
+    return lo;
+}
 
 // The value of the lane that is a fixed step away, over a row of sixteen lanes without a trip through LDS.
 template <int kCtl>
@@ -72,23 +98,44 @@ __device__ __forceinline__ float MaxOver(float v) {
     return OverLanes<kLanes>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// e^x for x <= 0 to about three units of 2^-24: the product with log2(e) in two parts, so that its rounding does not grow with x.  Below 2^-126: zero.
-__device__ __forceinline__ float ExpOfNegative(float x) {
-    constexpr float kLog2e = 1.44269502162933349609f, kLog2eRest = 1.925963033500e-8f, kLn2 = 0.693147182464599609375f;
-    const float hi = x * kLog2e;
-    const float lo = fmaf(x, kLog2e, -hi) + x * kLog2eRest;
-    const float e = __builtin_amdgcn_exp2f(hi);
-    return x < -87.33f ? 0.f : fmaf(e, lo * kLn2, e);  // (of -inf: lo is none)
+// 1 / v of numbers that neither it nor they are near the ends of fp32's range, to about a unit of 2^-24 (a division takes three times as long).
+__device__ __forceinline__ float Reciprocal(float v) {
+    const float r = __builtin_amdgcn_rcpf(v);
+    return fmaf(fmaf(-v, r, 1.f), r, r);
 }
 
-// sigmoid(x) and 1 - sigmoid(x), each to its own precision.
+constexpr float kLog2e = 1.44269502162933349609f;
+
+// e^(x - top) for x <= top: the product with log2(e) with what its rounding leaves, so that only the difference's own rounding is |x - top| units of 2^-24,
+// and the rest four.  0 of -inf, and below 2^-126.
+struct ExpFrom {
+    float top;
+    __device__ __forceinline__ explicit ExpFrom(float t) : top(t) {}
+    __device__ __forceinline__ float operator()(float x) const {
+        constexpr float kLn2 = 0.693147182464599609375f, kLog2eRest = 1.925963033500e-8f;
+        const float d = x - top, hi = d * kLog2e;
+        const float lo = fmaf(d, kLog2e, -hi) + d * kLog2eRest;
+        const float e = __builtin_amdgcn_exp2f(hi);
+        return d < -88.f ? 0.f : fmaf(e, lo * kLn2, e);  // (of -inf: lo is none)
+    }
+};
+
+// sigmoid(x) and 1 - sigmoid(x), each to its own precision: |x| + 4 units of 2^-24.  (Of e^-x past fp32's range the reciprocal is 0, and below a half the
+// difference from 1 is the more exact: no value needs a case of its own.)
 struct Sigmoid {
     float p, rest;
 };
 __device__ __forceinline__ Sigmoid SigmoidOf(float x) {
-    const float t = ExpOfNegative(-fabsf(x));
-    const float far = 1.f / (1.f + t), near = t * far;
-    return x < 0.f ? Sigmoid{near, far} : Sigmoid{far, near};
+    const float t = __builtin_amdgcn_exp2f(x * -kLog2e);
+    const float p = __builtin_amdgcn_rcpf(1.f + t);
+    return Sigmoid{p, p > 0.5f ? t * p : 1.f - p};
+}
+
+// -inf in an element type.
+template <typename Codec>
+__device__ __forceinline__ typename Codec::Storage Nothing() {
+    if constexpr (std::is_same_v<Codec, F32>) return -INFINITY;
+    else return std::is_same_v<Codec, F16> ? 0xfc00 : 0xff80;
 }
 
 // A row of experts lies over kLanes lanes in pieces of four: piece p of lane l holds experts 4 (p kLanes + l) to + 3.
@@ -98,22 +145,51 @@ struct RowOf {
     static constexpr int kWidth = kLanes * kEach;  // most experts
     __device__ static __forceinline__ int At(int p, int l) { return 4 * (p * kLanes + l); }
 
-    // Behind the last expert: `fill`.  A piece that is whole is one load, wherever it begins.
-    template <typename Codec>
-    __device__ static __forceinline__ void Load(const typename Codec::Storage* row, int experts, int l, float fill, float (&v)[kEach]) {
+    // A lane's pieces as they come from memory: one load each without a branch and without a use, so that several rows' are on their way together.  A piece
+    // that would end behind the row is the row's last four elements.
+    template <typename T>
+    struct Raw {
+        T e[kEach];
+    };
+    template <typename T>
+    __device__ static __forceinline__ Raw<T> Ask(const T* row, int experts, int l) {
+        Raw<T> raw;
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
-            const int at = At(p, l);
-            typename Codec::Storage raw[4];
-            if (at + 4 <= experts) {
-                __builtin_memcpy(raw, row + at, sizeof(raw));
+            if (kLanes == 2 && experts < 4) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * p + i] = Codec::Load(raw[i]);
+                for (int i = 0; i < 4; ++i) raw.e[4 * p + i] = row[min(i, experts - 1)];
             } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[4 * p + i] = at + i < experts ? Codec::Load(row[at + i]) : fill;
+                __builtin_memcpy(raw.e + 4 * p, row + min(At(p, l), experts - 4), 4 * sizeof(T));
             }
         }
+        return raw;
+    }
+    // Their elements in their places; behind the last expert: `fill`.
+    template <typename T>
+    __device__ static __forceinline__ void Place(const Raw<T>& raw, int experts, int l, T fill, T (&v)[kEach]) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[i] = raw.e[i];
+        if (experts == kWidth) return;
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+            const int at = At(p, l), behind = kLanes == 2 && experts < 4 ? 0 : at - min(at, experts - 4);
+            T* const e = v + 4 * p;
+            const bool one = (behind & 1) != 0, two = (behind & 2) != 0;  // three in two steps
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = one ? (i < 3 ? e[i + 1] : fill) : e[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = two ? (i < 2 ? e[i + 2] : fill) : e[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = at + i < experts ? e[i] : fill;
+        }
+    }
+    template <typename Codec>
+    __device__ static __forceinline__ void Logits(const Raw<typename Codec::Storage>& raw, int experts, int l, float (&v)[kEach]) {
+        typename Codec::Storage placed[kEach];
+        Place(raw, experts, l, Nothing<Codec>(), placed);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) v[i] = Codec::Load(placed[i]);
     }
     template <typename Codec>
     __device__ static __forceinline__ void Store(typename Codec::Storage* row, int experts, int l, const float (&v)[kEach]) {
@@ -135,59 +211,41 @@ struct RowOf {
     }
 };
 
-// Softmax of a row of logits: x -> p, and what makes a logit's p of it.  A row without a logit above -inf has zeros; NaN and +inf give NaN throughout.
-struct Softmax {
-    float top, inverse;
-    __device__ __forceinline__ float Of(float x) const { return ExpOfNegative(x - top) * inverse; }
-};
+// The largest of a row's logits, as the point that exponentials are taken from: 0 for a row without a logit above -inf.  A NaN is passed over.
 template <int kLanes, int kEach>
-__device__ __forceinline__ Softmax SoftmaxOf(float (&v)[kEach]) {
+__device__ __forceinline__ float TopOf(const float (&v)[kEach]) {
     float top = v[0];
 #pragma unroll
     for (int i = 1; i < kEach; ++i) top = fmaxf(top, v[i]);
     top = MaxOver<kLanes>(top);
-    if (top == -INFINITY) top = 0.f;
+    return top == -INFINITY ? 0.f : top;
+}
+
+// Softmax of a row of logits in their place.  A row without a logit above -inf has zeros; NaN and +inf give NaN throughout.
+template <int kLanes, int kEach>
+__device__ __forceinline__ void SoftmaxOf(float (&v)[kEach]) {
+    const ExpFrom e(TopOf<kLanes>(v));
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-        v[i] = ExpOfNegative(v[i] - top);
+        v[i] = e(v[i]);
         sum += v[i];
     }
     sum = SumOver<kLanes>(sum);
-    const Softmax s{top, sum == 0.f ? 0.f : 1.f / sum};
+    const float inverse = sum == 0.f ? 0.f : Reciprocal(sum);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) v[i] *= s.inverse;
-    return s;
+    for (int i = 0; i < kEach; ++i) v[i] *= inverse;
 }
 
-// Shares of the row's sum of sigmoid scores, from the scores p.  Where every score is nearly lost in fp32 they are in the proportions of e^x, taken from
-// the largest logit; a row without a logit above -inf has zeros.
+// Shares of the row's sum of sigmoid scores.  Where that sum is below kLostSum the scores are nearly or wholly lost in fp32: they are in the proportions of
+// e^x then, which is the softmax (a row without a logit above -inf has zeros).
+constexpr float kLostSum = 0x1p-60f;
 template <int kLanes, int kEach>
-__device__ __forceinline__ void SharesOf(const float (&x)[kEach], const float (&p)[kEach], float (&share)[kEach]) {
-    float sum = 0.f;
+__device__ __forceinline__ void LostSharesOf(const float (&x)[kEach], float (&share)[kEach]) {
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += p[i];
-    sum = SumOver<kLanes>(sum);
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) share[i] = p[i];
-    if (sum < 0x1p-60f) {  // (the lanes of a row agree)
-        float top = x[0];
-#pragma unroll
-        for (int i = 1; i < kEach; ++i) top = fmaxf(top, x[i]);
-        top = MaxOver<kLanes>(top);
-        sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            share[i] = top == -INFINITY ? 0.f : ExpOfNegative(x[i] - top);
-            sum += share[i];
-        }
-        sum = SumOver<kLanes>(sum);
-    }
-    const float inverse = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) share[i] *= inverse;
+    for (int i = 0; i < kEach; ++i) share[i] = x[i];
+    SoftmaxOf<kLanes>(share);
 }
-
 // f(lanes, pieces) of the layout for rows of so many experts, as integral constants: the fewest lanes whose pieces of four hold them, then the fewest pieces.
 template <typename F>
 void ForRowLayout(int64_t experts, F f) {
