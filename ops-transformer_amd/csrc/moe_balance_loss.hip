@@ -59,7 +59,7 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
     __shared__ int32_t picked[Row::kWidth];
     __shared__ int32_t live;
     __shared__ double finishing[kChunkWaves];
-    const int tid = threadIdx.x, wave = tid / kWave, lane = tid % kWave, l = lane % kLanes, group = lane / kLanes;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, l = lane % kLanes, side = lane / kLanes;
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x);
     auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
 
@@ -79,16 +79,18 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
     // each lane's first id, before the workgroup looks for their sequence.
     typename Row::template Raw<typename Codec::Storage> raw[kUnroll];
     int32_t rowIds[kUnroll], id = -1, rowId = -1;
+    // rows from `at` on, the same for the wave, its lanes `side` by side
     auto load = [&](int64_t at, int64_t end) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int64_t row = min(at + u * kStride, end - 1);
-            rowIds[u] = a.expertIdx[row * a.k];
-            raw[u] = Row::Ask(x + row * a.experts, a.experts, l);
+            const uint32_t beside = kRowsAtOnce == 1 ? 0 : min(static_cast<uint32_t>(side), static_cast<uint32_t>(end - 1 - row));
+            rowIds[u] = (a.expertIdx + row * a.k)[beside * static_cast<uint32_t>(a.k)];
+            raw[u] = Row::Ask(x + row * a.experts, beside * static_cast<uint32_t>(a.experts), a.experts, l);
         }
     };
     auto loadFirst = [&](int64_t begin, int64_t end) {
-        if (begin + wave * kRowsAtOnce + group < end) load(begin + wave * kRowsAtOnce + group, end);
+        if (begin + wave * kRowsAtOnce < end) load(begin + wave * kRowsAtOnce, end);
         if (tid < (end - begin) * a.k) {
             id = a.expertIdx[begin * a.k + tid];
             rowId = a.expertIdx[(begin + tid / a.k) * a.k];
@@ -132,13 +134,13 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
         for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
         int32_t counted = 0;
 #pragma unroll 1
-        for (int64_t row = at + wave * kRowsAtOnce + group; row < end; row += kUnroll * kStride) {
+        for (int64_t row = at + wave * kRowsAtOnce; row < end; row += kUnroll * kStride) {
             // Scores, for softmax before their division by the sum.  Row by row without a branch: the rows' reductions overlap.
             float p[kUnroll][kEach], total[kUnroll];
             bool counts[kUnroll], lost = false;
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                counts[u] = row + u * kStride < end && isExpert(rowIds[u]);
+                counts[u] = row + u * kStride + side < end && isExpert(rowIds[u]);
                 Row::template Logits<Codec>(raw[u], a.experts, l, p[u]);
             }
             if (row + kUnroll * kStride < end) load(row + kUnroll * kStride, end);
@@ -170,9 +172,9 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
             }
             if (kSigmoid && lost) {  // rare, and made again (the lanes of a row agree)
 #pragma unroll 1
-                for (int64_t again = row; again < min(row + kUnroll * kStride, end); again += kStride) {
+                for (int64_t again = row + side; again < min(row + kUnroll * kStride, end); again += kStride) {
                     float v[kEach], share[kEach], scores = 0.f;
-                    Row::template Logits<Codec>(Row::Ask(x + again * a.experts, a.experts, l), a.experts, l, v);
+                    Row::template Logits<Codec>(Row::Ask(x + again * a.experts, 0, a.experts, l), a.experts, l, v);
 #pragma unroll
                     for (int i = 0; i < kEach; ++i) scores += SigmoidOf(v[i]).p;
                     if (!(SumOver<kLanes>(scores) < kLostSum) || !isExpert(a.expertIdx[again * a.k])) continue;

@@ -51,70 +51,79 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
     constexpr int kRowsAtOnce = kWave / kLanes;
     __shared__ float4 scores[kGradWaves][kRowsAtOnce][Row::kWidth / 4];
     __shared__ float4 picked[kGradWaves][kRowsAtOnce][Row::kWidth / 4];  // zero between rows
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave, l = lane % kLanes, side = lane / kLanes;
+    using X = typename Codec::Storage;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, l = lane % kLanes, side = lane / kLanes;
     const float* const scoreOf = reinterpret_cast<const float*>(scores[wave][side]);
     float* const pickedOf = reinterpret_cast<float*>(picked[wave][side]);
     const bool weights = a.yGrad != nullptr, balance = a.lossGrad != nullptr;
     auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
-    auto yGradOf = [&](int64_t row, int j) {
-        const int64_t at = row * a.k + j;
-        return a.yGradIsFloat ? static_cast<const float*>(a.yGrad)[at] : Codec::Load(static_cast<const typename Codec::Storage*>(a.yGrad)[at]);
-    };
     // The rows of a wave follow each other, `side` by side: their sequence changes seldom, and with it the counts in registers.
-    const int64_t first = (GroupIndex() * kGradWaves + wave) * a.waveRows, last = min(first + a.waveRows, a.sequences.rows);
-    if (first >= last) return;
-    using Inputs = RowInputs<typename Row::template Raw<typename Codec::Storage>>;
+    const int64_t first = (GroupIndex() * kGradWaves + wave) * a.waveRows;
+    if (first >= a.sequences.rows) return;
+    const int32_t rows = static_cast<int32_t>(min(static_cast<int64_t>(a.waveRows), a.sequences.rows - first));
+    // What the wave's rows begin at, and the lane's own row behind those of the ones beside it.
+    const X* const xRows = static_cast<const X*>(a.x) + first * a.experts;
+    typename Out::Storage* const outRows = static_cast<typename Out::Storage*>(a.xGrad) + first * a.experts;
+    const int32_t* const idxRows = a.expertIdx + first * a.k;
+    const float* const yRowsFloat = static_cast<const float*>(a.yGrad) + first * a.k;
+    const X* const yRows = static_cast<const X*>(a.yGrad) + first * a.k;
+    auto yGradOf = [&](uint32_t at) { return a.yGradIsFloat ? yRowsFloat[at] : Codec::Load(yRows[at]); };
+    using Inputs = RowInputs<typename Row::template Raw<X>>;
     Inputs in;
-    auto load = [&](int64_t row) {
-        in.x = Row::Ask(static_cast<const typename Codec::Storage*>(a.x) + row * a.experts, a.experts, l);
-        in.first = a.expertIdx[row * a.k];
+    auto load = [&](int32_t row) {
+        const uint32_t pick = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.k);
+        in.x = Row::Ask(xRows, static_cast<uint32_t>(row) * static_cast<uint32_t>(a.experts), a.experts, l);
+        in.first = idxRows[pick];
         in.id = -1;
         in.y = 0.f;
         if (weights && l < a.k) {
-            in.id = a.expertIdx[row * a.k + l];
-            in.y = yGradOf(row, l);
+            in.id = idxRows[pick + l];
+            in.y = yGradOf(pick + l);
         }
     };
-    if (first + side < last) load(first + side);
+    if (side < rows) load(side);
     if (weights) {
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) picked[wave][side][Row::At(p, l) / 4] = float4{0.f, 0.f, 0.f, 0.f};
     }
-    int32_t sequence = -2;     // of the row, and where it ends
-    int64_t sequenceEnd = -1;
+    int32_t sequence = -2;     // of the row, and where it ends, from the wave's first row on
+    int32_t sequenceEnd = -1;
     bool inside = false;       // whether it is one
     float shareGrad[kEach];    // what its loss gives each share
 #pragma unroll
     for (int i = 0; i < kEach; ++i) shareGrad[i] = 0.f;
     // The loads of a sequence go out together, those of rows in none being of another one's.
     auto enter = [&](int32_t s, int64_t end) {
-        sequenceEnd = end;
+        sequenceEnd = static_cast<int32_t>(min(end - first, static_cast<int64_t>(1) << 30));
         sequence = s;
         inside = s >= 0 && s < a.sequences.count;
         const int32_t at = s < 0 ? 0 : min(s, a.sequences.count - 1);
-        const int32_t rows = a.seqRows[at];
+        const int32_t live = a.seqRows[at];
         const float lossGrad = a.lossGrad[at];
-        const auto raw = Row::Ask(a.counts + static_cast<int64_t>(at) * a.experts, a.experts, l);
+        const auto raw = Row::Ask(a.counts, static_cast<uint32_t>(at) * static_cast<uint32_t>(a.experts), a.experts, l);
         int32_t counts[kEach];
         Row::Place(raw, a.experts, l, 0, counts);
-        const float n = static_cast<float>(rows);
-        const float each = rows > 0 ? lossGrad * (static_cast<float>(a.experts) / static_cast<float>(a.k)) / n / n : 0.f;
+        const float n = static_cast<float>(live);
+        const float each = live > 0 ? lossGrad * (static_cast<float>(a.experts) / static_cast<float>(a.k)) / n / n : 0.f;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) shareGrad[i] = rows > 0 ? each * static_cast<float>(counts[i]) : 0.f;
+        for (int i = 0; i < kEach; ++i) shareGrad[i] = live > 0 ? each * static_cast<float>(counts[i]) : 0.f;
     };
     if (balance) {
         int64_t end;
         const int32_t s = a.sequences.Of(first, end);
         enter(s, end);
     }
-    for (int64_t row = first + side; row < last; row += kRowsAtOnce) {
+    for (int32_t base = 0; base < rows; base += kRowsAtOnce) {
+        const int32_t row = base + side;
+        if (row >= rows) break;  // (the lanes of a row agree)
         if (balance && row >= sequenceEnd && sequence < a.sequences.count) {
             int64_t end;
-            const int32_t s = SequenceBehind(a.sequences, sequence, row, end);
+            const int32_t s = SequenceBehind(a.sequences, sequence, first + row, end);
             enter(s, end);
         }
         const Inputs now = in;
-        if (row + kRowsAtOnce < last) load(row + kRowsAtOnce);
+        if (row + kRowsAtOnce < rows) load(row + kRowsAtOnce);
+        const uint32_t pick = static_cast<uint32_t>(row) * static_cast<uint32_t>(a.k);
         float x[kEach];
         Row::template Logits<Codec>(now.x, a.experts, l, x);
         // p: sigmoid's score, with rest = 1 - p, or softmax's before its division by the sum
@@ -147,10 +156,10 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
                 weighted = now.y * pickedSum;
             }
             for (int j = l + kLanes; j < a.k; j += kLanes) {
-                const int32_t id = a.expertIdx[row * a.k + j];
+                const int32_t id = idxRows[pick + j];
                 if (!isExpert(id)) continue;
                 pickedSum += scoreOf[id];
-                weighted = fmaf(yGradOf(row, j), scoreOf[id], weighted);
+                weighted = fmaf(yGradOf(pick + j), scoreOf[id], weighted);
             }
         }
         sum = SumOver<kLanes>(sum);
@@ -172,14 +181,15 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
             if (a.renorm) {
                 const float total = pickedSum + a.eps;
                 const bool none = pickedSum == 0.f;
-                scale = none ? 0.f : a.factor / total;
-                mean = none ? 0.f : weighted / total;
-                all = none ? 0.f : a.factor * mean * (a.eps / total);
+                const float part = none ? 0.f : 1.f / total;
+                scale = a.factor * part;
+                mean = weighted * part;
+                all = scale * weighted * (a.eps * part);
             }
             if (isExpert(now.id)) atomicAdd(pickedOf + now.id, scale * (now.y - mean));
             for (int j = l + kLanes; j < a.k; j += kLanes) {
-                const int32_t id = a.expertIdx[row * a.k + j];
-                if (isExpert(id)) atomicAdd(pickedOf + id, scale * (yGradOf(row, j) - mean));
+                const int32_t id = idxRows[pick + j];
+                if (isExpert(id)) atomicAdd(pickedOf + id, scale * (yGradOf(pick + j) - mean));
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -222,7 +232,7 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
         const bool live = isExpert(now.first);
 #pragma unroll
         for (int i = 0; i < kEach; ++i) grad[i] = live ? grad[i] : 0.f;
-        Row::template Store<Out>(static_cast<typename Out::Storage*>(a.xGrad) + row * a.experts, a.experts, l, grad);
+        Row::template Store<Out>(outRows, static_cast<uint32_t>(row) * static_cast<uint32_t>(a.experts), a.experts, l, grad);
     }
 }
 

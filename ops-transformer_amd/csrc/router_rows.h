@@ -151,16 +151,17 @@ struct RowOf {
     struct Raw {
         T e[kEach];
     };
+    // (`rows`, the same for the wave, and where the lane's row begins behind it: an address in scalar registers with 32 bits of the lane's own.)
     template <typename T>
-    __device__ static __forceinline__ Raw<T> Ask(const T* row, int experts, int l) {
+    __device__ static __forceinline__ Raw<T> Ask(const T* rows, uint32_t begin, int experts, int l) {
         Raw<T> raw;
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
             if (kLanes == 2 && experts < 4) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) raw.e[4 * p + i] = row[min(i, experts - 1)];
+                for (int i = 0; i < 4; ++i) raw.e[4 * p + i] = rows[begin + static_cast<uint32_t>(min(i, experts - 1))];
             } else {
-                __builtin_memcpy(raw.e + 4 * p, row + min(At(p, l), experts - 4), 4 * sizeof(T));
+                __builtin_memcpy(raw.e + 4 * p, rows + (begin + static_cast<uint32_t>(min(At(p, l), experts - 4))), 4 * sizeof(T));
             }
         }
         return raw;
@@ -192,19 +193,20 @@ struct RowOf {
         for (int i = 0; i < kEach; ++i) v[i] = Codec::Load(placed[i]);
     }
     template <typename Codec>
-    __device__ static __forceinline__ void Store(typename Codec::Storage* row, int experts, int l, const float (&v)[kEach]) {
+    __device__ static __forceinline__ void Store(typename Codec::Storage* rows, uint32_t begin, int experts, int l, const float (&v)[kEach]) {
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
             const int at = At(p, l);
+            typename Codec::Storage* const row = rows + (begin + static_cast<uint32_t>(at));
             if (at + 4 <= experts) {
                 typename Codec::Storage raw[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) raw[i] = Codec::Store(v[4 * p + i]);
-                __builtin_memcpy(row + at, raw, sizeof(raw));
+                __builtin_memcpy(row, raw, sizeof(raw));
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (at + i < experts) row[at + i] = Codec::Store(v[4 * p + i]);
+                    if (at + i < experts) row[i] = Codec::Store(v[4 * p + i]);
                 }
             }
         }
