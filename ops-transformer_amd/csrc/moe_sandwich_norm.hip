@@ -47,117 +47,128 @@ __device__ __forceinline__ float RowGate(const SandwichArgs& a, int64_t row) {
 }
 
 // Rows in pieces of eight elements, up to kPackets of them a lane; a workgroup takes every gridDim.x-th row and asks for the next one before the
-// present one is reduced.  Gammas and a gate per channel stay in registers.  Pieces are read and written where they lie (see norm_rows.h).
+// present one is begun (where the registers hold both, else before it is reduced the second time).  Gammas and a gate per channel stay in registers.
 constexpr int kMaxPacketThreads = 512;
 constexpr int kMaxPackets = 4;
+constexpr int64_t kCus = 256, kWavesACu = 16;
 
-template <typename Codec, typename Gamma, int kPackets, int kGate>
+template <typename Codec, int kPackets, bool kGate>
+struct NormRows {
+    Packet<Codec> x[kPackets], residual[kPackets], gate[kGate ? kPackets : 1];
+    float rowGate = 1.f;
+};
+
+template <typename Codec, typename Gamma, int kPackets, int kGate, bool kTail>
 __global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(SandwichArgs a) {
-    using P = Packet<Codec>;
     using Storage = typename Codec::Storage;
     constexpr int kMaxWaves = kMaxPacketThreads / kWave;
+    constexpr bool kHeld = kGate == kHeldPackets, kRead = kGate == kReadPackets;
+    constexpr bool kEarly = kPackets == 1 || (kPackets == 2 && sizeof(Storage) == 2);
     __shared__ float postSums[2][kMaxWaves][1];
     __shared__ float2 partial[2][kMaxWaves];
     const int threads = blockDim.x, waves = threads / kWave, tid = threadIdx.x;
     const int cols = static_cast<int>(a.cols);
     const bool post = a.post != nullptr, pre = a.pre != nullptr;
-    P x[kPackets], r[kPackets], gateRow[kGate == kReadPackets ? kPackets : 1];
-    Packet<Gamma> postGamma[kPackets], preGamma[kPackets];
-    float gateHeld[kGate == kHeldPackets ? kPackets : 1][8];
-    float rowGate = 1.f;
-    bool here[kPackets];
-    auto at = [&](int p) { return (p * threads + tid) * 8; };
-    auto count = [&](int p) { return min(cols - at(p), 8); };
+    const Pieces<kPackets, kTail> at(cols, threads, tid);
+    Packet<Gamma> postGamma[kPackets], preGamma[kPackets], gateHeld[kHeld ? kPackets : 1];
 #pragma unroll
     for (int p = 0; p < kPackets; ++p) {
-        here[p] = at(p) < cols;
-        if (!here[p]) continue;
-        if (post) postGamma[p] = LoadPacket<false, Gamma>(a.post, at(p), count(p));
-        if (pre) preGamma[p] = LoadPacket<false, Gamma>(a.pre, at(p), count(p));
-        if constexpr (kGate == kHeldPackets) {
-            Unpack<Gamma>(LoadPacket<false, Gamma>(a.gate, at(p), count(p)), gateHeld[p]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) gateHeld[p][i] = Gated(gateHeld[p][i], a.sigmoid);
-        }
+        if (post) postGamma[p] = at.template Load<Gamma>(a.post, 0, p);
+        if (pre) preGamma[p] = at.template Load<Gamma>(a.pre, 0, p);
+        if constexpr (kHeld) gateHeld[p] = at.template Load<Gamma>(a.gate, 0, p);
     }
-    auto load = [&](int64_t row) {
+    using Rows = NormRows<Codec, kPackets, kRead>;
+    auto load = [&](Rows& to, int64_t row) {
+        const int64_t begin = row * cols;
 #pragma unroll
         for (int p = 0; p < kPackets; ++p) {
-            if (!here[p]) continue;
-            x[p] = LoadPacket<false, Codec>(a.x, row * cols + at(p), count(p));
-            r[p] = LoadPacket<false, Codec>(a.residual, row * cols + at(p), count(p));
-            if constexpr (kGate == kReadPackets) gateRow[p] = LoadPacket<false, Codec>(a.gate, row * cols + at(p), count(p));
+            to.x[p] = at.template Load<Codec>(a.x, begin, p);
+            to.residual[p] = at.template Load<Codec>(a.residual, begin, p);
+            if constexpr (kRead) to.gate[p] = at.template Load<Codec>(a.gate, begin, p);
         }
-        if constexpr (kGate == kNoPackets) rowGate = RowGate<Codec>(a, row);
+        if constexpr (kGate == kNoPackets) to.rowGate = RowGate<Codec>(a, row);
     };
     int64_t row = blockIdx.x;
-    load(row);
-    for (int parity = 0; row < a.rows; parity ^= 1) {
+    // One row; `following` takes the next one where it is asked for early, else `in` does.
+    auto step = [&](Rows& in, Rows& following, int parity) __attribute__((always_inline)) {
+        const int64_t begin = row * cols, next = row + gridDim.x;
+        if constexpr (kEarly) load(following, min(next, a.rows - 1));
+#pragma unroll
+        for (int p = 0; p < kPackets; ++p) {
+            HoldPacked<Gamma>(postGamma[p]);
+            HoldPacked<Gamma>(preGamma[p]);
+            if constexpr (kHeld) HoldPacked<Gamma>(gateHeld[p]);
+        }
         float postRstd = 0.f;
         if (post) {
             float squares[1] = {0.f};
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
-                if (!here[p]) continue;
-                float v[8];
-                Unpack<Codec>(x[p], v);
+                float v[8], part = 0.f;
+                Unpack<Codec>(in.x[p], v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) squares[0] = fmaf(v[i], v[i], squares[0]);
+                for (int i = 0; i < 8; ++i) part = fmaf(at.Own(v[i], p, i), v[i], part);
+                squares[0] += at.Counted(part, p);
             }
             SumsOverGroup<1, kMaxWaves>(squares, waves, parity, postSums);
             postRstd = FactorOf(squares[0], a.cols, a.eps);
             if (a.postRstd != nullptr && tid == 0) a.postRstd[row] = postRstd;
         }
-        P s[kPackets];
+        Packet<Codec> s[kPackets];
         float sumSquares = 0.f;
         uint32_t maxBits = 0;
 #pragma unroll
         for (int p = 0; p < kPackets; ++p) {
-            if (!here[p]) continue;
-            float v[8], w[8];
-            Unpack<Codec>(x[p], v);
-            Unpack<Codec>(r[p], w);
+            float v[8], w[8], g[8];
+            Unpack<Codec>(in.x[p], v);
+            Unpack<Codec>(in.residual[p], w);
             if (post) {
-                float g[8];
                 Unpack<Gamma>(postGamma[p], g);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = v[i] * postRstd * g[i];
             }
-            if constexpr (kGate == kHeldPackets) {
+            if constexpr (kHeld) {
+                Unpack<Gamma>(gateHeld[p], g);
+                OpenGates(g, a.sigmoid);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= gateHeld[p][i];
-            } else if constexpr (kGate == kReadPackets) {
-                float g[8];
-                Unpack<Codec>(gateRow[p], g);
+                for (int i = 0; i < 8; ++i) v[i] *= g[i];
+            } else if constexpr (kRead) {
+                Unpack<Codec>(in.gate[p], g);
+                OpenGates(g, a.sigmoid);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= Gated(g[i], a.sigmoid);
+                for (int i = 0; i < 8; ++i) v[i] *= g[i];
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] *= rowGate;
+                for (int i = 0; i < 8; ++i) v[i] *= in.rowGate;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = fmaf(a.residualScale, w[i], a.branchScale * v[i]);
             s[p] = Pack<Codec>(v);
-            StorePacket<false, Storage>(a.sum, row * cols + at(p), count(p), s[p]);
+            at.template StoreOwn<Storage>(a.sum, begin, p, s[p]);  // it may lie where another lane has yet to read what is not its own
             if (!pre) continue;
             Unpack<Codec>(s[p], v);
-            float g[8];
             Unpack<Gamma>(preGamma[p], g);
+            float part = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sumSquares = fmaf(v[i], v[i], sumSquares);
+            for (int i = 0; i < 8; ++i) part = fmaf(at.Own(v[i], p, i), v[i], part);
+            sumSquares += at.Counted(part, p);
             if (a.y != nullptr) {
+                float smooth[8];
                 if (a.smooth != nullptr) {
-                    const Packet<F32> smooth = LoadPacket<false, F32>(a.smooth, at(p), count(p));
+                    Unpack<F32>(at.template Load<F32>(a.smooth, 0, p), smooth);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) maxBits = max(maxBits, __float_as_uint(fabsf(v[i] * g[i] * reinterpret_cast<const float*>(&smooth)[i])));
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) maxBits = max(maxBits, __float_as_uint(fabsf(v[i] * g[i])));
+                    for (int i = 0; i < 8; ++i) g[i] *= smooth[i];
                 }
+                uint32_t most = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(fabsf(at.Own(v[i] * g[i], p, i))));
+                if (kTail || at.skip[p] == 0) maxBits = max(maxBits, most);
             }
         }
-        const int64_t next = row + gridDim.x;
-        if (next < a.rows) load(next);
+        if constexpr (!kEarly) {
+            __builtin_amdgcn_sched_barrier(0);  // not in front of the last uses
+            load(in, min(next, a.rows - 1));
+        }
         if (pre) {
             sumSquares = SumOver<kWave>(sumSquares);
             if (a.y != nullptr) maxBits = WaveMax(maxBits);
@@ -178,7 +189,6 @@ __global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(Sandw
             }
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
-                if (!here[p]) continue;
                 float v[8], g[8];
                 Unpack<Codec>(s[p], v);
                 Unpack<Gamma>(preGamma[p], g);
@@ -186,26 +196,37 @@ __global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(Sandw
                     float n[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) n[i] = v[i] * scales.r * g[i];
-                    StorePacket<false, Storage>(a.norm, row * cols + at(p), count(p), Pack<Codec>(n));
+                    at.template StoreOwn<Storage>(a.norm, begin, p, Pack<Codec>(n));
                 }
                 if (a.y != nullptr) {
                     float smooth[8];
                     if (a.smooth != nullptr) {
-                        Unpack<F32>(LoadPacket<false, F32>(a.smooth, at(p), count(p)), smooth);
-                    } else {
+                        Unpack<F32>(at.template Load<F32>(a.smooth, 0, p), smooth);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) smooth[i] = 1.f;
+                        for (int i = 0; i < 8; ++i) g[i] *= smooth[i];
                     }
                     uint32_t q[2] = {0, 0};
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        q[i / 4] |= (static_cast<uint32_t>(Quantised(v[i] * g[i] * smooth[i], scales)) & 0xffu) << (i % 4 * 8);
-                    }
-                    StorePacket<false, int8_t>(a.y, row * cols + at(p), count(p), uint2{q[0], q[1]});
+                    for (int i = 0; i < 8; ++i) q[i / 4] |= (static_cast<uint32_t>(Quantised(v[i] * g[i], scales)) & 0xffu) << (i % 4 * 8);
+                    at.template StoreOwn<int8_t>(a.y, begin, p, uint2{q[0], q[1]});
                 }
             }
         }
         row = next;
+    };
+    Rows first;
+    load(first, row);
+    if constexpr (kEarly) {
+        // The two rows take turns where they lie: moved, a row's loads would have to have ended, and the stores behind them.
+        Rows second;
+        while (true) {
+            step(first, second, 0);
+            if (row >= a.rows) break;
+            step(second, first, 1);
+            if (row >= a.rows) break;
+        }
+    } else {
+        for (int parity = 0; row < a.rows; parity ^= 1) step(first, first, parity);
     }
 }
 
@@ -290,10 +311,10 @@ class SandwichExecutor : public aclOpExecutor {
     void LaunchPackets(hipStream_t stream) const {
         const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
         const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
-        int64_t groups = args.rows;
-        const int64_t most = threads >= 256 ? 4096 : 2048;
-        if (groups > most) groups = most;
-        hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kGate>), dim3(static_cast<unsigned>(groups)), dim3(threads), 0, stream, args);
+        const int64_t groups = std::min<int64_t>(args.rows, kCus * (kWavesACu * kWave / threads));
+        const dim3 grid(static_cast<unsigned>(groups));
+        if (args.cols % 8 != 0) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kGate, true>), grid, dim3(threads), 0, stream, args);
+        else hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kGate, false>), grid, dim3(threads), 0, stream, args);
     }
 
     template <typename Codec, typename Gamma, int kPackets>
@@ -311,10 +332,10 @@ class SandwichExecutor : public aclOpExecutor {
             using Codec = decltype(codec);
             using Gamma = decltype(gamma);
             const int64_t lanes = (args.cols + 7) / 8;
-            if (lanes <= kMaxPacketThreads) ForGate<Codec, Gamma, 1>(stream);
+            if (args.cols < 8 || lanes > kMaxPackets * kMaxPacketThreads) hipLaunchKernelGGL((SandwichAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
+            else if (lanes <= kMaxPacketThreads) ForGate<Codec, Gamma, 1>(stream);
             else if (lanes <= 2 * kMaxPacketThreads) ForGate<Codec, Gamma, 2>(stream);
-            else if (lanes <= kMaxPackets * kMaxPacketThreads) ForGate<Codec, Gamma, kMaxPackets>(stream);
-            else hipLaunchKernelGGL((SandwichAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
+            else ForGate<Codec, Gamma, kMaxPackets>(stream);
         });
         const hipError_t err = hipGetLastError();
         OPAPI_CHECK(err == hipSuccess, ACLNN_ERR_RUNTIME_ERROR, "aclnnMoeSandwichNorm: launch failed: %s", hipGetErrorString(err));

@@ -11,8 +11,9 @@ namespace {
 
 using namespace moe_front;
 
-// Column sums, by their place in the workspace.
-enum { kPostSums, kPreSums, kGateSums, kColumnSums };
+// Column sums, by their place in the workspace: of dn s^, and of the branch.  Where a gate per channel opens by g, postGammaGrad = g S and gateGrad = slope
+// postGamma S of the one S = sum of dv x^; else S = sum of du x^ is postGammaGrad itself.
+enum { kPreSums, kBranchSums, kColumnSums };
 
 struct SandwichGradArgs {
     const void* x;           // read where there is a post norm or a gate
@@ -27,8 +28,10 @@ struct SandwichGradArgs {
     void* xGrad;             // optional
     void* residualGrad;      // optional
     void* gateGrad;          // optional
-    float* columnGrads[kColumnSums];  // outputs, optional
-    float* columnSums[kColumnSums];   // workspace: [groups, cols] each
+    float* preGammaGrad;     // optional
+    float* postGammaGrad;    // optional
+    float* channelGrad;      // optional: gateGrad of a gate per channel
+    float* columnSums[kColumnSums];  // workspace: [groups, cols] each, null where not wanted
     float* rowMeans;         // workspace of rows in two passes: [rows, 2]
     int64_t rows;
     int64_t cols;
@@ -53,194 +56,263 @@ __device__ __forceinline__ float RawRowGate(const SandwichGradArgs& a, int64_t r
 
 constexpr int kMaxPacketThreads = 512;
 
-template <typename Codec, typename Gamma, int kPackets, int kGate>
+// What is read of a row.
+template <typename Codec, int kPackets, bool kGate>
+struct GradRows {
+    Packet<Codec> x[kPackets], s[kPackets], sumGrad[kPackets], normGrad[kPackets], gate[kGate ? kPackets : 1];
+    float postRstd = 1.f, preRstd = 0.f, rawGate = 0.f;
+};
+
+// kSumsInLds: the column sums of a workgroup, where its registers have no room for them beside the row.
+template <typename Codec, typename Gamma, int kPackets>
+constexpr bool kSumsInLds = kPackets == 4 || (kPackets == 2 && sizeof(typename Codec::Storage) + sizeof(typename Gamma::Storage) == 8);
+
+template <typename Codec, typename Gamma, int kPackets, int kGate, bool kPre, bool kTail>
 __global__ __launch_bounds__(kMaxPacketThreads) void SandwichGradKernel(SandwichGradArgs a) {
-    using P = Packet<Codec>;
     using Storage = typename Codec::Storage;
     constexpr int kMaxWaves = kMaxPacketThreads / kWave;
     constexpr bool kHeld = kGate == kHeldPackets, kRead = kGate == kReadPackets;
+    constexpr bool kLds = kSumsInLds<Codec, Gamma, kPackets>;
+    // Where the registers hold a second row, the next one is asked for before the present one is begun, else when its loads have found their last use.
+    constexpr bool kEarly = kPackets == 1 || (kPackets == 2 && sizeof(Storage) == 2);
+    // Weights stay in registers, packed, or are read again for every row, from the caches.
+    constexpr bool kHoldWeights = kPackets < 4;
     __shared__ float preSums[2][kMaxWaves][1];
     __shared__ float postSums[2][kMaxWaves][2];
+    extern __shared__ float4 ldsSums[];  // kLds: [kColumnSums][kPackets][2][threads], each lane its own
     const int threads = blockDim.x, waves = threads / kWave, tid = threadIdx.x;
     const int cols = static_cast<int>(a.cols);
     const float each = 1.f / static_cast<float>(a.cols);
-    const bool post = a.post != nullptr, pre = a.pre != nullptr, gated = a.gateKind != kGateNone, rowGated = a.gateKind == kGateRow;
-    const bool needsX = post || gated, sums = a.sumGrad != nullptr;
-    P x[kPackets], s[kPackets], sumGrad[kPackets], normGrad[kPackets], gateRow[kRead ? kPackets : 1];
-    Packet<Gamma> postGamma[kPackets], preGamma[kPackets];
-    float gateHeld[kHeld ? kPackets : 1][8];
-    float postSum[kPackets][8], preSum[kPackets][8], gateSum[kHeld ? kPackets : 1][8];
-    float postRstd = 1.f, preRstd = 0.f, rawGate = 0.f;
-    bool here[kPackets];
-    auto at = [&](int p) { return (p * threads + tid) * 8; };
-    auto count = [&](int p) { return min(cols - at(p), 8); };
+    const bool post = a.post != nullptr, gated = a.gateKind != kGateNone, rowGated = a.gateKind == kGateRow;
+    const bool sums = a.sumGrad != nullptr, branchSums = post || kHeld;
+    const Pieces<kPackets, kTail> at(cols, threads, tid);
+    constexpr int kHeldPackets = kHoldWeights ? kPackets : 1;
+    Packet<Gamma> postHeld[kHeldPackets], preHeld[kPre ? kHeldPackets : 1], gateHeld[kHeld ? kHeldPackets : 1];
+    auto weights = [&](const Packet<Gamma>* held, const void* w, int p) {
+        if constexpr (kHoldWeights) return held[p];
+        else return at.template Load<Gamma>(w, 0, p);
+    };
+    float sumHeld[kLds ? 1 : kColumnSums][kLds ? 1 : kPackets][8];
+    auto addToColumns = [&](int which, int p, const float (&v)[8]) {
+        if constexpr (kLds) {
+            float4* const to = ldsSums + ((which * kPackets + p) * 2) * threads + tid;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float4 t = to[h * threads];
+                t.x += v[4 * h];
+                t.y += v[4 * h + 1];
+                t.z += v[4 * h + 2];
+                t.w += v[4 * h + 3];
+                to[h * threads] = t;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sumHeld[which][p][i] += v[i];
+        }
+    };
 #pragma unroll
     for (int p = 0; p < kPackets; ++p) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            postSum[p][i] = preSum[p][i] = 0.f;
-            if constexpr (kHeld) gateSum[p][i] = 0.f;
-        }
-        here[p] = at(p) < cols;
-        if (!here[p]) continue;
-        if (post) postGamma[p] = LoadPacket<false, Gamma>(a.post, at(p), count(p));
-        if (pre) preGamma[p] = LoadPacket<false, Gamma>(a.pre, at(p), count(p));
-        if constexpr (kHeld) {
-            Unpack<Gamma>(LoadPacket<false, Gamma>(a.gate, at(p), count(p)), gateHeld[p]);
+        for (int c = 0; c < kColumnSums; ++c) {
+            if constexpr (kLds) {
+                ldsSums[((c * kPackets + p) * 2) * threads + tid] = ldsSums[((c * kPackets + p) * 2 + 1) * threads + tid] = float4{0.f, 0.f, 0.f, 0.f};
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) gateHeld[p][i] = Gated(gateHeld[p][i], a.sigmoid);
+                for (int i = 0; i < 8; ++i) sumHeld[c][p][i] = 0.f;
+            }
+        }
+        if constexpr (kHoldWeights) {
+            if (post) postHeld[p] = at.template Load<Gamma>(a.post, 0, p);
+            if constexpr (kPre) preHeld[p] = at.template Load<Gamma>(a.pre, 0, p);
+            if constexpr (kHeld) gateHeld[p] = at.template Load<Gamma>(a.gate, 0, p);
         }
     }
-    auto load = [&](int64_t row) {
+    // Every row's loads, and as many: of tensors that are absent or not needed another one's are loaded in their place, which are at hand then.
+    const void* const readX = post || gated ? a.x : kPre ? a.s : a.sumGrad;
+    const void* const readSumGrad = sums ? a.sumGrad : a.normGrad;
+    const float* const readRstd = post ? a.postRstd : kPre ? a.preRstd : nullptr;
+    auto load = [&](GradRows<Codec, kPackets, kRead>& to, int64_t row) {
+        const int64_t begin = row * cols;
 #pragma unroll
         for (int p = 0; p < kPackets; ++p) {
-            if (!here[p]) continue;
-            const int64_t from = row * cols + at(p);
-            if (pre) {
-                s[p] = LoadPacket<false, Codec>(a.s, from, count(p));
-                normGrad[p] = LoadPacket<false, Codec>(a.normGrad, from, count(p));
+            if constexpr (kPre) {
+                to.s[p] = at.template Load<Codec>(a.s, begin, p);
+                to.normGrad[p] = at.template Load<Codec>(a.normGrad, begin, p);
             }
-            if (sums) sumGrad[p] = LoadPacket<false, Codec>(a.sumGrad, from, count(p));
-            if (needsX) x[p] = LoadPacket<false, Codec>(a.x, from, count(p));
-            if constexpr (kRead) gateRow[p] = LoadPacket<false, Codec>(a.gate, from, count(p));
+            to.sumGrad[p] = at.template Load<Codec>(readSumGrad, begin, p);
+            to.x[p] = at.template Load<Codec>(readX, begin, p);
+            if constexpr (kRead) to.gate[p] = at.template Load<Codec>(a.gate, begin, p);
         }
-        if (post) postRstd = a.postRstd[row];
-        if (pre) preRstd = a.preRstd[row];
-        if (kGate == kNoPackets && rowGated) rawGate = RawRowGate<Codec>(a, row);
+        if (readRstd != nullptr) to.postRstd = readRstd[row];
+        if constexpr (kPre) to.preRstd = a.preRstd[row];
+        if (kGate == kNoPackets && rowGated) to.rawGate = RawRowGate<Codec>(a, row);
     };
     int64_t row = blockIdx.x;
-    if (row < a.rows) load(row);
-    for (int parity = 0; row < a.rows; parity ^= 1) {
-        // dS
-        float d[kPackets][8];
-        float preMean[1] = {0.f};
-        if (pre) {
+    // One row; `following` takes the next one where it is asked for early, else `in` does.
+    auto step = [&](GradRows<Codec, kPackets, kRead>& in, GradRows<Codec, kPackets, kRead>& following, int parity) __attribute__((always_inline)) {
+        const int64_t begin = row * cols, next = row + gridDim.x;
+        if constexpr (kEarly) load(following, min(next, a.rows - 1));
+        if constexpr (kHoldWeights) {
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
-                if (!here[p]) continue;
-                float v[8], g[8];
-                Unpack<Codec>(s[p], v);
-                Unpack<Codec>(normGrad[p], d[p]);
-                Unpack<Gamma>(preGamma[p], g);
+                HoldPacked<Gamma>(postHeld[p]);
+                if constexpr (kPre) HoldPacked<Gamma>(preHeld[p]);
+                if constexpr (kHeld) HoldPacked<Gamma>(gateHeld[p]);
+            }
+        }
+        const float postRstd = post ? in.postRstd : 1.f, raw = in.rawGate;
+        // dS
+        float d[kPackets][8];
+        if constexpr (kPre) {
+            const float preRstd = in.preRstd;
+            float preMean[1] = {0.f};
+#pragma unroll
+            for (int p = 0; p < kPackets; ++p) {
+                float v[8], g[8], terms[8], part = 0.f;
+                Unpack<Codec>(in.s[p], v);
+                Unpack<Codec>(in.normGrad[p], d[p]);
+                Unpack<Gamma>(weights(preHeld, a.pre, p), g);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float normed = v[i] * preRstd;
-                    preSum[p][i] = fmaf(d[p][i], normed, preSum[p][i]);
+                    terms[i] = d[p][i] * (v[i] * preRstd);
+                    part = fmaf(at.Own(terms[i], p, i), g[i], part);
                     d[p][i] *= g[i];
-                    preMean[0] = fmaf(d[p][i], normed, preMean[0]);
                 }
+                addToColumns(kPreSums, p, terms);
+                preMean[0] += at.Counted(part, p);
             }
             SumsOverGroup<1, kMaxWaves>(preMean, waves, parity, preSums);
             preMean[0] *= each;
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
-                if (!here[p]) continue;
                 float v[8];
-                Unpack<Codec>(s[p], v);
+                Unpack<Codec>(in.s[p], v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) d[p][i] = preRstd * (d[p][i] - v[i] * preRstd * preMean[0]);
             }
         }
 #pragma unroll
         for (int p = 0; p < kPackets; ++p) {
-            if (!here[p]) continue;
-            if (sums) {
+            if (!kPre || sums) {
                 float v[8];
-                Unpack<Codec>(sumGrad[p], v);
+                Unpack<Codec>(in.sumGrad[p], v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[p][i] = pre ? d[p][i] + v[i] : v[i];
+                for (int i = 0; i < 8; ++i) d[p][i] = kPre ? d[p][i] + v[i] : v[i];
             }
             if (a.residualGrad != nullptr) {
                 float v[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = a.residualScale * d[p][i];
-                StorePacket<false, Storage>(a.residualGrad, row * cols + at(p), count(p), Pack<Codec>(v));
+                at.template Store<Storage>(a.residualGrad, begin, p, Pack<Codec>(v));
             }
         }
         // through the gate and the post norm's weights
-        const float rowGate = rowGated ? Gated(rawGate, a.sigmoid) : 1.f;
+        const float rowGate = rowGated ? Gated(raw, a.sigmoid) : 1.f;
         float rowSums[2] = {0.f, 0.f};  // du postGamma x^, dv u
 #pragma unroll
         for (int p = 0; p < kPackets; ++p) {
-            if (!here[p]) continue;
-            float xs[8], g[8];
-            if (needsX) Unpack<Codec>(x[p], xs);
-            if (post) Unpack<Gamma>(postGamma[p], g);
-            float gateEach[8], gateGrad[8];
-            if constexpr (kRead) Unpack<Codec>(gateRow[p], gateEach);
+            float xs[8], g[8], gate[8], gateGrad[8], terms[8], parts[2] = {0.f, 0.f};
+            Unpack<Codec>(in.x[p], xs);
+            if (post) {
+                Unpack<Gamma>(weights(postHeld, a.post, p), g);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) g[i] = 1.f;
+            }
+            float slope[8];
+            if constexpr (kRead) {
+                Unpack<Codec>(in.gate[p], gate);
+                OpenGates(gate, slope, a.sigmoid);
+            } else if constexpr (kHeld) {
+                Unpack<Gamma>(weights(gateHeld, a.gate, p), gate);
+                OpenGates(gate, a.sigmoid);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float v = a.branchScale * d[p][i];
-                const float normed = needsX ? xs[i] * postRstd : 0.f;
-                const float u = post ? normed * g[i] : normed;
+                const float normed = xs[i] * postRstd;
                 if constexpr (kHeld) {
-                    gateSum[p][i] = fmaf(v, u, gateSum[p][i]);
-                    v *= gateHeld[p][i];
+                    terms[i] = v * normed;
+                    v *= gate[i];
                 } else if constexpr (kRead) {
-                    float open = gateEach[i], slope = 1.f;
-                    if (a.sigmoid) {
-                        const Sigmoid sg = SigmoidOf(gateEach[i]);
-                        open = sg.p;
-                        slope = sg.p * sg.rest;
-                    }
-                    gateGrad[i] = v * u * slope;
-                    v *= open;
+                    gateGrad[i] = v * (normed * g[i]) * slope[i];
+                    v *= gate[i];
+                    terms[i] = v * normed;
                 } else {
-                    rowSums[1] = fmaf(v, u, rowSums[1]);
+                    parts[1] = fmaf(at.Own(v * normed, p, i), g[i], parts[1]);
                     v *= rowGate;
+                    terms[i] = v * normed;
                 }
-                if (post) {
-                    postSum[p][i] = fmaf(v, normed, postSum[p][i]);
-                    v *= g[i];
-                    rowSums[0] = fmaf(v, normed, rowSums[0]);
-                }
+                v *= g[i];
+                parts[0] = fmaf(at.Own(v, p, i), normed, parts[0]);
                 d[p][i] = v;
             }
+            if (branchSums) addToColumns(kBranchSums, p, terms);
+            rowSums[0] += at.Counted(parts[0], p);
+            rowSums[1] += at.Counted(parts[1], p);
             if constexpr (kRead) {
-                if (a.gateGrad != nullptr) StorePacket<false, Storage>(a.gateGrad, row * cols + at(p), count(p), Pack<Codec>(gateGrad));
+                if (a.gateGrad != nullptr) at.template Store<Storage>(a.gateGrad, begin, p, Pack<Codec>(gateGrad));
             }
         }
-        // The row's own values are needed once more: x is unpacked before the next row's loads take its place.
-        const float rstd = postRstd, raw = rawGate;
-        float xs[kPackets][8];
-        if (post) {
+        Packet<Codec> x[kPackets];  // needed once more
 #pragma unroll
-            for (int p = 0; p < kPackets; ++p) {
-                if (here[p]) Unpack<Codec>(x[p], xs[p]);
-            }
+        for (int p = 0; p < kPackets; ++p) x[p] = in.x[p];
+        if constexpr (!kEarly) {
+            __builtin_amdgcn_sched_barrier(0);  // not in front of the last uses
+            load(in, min(next, a.rows - 1));
         }
-        const int64_t next = row + gridDim.x;
-        if (next < a.rows) load(next);
         if (post || rowGated) SumsOverGroup<2, kMaxWaves>(rowSums, waves, parity, postSums);
         if (rowGated && a.gateGrad != nullptr && tid == 0) static_cast<float*>(a.gateGrad)[row] = rowSums[1] * GateSlope(raw, a.sigmoid);
         if (a.xGrad != nullptr) {
             const float mean = rowSums[0] * each;
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
-                if (!here[p]) continue;
                 if (post) {
+                    float xs[8];
+                    Unpack<Codec>(x[p], xs);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) d[p][i] = rstd * (d[p][i] - xs[p][i] * rstd * mean);
+                    for (int i = 0; i < 8; ++i) d[p][i] = postRstd * (d[p][i] - xs[i] * postRstd * mean);
                 }
-                StorePacket<false, Storage>(a.xGrad, row * cols + at(p), count(p), Pack<Codec>(d[p]));
+                at.template Store<Storage>(a.xGrad, begin, p, Pack<Codec>(d[p]));
             }
         }
         row = next;
+    };
+    GradRows<Codec, kPackets, kRead> first;
+    load(first, row);
+    if constexpr (kPackets == 1) {
+        // The two rows take turns where they lie: moved, a row's loads would have to have ended, and the stores behind them.
+        GradRows<Codec, kPackets, kRead> second;
+        while (true) {
+            step(first, second, 0);
+            if (row >= a.rows) break;
+            step(second, first, 1);
+            if (row >= a.rows) break;
+        }
+    } else if constexpr (kEarly) {
+        GradRows<Codec, kPackets, kRead> second;
+        for (int parity = 0; row < a.rows; parity ^= 1) {
+            step(first, second, parity);
+            first = second;
+        }
+    } else {
+        for (int parity = 0; row < a.rows; parity ^= 1) step(first, first, parity);
     }
     const int64_t mine = static_cast<int64_t>(blockIdx.x) * cols;
-    auto leave = [&](int which, const float (&sum)[8], int p) {
-        if (a.columnGrads[which] == nullptr) return;
-        float* const to = a.columnSums[which] + mine + at(p);
-        for (int i = 0; i < 8; ++i) {
-            if (i < count(p)) to[i] = sum[i];
-        }
-    };
 #pragma unroll
-    for (int p = 0; p < kPackets; ++p) {
-        if (!here[p]) continue;
-        leave(kPostSums, postSum[p], p);
-        leave(kPreSums, preSum[p], p);
-        if constexpr (kHeld) leave(kGateSums, gateSum[p], p);
+    for (int c = 0; c < kColumnSums; ++c) {
+        if (a.columnSums[c] == nullptr) continue;
+#pragma unroll
+        for (int p = 0; p < kPackets; ++p) {
+            Packet<F32> piece;
+            if constexpr (kLds) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) piece.q[h] = __builtin_bit_cast(uint4, ldsSums[((c * kPackets + p) * 2 + h) * threads + tid]);
+            } else {
+                __builtin_memcpy(&piece, sumHeld[c][p], sizeof(piece));
+            }
+            at.template Store<float>(a.columnSums[c], mine, p, piece);
+        }
     }
 }
 
@@ -332,17 +404,16 @@ __global__ __launch_bounds__(kAnyThreads) void SandwichGradColumnsKernel(Sandwic
     const int64_t group = GroupIndex() / blocks;
     const int64_t c = GroupIndex() % blocks * kAnyThreads + threadIdx.x;
     if (group >= a.groups || c >= a.cols) return;
-    float sums[kColumnSums] = {0.f, 0.f, 0.f};
+    float sums[kColumnSums] = {0.f, 0.f};
     for (int64_t row = group; row < a.rows; row += a.groups) {
         const Element<Codec, Gamma> el(a, row);
         if (a.pre != nullptr) sums[kPreSums] = fmaf(el.Value(a.normGrad, c), el.NormedSum(c), sums[kPreSums]);
-        if (a.post == nullptr && a.gateKind != kGateChannel) continue;
-        const float v = a.branchScale * el.SumGrad(c, a.rowMeans[row]), normed = el.NormedX(c);
-        sums[kGateSums] = fmaf(v, el.Unit(c, normed), sums[kGateSums]);
-        sums[kPostSums] = fmaf(v * el.Open(c), normed, sums[kPostSums]);
+        if (a.columnSums[kBranchSums] == nullptr) continue;
+        const float v = a.branchScale * el.SumGrad(c, a.rowMeans[row]);
+        sums[kBranchSums] = fmaf(a.gateKind == kGateChannel ? v : v * el.Open(c), el.NormedX(c), sums[kBranchSums]);
     }
     for (int i = 0; i < kColumnSums; ++i) {
-        if (a.columnGrads[i] != nullptr) a.columnSums[i][group * a.cols + c] = sums[i];
+        if (a.columnSums[i] != nullptr) a.columnSums[i][group * a.cols + c] = sums[i];
     }
 }
 
@@ -354,25 +425,37 @@ __global__ __launch_bounds__(kFinishThreads) void SandwichGradFinishKernel(Sandw
     constexpr int kRuns = kFinishThreads / kWave;
     __shared__ double sums[kRuns][kWave];
     const int which = blockIdx.y;
-    if (a.columnGrads[which] == nullptr) return;
+    const float* const columnSums = a.columnSums[which];  // (of no rows: none, and the sums are zeros)
+    if (which == kPreSums ? a.preGammaGrad == nullptr : a.postGammaGrad == nullptr && a.channelGrad == nullptr) return;
     const int run = threadIdx.x / kWave, lane = threadIdx.x % kWave;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * kWave + lane;
     double sum = 0.0;
     if (c < a.cols) {
-#pragma unroll 4
-        for (int64_t g = run; g < a.groups; g += kRuns) sum += a.columnSums[which][g * a.cols + c];
+#pragma unroll 8
+        for (int64_t g = run; g < a.groups; g += kRuns) sum += columnSums[g * a.cols + c];
     }
     sums[run][lane] = sum;
     __syncthreads();
     if (run != 0 || c >= a.cols) return;
     sum = 0.0;
     for (int r = 0; r < kRuns; ++r) sum += sums[r][lane];
-    if (which == kGateSums) sum *= GateSlope(Gamma::Load(static_cast<const typename Gamma::Storage*>(a.gate)[c]), a.sigmoid);
-    a.columnGrads[which][c] = static_cast<float>(sum);
+    if (which == kPreSums) {
+        a.preGammaGrad[c] = static_cast<float>(sum);
+        return;
+    }
+    auto weight = [&](const void* w) { return Gamma::Load(static_cast<const typename Gamma::Storage*>(w)[c]); };
+    if (a.gateKind != kGateChannel) {
+        a.postGammaGrad[c] = static_cast<float>(sum);
+        return;
+    }
+    const float gate = weight(a.gate);
+    if (a.postGammaGrad != nullptr) a.postGammaGrad[c] = static_cast<float>(sum * Gated(gate, a.sigmoid));
+    if (a.channelGrad != nullptr) a.channelGrad[c] = static_cast<float>(sum * GateSlope(gate, a.sigmoid) * (a.post != nullptr ? weight(a.post) : 1.f));
 }
 
-// Rows of up to 8192 values stay in registers, with what their columns owe.
-constexpr int kMaxPackets = 2;
+// Rows of eight to 16384 values are one workgroup's at a time.
+constexpr int kMaxPackets = 4;
+constexpr int64_t kCus = 256;
 constexpr int64_t kPacketCols = 8ll * kMaxPacketThreads * kMaxPackets;
 
 class SandwichGradExecutor : public aclOpExecutor {
@@ -383,12 +466,15 @@ class SandwichGradExecutor : public aclOpExecutor {
     uint64_t offMeans = 0, offSums = 0;
     int threads = 0;
 
-    bool Columns() const { return args.columnGrads[kPostSums] != nullptr || args.columnGrads[kPreSums] != nullptr || args.columnGrads[kGateSums] != nullptr; }
+    // Which column sums are wanted.
+    bool Wants(int which) const { return which == kPreSums ? args.preGammaGrad != nullptr : args.postGammaGrad != nullptr || args.channelGrad != nullptr; }
+    bool Columns() const { return Wants(kPreSums) || Wants(kBranchSums); }
+    bool InPackets() const { return args.cols >= 8 && args.cols <= kPacketCols; }
 
     // Returns the workspace's size.
     uint64_t Plan() {
         uint64_t bytes = 0;
-        if (args.cols > kPacketCols) {
+        if (!InPackets()) {
             args.groups = (args.rows + kColumnRows - 1) / kColumnRows;
             // enough workgroups side by side for the columns' sums of short batches
             const int64_t blocks = (args.cols + kAnyThreads - 1) / kAnyThreads;
@@ -397,26 +483,51 @@ class SandwichGradExecutor : public aclOpExecutor {
             bytes = opapi::AlignUp(4 * static_cast<uint64_t>(args.rows), 16);
         } else {
             const int64_t lanes = (args.cols + 7) / 8;
-            const int64_t packets = lanes <= kMaxPacketThreads ? 1 : kMaxPackets;
+            const int64_t packets = lanes <= kMaxPacketThreads ? 1 : lanes <= 2 * kMaxPacketThreads ? 2 : kMaxPackets;
             threads = static_cast<int>(((lanes + packets - 1) / packets + kWave - 1) / kWave * kWave);
-            args.groups = 256 * std::max(1, kMaxPacketThreads / threads);
+            const int64_t waves = threads / kWave;
+            args.groups = kCus * std::max<int64_t>(1, kMaxPacketThreads / kWave / waves);
+            if (packets == 1 && waves > 4 && args.rows >= 8 * 2 * kCus) args.groups = 2 * kCus;
             if (args.groups < (args.rows + kColumnRows - 1) / kColumnRows) args.groups = (args.rows + kColumnRows - 1) / kColumnRows;
             if (args.groups > args.rows) args.groups = args.rows;
         }
         offSums = bytes;
-        for (float* grads : args.columnGrads) {
-            if (grads != nullptr) bytes += opapi::AlignUp(4 * static_cast<uint64_t>(args.groups) * static_cast<uint64_t>(args.cols), 16);
+        for (int i = 0; i < kColumnSums; ++i) {
+            if (Wants(i)) bytes += opapi::AlignUp(4 * static_cast<uint64_t>(args.groups) * static_cast<uint64_t>(args.cols), 16);
         }
         return bytes;
     }
 
+    template <typename Codec, typename Gamma, int kPackets, int kGate, bool kPre, bool kTail>
+    hipError_t LaunchKernel(hipStream_t stream) const {
+        const auto kernel = SandwichGradKernel<Codec, Gamma, kPackets, kGate, kPre, kTail>;
+        int lds = 0;
+        if constexpr (kSumsInLds<Codec, Gamma, kPackets>) {
+            static std::atomic<uint64_t> done{0};
+            constexpr int kMost = kColumnSums * kPackets * 2 * kMaxPacketThreads * static_cast<int>(sizeof(float4));
+            lds = kMost / kMaxPacketThreads * threads;
+            const hipError_t e = opapi::EnsureDynamicLds(reinterpret_cast<const void*>(kernel), kMost, done);
+            if (e != hipSuccess) return e;
+        }
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(args.groups)), dim3(static_cast<unsigned>(threads)), static_cast<unsigned>(lds), stream, args);
+        return hipSuccess;
+    }
+
+    template <typename Codec, typename Gamma, int kPackets, int kGate>
+    hipError_t LaunchPackets(hipStream_t stream) const {
+        const bool tail = args.cols % 8 != 0;
+        if (args.pre != nullptr) {
+            return tail ? LaunchKernel<Codec, Gamma, kPackets, kGate, true, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kGate, true, false>(stream);
+        }
+        return tail ? LaunchKernel<Codec, Gamma, kPackets, kGate, false, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kGate, false, false>(stream);
+    }
+
     template <typename Codec, typename Gamma, int kPackets>
-    void ForGate(hipStream_t stream) const {
+    hipError_t ForGate(hipStream_t stream) const {
         const int packets = GatePackets(args.gateKind);
-        const dim3 grid(static_cast<unsigned>(args.groups));
-        if (packets == kHeldPackets) hipLaunchKernelGGL((SandwichGradKernel<Codec, Gamma, kPackets, kHeldPackets>), grid, dim3(threads), 0, stream, args);
-        else if (packets == kReadPackets) hipLaunchKernelGGL((SandwichGradKernel<Codec, Gamma, kPackets, kReadPackets>), grid, dim3(threads), 0, stream, args);
-        else hipLaunchKernelGGL((SandwichGradKernel<Codec, Gamma, kPackets, kNoPackets>), grid, dim3(threads), 0, stream, args);
+        if (packets == kHeldPackets) return LaunchPackets<Codec, Gamma, kPackets, kHeldPackets>(stream);
+        if (packets == kReadPackets) return LaunchPackets<Codec, Gamma, kPackets, kReadPackets>(stream);
+        return LaunchPackets<Codec, Gamma, kPackets, kNoPackets>(stream);
     }
 
     aclnnStatus Run(void* workspace, hipStream_t stream) override {
@@ -425,23 +536,27 @@ class SandwichGradExecutor : public aclOpExecutor {
         args.rowMeans = reinterpret_cast<float*>(at);
         at += offSums;
         for (int i = 0; i < kColumnSums; ++i) {
-            if (args.columnGrads[i] == nullptr) continue;
+            if (!Wants(i)) continue;
             args.columnSums[i] = reinterpret_cast<float*>(at);
             at += opapi::AlignUp(4 * static_cast<uint64_t>(args.groups) * static_cast<uint64_t>(args.cols), 16);
         }
+        hipError_t err = hipSuccess;
         ForTypes(dtype, weightType, [&](auto codec, auto gamma) {
             using Codec = decltype(codec);
             using Gamma = decltype(gamma);
             if (args.rows > 0) {
                 opapi::KernelTimer timer("sandwich_norm_grad", stream);
-                if (args.cols > kPacketCols) {
+                const int64_t lanes = (args.cols + 7) / 8;
+                if (!InPackets()) {
                     hipLaunchKernelGGL((SandwichGradRowsKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
                     const int64_t blocks = (args.cols + kAnyThreads - 1) / kAnyThreads;
                     if (Columns()) hipLaunchKernelGGL((SandwichGradColumnsKernel<Codec, Gamma>), GridOf(blocks * args.groups), dim3(kAnyThreads), 0, stream, args);
-                } else if (args.cols <= 8 * kMaxPacketThreads) {
-                    ForGate<Codec, Gamma, 1>(stream);
+                } else if (lanes <= kMaxPacketThreads) {
+                    err = ForGate<Codec, Gamma, 1>(stream);
+                } else if (lanes <= 2 * kMaxPacketThreads) {
+                    err = ForGate<Codec, Gamma, 2>(stream);
                 } else {
-                    ForGate<Codec, Gamma, kMaxPackets>(stream);
+                    err = ForGate<Codec, Gamma, kMaxPackets>(stream);
                 }
             }
             if (Columns()) {
@@ -450,7 +565,7 @@ class SandwichGradExecutor : public aclOpExecutor {
                 hipLaunchKernelGGL((SandwichGradFinishKernel<Gamma>), grid, dim3(kFinishThreads), 0, stream, args);
             }
         });
-        const hipError_t err = hipGetLastError();
+        if (err == hipSuccess) err = hipGetLastError();
         OPAPI_CHECK(err == hipSuccess, ACLNN_ERR_RUNTIME_ERROR, "aclnnMoeSandwichNormGrad: launch failed: %s", hipGetErrorString(err));
         return ACLNN_SUCCESS;
     }
@@ -529,9 +644,9 @@ extern "C" aclnnStatus aclnnMoeSandwichNormGradGetWorkspaceSize(
     OPAPI_BIND(ex, preRstdOptional, &a.preRstd);
     a.xGrad = DataPtr(xGradOutOptional);
     a.residualGrad = DataPtr(residualGradOutOptional);
-    a.columnGrads[kPostSums] = reinterpret_cast<float*>(DataPtr(postGammaGradOutOptional));
-    a.columnGrads[kPreSums] = reinterpret_cast<float*>(DataPtr(preGammaGradOutOptional));
-    if (shape.gateKind == kGateChannel) a.columnGrads[kGateSums] = reinterpret_cast<float*>(DataPtr(gateGradOutOptional));
+    a.postGammaGrad = reinterpret_cast<float*>(DataPtr(postGammaGradOutOptional));
+    a.preGammaGrad = reinterpret_cast<float*>(DataPtr(preGammaGradOutOptional));
+    if (shape.gateKind == kGateChannel) a.channelGrad = reinterpret_cast<float*>(DataPtr(gateGradOutOptional));
     else a.gateGrad = DataPtr(gateGradOutOptional);
     a.rows = shape.rows;
     a.cols = shape.cols;

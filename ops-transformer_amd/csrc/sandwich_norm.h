@@ -18,6 +18,23 @@ constexpr int kNoPackets = 0, kHeldPackets = 1, kReadPackets = 2;
 inline int GatePackets(int kind) { return kind == kGateChannel ? kHeldPackets : kind == kGateEach ? kReadPackets : kNoPackets; }
 
 __device__ __forceinline__ float Gated(float gate, int sigmoid) { return sigmoid ? SigmoidOf(gate).p : gate; }
+// Eight gates opened (and their slopes), the choice made once: made element by element both sides are worked out.
+__device__ __forceinline__ void OpenGates(float (&gate)[8], int sigmoid) {
+    if (!sigmoid) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) gate[i] = SigmoidOf(gate[i]).p;
+}
+__device__ __forceinline__ void OpenGates(float (&gate)[8], float (&slope)[8], int sigmoid) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) slope[i] = 1.f;
+    if (!sigmoid) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const Sigmoid s = SigmoidOf(gate[i]);
+        gate[i] = s.p;
+        slope[i] = s.p * s.rest;
+    }
+}
 
 // kCount sums over a workgroup, the same bits in every lane.  `parity` alternates between calls that follow each other: one barrier a call.
 template <int kCount, int kMaxWaves>
@@ -37,6 +54,64 @@ __device__ __forceinline__ void SumsOverGroup(float (&v)[kCount], int waves, int
         for (int i = 0; i < kCount; ++i) v[i] += lds[parity][w][i];
     }
 }
+
+// The piece itself, through a statement the optimiser cannot see through: what a loop makes of it is not made in front of the loop and held (weights of 16
+// bits, unpacked, take twice their registers, and a gate's sigmoid as many again).
+template <typename Codec>
+__device__ __forceinline__ void HoldPacked(Packet<Codec>& piece) {
+    if constexpr (sizeof(typename Codec::Storage) == 4) return;
+#pragma unroll
+    for (uint4& q : piece.q) asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w));
+}
+
+// Where a lane's pieces of eight elements lie in a row of `cols`, at least eight.  Every lane has each of its pieces: one that would end behind the row is the
+// row's last eight elements, the first `skip` of which are other lanes' (all eight of a piece that would begin behind it; kTail: cols is no multiple of eight,
+// else there are no others).  So loads are without a branch, the compiler knows how many there are, and a wait for one row's need not be one for the
+// next row's: with branches 8192 x 7168 rows waited for all of them.
+template <int kPackets, bool kTail>
+struct Pieces {
+    uint32_t from[kPackets];
+    int skip[kPackets];
+
+    __device__ __forceinline__ Pieces(int cols, int threads, int tid) {
+#pragma unroll
+        for (int p = 0; p < kPackets; ++p) {
+            const int at = (p * threads + tid) * 8;
+            from[p] = static_cast<uint32_t>(min(at, cols - 8));
+            skip[p] = min(at - static_cast<int>(from[p]), 8);
+        }
+    }
+    // Sums are of the lane's own elements: Own() of each term, Counted() of the piece's.
+    __device__ __forceinline__ float Own(float v, int p, int i) const { return kTail && i < skip[p] ? 0.f : v; }
+    __device__ __forceinline__ float Counted(float part, int p) const { return kTail || skip[p] == 0 ? part : 0.f; }
+    // `row`: where the row begins, the same for the wave.
+    template <typename Codec>
+    __device__ __forceinline__ Packet<Codec> Load(const void* base, int64_t row, int p) const {
+        Packet<Codec> piece;
+        __builtin_memcpy(&piece, static_cast<const typename Codec::Storage*>(base) + row + from[p], sizeof(piece));
+        return piece;
+    }
+    // All eight: what two lanes have of an element has to be the same bits.
+    template <typename Storage, typename P>
+    __device__ __forceinline__ void Store(void* base, int64_t row, int p, const P& piece) const {
+        __builtin_memcpy(static_cast<Storage*>(base) + row + from[p], &piece, sizeof(piece));
+    }
+    // The lane's own.
+    template <typename Storage, typename P>
+    __device__ __forceinline__ void StoreOwn(void* base, int64_t row, int p, const P& piece) const {
+        Storage* const to = static_cast<Storage*>(base) + row + from[p];
+        if (skip[p] == 0) {
+            __builtin_memcpy(to, &piece, sizeof(piece));
+        } else if (kTail) {
+            Storage raw[8];
+            __builtin_memcpy(raw, &piece, sizeof(piece));
+#pragma unroll
+            for (int i = 1; i < 8; ++i) {
+                if (i >= skip[p]) to[i] = raw[i];
+            }
+        }
+    }
+};
 
 // The weights that go with the channels, gammas and a gate per channel, share a type: x's, or FLOAT.
 struct SandwichShape {
