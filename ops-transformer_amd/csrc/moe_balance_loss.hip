@@ -48,25 +48,28 @@ constexpr int kFinishThreads = 1024;
 constexpr int kFinishFew = 64, kFinishMany = 256;
 constexpr int64_t kFewPieces = 64;
 
-template <typename Codec, int kLanes, int kPieces, bool kSigmoid>
+template <typename Codec, int kLanes, int kPieces, bool kSigmoid, bool kCut>
 __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs a) {
     using Row = RowOf<kLanes, kPieces>;
     constexpr int kEach = Row::kEach;
     constexpr int kRowsAtOnce = kWave / kLanes;
     constexpr int kUnroll = UnrollOf(kPieces);
     constexpr int kStride = kChunkWaves * kRowsAtOnce;
-    __shared__ alignas(16) float sums[kChunkWaves][Row::kWidth];
-    __shared__ int32_t picked[Row::kWidth];
-    __shared__ int32_t live;
+    // kCut: sequences may end inside a chunk.  The rows of two go in one pass, where LDS has room for both tables (packed batch of 3011 x 160 in 7
+    // sequences 12.3 -> 11.0 us; without offsets the second sums cost 0.7 us for nothing).
+    constexpr int kAtOnce = kCut && kPieces <= 2 ? 2 : 1;
+    __shared__ alignas(16) float sums[kAtOnce][kChunkWaves][Row::kWidth];
+    __shared__ int32_t picked[kAtOnce][Row::kWidth];
+    __shared__ int32_t live[kAtOnce];
     __shared__ double finishing[kChunkWaves];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, l = lane % kLanes, side = lane / kLanes;
     const typename Codec::Storage* const x = static_cast<const typename Codec::Storage*>(a.x);
     auto isExpert = [&](int32_t id) { return static_cast<uint32_t>(id) < static_cast<uint32_t>(a.experts); };
 
-    auto totalOf = [&](int e) {
+    auto totalOf = [&](int q, int e) {
         float total = 0.f;
 #pragma unroll
-        for (int w = 0; w < kChunkWaves; ++w) total += sums[w][e];
+        for (int w = 0; w < kChunkWaves; ++w) total += sums[q][w][e];
         return total;
     };
     const Sequences& seqs = a.sequences;
@@ -97,42 +100,44 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
         }
     };
     loadFirst(first, last);
-    for (int e = tid; e < a.experts; e += kChunkThreads) picked[e] = 0;
-    if (tid == 0) live = 0;
+#pragma unroll
+    for (int q = 0; q < kAtOnce; ++q) {
+        for (int e = tid; e < a.experts; e += kChunkThreads) picked[q][e] = 0;
+        if (tid == 0) live[q] = 0;
+    }
     if (blockIdx.x == 0 && !a.alone) {  // for the second kernel
         for (int s = tid; s < seqs.count; s += kChunkThreads) a.tickets[s] = 0;
     }
     __syncthreads();
-    int32_t s = -1;
-    int64_t following = first;  // where the sequence behind s ends
     for (int64_t at = first;;) {
-        int64_t end = last;
+        int32_t s = 0;
+        int64_t border = last, end = last;  // of sequence s, and of the rows of this pass: those behind the border are of sequence s + 1
         if (!a.alone) {
             if (at >= last) return;
-            if (seqs.offsets == nullptr) {
-                s = 0;
-            } else {
-                // `at` is in the next sequence, unless some have no rows; whatever the offsets are, s starts at or in front of it and ends behind it
-                if (following > at) {
-                    end = following;
-                    ++s;
-                } else {
-                    s = seqs.Of(at, end);
-                }
+            if constexpr (kCut) {
+                // whatever the offsets are, s starts at or in front of `at` and ends behind it
+                int64_t beyond;
+                s = seqs.Of(at, border, beyond);
                 if (s >= seqs.count) return;
-                end = min(last, end);
-            }
-            if (s < 0) {
-                at = end;
-                following = 0;
-                if (at < last) loadFirst(at, last);
-                continue;
+                border = min(last, border);
+                end = border;
+                if (s < 0) {
+                    at = border;
+                    if (at < last) loadFirst(at, last);
+                    continue;
+                }
+                if (kAtOnce == 2 && border < last && s + 1 < seqs.count) end = max(border, min(last, beyond >= 0 ? beyond : seqs.Start(s + 2)));
             }
         }
-        float sum[kEach];
+        const bool both = end > border;
+        float sum[kAtOnce][kEach];
+        int32_t counted[kAtOnce];
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) sum[i] = 0.f;
-        int32_t counted = 0;
+        for (int q = 0; q < kAtOnce; ++q) {
+            counted[q] = 0;
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) sum[q][i] = 0.f;
+        }
 #pragma unroll 1
         for (int64_t row = at + wave * kRowsAtOnce; row < end; row += kUnroll * kStride) {
             // Scores, for softmax before their division by the sum.  Row by row without a branch: the rows' reductions overlap.
@@ -161,14 +166,20 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
             }
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                counted += counts[u] && l == 0 ? 1 : 0;
+                const bool behind = kAtOnce == 2 && row + u * kStride + side >= border;
+#pragma unroll
+                for (int q = 0; q < kAtOnce; ++q) counted[q] += counts[u] && l == 0 && behind == (q == 1) ? 1 : 0;
                 if (kSigmoid && counts[u] && total[u] < kLostSum) {
                     lost = true;
                     counts[u] = false;
                 }
                 const float inverse = total[u] == 0.f ? 0.f : Reciprocal(total[u]);
 #pragma unroll
-                for (int i = 0; i < kEach; ++i) sum[i] = counts[u] ? fmaf(p[u][i], inverse, sum[i]) : sum[i];
+                for (int q = 0; q < kAtOnce; ++q) {
+                    const bool here = counts[u] && behind == (q == 1);
+#pragma unroll
+                    for (int i = 0; i < kEach; ++i) sum[q][i] = here ? fmaf(p[u][i], inverse, sum[q][i]) : sum[q][i];
+                }
             }
             if (kSigmoid && lost) {  // rare, and made again (the lanes of a row agree)
 #pragma unroll 1
@@ -180,59 +191,70 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
                     if (!(SumOver<kLanes>(scores) < kLostSum) || !isExpert(a.expertIdx[again * a.k])) continue;
                     LostSharesOf<kLanes>(v, share);
 #pragma unroll
-                    for (int i = 0; i < kEach; ++i) sum[i] += share[i];
+                    for (int q = 0; q < kAtOnce; ++q) {
+#pragma unroll
+                        for (int i = 0; i < kEach; ++i) sum[q][i] += (kAtOnce == 2 && again >= border) == (q == 1) ? share[i] : 0.f;
+                    }
                 }
             }
         }
-        counted = WaveSum(counted);
-        if (lane == 0 && counted != 0) atomicAdd(&live, counted);
-        const int32_t ids = static_cast<int32_t>(end - at) * a.k;
-        if (tid < ids && isExpert(rowId) && isExpert(id)) atomicAdd(&picked[id], 1);
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+            counted[q] = WaveSum(counted[q]);
+            if (lane == 0 && counted[q] != 0) atomicAdd(&live[q], counted[q]);
+        }
+        const int32_t ids = static_cast<int32_t>(end - at) * a.k, idsBefore = static_cast<int32_t>(border - at) * a.k;
+        if (tid < ids && isExpert(rowId) && isExpert(id)) atomicAdd(&picked[kAtOnce == 2 && tid >= idsBefore ? 1 : 0][id], 1);
 #pragma unroll 1
         for (int32_t i = tid + kChunkThreads; i < ids; i += kChunkThreads) {
             const int32_t* const idx = a.expertIdx + at * a.k;
             const int32_t more = idx[i];
-            if (isExpert(idx[i / a.k * a.k]) && isExpert(more)) atomicAdd(&picked[more], 1);
+            if (isExpert(idx[i / a.k * a.k]) && isExpert(more)) atomicAdd(&picked[kAtOnce == 2 && i >= idsBefore ? 1 : 0][more], 1);
         }
-        if (end < last) {  // what comes behind this sequence, on its way meanwhile
-            loadFirst(end, last);
-            following = s + 2 <= seqs.count ? seqs.Start(s + 2) : 0;
-        }
+        if (end < last) loadFirst(end, last);  // what comes behind, on its way meanwhile
         // the rows side by side in a wave; the waves are added up when they are read
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
+        for (int q = 0; q < kAtOnce; ++q) {
+            if (q == 1 && !both) break;
 #pragma unroll
-            for (int d = kLanes; d < kWave; d <<= 1) sum[i] += __shfl_xor(sum[i], d);
-        }
-        if (lane < kLanes) {
+            for (int i = 0; i < kEach; ++i) {
 #pragma unroll
-            for (int p = 0; p < kPieces; ++p) *reinterpret_cast<float4*>(&sums[wave][Row::At(p, l)]) = float4{sum[4 * p], sum[4 * p + 1], sum[4 * p + 2], sum[4 * p + 3]};
+                for (int d = kLanes; d < kWave; d <<= 1) sum[q][i] += __shfl_xor(sum[q][i], d);
+            }
+            if (lane < kLanes) {
+#pragma unroll
+                for (int p = 0; p < kPieces; ++p) {
+                    *reinterpret_cast<float4*>(&sums[q][wave][Row::At(p, l)]) = float4{sum[q][4 * p], sum[q][4 * p + 1], sum[q][4 * p + 2], sum[q][4 * p + 3]};
+                }
+            }
         }
         __syncthreads();
         if (a.alone) break;
-        const int64_t piece = static_cast<int64_t>(blockIdx.x) + s;
+        for (int q = 0; q < (both ? 2 : 1); ++q) {
+            const int64_t piece = static_cast<int64_t>(blockIdx.x) + s + q;
 #pragma unroll 1
-        for (int e = tid; e < a.experts; e += kChunkThreads) {
-            a.pieceSums[piece * a.experts + e] = totalOf(e);
-            a.pieceCounts[piece * a.experts + e] = picked[e];
-            picked[e] = 0;  // for the next sequence
-        }
-        if (tid == 0) {
-            a.pieceRows[piece] = live;
-            live = 0;
+            for (int e = tid; e < a.experts; e += kChunkThreads) {
+                a.pieceSums[piece * a.experts + e] = totalOf(q, e);
+                a.pieceCounts[piece * a.experts + e] = picked[q][e];
+                picked[q][e] = 0;  // for the next sequences
+            }
+            if (tid == 0) {
+                a.pieceRows[piece] = live[q];
+                live[q] = 0;
+            }
         }
         at = end;
         if (at >= last) return;
         __syncthreads();
     }
-    const double n = live > 0 ? live : 1;
+    const double n = live[0] > 0 ? live[0] : 1;
     double loss = 0.0;
 #pragma unroll 1
     for (int e = tid; e < a.experts; e += kChunkThreads) {
-        const double mean = totalOf(e) / n;
-        a.counts[e] = picked[e];
+        const double mean = totalOf(0, e) / n;
+        a.counts[e] = picked[0][e];
         if (a.prob != nullptr) a.prob[e] = static_cast<float>(mean);
-        loss += mean * picked[e];
+        loss += mean * picked[0][e];
     }
     loss = WaveSum(loss);
     if (lane == 0) finishing[wave] = loss;
@@ -241,7 +263,7 @@ __global__ __launch_bounds__(kChunkThreads) void BalanceChunkKernel(BalanceArgs 
     loss = 0.0;
     for (int w = 0; w < kChunkWaves; ++w) loss += finishing[w];
     a.loss[0] = static_cast<float>(loss * a.experts / (a.k * n));
-    a.rowsOut[0] = live;
+    a.rowsOut[0] = live[0];
 }
 
 // A sequence and kExperts of its experts: the pieces' sums in their order, in runs side by side.  Where one workgroup does not hold all experts, the one
@@ -329,8 +351,10 @@ class BalanceExecutor : public aclOpExecutor {
         ForRowLayout(args.experts, [&](auto lanes, auto pieces) {
             constexpr int kLanes = decltype(lanes)::value, kPieces = decltype(pieces)::value;
             const dim3 grid(static_cast<unsigned>(args.chunks));
-            if (args.sigmoid) hipLaunchKernelGGL((BalanceChunkKernel<Codec, kLanes, kPieces, true>), grid, dim3(kChunkThreads), 0, stream, args);
-            else hipLaunchKernelGGL((BalanceChunkKernel<Codec, kLanes, kPieces, false>), grid, dim3(kChunkThreads), 0, stream, args);
+            const bool cut = args.sequences.offsets != nullptr && !args.alone;
+            auto launch = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(kChunkThreads), 0, stream, args); };
+            if (args.sigmoid) cut ? launch(BalanceChunkKernel<Codec, kLanes, kPieces, true, true>) : launch(BalanceChunkKernel<Codec, kLanes, kPieces, true, false>);
+            else cut ? launch(BalanceChunkKernel<Codec, kLanes, kPieces, false, true>) : launch(BalanceChunkKernel<Codec, kLanes, kPieces, false, false>);
         });
     }
 

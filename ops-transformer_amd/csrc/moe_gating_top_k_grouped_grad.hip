@@ -109,8 +109,8 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
         for (int i = 0; i < kEach; ++i) shareGrad[i] = live > 0 ? each * static_cast<float>(counts[i]) : 0.f;
     };
     if (balance) {
-        int64_t end;
-        const int32_t s = a.sequences.Of(first, end);
+        int64_t end, beyond;
+        const int32_t s = a.sequences.Of(first, end, beyond);
         enter(s, end);
     }
     for (int32_t base = 0; base < rows; base += kRowsAtOnce) {
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
             if (a.renorm) {
                 const float total = pickedSum + a.eps;
                 const bool none = pickedSum == 0.f;
-                const float part = none ? 0.f : 1.f / total;
+                const float part = none ? 0.f : __builtin_amdgcn_rcpf(total);
                 scale = a.factor * part;
                 mean = weighted * part;
                 all = scale * weighted * (a.eps * part);

@@ -28,10 +28,12 @@ struct Sequences {
     }
     // The last sequence that starts at or in front of `row`, the same in all lanes of a whole wave: -1 in front of the first, `count` behind the last.  The
     // lanes look at 64 places at a time, so that the round trips are one for up to 63 sequences and four for the most.  Whatever the offsets are, the
-    // sequence starts at or in front of the row, and the next one, at `end`, behind it (behind the last: all rows).
-    __device__ __forceinline__ int32_t Of(int64_t row, int64_t& end) const {
+    // sequence starts at or in front of the row, and the next one, at `end`, behind it (behind the last: all rows).  `beyond`: where the next one
+    // ends, if it was seen on the way; else -1.
+    __device__ __forceinline__ int32_t Of(int64_t row, int64_t& end, int64_t& beyond) const {
         int32_t lo = -1, hi = count + 1;
         end = rows;
+        beyond = -1;
         while (hi - lo > 1) {
             const int32_t step = (hi - lo - 2) / kWave + 1;
             const int32_t at = lo + (static_cast<int32_t>(threadIdx.x % kWave) + 1) * step;
@@ -39,6 +41,7 @@ struct Sequences {
             const uint64_t behind = __ballot(at >= hi || start > row);
             const int32_t steps = behind == 0 ? kWave : __builtin_ctzll(behind);  // that do not lead behind the row
             if (behind != 0 && lo + (steps + 1) * step < hi) {
+                if (step == 1 && steps + 1 < kWave && lo + steps + 2 < hi) beyond = __shfl(start, steps + 1);
                 hi = lo + (steps + 1) * step;
                 end = __shfl(start, steps);
             }
