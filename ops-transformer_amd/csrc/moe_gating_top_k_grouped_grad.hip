@@ -1,9 +1,9 @@
 // aclnnMoeGatingTopKGroupedGrad for gfx950: the gradients of picked weights and of the balance loss with respect to the logits.
 //
-// Both are a row's scores times something less a mean, and the scores are made anew from the logits: one read and one write of a row.  With q_j = p_j / t
-// of the picked ones and A = sum dy_j p_j, the renormalised weights have dp_j = F (dy_j - A / t) / t, and their mean under the softmax is
-// F A / t (1 - sum p / t) = F (A / t) (eps / t): formed so, it is not the difference of two sums that cancel.  The picks' dp goes through LDS from the lane
-// that has the pick to the one that has the expert.
+// Both are a row's scores times something less a mean, and the scores are made anew from the logits: one read and one write of a row.  With t = sum p + eps of
+// the picked ones, q_j = p_j / t and M = sum dy_j q_j, the renormalised weights have p_j dp_j = F q_j (dy_j - M), and the mean of dp under the softmax is
+// F M (1 - sum p / t) = F M eps / t: formed so, it is not the difference of two sums that cancel.  The picks' p dp goes through LDS from the lane that has
+// the pick to the one that has the expert.
 #include "router_rows.h"
 
 #include "aclnnop/aclnn_moe_gating_top_k_grouped_grad.h"
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
 #pragma unroll
             for (int i = 0; i < kEach; ++i) p[i] = e(x[i]);
         }
-        float sum = 0.f, shared = 0.f, pickedSum = 0.f, weighted = 0.f;
+        float sum = 0.f, shared = 0.f, score = 0.f, pickedSum = 0.f, weighted = 0.f;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) {
             sum += p[i];
@@ -152,8 +152,9 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
             if (isExpert(now.id)) {
-                pickedSum = scoreOf[now.id];
-                weighted = now.y * pickedSum;
+                score = scoreOf[now.id];
+                pickedSum = score;
+                weighted = now.y * score;
             }
             for (int j = l + kLanes; j < a.k; j += kLanes) {
                 const int32_t id = idxRows[pick + j];
@@ -170,26 +171,24 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
         }
         const float inverse = sum == 0.f ? 0.f : Reciprocal(sum);
         if constexpr (!kSigmoid) {
-            pickedSum *= inverse;
-            weighted *= inverse;
 #pragma unroll
             for (int i = 0; i < kEach; ++i) p[i] *= inverse;
         }
         float grad[kEach];
         if (weights) {
-            float mean = 0.f, scale = a.factor, all = a.factor * weighted;
+            // The picked scores are divided once, softmax's by the row's sum or by the picked ones': first by the one and then by the other, small ones
+            // would be lost between.
+            const float whole = kSigmoid ? 1.f : sum;
+            float mean = 0.f, part = kSigmoid ? 1.f : inverse, all = a.factor * (weighted * part);
             if (a.renorm) {
-                const float total = pickedSum + a.eps;
-                const bool none = pickedSum == 0.f;
-                const float part = none ? 0.f : __builtin_amdgcn_rcpf(total);
-                scale = a.factor * part;
+                part = pickedSum < 0x1p-126f ? 0.f : __builtin_amdgcn_rcpf(fmaf(a.eps, whole, pickedSum));
                 mean = weighted * part;
-                all = scale * weighted * (a.eps * part);
+                all = a.factor * mean * (a.eps * whole * part);
             }
-            if (isExpert(now.id)) atomicAdd(pickedOf + now.id, scale * (now.y - mean));
+            if (isExpert(now.id)) atomicAdd(pickedOf + now.id, a.factor * (score * part) * (now.y - mean));
             for (int j = l + kLanes; j < a.k; j += kLanes) {
                 const int32_t id = idxRows[pick + j];
-                if (isExpert(id)) atomicAdd(pickedOf + id, scale * (yGradOf(pick + j) - mean));
+                if (isExpert(id)) atomicAdd(pickedOf + id, a.factor * (scoreOf[id] * part) * (yGradOf(pick + j) - mean));
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -201,8 +200,8 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
                 const float d[4] = {dp.x, dp.y, dp.z, dp.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if constexpr (kSigmoid) grad[4 * q + i] = d[i] * (p[4 * q + i] * rest[4 * q + i]);
-                    else grad[4 * q + i] = p[4 * q + i] * (d[i] - all);
+                    if constexpr (kSigmoid) grad[4 * q + i] = d[i] * rest[4 * q + i];
+                    else grad[4 * q + i] = fmaf(p[4 * q + i], -all, d[i]);
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

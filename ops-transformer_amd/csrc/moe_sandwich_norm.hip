@@ -107,7 +107,10 @@ __global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(Sandw
                 float v[8], part = 0.f;
                 Unpack<Codec>(in.x[p], v);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) part = fmaf(at.Own(v[i], p, i), v[i], part);
+                for (int i = 0; i < 8; ++i) {
+                    const float own = at.Own(v[i], p, i);
+                    part = fmaf(own, own, part);
+                }
                 squares[0] += at.Counted(part, p);
             }
             SumsOverGroup<1, kMaxWaves>(squares, waves, parity, postSums);
@@ -150,7 +153,10 @@ __global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(Sandw
             Unpack<Gamma>(preGamma[p], g);
             float part = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) part = fmaf(at.Own(v[i], p, i), v[i], part);
+            for (int i = 0; i < 8; ++i) {
+                const float own = at.Own(v[i], p, i);  // twice: of another lane's element there may be an infinite value here, made of its sum in place
+                part = fmaf(own, own, part);
+            }
             sumSquares += at.Counted(part, p);
             if (a.y != nullptr) {
                 float smooth[8];

@@ -348,6 +348,22 @@ def test_grad_rows_of_unusual_values(aclnn, dev, score):
         assert not got[1].any() and not got[8].any()
 
 
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("E", [96, 2048])
+def test_grad_of_picks_with_small_scores(aclnn, dev, E, score):
+    """Picks far below the row's top, with nothing added to their sum: their shares of it are ordinary numbers, though a score divided by the row's sum, or one
+    divided by the sum of the scores, would leave fp32."""
+    T, k = 40, 4
+    x, _ = _router_inputs(T, E, k, torch.float32, 17)
+    idx = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:k] for t in range(T)]).int()
+    x = x.clamp(-2, 2)
+    x.scatter_add_(1, idx.long(), torch.full((T, k), -82.0))        # e^(-82 - 2 - 2) is above 2^-126, and divided by the sum of a row it is below
+    dy = torch.randn((T, k), generator=torch.Generator().manual_seed(18))
+    for eps in (0.0, 2.0 ** -120):
+        got = aclnn.moe_gating_top_k_grouped_grad(*_on(dev, x, idx, dy), score_type=score, renorm=1, eps=eps)
+        _check_grad(got, x, idx, dy, None, None, None, None, score, 1, 1.0, eps)
+
+
 def test_grad_against_differences(aclnn, dev):
     """Along random directions: the definition's central differences in 64 bits (their own error: h^2 of third derivatives below 1, and 2^-53 / h of the value)."""
     T, E, k = 40, 24, 3
@@ -515,6 +531,32 @@ def test_sandwich_rows_of_unusual_values(aclnn, dev, H):
         _check_sandwich(x[rows], res[rows], post, gate[rows], pre, [t[rows] for t in (total, norm, y, scale, post_rstd, pre_rstd)])
     nothing = aclnn.moe_sandwich_norm(*_on(dev, torch.zeros(2, H), torch.zeros(2, H), post, None, pre), epsilon=0.0, output_rstd=True)
     assert not any(t.any() for t in nothing if t is not None)
+
+
+def test_sandwich_in_place_beside_sums_near_the_top(aclnn, dev):
+    """The sum in the residual's place where a lane's last piece reaches back over another wave's: what that one has written there already, taken for the
+    residual once more, would be past the type's range, and must not come into the row's norm."""
+    T, H = 600, 1031
+    x = torch.full((T, H), 3e4, dtype=torch.float16)
+    res = torch.full((T, H), 2.5e4, dtype=torch.float16)
+    pre = torch.ones(H, dtype=torch.float16)
+    for _ in range(3):
+        x_dev, res_dev, pre_dev = _on(dev, x, res, pre)
+        out = (res_dev, torch.empty_like(x_dev), torch.empty((T, H), dtype=torch.int8, device=dev), torch.empty(T, device=dev), None, torch.empty(T, device=dev))
+        _check_sandwich(x, res, None, None, pre, aclnn.moe_sandwich_norm(x_dev, res_dev, pre_gamma=pre_dev, out=out))
+
+
+def test_sandwich_gate_of_one_row_for_all(aclnn, dev):
+    """A gate with a stride of zero over the rows is read as a gate of its own for each of them."""
+    T, H = 19, 1000
+    x, res, post, gate, pre = _sandwich_inputs(T, H, torch.bfloat16, 8, gate="each")
+    shared = gate[:1].expand(T, H)
+    _check_sandwich(x, res, post, shared, pre, aclnn.moe_sandwich_norm(*_on(dev, x, res, post), gate[:1].to(dev).expand(T, H), pre.to(dev), gate_type=1), 1)
+    ins = list(_grad_inputs(T, H, torch.bfloat16, 8, True, True, "each", False, 1))
+    ins[5] = shared
+    given = _on(dev, *ins)
+    given[5] = gate[:1].to(dev).expand(T, H)
+    _check_sandwich_grad(aclnn.moe_sandwich_norm_grad(*given, gate_type=1), *ins, 1, 1.0, 1.0)
 
 
 def test_sandwich_long_batches_and_empty_ones(aclnn, dev):
