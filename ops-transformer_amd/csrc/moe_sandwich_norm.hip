@@ -48,7 +48,7 @@ __device__ __forceinline__ float RowGate(const SandwichArgs& a, int64_t row) {
 
 // Rows in pieces of eight elements, up to kPackets of them a lane; a workgroup takes every gridDim.x-th row and asks for the next one before the
 // present one is begun (where the registers hold both, else before it is reduced the second time).  Gammas and a gate per channel stay in registers.
-constexpr int kMaxPacketThreads = 512;
+constexpr int kFewThreads = 512, kManyThreads = 768;
 constexpr int kMaxPackets = 4;
 constexpr int64_t kCus = 256, kWavesACu = 16;
 
@@ -58,10 +58,10 @@ struct NormRows {
     float rowGate = 1.f;
 };
 
-template <typename Codec, typename Gamma, int kPackets, int kGate, bool kTail>
-__global__ __launch_bounds__(kMaxPacketThreads) void SandwichPacketsKernel(SandwichArgs a) {
+template <typename Codec, typename Gamma, int kPackets, int kThreads, int kGate, bool kTail>
+__global__ __launch_bounds__(kThreads) void SandwichPacketsKernel(SandwichArgs a) {
     using Storage = typename Codec::Storage;
-    constexpr int kMaxWaves = kMaxPacketThreads / kWave;
+    constexpr int kMaxWaves = kThreads / kWave;
     constexpr bool kHeld = kGate == kHeldPackets, kRead = kGate == kReadPackets;
     constexpr bool kEarly = kPackets == 1 || (kPackets == 2 && sizeof(Storage) == 2);
     __shared__ float postSums[2][kMaxWaves][1];
@@ -313,22 +313,22 @@ class SandwichExecutor : public aclOpExecutor {
     aclDataType dtype = ACL_FLOAT;
     aclDataType weightType = ACL_FLOAT;
 
-    template <typename Codec, typename Gamma, int kPackets, int kGate>
+    template <typename Codec, typename Gamma, int kPackets, int kThreads, int kGate>
     void LaunchPackets(hipStream_t stream) const {
         const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
         const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
         const int64_t groups = std::min<int64_t>(args.rows, kCus * (kWavesACu * kWave / threads));
         const dim3 grid(static_cast<unsigned>(groups));
-        if (args.cols % 8 != 0) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kGate, true>), grid, dim3(threads), 0, stream, args);
-        else hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kGate, false>), grid, dim3(threads), 0, stream, args);
+        if (args.cols % 8 != 0) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, true>), grid, dim3(threads), 0, stream, args);
+        else hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, false>), grid, dim3(threads), 0, stream, args);
     }
 
-    template <typename Codec, typename Gamma, int kPackets>
+    template <typename Codec, typename Gamma, int kPackets, int kThreads>
     void ForGate(hipStream_t stream) const {
         const int packets = GatePackets(args.gateKind);
-        if (packets == kHeldPackets) LaunchPackets<Codec, Gamma, kPackets, kHeldPackets>(stream);
-        else if (packets == kReadPackets) LaunchPackets<Codec, Gamma, kPackets, kReadPackets>(stream);
-        else LaunchPackets<Codec, Gamma, kPackets, kNoPackets>(stream);
+        if (packets == kHeldPackets) LaunchPackets<Codec, Gamma, kPackets, kThreads, kHeldPackets>(stream);
+        else if (packets == kReadPackets) LaunchPackets<Codec, Gamma, kPackets, kThreads, kReadPackets>(stream);
+        else LaunchPackets<Codec, Gamma, kPackets, kThreads, kNoPackets>(stream);
     }
 
     aclnnStatus Run(void*, hipStream_t stream) override {
@@ -338,10 +338,17 @@ class SandwichExecutor : public aclOpExecutor {
             using Codec = decltype(codec);
             using Gamma = decltype(gamma);
             const int64_t lanes = (args.cols + 7) / 8;
-            if (args.cols < 8 || lanes > kMaxPackets * kMaxPacketThreads) hipLaunchKernelGGL((SandwichAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
-            else if (lanes <= kMaxPacketThreads) ForGate<Codec, Gamma, 1>(stream);
-            else if (lanes <= 2 * kMaxPacketThreads) ForGate<Codec, Gamma, 2>(stream);
-            else ForGate<Codec, Gamma, kMaxPackets>(stream);
+            if (args.cols < 8 || lanes > kMaxPackets * kFewThreads) {
+                hipLaunchKernelGGL((SandwichAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
+            } else if (lanes <= kFewThreads) {
+                ForGate<Codec, Gamma, 1, kFewThreads>(stream);
+            } else if (lanes <= 2 * kFewThreads) {
+                ForGate<Codec, Gamma, 2, kFewThreads>(stream);
+            } else if (lanes <= 2 * kManyThreads) {
+                ForGate<Codec, Gamma, 2, kManyThreads>(stream);
+            } else {
+                ForGate<Codec, Gamma, kMaxPackets, kFewThreads>(stream);
+            }
         });
         const hipError_t err = hipGetLastError();
         OPAPI_CHECK(err == hipSuccess, ACLNN_ERR_RUNTIME_ERROR, "aclnnMoeSandwichNorm: launch failed: %s", hipGetErrorString(err));

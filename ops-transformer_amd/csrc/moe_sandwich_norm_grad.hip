@@ -54,7 +54,7 @@ __device__ __forceinline__ float RawRowGate(const SandwichGradArgs& a, int64_t r
     return a.gateIsFloat ? static_cast<const float*>(a.gate)[row] : Codec::Load(static_cast<const typename Codec::Storage*>(a.gate)[row]);
 }
 
-constexpr int kMaxPacketThreads = 512;
+constexpr int kFewThreads = 512, kManyThreads = 768;
 
 // What is read of a row.
 template <typename Codec, int kPackets, bool kGate>
@@ -64,19 +64,19 @@ struct GradRows {
 };
 
 // kSumsInLds: the column sums of a workgroup, where its registers have no room for them beside the row.
-template <typename Codec, typename Gamma, int kPackets>
-constexpr bool kSumsInLds = kPackets == 4 || (kPackets == 2 && sizeof(typename Codec::Storage) + sizeof(typename Gamma::Storage) == 8);
+template <typename Codec, typename Gamma, int kPackets, int kThreads>
+constexpr bool kSumsInLds = kPackets == 4 || kThreads == kManyThreads || (kPackets == 2 && sizeof(typename Codec::Storage) + sizeof(typename Gamma::Storage) == 8);
 
-template <typename Codec, typename Gamma, int kPackets, int kGate, bool kPre, bool kTail>
-__global__ __launch_bounds__(kMaxPacketThreads) void SandwichGradKernel(SandwichGradArgs a) {
+template <typename Codec, typename Gamma, int kPackets, int kThreads, int kGate, bool kPre, bool kTail>
+__global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs a) {
     using Storage = typename Codec::Storage;
-    constexpr int kMaxWaves = kMaxPacketThreads / kWave;
+    constexpr int kMaxWaves = kThreads / kWave;
     constexpr bool kHeld = kGate == kHeldPackets, kRead = kGate == kReadPackets;
-    constexpr bool kLds = kSumsInLds<Codec, Gamma, kPackets>;
+    constexpr bool kLds = kSumsInLds<Codec, Gamma, kPackets, kThreads>;
     // Where the registers hold a second row, the next one is asked for before the present one is begun, else when its loads have found their last use.
     constexpr bool kEarly = kPackets == 1 || (kPackets == 2 && sizeof(Storage) == 2);
     // Weights stay in registers, packed, or are read again for every row, from the caches.
-    constexpr bool kHoldWeights = kPackets < 4;
+    constexpr bool kHoldWeights = kPackets < 4 && kThreads == kFewThreads;
     __shared__ float preSums[2][kMaxWaves][1];
     __shared__ float postSums[2][kMaxWaves][2];
     extern __shared__ float4 ldsSums[];  // kLds: [kColumnSums][kPackets][2][threads], each lane its own
@@ -454,9 +454,9 @@ __global__ __launch_bounds__(kFinishThreads) void SandwichGradFinishKernel(Sandw
 }
 
 // Rows of eight to 16384 values are one workgroup's at a time.
-constexpr int kMaxPackets = 4;
 constexpr int64_t kCus = 256;
-constexpr int64_t kPacketCols = 8ll * kMaxPacketThreads * kMaxPackets;
+constexpr int kMaxPackets = 4;
+constexpr int64_t kPacketCols = 8ll * kFewThreads * kMaxPackets;
 
 class SandwichGradExecutor : public aclOpExecutor {
    public:
@@ -483,10 +483,10 @@ class SandwichGradExecutor : public aclOpExecutor {
             bytes = opapi::AlignUp(4 * static_cast<uint64_t>(args.rows), 16);
         } else {
             const int64_t lanes = (args.cols + 7) / 8;
-            const int64_t packets = lanes <= kMaxPacketThreads ? 1 : lanes <= 2 * kMaxPacketThreads ? 2 : kMaxPackets;
+            const int64_t packets = lanes <= kFewThreads ? 1 : lanes <= 2 * kManyThreads ? 2 : kMaxPackets;
             threads = static_cast<int>(((lanes + packets - 1) / packets + kWave - 1) / kWave * kWave);
             const int64_t waves = threads / kWave;
-            args.groups = kCus * std::max<int64_t>(1, kMaxPacketThreads / kWave / waves);
+            args.groups = kCus * std::max<int64_t>(1, kFewThreads / kWave / waves);
             if (packets == 1 && waves > 4 && args.rows >= 8 * 2 * kCus) args.groups = 2 * kCus;
             if (args.groups < (args.rows + kColumnRows - 1) / kColumnRows) args.groups = (args.rows + kColumnRows - 1) / kColumnRows;
             if (args.groups > args.rows) args.groups = args.rows;
@@ -498,14 +498,14 @@ class SandwichGradExecutor : public aclOpExecutor {
         return bytes;
     }
 
-    template <typename Codec, typename Gamma, int kPackets, int kGate, bool kPre, bool kTail>
+    template <typename Codec, typename Gamma, int kPackets, int kThreads, int kGate, bool kPre, bool kTail>
     hipError_t LaunchKernel(hipStream_t stream) const {
-        const auto kernel = SandwichGradKernel<Codec, Gamma, kPackets, kGate, kPre, kTail>;
+        const auto kernel = SandwichGradKernel<Codec, Gamma, kPackets, kThreads, kGate, kPre, kTail>;
         int lds = 0;
-        if constexpr (kSumsInLds<Codec, Gamma, kPackets>) {
+        if constexpr (kSumsInLds<Codec, Gamma, kPackets, kThreads>) {
             static std::atomic<uint64_t> done{0};
-            constexpr int kMost = kColumnSums * kPackets * 2 * kMaxPacketThreads * static_cast<int>(sizeof(float4));
-            lds = kMost / kMaxPacketThreads * threads;
+            constexpr int kMost = kColumnSums * kPackets * 2 * kThreads * static_cast<int>(sizeof(float4));
+            lds = kMost / kThreads * threads;
             const hipError_t e = opapi::EnsureDynamicLds(reinterpret_cast<const void*>(kernel), kMost, done);
             if (e != hipSuccess) return e;
         }
@@ -513,21 +513,21 @@ class SandwichGradExecutor : public aclOpExecutor {
         return hipSuccess;
     }
 
-    template <typename Codec, typename Gamma, int kPackets, int kGate>
+    template <typename Codec, typename Gamma, int kPackets, int kThreads, int kGate>
     hipError_t LaunchPackets(hipStream_t stream) const {
         const bool tail = args.cols % 8 != 0;
         if (args.pre != nullptr) {
-            return tail ? LaunchKernel<Codec, Gamma, kPackets, kGate, true, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kGate, true, false>(stream);
+            return tail ? LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, true, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, true, false>(stream);
         }
-        return tail ? LaunchKernel<Codec, Gamma, kPackets, kGate, false, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kGate, false, false>(stream);
+        return tail ? LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, false, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, false, false>(stream);
     }
 
-    template <typename Codec, typename Gamma, int kPackets>
+    template <typename Codec, typename Gamma, int kPackets, int kThreads>
     hipError_t ForGate(hipStream_t stream) const {
         const int packets = GatePackets(args.gateKind);
-        if (packets == kHeldPackets) return LaunchPackets<Codec, Gamma, kPackets, kHeldPackets>(stream);
-        if (packets == kReadPackets) return LaunchPackets<Codec, Gamma, kPackets, kReadPackets>(stream);
-        return LaunchPackets<Codec, Gamma, kPackets, kNoPackets>(stream);
+        if (packets == kHeldPackets) return LaunchPackets<Codec, Gamma, kPackets, kThreads, kHeldPackets>(stream);
+        if (packets == kReadPackets) return LaunchPackets<Codec, Gamma, kPackets, kThreads, kReadPackets>(stream);
+        return LaunchPackets<Codec, Gamma, kPackets, kThreads, kNoPackets>(stream);
     }
 
     aclnnStatus Run(void* workspace, hipStream_t stream) override {
@@ -551,12 +551,14 @@ class SandwichGradExecutor : public aclOpExecutor {
                     hipLaunchKernelGGL((SandwichGradRowsKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
                     const int64_t blocks = (args.cols + kAnyThreads - 1) / kAnyThreads;
                     if (Columns()) hipLaunchKernelGGL((SandwichGradColumnsKernel<Codec, Gamma>), GridOf(blocks * args.groups), dim3(kAnyThreads), 0, stream, args);
-                } else if (lanes <= kMaxPacketThreads) {
-                    err = ForGate<Codec, Gamma, 1>(stream);
-                } else if (lanes <= 2 * kMaxPacketThreads) {
-                    err = ForGate<Codec, Gamma, 2>(stream);
+                } else if (lanes <= kFewThreads) {
+                    err = ForGate<Codec, Gamma, 1, kFewThreads>(stream);
+                } else if (lanes <= 2 * kFewThreads) {
+                    err = ForGate<Codec, Gamma, 2, kFewThreads>(stream);
+                } else if (lanes <= 2 * kManyThreads) {
+                    err = ForGate<Codec, Gamma, 2, kManyThreads>(stream);
                 } else {
-                    err = ForGate<Codec, Gamma, kMaxPackets>(stream);
+                    err = ForGate<Codec, Gamma, kMaxPackets, kFewThreads>(stream);
                 }
             }
             if (Columns()) {
