@@ -40,9 +40,9 @@ constexpr int kChunkWaves = kChunkThreads / kWave;
 // A lane's rows in flight: their loads and reductions overlap.
 constexpr int UnrollOf(int pieces) { return pieces <= 2 ? 2 : 1; }
 // Chunks: as many as there are CUs, of at least the rows that a workgroup has in flight at once, and of at most so many that a lane's fp32 sums stay short.
-constexpr int64_t kMostChunks = 256, kMaxChunkRows = 4096;
+constexpr int64_t kMostChunks = 256, kMinChunkRows = 128, kMaxChunkRows = 4096;
 // One sequence of up to so many such passes is one workgroup's: it spares the second launch.
-constexpr int64_t kAlonePasses = 8;
+constexpr int64_t kAlonePasses = 6;
 // A workgroup of the second kernel takes few experts in many runs of pieces, or, where a sequence has few pieces, many in few.
 constexpr int kFinishThreads = 1024;
 constexpr int kFinishFew = 64, kFinishMany = 256;
@@ -440,7 +440,7 @@ extern "C" aclnnStatus aclnnMoeBalanceLossGetWorkspaceSize(const aclTensor* x, c
     ForRowLayout(experts, [&](auto lanes, auto pieces) { passRows = kChunkWaves * (kWave / decltype(lanes)::value) * UnrollOf(decltype(pieces)::value); });
     a.alone = sequences == 1 && rows <= kAlonePasses * passRows;
     int64_t chunkRows = (rows + kMostChunks - 1) / kMostChunks;
-    if (chunkRows < 2 * passRows) chunkRows = 2 * passRows;
+    chunkRows = std::max(chunkRows, std::min<int64_t>(2 * passRows, kMinChunkRows));
     if (chunkRows > kMaxChunkRows) chunkRows = kMaxChunkRows;
     a.chunkRows = static_cast<int32_t>(chunkRows);
     a.chunks = a.alone ? 1 : static_cast<int32_t>((rows + chunkRows - 1) / chunkRows);

@@ -247,7 +247,7 @@ class GatingGradExecutor : public aclOpExecutor {
         ForRowLayout(args.experts, [&](auto lanes, auto pieces) {
             constexpr int kLanes = decltype(lanes)::value, kPieces = decltype(pieces)::value;
             constexpr int64_t kRowsAtOnce = kWave / kLanes;
-            const int64_t waves = 8 * 1024;  // two rounds of the chip's 256 x 4 SIMDs, four waves each
+            const int64_t waves = 4 * 1024;
             int64_t each = (args.sequences.rows + waves - 1) / waves;
             each = (each + kRowsAtOnce - 1) / kRowsAtOnce * kRowsAtOnce;
             if (each > 64 * kRowsAtOnce) each = 64 * kRowsAtOnce;

@@ -50,7 +50,7 @@ __device__ __forceinline__ float RowGate(const SandwichArgs& a, int64_t row) {
 // present one is begun (where the registers hold both, else before it is reduced the second time).  Gammas and a gate per channel stay in registers.
 constexpr int kFewThreads = 512, kManyThreads = 768;
 constexpr int kMaxPackets = 4;
-constexpr int64_t kCus = 256, kWavesACu = 16;
+constexpr int64_t kCus = 256;
 
 template <typename Codec, int kPackets, bool kGate>
 struct NormRows {
@@ -317,9 +317,11 @@ class SandwichExecutor : public aclOpExecutor {
     void LaunchPackets(hipStream_t stream) const {
         const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
         const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
-        const int64_t groups = std::min<int64_t>(args.rows, kCus * (kWavesACu * kWave / threads));
+        const bool tail = args.cols % 8 != 0;
+        const int64_t each = kPackets == 1 ? 16 * kWave / threads : tail && kThreads == kFewThreads ? 2 : std::max(1, 12 * kWave / threads);
+        const int64_t groups = std::min<int64_t>(args.rows, kCus * each);
         const dim3 grid(static_cast<unsigned>(groups));
-        if (args.cols % 8 != 0) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, true>), grid, dim3(threads), 0, stream, args);
+        if (tail) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, true>), grid, dim3(threads), 0, stream, args);
         else hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, false>), grid, dim3(threads), 0, stream, args);
     }
 
