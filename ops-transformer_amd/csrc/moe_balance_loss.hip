@@ -4,6 +4,10 @@
 // chunk or to the next sequence: the piece that chunk c has of sequence s is number c + s, and of s there are pieces from its first chunk to its
 // last.  So the pieces' sums lie in a table of chunks + sequences entries without a count or an offset made beforehand, and a second kernel adds up those
 // of each sequence in their order.  One chunk and one sequence: the first kernel finishes by itself.
+//
+// What bounds it: round trips and launches, not bytes.  16384 x 256 fp32 rows (17 MB, 3.3 us at a copy's 5.2 TB/s) take 12.6 us, 7.3 of them this kernel's
+// (a pass of 32 rows per workgroup is a load, a row's sum across the lanes, a reciprocal) and 5 the second one's, which waits for sums that other XCDs
+// wrote.  Its work in the first kernel's last workgroup would need counters that somebody has set to zero before, a launch again.
 #include "router_rows.h"
 
 #include "aclnnop/aclnn_moe_balance_loss.h"
@@ -37,13 +41,17 @@ struct BalanceArgs {
 
 constexpr int kChunkThreads = 512;
 constexpr int kChunkWaves = kChunkThreads / kWave;
-// A lane's rows in flight: their loads and reductions overlap.
+// A lane's rows in flight: their loads and reductions overlap (4096 x 256 in four sequences 11.1 us, with one row 12.6; rows of more than 512 experts have no
+// registers for two: 2048 x 2048 17.6 us, with two 19.9).
 constexpr int UnrollOf(int pieces) { return pieces <= 2 ? 2 : 1; }
-// Chunks: as many as there are CUs, of at least the rows that a workgroup has in flight at once, and of at most so many that a lane's fp32 sums stay short.
+// Chunks: as many as there are CUs (16384 x 256 12.6 us; with 128 14.9, with 512 15.6), of at least two passes, whose loads overlap, or kMinChunkRows where a
+// pass holds many narrow rows (16384 x 8 in eight sequences 10.1 us; of two passes, 1024 rows, 13.5), and of at most so many that a lane's fp32 sums stay short.
 constexpr int64_t kMostChunks = 256, kMinChunkRows = 128, kMaxChunkRows = 4096;
-// One sequence of up to so many such passes is one workgroup's: it spares the second launch.
+// One sequence of up to so many passes is one workgroup's: it spares the second launch (96 x 256, six passes: 7.0 us, in two launches 8.1; eight passes of
+// 128 rows 8.5 and 8.1, of 4096 rows of eight experts 14.7 and 9.5).
 constexpr int64_t kAlonePasses = 6;
-// A workgroup of the second kernel takes few experts in many runs of pieces, or, where a sequence has few pieces, many in few.
+// A workgroup of the second kernel takes few experts in many runs of pieces, or, where a sequence has few pieces, many in few: 16384 x 256 in one sequence
+// (256 pieces) 12.6 us with few and 16.6 with many, in 64 sequences (five pieces) 19.0 and 14.9.  Fewer than 64 leave more parts of the loss to join (32: 13.5).
 constexpr int kFinishThreads = 1024;
 constexpr int kFinishFew = 64, kFinishMany = 256;
 constexpr int64_t kFewPieces = 64;

@@ -4,6 +4,10 @@
 // the picked ones, q_j = p_j / t and M = sum dy_j q_j, the renormalised weights have p_j dp_j = F q_j (dy_j - M), and the mean of dp under the softmax is
 // F M (1 - sum p / t) = F M eps / t: formed so, it is not the difference of two sums that cancel.  The picks' p dp goes through LDS from the lane that has
 // the pick to the one that has the expert.
+//
+// What bounds it: few rows, a launch and two round trips (256 x 8: 4.2 us, most of it the host's); many, vector instructions (16384 x 256 fp32: 10.4 us,
+// 60 % of the SIMDs' issue, where the bytes, 34.6 MB, take 6.7 at a copy's rate): a score is six instructions, its gradient ten, and four sums
+// cross the lanes.
 #include "router_rows.h"
 
 #include "aclnnop/aclnn_moe_gating_top_k_grouped_grad.h"
@@ -42,8 +46,8 @@ struct RowInputs {
     float y;
 };
 
-// What bounds it: the chain of a row's steps, and its arithmetic.  Scores are held unnormalised, so that their sum, that of the picked ones and both
-// means are reduced side by side.
+// A row has the fewest lanes that hold it, four experts each, as the balance's kernel has it, and a wave's rows follow each other, the next asked for before the
+// present one is done.  Scores are held unnormalised, so that their sum, that of the picked ones and both means are reduced side by side.
 template <typename Codec, typename Out, int kLanes, int kPieces, bool kSigmoid>
 __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
     using Row = RowOf<kLanes, kPieces>;
@@ -247,6 +251,7 @@ class GatingGradExecutor : public aclOpExecutor {
         ForRowLayout(args.experts, [&](auto lanes, auto pieces) {
             constexpr int kLanes = decltype(lanes)::value, kPieces = decltype(pieces)::value;
             constexpr int64_t kRowsAtOnce = kWave / kLanes;
+            // As many waves as the registers let the 256 x 4 SIMDs hold at once: 16384 x 256 10.4 us, half as many 12.9, twice 10.9, four times 12.3.
             const int64_t waves = 4 * 1024;
             int64_t each = (args.sequences.rows + waves - 1) / waves;
             each = (each + kRowsAtOnce - 1) / kRowsAtOnce * kRowsAtOnce;

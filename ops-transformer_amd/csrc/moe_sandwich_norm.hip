@@ -1,7 +1,9 @@
 // aclnnMoeSandwichNorm for gfx950: s = a residual + b gate * (rms_norm(x) * postGamma), n = rms_norm(s) * preGamma, int8 rows of n * smooth.
 //
 // Two reductions over a row, the second on what the first one settles: the row stays in registers from its load to its last output, so it crosses the
-// memory once.  Sums, factors, u, v and n are fp32; what is rounded is s (to the stream's type, and that rounded value is what is normalised), n where it
+// memory once, and the memory bounds it: 8192 x 7168 bf16 with a gate per channel (470 MB) 87.9 us, 5.35 TB/s, part of them from the memory-side cache;
+// 4096 x 12000 77.5 (393 MB, 5.1 TB/s); 64 x 4096 a launch, 5.0.  Rows of 16 bits off the four-byte grid take 1.4 times as long (4096 x 7167 63, where their
+// bytes take 45): their loads and stores of eight elements straddle words.  Sums, factors, u, v and n are fp32; what is rounded is s (to the stream's type, and that rounded value is what is normalised), n where it
 // leaves, and y, which is made as aclnnMoeAddRmsNormQuant makes it (norm_rows.h).
 #include "sandwich_norm.h"
 
@@ -48,6 +50,8 @@ __device__ __forceinline__ float RowGate(const SandwichArgs& a, int64_t row) {
 
 // Rows in pieces of eight elements, up to kPackets of them a lane; a workgroup takes every gridDim.x-th row and asks for the next one before the
 // present one is begun (where the registers hold both, else before it is reduced the second time).  Gammas and a gate per channel stay in registers.
+// Up to 4096 values a lane has one piece, up to 12288 two on up to 768 lanes, up to 16384 four on 512: four of 9000 columns' take 71.5 us at 4096 rows
+// where two take 60.9, and more than 768 lanes have no registers for two.
 constexpr int kFewThreads = 512, kManyThreads = 768;
 constexpr int kMaxPackets = 4;
 constexpr int64_t kCus = 256;
@@ -318,6 +322,8 @@ class SandwichExecutor : public aclOpExecutor {
         const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
         const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
         const bool tail = args.cols % 8 != 0;
+        // Workgroups a CU.  One piece: 16 waves (8192 x 4096 38.4 us; 12 waves, which is one workgroup, 42.6; 32 41).  Two: 12 (8192 x 7168 87.9, with two workgroups
+        // 93.1; 8192 x 4608 59.9 with two, 67.7 with three), and two workgroups where the tail's instructions want company (4096 x 7167 63.0, with one 82).
         const int64_t each = kPackets == 1 ? 16 * kWave / threads : tail && kThreads == kFewThreads ? 2 : std::max(1, 12 * kWave / threads);
         const int64_t groups = std::min<int64_t>(args.rows, kCus * each);
         const dim3 grid(static_cast<unsigned>(groups));

@@ -1,7 +1,8 @@
 // aclnnMoeSandwichNormGrad for gfx950: from the gradients of the sum and of its norm to those of the block's output, the residual, both gammas and the gate.
 //
 // With x^ = x postRstd and s^ = s preRstd a row needs one sum behind the other, sum(dn preGamma s^) for dS and sum(du postGamma x^) for xGrad: it stays in
-// registers from its loads to its stores.  A workgroup takes every gridDim.x-th row and adds up what its lanes' columns owe the gammas and a gate per
+// registers from its loads to its stores, and the memory bounds it: 8192 x 7168 bf16 with both norms (705 MB) 137 us, 5.15 TB/s; 4096 x 12000 138 (590 MB);
+// rows of 16 bits off the four-byte grid 1.45 times their bytes' time (4096 x 7167 100 us).  Few rows: two launches (64 x 7168 9.5 us).  A workgroup takes every gridDim.x-th row and adds up what its lanes' columns owe the gammas and a gate per
 // channel in registers; a second kernel adds up the workgroups.
 #include "sandwich_norm.h"
 
@@ -63,7 +64,8 @@ struct GradRows {
     float postRstd = 1.f, preRstd = 0.f, rawGate = 0.f;
 };
 
-// kSumsInLds: the column sums of a workgroup, where its registers have no room for them beside the row.
+// kSumsInLds: the column sums of a workgroup, where its registers have no room for them beside the row (each lane adds to its own 16 bytes, no conflicts:
+// with them in registers 4096 x 12000 rows went to scratch memory and took 912 us).
 template <typename Codec, typename Gamma, int kPackets, int kThreads>
 constexpr bool kSumsInLds = kPackets == 4 || kThreads == kManyThreads || (kPackets == 2 && sizeof(typename Codec::Storage) + sizeof(typename Gamma::Storage) == 8);
 
@@ -453,7 +455,9 @@ __global__ __launch_bounds__(kFinishThreads) void SandwichGradFinishKernel(Sandw
     if (a.channelGrad != nullptr) a.channelGrad[c] = static_cast<float>(sum * GateSlope(gate, a.sigmoid) * (a.post != nullptr ? weight(a.post) : 1.f));
 }
 
-// Rows of eight to 16384 values are one workgroup's at a time.
+// Rows of eight to 16384 values are one workgroup's at a time: one piece a lane up to 4096 values, two on up to 512 lanes, two on up to 768, whose 168 registers
+// hold them with the sums in LDS (4096 x 12000 bf16 138 us, 2048 x 12000 fp32 139; four pieces on 384 lanes 157 and 238; two on 1024, with 128 registers, 202
+// and 211), and four above 12288 values (3000 x 16384 156 us; an element at a time 755).
 constexpr int64_t kCus = 256;
 constexpr int kMaxPackets = 4;
 constexpr int64_t kPacketCols = 8ll * kFewThreads * kMaxPackets;
@@ -487,6 +491,9 @@ class SandwichGradExecutor : public aclOpExecutor {
             threads = static_cast<int>(((lanes + packets - 1) / packets + kWave - 1) / kWave * kWave);
             const int64_t waves = threads / kWave;
             args.groups = kCus * std::max<int64_t>(1, kFewThreads / kWave / waves);
+            // Above, a CU's workgroups have eight waves together; twelve or more (twice the workgroups) cost more in column sums than they hide: 8192 x 7168
+            // 152 us instead of 137, 16384 x 1024 53 instead of 47, and half as many there 109.  Workgroups of five to eight waves with one piece a lane and many rows
+            // have registers for two a CU: 8192 x 4096 55.8 us, with one 63.6; 2880 columns with a gate each 151 and 196.
             if (packets == 1 && waves > 4 && args.rows >= 8 * 2 * kCus) args.groups = 2 * kCus;
             if (args.groups < (args.rows + kColumnRows - 1) / kColumnRows) args.groups = (args.rows + kColumnRows - 1) / kColumnRows;
             if (args.groups > args.rows) args.groups = args.rows;

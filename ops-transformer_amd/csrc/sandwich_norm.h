@@ -67,7 +67,7 @@ __device__ __forceinline__ void HoldPacked(Packet<Codec>& piece) {
 // Where a lane's pieces of eight elements lie in a row of `cols`, at least eight.  Every lane has each of its pieces: one that would end behind the row is the
 // row's last eight elements, the first `skip` of which are other lanes' (all eight of a piece that would begin behind it; kTail: cols is no multiple of eight,
 // else there are no others).  So loads are without a branch, the compiler knows how many there are, and a wait for one row's need not be one for the
-// next row's: with branches 8192 x 7168 rows waited for all of them.
+// next row's: with branches 8192 x 7168 rows waited for all of them (105 us instead of 93 with two workgroups a CU).
 template <int kPackets, bool kTail>
 struct Pieces {
     uint32_t from[kPackets];
