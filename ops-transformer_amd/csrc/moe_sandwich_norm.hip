@@ -322,9 +322,11 @@ class SandwichExecutor : public aclOpExecutor {
         const int64_t lanes = ((args.cols + 7) / 8 + kPackets - 1) / kPackets;
         const int threads = static_cast<int>((lanes + kWave - 1) / kWave * kWave);
         const bool tail = args.cols % 8 != 0;
-        // Workgroups a CU.  One piece: 16 waves (8192 x 4096 38.4 us; 12 waves, which is one workgroup, 42.6; 32 41).  Two: 12 (8192 x 7168 87.9, with two workgroups
-        // 93.1; 8192 x 4608 59.9 with two, 67.7 with three), and two workgroups where the tail's instructions want company (4096 x 7167 63.0, with one 82).
-        const int64_t each = kPackets == 1 ? 16 * kWave / threads : tail && kThreads == kFewThreads ? 2 : std::max(1, 12 * kWave / threads);
+        // Workgroups a CU.  One piece: 16 waves, and three workgroups of five or six (8192 x 2880 38.5 us, with two of six 42.9, with four 39.3; with a gate a row
+        // 42.7, 53.4 and 42.4; 8192 x 4096 38.4 with two, with one 42.6, with four 41; 8192 x 1024 13.2 with eight, with ten 14.3).  Two: 12 waves (8192 x 7168
+        // 87.9 with one workgroup, with two 93.1; 8192 x 4608 59.9 with two, with three 67.7), and two workgroups where the tail's instructions want company
+        // (4096 x 7167 63.0, with one 82).
+        const int64_t each = kPackets == 1 ? (threads > 4 * kWave ? 18 : 16) * kWave / threads : tail && kThreads == kFewThreads ? 2 : std::max(1, 12 * kWave / threads);
         const int64_t groups = std::min<int64_t>(args.rows, kCus * each);
         const dim3 grid(static_cast<unsigned>(groups));
         if (tail) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, true>), grid, dim3(threads), 0, stream, args);
