@@ -2,8 +2,10 @@
 //
 // With x^ = x postRstd and s^ = s preRstd a row needs one sum behind the other, sum(dn preGamma s^) for dS and sum(du postGamma x^) for xGrad: it stays in
 // registers from its loads to its stores, and the memory bounds it: 8192 x 7168 bf16 with both norms (705 MB) 137 us, 5.15 TB/s; 4096 x 12000 138 (590 MB);
-// rows of 16 bits off the four-byte grid 1.45 times their bytes' time (4096 x 7167 100 us).  Few rows: two launches (64 x 7168 9.5 us).  A workgroup takes every gridDim.x-th row and adds up what its lanes' columns owe the gammas and a gate per
-// channel in registers; a second kernel adds up the workgroups.
+// rows of 16 bits off the four-byte grid 1.45 times their bytes' time (4096 x 7167 100 us).  Few rows: two launches (64 x 4096 9.7 us).
+//
+// A workgroup takes every gridDim.x-th row, or several short ones at once, and adds up what its lanes' columns owe the gammas and a gate per channel in
+// registers; a second kernel adds up the workgroups.
 #include "sandwich_norm.h"
 
 #include "aclnnop/aclnn_moe_sandwich_norm_grad.h"
@@ -37,6 +39,7 @@ struct SandwichGradArgs {
     int64_t rows;
     int64_t cols;
     int64_t groups;          // that columns are summed over
+    int32_t rowThreads;      // of a workgroup, which takes as many rows at once as it has times these
     int32_t gateKind;
     int32_t sigmoid;
     int32_t gateIsFloat;
@@ -82,7 +85,10 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
     __shared__ float preSums[2][kMaxWaves][1];
     __shared__ float postSums[2][kMaxWaves][2];
     extern __shared__ float4 ldsSums[];  // kLds: [kColumnSums][kPackets][2][threads], each lane its own
-    const int threads = blockDim.x, waves = threads / kWave, tid = threadIdx.x;
+    // One piece a lane: rows of few waves lie side by side in a workgroup.
+    const int threads = kPackets == 1 ? a.rowThreads : blockDim.x, waves = threads / kWave;
+    const int side = kPackets == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / threads) : 0, sides = kPackets == 1 ? blockDim.x / threads : 1;
+    const int tid = threadIdx.x - side * threads;
     const int cols = static_cast<int>(a.cols);
     const float each = 1.f / static_cast<float>(a.cols);
     const bool post = a.post != nullptr, gated = a.gateKind != kGateNone, rowGated = a.gateKind == kGateRow;
@@ -95,7 +101,7 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
         else return at.template Load<Gamma>(w, 0, p);
     };
     float sumHeld[kLds ? 1 : kColumnSums][kLds ? 1 : kPackets][8];
-    auto addToColumns = [&](int which, int p, const float (&v)[8]) {
+    auto addToColumns = [&](int which, int p, const float (&v)[8], bool counts) {
         if constexpr (kLds) {
             float4* const to = ldsSums + ((which * kPackets + p) * 2) * threads + tid;
 #pragma unroll
@@ -107,7 +113,7 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
                 t.w += v[4 * h + 3];
                 to[h * threads] = t;
             }
-        } else {
+        } else if (counts) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sumHeld[which][p][i] += v[i];
         }
@@ -149,11 +155,14 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
         if constexpr (kPre) to.preRstd = a.preRstd[row];
         if (kGate == kNoPackets && rowGated) to.rawGate = RawRowGate<Codec>(a, row);
     };
-    int64_t row = blockIdx.x;
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * sides;
+    int64_t base = static_cast<int64_t>(blockIdx.x) * sides;  // the first of the rows side by side: it goes on for all or for none
     // One row; `following` takes the next one where it is asked for early, else `in` does.
     auto step = [&](GradRows<Codec, kPackets, kRead>& in, GradRows<Codec, kPackets, kRead>& following, int parity) __attribute__((always_inline)) {
-        const int64_t begin = row * cols, next = row + gridDim.x;
-        if constexpr (kEarly) load(following, min(next, a.rows - 1));
+        // Behind the last row: that one once more, which counts in no column.
+        const int64_t row = min(base + side, a.rows - 1), begin = row * cols, next = min(base + side + stride, a.rows - 1);
+        const bool counts = kPackets > 1 || base + side < a.rows;
+        if constexpr (kEarly) load(following, next);
         if constexpr (kHoldWeights) {
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
@@ -180,10 +189,10 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
                     part = fmaf(at.Own(terms[i], p, i), g[i], part);
                     d[p][i] *= g[i];
                 }
-                addToColumns(kPreSums, p, terms);
+                addToColumns(kPreSums, p, terms, counts);
                 preMean[0] += at.Counted(part, p);
             }
-            SumsOverGroup<1, kMaxWaves>(preMean, waves, parity, preSums);
+            SumsOverGroup<1, kMaxWaves>(preMean, waves, parity, preSums, side * waves);
             preMean[0] *= each;
 #pragma unroll
             for (int p = 0; p < kPackets; ++p) {
@@ -249,7 +258,7 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
                 parts[0] = fmaf(at.Own(v, p, i), normed, parts[0]);
                 d[p][i] = v;
             }
-            if (branchSums) addToColumns(kBranchSums, p, terms);
+            if (branchSums) addToColumns(kBranchSums, p, terms, counts);
             rowSums[0] += at.Counted(parts[0], p);
             rowSums[1] += at.Counted(parts[1], p);
             if constexpr (kRead) {
@@ -261,9 +270,9 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
         for (int p = 0; p < kPackets; ++p) x[p] = in.x[p];
         if constexpr (!kEarly) {
             __builtin_amdgcn_sched_barrier(0);  // not in front of the last uses
-            load(in, min(next, a.rows - 1));
+            load(in, next);
         }
-        if (post || rowGated) SumsOverGroup<2, kMaxWaves>(rowSums, waves, parity, postSums);
+        if (post || rowGated) SumsOverGroup<2, kMaxWaves>(rowSums, waves, parity, postSums, side * waves);
         if (rowGated && a.gateGrad != nullptr && tid == 0) static_cast<float*>(a.gateGrad)[row] = rowSums[1] * GateSlope(raw, a.sigmoid);
         if (a.xGrad != nullptr) {
             const float mean = rowSums[0] * each;
@@ -278,27 +287,48 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
                 at.template Store<Storage>(a.xGrad, begin, p, Pack<Codec>(d[p]));
             }
         }
-        row = next;
+        base += stride;
     };
     GradRows<Codec, kPackets, kRead> first;
-    load(first, row);
+    load(first, min(base + side, a.rows - 1));
     if constexpr (kPackets == 1) {
         // The two rows take turns where they lie: moved, a row's loads would have to have ended, and the stores behind them.
         GradRows<Codec, kPackets, kRead> second;
         while (true) {
             step(first, second, 0);
-            if (row >= a.rows) break;
+            if (base >= a.rows) break;
             step(second, first, 1);
-            if (row >= a.rows) break;
+            if (base >= a.rows) break;
         }
     } else if constexpr (kEarly) {
         GradRows<Codec, kPackets, kRead> second;
-        for (int parity = 0; row < a.rows; parity ^= 1) {
+        for (int parity = 0; base < a.rows; parity ^= 1) {
             step(first, second, parity);
             first = second;
         }
     } else {
-        for (int parity = 0; row < a.rows; parity ^= 1) step(first, first, parity);
+        for (int parity = 0; base < a.rows; parity ^= 1) step(first, first, parity);
+    }
+    if (kPackets == 1 && sides > 1) {  // the sums of the rows side by side, to the first of them
+        static_assert(kPackets > 1 || kLds || kColumnSums * kPackets * 8 == 16, "four pieces of four");
+        float4* const to = ldsSums + threadIdx.x;
+        if constexpr (!kLds) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) to[q * blockDim.x] = *reinterpret_cast<const float4*>(&sumHeld[q / 2][0][q % 2 * 4]);
+            __syncthreads();
+            if (side > 0) return;
+            for (int s = 1; s < sides; ++s) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const float4 more = to[q * blockDim.x + s * threads];
+                    float* const sum = &sumHeld[q / 2][0][q % 2 * 4];
+                    sum[0] += more.x;
+                    sum[1] += more.y;
+                    sum[2] += more.z;
+                    sum[3] += more.w;
+                }
+            }
+        }
     }
     const int64_t mine = static_cast<int64_t>(blockIdx.x) * cols;
 #pragma unroll
@@ -468,7 +498,7 @@ class SandwichGradExecutor : public aclOpExecutor {
     aclDataType dtype = ACL_FLOAT;
     aclDataType weightType = ACL_FLOAT;
     uint64_t offMeans = 0, offSums = 0;
-    int threads = 0;
+    int threads = 0, sides = 1;  // of a row; rows side by side in a workgroup
 
     // Which column sums are wanted.
     bool Wants(int which) const { return which == kPreSums ? args.preGammaGrad != nullptr : args.postGammaGrad != nullptr || args.channelGrad != nullptr; }
@@ -490,13 +520,18 @@ class SandwichGradExecutor : public aclOpExecutor {
             const int64_t packets = lanes <= kFewThreads ? 1 : lanes <= 2 * kManyThreads ? 2 : kMaxPackets;
             threads = static_cast<int>(((lanes + packets - 1) / packets + kWave - 1) / kWave * kWave);
             const int64_t waves = threads / kWave;
-            args.groups = kCus * std::max<int64_t>(1, kFewThreads / kWave / waves);
+            // Rows of one or two waves lie side by side in a workgroup of eight, whose column sums are joined before they leave it (8192 x 512 15.5 us, a
+            // workgroup each 20.5; 16384 x 1024 45.4 and 47.8); of four they would wait for each other (16384 x 2048 83.8 and 81.9).
+            sides = packets == 1 && waves <= 2 ? kFewThreads / kWave / waves : 1;
+            args.rowThreads = threads;
+            args.groups = kCus * std::max<int64_t>(1, kFewThreads / kWave / (waves * sides));
             // Above, a CU's workgroups have eight waves together; twelve or more (twice the workgroups) cost more in column sums than they hide: 8192 x 7168
-            // 152 us instead of 137, 16384 x 1024 53 instead of 47, and half as many there 109.  Workgroups of five to eight waves with one piece a lane and many rows
+            // 152 us instead of 137, 4096 x 4608 65 instead of 60.  Workgroups of five to eight waves with one piece a lane and many rows
             // have registers for two a CU: 8192 x 4096 55.8 us, with one 63.6; 2880 columns with a gate each 151 and 196.
             if (packets == 1 && waves > 4 && args.rows >= 8 * 2 * kCus) args.groups = 2 * kCus;
+            const int64_t rows = (args.rows + sides - 1) / sides;  // one behind the other
             if (args.groups < (args.rows + kColumnRows - 1) / kColumnRows) args.groups = (args.rows + kColumnRows - 1) / kColumnRows;
-            if (args.groups > args.rows) args.groups = args.rows;
+            if (args.groups > rows) args.groups = rows;
         }
         offSums = bytes;
         for (int i = 0; i < kColumnSums; ++i) {
@@ -516,7 +551,9 @@ class SandwichGradExecutor : public aclOpExecutor {
             const hipError_t e = opapi::EnsureDynamicLds(reinterpret_cast<const void*>(kernel), kMost, done);
             if (e != hipSuccess) return e;
         }
-        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(args.groups)), dim3(static_cast<unsigned>(threads)), static_cast<unsigned>(lds), stream, args);
+        if (sides > 1) lds = sides * threads * kColumnSums * 8 * static_cast<int>(sizeof(float));
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(args.groups)), dim3(static_cast<unsigned>(sides * threads)), static_cast<unsigned>(lds), stream,
+                           args);
         return hipSuccess;
     }
 

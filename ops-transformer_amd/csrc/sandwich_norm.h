@@ -36,9 +36,10 @@ __device__ __forceinline__ void OpenGates(float (&gate)[8], float (&slope)[8], i
     }
 }
 
-// kCount sums over a workgroup, the same bits in every lane.  `parity` alternates between calls that follow each other: one barrier a call.
+// kCount sums over a workgroup, or `waves` of it from `first` on, the same bits in every lane.  `parity` alternates between calls that follow each other: one
+// barrier a call.
 template <int kCount, int kMaxWaves>
-__device__ __forceinline__ void SumsOverGroup(float (&v)[kCount], int waves, int parity, float (&lds)[2][kMaxWaves][kCount]) {
+__device__ __forceinline__ void SumsOverGroup(float (&v)[kCount], int waves, int parity, float (&lds)[2][kMaxWaves][kCount], int first = 0) {
 #pragma unroll
     for (int i = 0; i < kCount; ++i) v[i] = SumOver<kWave>(v[i]);
     if (waves == 1) return;
@@ -48,10 +49,10 @@ __device__ __forceinline__ void SumsOverGroup(float (&v)[kCount], int waves, int
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) v[i] = lds[parity][0][i];
+    for (int i = 0; i < kCount; ++i) v[i] = lds[parity][first][i];
     for (int w = 1; w < waves; ++w) {
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) v[i] += lds[parity][w][i];
+        for (int i = 0; i < kCount; ++i) v[i] += lds[parity][first + w][i];
     }
 }
 
