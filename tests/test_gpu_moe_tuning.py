@@ -546,6 +546,43 @@ def test_sandwich_in_place_beside_sums_near_the_top(aclnn, dev):
         _check_sandwich(x, res, None, None, pre, aclnn.moe_sandwich_norm(x_dev, res_dev, pre_gamma=pre_dev, out=out))
 
 
+# More rows than workgroups, so that workgroups go on to a second row and some to a third: one piece a lane (1280, 2048 and 768 workgroups), two on up to 512 lanes
+# (512, 256), two on up to 768 and four (256; 512 off the eight).
+LOOPS = [(2600, 1031), (4200, 1000), (1600, 2880), (1100, 5000), (1100, 7167), (600, 8192), (600, 8200), (600, 9001), (600, 12000), (600, 12304), (1100, 16381),
+         (600, 16384)]
+
+
+@pytest.mark.parametrize("dtype_name", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("T,H", LOOPS)
+def test_sandwich_more_rows_than_workgroups(aclnn, dev, T, H, dtype_name):
+    """The same bits as in calls that give every row a workgroup of its own, the sum apart and in the place of either input; the last rows against the formula."""
+    dtype = TORCH[dtype_name]
+    smooth = torch.exp(0.3 * torch.randn(H, generator=torch.Generator().manual_seed(H)))
+    for i, (post, pre, gate) in enumerate([(True, True, "row"), (False, True, "each"), (True, False, "channel")]):
+        few = _sandwich_inputs(211, H, dtype, T + i, post, pre, gate, dtype_name == "f16")
+        at = [(torch.arange(T) * step + 3) % 211 for step in (1, 7, 5)]             # rows a workgroup apart are others
+        ins = [few[0][at[0]], few[1][at[1]], few[2], few[3] if gate == "channel" else few[3][at[2]], few[4]]
+        given = _on(dev, *ins)
+        kw = dict(gate_type=i % 2, residual_scale=0.9, branch_scale=0.25)
+        if pre:
+            kw["smooth_scale"] = smooth.to(dev)
+        whole = aclnn.moe_sandwich_norm(*given, quantise=pre, output_rstd=True, **kw)
+        _check_sandwich(*[t[-40:] if j in (0, 1) or j == 3 and gate != "channel" else t for j, t in enumerate(ins)],
+                        [None if t is None else t[-40:] for t in whole], i % 2, 0.9, 0.25, 1e-6, smooth if pre else None)
+        for begin in range(0, T, 200):
+            part = slice(begin, begin + 200)
+            alone = aclnn.moe_sandwich_norm(given[0][part], given[1][part], given[2], given[3] if gate == "channel" else given[3][part], given[4], quantise=pre,
+                                            output_rstd=True, **kw)
+            for a, b in zip(alone, whole):
+                assert (a is None) == (b is None) and (a is None or torch.equal(a, b[part])), begin
+        for which in (0, 1):
+            pair = [given[0].clone(), given[1].clone()]
+            out = (pair[which],) + tuple(None if t is None else torch.empty_like(t) for t in whole[1:])
+            for a, b in zip(aclnn.moe_sandwich_norm(*pair, *given[2:], out=out, **kw), whole):
+                assert (a is None) == (b is None) and (a is None or torch.equal(a, b))
+            assert torch.equal(pair[1 - which], given[1 - which])
+
+
 def test_sandwich_gate_of_one_row_for_all(aclnn, dev):
     """A gate with a stride of zero over the rows is read as a gate of its own for each of them."""
     T, H = 19, 1000
