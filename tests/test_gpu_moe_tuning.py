@@ -712,6 +712,14 @@ def test_sandwich_grad_outputs_alone(aclnn, dev, H):
         _check_sandwich_grad(aclnn.moe_sandwich_norm_grad(*only), *[None if t is None else t.cpu() for t in only], 0, 1.0, 1.0)
 
 
+@pytest.mark.parametrize("T,H", [(1100000, 7), (1100000, 3)])
+def test_sandwich_grad_columns_of_long_batches(aclnn, dev, T, H):
+    """So many rows that a group of the columns' sums has 512 of them, an element at a time."""
+    for gate, dtype in [("channel", torch.float32), ("row", torch.bfloat16)]:
+        ins = _grad_inputs(T, H, dtype, H, True, True, gate, False, 1)
+        _check_sandwich_grad(aclnn.moe_sandwich_norm_grad(*_on(dev, *ins), gate_type=1), *ins, 1, 1.0, 1.0)
+
+
 def test_sandwich_grad_strides_and_offsets(aclnn, dev):
     for H in (1001, 4096, 9000):
         ins = _on(dev, *_grad_inputs(9, H, torch.bfloat16, H, True, True, "each", False))
@@ -860,6 +868,36 @@ def test_behind_two_to_the_31_elements(aclnn, dev):
     tol = 2 * _norm_error(H) + 20 * U
     for g, (value, mass) in zip(grads[:2], want[:2]):
         _within(g[-30:], value, tol * mass + _half(g.dtype) * (value.abs() + tol * mass) + _tiny(g.dtype))
+
+
+def test_column_sums_behind_two_to_the_31_elements(aclnn, dev):
+    """Rows of which all but the last are alike: what they add to the columns has a closed form."""
+    T, H, n = 530000, 4096, 30                              # 2.17e9 values
+    x = torch.zeros((T, H), dtype=torch.bfloat16, device=dev)
+    ones = torch.ones((T, H), dtype=torch.bfloat16, device=dev)
+    ins = _grad_inputs(n, H, torch.bfloat16, 4, True, True, "channel", False)
+    sums, norm_grad = ones.clone(), ones.clone()
+    x[-n:], sums[-n:], ones[-n:], norm_grad[-n:] = [t.to(dev) for t in ins[:4]]
+    post_rstd, pre_rstd = torch.full((T,), 3.0, device=dev), torch.full((T,), 0.5, device=dev)
+    post_rstd[-n:], pre_rstd[-n:] = ins[7].to(dev), ins[8].to(dev)
+    post, gate, pre = ins[4:7]
+    out = (None, None) + tuple(torch.empty(H, device=dev) for _ in range(3))
+    got = aclnn.moe_sandwich_norm_grad(x, sums, ones, norm_grad, *_on(dev, post, gate, pre), post_rstd, pre_rstd, out=out)[2:]
+    want = list(_sandwich_grad_want(*ins, 0, 1.0, 1.0)[2:])
+    # The rows alike have x = 0: nothing for the post norm and the gate; the pre norm gets 1 * 1 * 0.5 a row.
+    want[2] = want[2][0] + (T - n) * 0.5, want[2][1] + (T - n) * 0.5
+    tol = 2 * _norm_error(H) + (512 + 2 + 20) * U
+    for g, (value, mass) in zip(got, want):
+        _within(g, value, tol * mass + _half(g.dtype) * (value.abs() + tol * mass))
+    # and with a value there: a row has v = d S = 1 + 0.5 (pre - 0.5 mean(pre) 0.5), x^ = 0.25 * 3
+    x[:-n] = 0.25
+    got = aclnn.moe_sandwich_norm_grad(x, sums, ones, norm_grad, *_on(dev, post, gate, pre), post_rstd, pre_rstd, out=out)[2:]
+    p, o, g = pre.double(), post.double(), gate.double()
+    v, m = 1 + 0.5 * (p - 0.25 * p.mean()), 1 + 0.5 * (p.abs() + 0.25 * p.abs().mean())
+    first = _sandwich_grad_want(*ins, 0, 1.0, 1.0)[2:4]
+    for got_, (value, mass), one, size in zip(got[:2], first, [v * g * 0.75, v * 0.75 * o], [m * g.abs() * 0.75, m * 0.75 * o.abs()]):
+        value, mass = value + (T - n) * one, mass + (T - n) * size
+        _within(got_, value, tol * mass + _half(got_.dtype) * (value.abs() + tol * mass))
 
 
 # ------------------------------------------------------------------------------------------------ together
