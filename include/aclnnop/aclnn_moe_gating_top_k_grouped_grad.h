@@ -10,7 +10,8 @@
  * and, for rows of sequence s, with r and n as in aclnn_moe_balance_loss.h, added to it:
  *   dr_e = lossGrad_s * E / (k n^2) * counts_se
  *   r (dr - sum_e dr_e r_e)  (softmax),  r (1 - p) (dr - sum_e dr_e r_e)  (sigmoid)
- * A row whose first id lies outside [0, E) has zeros; another such id has no part in the sums; with renorm a row whose picked p are all zero has dp = 0.
+ * A row whose first id lies outside [0, E) has zeros; another such id has no part in the sums; with renorm a row whose picked p are all zero in 64 bits (the
+ * choice has its weights in them) has dp = 0; picked p that only fp32 loses have their shares all the same.
  * Rows in no sequence have no gradient of the loss.  Everything is fp32, rounded once to xGrad's type.
  *
  * x, expertIdx, seqOffsetsOptional: as aclnnMoeBalanceLoss takes them; yGradOptional of x's type or FLOAT, expertIdx's extents; lossGradOptional FLOAT [S],

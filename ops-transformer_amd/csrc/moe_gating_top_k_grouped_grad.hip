@@ -150,11 +150,13 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
             sum += p[i];
             shared = fmaf(shareGrad[i], p[i], shared);
         }
-        if (weights) {
+        // The lane's part of the picks' sums, of scores that go through LDS.
+        auto pickSums = [&](const float (&s)[kEach]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int q = 0; q < kPieces; ++q) scores[wave][side][Row::At(q, l) / 4] = float4{p[4 * q], p[4 * q + 1], p[4 * q + 2], p[4 * q + 3]};
+            for (int q = 0; q < kPieces; ++q) scores[wave][side][Row::At(q, l) / 4] = float4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             __builtin_amdgcn_wave_barrier();
+            score = pickedSum = weighted = 0.f;
             if (isExpert(now.id)) {
                 score = scoreOf[now.id];
                 pickedSum = score;
@@ -166,12 +168,41 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
                 pickedSum += scoreOf[id];
                 weighted = fmaf(yGradOf(pick + j), scoreOf[id], weighted);
             }
-        }
+        };
+        if (weights) pickSums(p);
         sum = SumOver<kLanes>(sum);
         shared = SumOver<kLanes>(shared);
         if (weights) {
             pickedSum = SumOver<kLanes>(pickedSum);
             weighted = SumOver<kLanes>(weighted);
+        }
+        float eps = kSigmoid ? a.eps : a.eps * sum;  // beside the picks' scores as they are held
+        if (__builtin_expect(weights && a.renorm && pickedSum < kLostSum, 0)) {
+            // Rare (the lanes of a row agree): scores, or their products with yGrad, are nearly or wholly lost in fp32.  They are taken from the largest pick
+            // then instead of from the row's top, or from 1.  (16384 x 256: 1 % of its time for the branch, 3 % of the weights' alone.)
+            const X* const logits = xRows + static_cast<uint32_t>(row) * static_cast<uint32_t>(a.experts);
+            float top = isExpert(now.id) ? Codec::Load(logits[now.id]) : -INFINITY;
+            for (int j = l + kLanes; j < a.k; j += kLanes) {
+                const int32_t id = idxRows[pick + j];
+                if (isExpert(id)) top = fmaxf(top, Codec::Load(logits[id]));
+            }
+            top = MaxOver<kLanes>(top);
+            const float up = (kSigmoid ? 0.f : TopOf<kLanes>(x)) - top;  // e^up times as large
+            if (up > kLostIn64) {
+                pickedSum = 0.f;
+            } else {
+                const ExpFrom e(top);
+                float s[kEach];
+#pragma unroll
+                for (int i = 0; i < kEach; ++i) s[i] = kSigmoid ? e(x[i]) * rest[i] : e(x[i]);
+                pickSums(s);
+                pickedSum = SumOver<kLanes>(pickedSum);
+                weighted = SumOver<kLanes>(weighted);
+                const float half = ExpFrom(-0.5f * up)(0.f);
+                eps = a.eps * half * half * (kSigmoid ? 1.f : sum);
+                if (a.eps == 0.f) eps = 0.f;
+                else if (up > 176.f || !(eps < 1e37f)) eps = pickedSum = 0.f;  // beside eps they are below fp32's range
+            }
         }
         const float inverse = sum == 0.f ? 0.f : Reciprocal(sum);
         if constexpr (!kSigmoid) {
@@ -182,12 +213,11 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
         if (weights) {
             // The picked scores are divided once, softmax's by the row's sum or by the picked ones': first by the one and then by the other, small ones
             // would be lost between.
-            const float whole = kSigmoid ? 1.f : sum;
             float mean = 0.f, part = kSigmoid ? 1.f : inverse, all = a.factor * (weighted * part);
             if (a.renorm) {
-                part = pickedSum < 0x1p-126f ? 0.f : __builtin_amdgcn_rcpf(fmaf(a.eps, whole, pickedSum));
+                part = pickedSum == 0.f ? 0.f : Reciprocal(eps + pickedSum);
                 mean = weighted * part;
-                all = a.factor * mean * (a.eps * whole * part);
+                all = a.factor * mean * (eps * part);
             }
             if (isExpert(now.id)) atomicAdd(pickedOf + now.id, a.factor * (score * part) * (now.y - mean));
             for (int j = l + kLanes; j < a.k; j += kLanes) {

@@ -245,6 +245,8 @@ __device__ __forceinline__ void SoftmaxOf(float (&v)[kEach]) {
 // Shares of the row's sum of sigmoid scores.  Where that sum is below kLostSum the scores are nearly or wholly lost in fp32: they are in the proportions of
 // e^x then, which is the softmax (a row without a logit above -inf has zeros).
 constexpr float kLostSum = 0x1p-60f;
+// e^-v of a v above this is zero in 64 bits, too.
+constexpr float kLostIn64 = 745.f;
 template <int kLanes, int kEach>
 __device__ __forceinline__ void LostSharesOf(const float (&x)[kEach], float (&share)[kEach]) {
 #pragma unroll

@@ -364,6 +364,35 @@ def test_grad_of_picks_with_small_scores(aclnn, dev, E, score):
         _check_grad(got, x, idx, dy, None, None, None, None, score, 1, 1.0, eps)
 
 
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("E,k", [(8, 2), (16, 12), (96, 4), (256, 8), (2048, 4)])
+def test_grad_of_picks_whose_scores_fp32_loses(aclnn, dev, E, k, score):
+    """Weights of picks far below the row's top, or of sigmoid scores below fp32's range: the choice has their shares in 64 bits, and so has the gradient; and small
+    gradients of small scores, whose products fp32 does not hold.  Every second row is an ordinary one."""
+    T = 75
+    x, _ = _router_inputs(T, E, k, torch.float32, 27)
+    g = torch.Generator().manual_seed(28)
+    idx = torch.stack([torch.randperm(E, generator=g)[:k] for _ in range(T)]).int()
+    idx[4, 1], idx[6, 0], idx[9, 1] = -1, E, idx[9, 0]
+    dy = torch.randn((T, k), generator=g)
+    for down, size, eps in [(80.0, 1e-8, 0.0), (60.0, 1e-25, 1e-20), (95.0, 1.0, 0.0), (100.0, 1e-3, 2.0 ** -140), (95.0, 1.0, 1e-20), (400.0, 1.0, 0.0),
+                            (400.0, 1.0, 1e-20), (45.0, 1.0, 1e-20)]:
+        low = x.clone()
+        low[::2].scatter_add_(1, idx[::2].long().clamp(0, E - 1), torch.full((T // 2 + 1, k), -down))
+        low[10, idx[10].long()] = torch.finfo(torch.float32).min                     # nothing is left of these in 64 bits either
+        low[12, idx[12].long()] = -math.inf
+        low[14, idx[14, 0].long()] = -math.inf
+        y = dy * size
+        got = aclnn.moe_gating_top_k_grouped_grad(*_on(dev, low, idx, y), score_type=score, renorm=1, eps=eps)
+        want, mass = _grad_want(low, idx, y, None, None, None, None, score, 1, 1.0, eps)
+        kept = torch.isfinite(low) & (low > -1e30)
+        tol = (6 * (2 * (down + 10) + E / 64 + 20) + 10) * U
+        _within(got, want, tol * mass + U * want.abs() + 2.0 ** -126 * kept + 2.0 ** -100 * mass)
+        assert not got[10].any() and not got[12].any() and not got[6].any()
+        for again in range(2):
+            assert torch.equal(got, aclnn.moe_gating_top_k_grouped_grad(*_on(dev, low, idx, y), score_type=score, renorm=1, eps=eps))
+
+
 def test_grad_against_differences(aclnn, dev):
     """Along random directions: the definition's central differences in 64 bits (their own error: h^2 of third derivatives below 1, and 2^-53 / h of the value)."""
     T, E, k = 40, 24, 3
