@@ -15,7 +15,8 @@
  * NaN.  Probabilities are summed in fp32 over up to 4096 rows, those sums in 64 bits, all in a fixed order: equal calls
  * give equal bits.
  *
- * x: FLOAT, FLOAT16 or BF16, rank 2 or 3, at most 2^26 rows and 2048 experts; expertIdx INT32 of x's extents with the last replaced by k, 1 to 64;
+ * x: FLOAT, FLOAT16 or BF16, rank 2 or 3, at most 2^26 rows and 2048 experts; expertIdx INT32 of x's extents with the last replaced by k, 1 to 64, at most
+ * 2^31 - 1 ids in all, of which one expert may be every one;
  * seqOffsetsOptional INT32 or INT64 [S + 1], S from 1 to 2^20, not falling (else: unspecified values, no access outside the tensors); lossOut FLOAT [S]; countsOut
  * INT32 [S, E]; rowsOut INT32 [S]; probOutOptional FLOAT [S, E] ([1] and [1, E] without seqOffsets).  Inputs may be strided views; outputs are contiguous
  * and share no memory with an input or with each other.  The workspace is 16-byte aligned and one per stream.

@@ -416,6 +416,7 @@ extern "C" aclnnStatus aclnnMoeBalanceLossGetWorkspaceSize(const aclTensor* x, c
     int64_t rows = 0, experts = 0, k = 0, sequences = 0;
     const aclnnStatus router = CheckRouterRows(x, expertIdx, seqOffsetsOptional, scoreType, &rows, &experts, &k, &sequences);
     if (router != ACLNN_SUCCESS) return router;
+    OPAPI_CHECK(rows * k <= 2147483647ll, kInvalid, "x has %lld rows of %lld picks; counts in INT32 hold up to 2147483647 ids", (long long)rows, (long long)k);
     OPAPI_CHECK(lossOut->dtype == ACL_FLOAT && HasExtents(lossOut, {sequences}), kInvalid, "lossOut %s must be FLOAT [%lld]", ShapeStr(lossOut).c_str(),
                 (long long)sequences);
     OPAPI_CHECK(rowsOut->dtype == ACL_INT32 && HasExtents(rowsOut, {sequences}), kInvalid, "rowsOut %s must be INT32 [%lld]", ShapeStr(rowsOut).c_str(),

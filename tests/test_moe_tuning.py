@@ -87,6 +87,14 @@ def test_balance_invalid(aclnn, kw, fragment):
     _check_invalid(aclnn, "aclnnMoeBalanceLoss", _balance(aclnn, **kw), fragment)
 
 
+def test_balance_counts_fit_their_type(aclnn):
+    """One expert may be every id of every row: as many as INT32 holds are taken, no more."""
+    for rows, k in [((1 << 25) - 1, 64), (1 << 26, 31)]:
+        assert _status(aclnn, "aclnnMoeBalanceLoss", _balance(aclnn, shape=(rows, 4), k=k, x_at=1 << 45, idx_at=1 << 46))[0] == 0
+    for rows, k in [(1 << 25, 64), (1 << 26, 32), ((1 << 31) // 63 + 1, 63)]:
+        _check_invalid(aclnn, "aclnnMoeBalanceLoss", _balance(aclnn, shape=(rows, 4), k=k, sequences=3), "2147483647 ids")
+
+
 def test_balance_nulls(aclnn):
     for pos in (0, 1, 4, 5, 6):
         args = _balance(aclnn)
