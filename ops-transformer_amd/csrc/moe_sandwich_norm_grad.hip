@@ -35,7 +35,7 @@ struct SandwichGradArgs {
     float* postGammaGrad;    // optional
     float* channelGrad;      // optional: gateGrad of a gate per channel
     float* columnSums[kColumnSums];  // workspace: [groups, cols] each, null where not wanted
-    float* rowMeans;         // workspace of rows in two passes: [rows, 2]
+    float* rowMeans;         // workspace of longer rows: [rows]
     int64_t rows;
     int64_t cols;
     int64_t groups;          // that columns are summed over
@@ -348,7 +348,7 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
     }
 }
 
-// Longer rows, read behind each sum again: a workgroup a row, which leaves the row's two means for the columns' sums.
+// Longer rows, read behind each sum again: a workgroup a row, which leaves the pre norm's mean of the row for the columns' sums.
 constexpr int kAnyThreads = 256;
 
 __device__ __forceinline__ double SumOfGroup(double v, double (&lds)[kAnyThreads / kWave]) {
