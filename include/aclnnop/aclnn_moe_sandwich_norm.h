@@ -13,11 +13,11 @@
  * Rows of zeros, of a NaN or an infinity, and what epsilon 0 does to rows of nothing: as in aclnn_moe_add_rms_norm_quant.h (a factor of 0 stands for 1 / 0).
  *
  * x, residual, sumOut, normOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents, at most 2^26 rows.  postGammaOptional and preGammaOptional
- * [H] of x's type or FLOAT, equal types; normOut, yOut, smoothScale and preRstdOut need preGamma, postRstdOut needs postGamma.  gateOptional, by its extents: [H] (a
- * value per channel, of the gammas' type; of x's type or FLOAT without one), x's extents with the last one 1 (a value per row; x's type or FLOAT), or x's extents
- * (a value each; x's type; where H is 1, a value per row).  smoothScaleOptional FLOAT [H]; yOutOptional INT8 of x's extents with scaleOutOptional; scaleOutOptional, postRstdOutOptional and
- * preRstdOutOptional FLOAT of x's extents without the last.  Inputs may be strided views; outputs are contiguous.  sumOut may be x's or residual's own memory,
- * entirely; no other output may share memory with an input or another output.
+ * [H] of x's type or FLOAT, equal types; normOut, yOut, smoothScale and preRstdOut need preGamma, postRstdOut needs postGamma.  gateOptional, by its extents:
+ * [H] (a value per channel, of the gammas' type; of x's type or FLOAT without one), x's extents with the last one 1 (a value per row; x's type or FLOAT), or
+ * x's extents (a value each; x's type; where H is 1, a value per row).  smoothScaleOptional FLOAT [H]; yOutOptional INT8 of x's extents with scaleOutOptional;
+ * scaleOutOptional, postRstdOutOptional and preRstdOutOptional FLOAT of x's extents without the last.  Inputs may be strided views; outputs are contiguous.
+ * sumOut may be x's or residual's own memory, entirely; no other output may share memory with an input or another output.
  */
 #ifndef OPS_TRANSFORMER_AMD_ACLNN_MOE_SANDWICH_NORM_H_
 #define OPS_TRANSFORMER_AMD_ACLNN_MOE_SANDWICH_NORM_H_

@@ -12,8 +12,8 @@
  * calls give equal bits.
  *
  * x, sum, sumGradOptional, normGradOptional, residualGradOutOptional, xGradOutOptional: FLOAT, FLOAT16 or BF16 (equal), rank 2 or 3, equal extents, at
- * most 2^26 rows of at most 2^24 values; gammas and gate as there.  normGrad, preGamma and preRstd belong together, and sum with them (not read without), postGamma and postRstd
- * do; sumGrad or normGrad or both.   postRstdOptional, preRstdOptional FLOAT of x's extents without the last.  postGammaGradOutOptional and
+ * most 2^26 rows of at most 2^24 values; gammas and gate as there.  normGrad, preGamma and preRstd belong together, and sum with them (not read without),
+ * postGamma and postRstd do; sumGrad or normGrad or both.  postRstdOptional, preRstdOptional FLOAT of x's extents without the last.  postGammaGradOutOptional and
  * preGammaGradOutOptional FLOAT [H]; gateGradOutOptional FLOAT of the gate's extents where it is shared, of x's type where it is not; each with its input
  * only.  At least one output.  Inputs may be strided views; outputs are contiguous and share no memory with an input or with each other.  The workspace is
  * 16-byte aligned and one per stream.

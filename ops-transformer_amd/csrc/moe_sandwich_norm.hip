@@ -3,8 +3,8 @@
 // Two reductions over a row, the second on what the first one settles: the row stays in registers from its load to its last output, so it crosses the
 // memory once, and the memory bounds it: 8192 x 7168 bf16 with a gate per channel (470 MB) 87.9 us, 5.35 TB/s, part of them from the memory-side cache;
 // 4096 x 12000 77.5 (393 MB, 5.1 TB/s); 64 x 4096 a launch, 5.0.  Rows of 16 bits off the four-byte grid take 1.4 times as long (4096 x 7167 63, where their
-// bytes take 45): their loads and stores of eight elements straddle words.  Sums, factors, u, v and n are fp32; what is rounded is s (to the stream's type, and that rounded value is what is normalised), n where it
-// leaves, and y, which is made as aclnnMoeAddRmsNormQuant makes it (norm_rows.h).
+// bytes take 45): their loads and stores of eight elements straddle words.  Sums, factors, u, v and n are fp32; what is rounded is s (to the stream's type, and
+// that rounded value is what is normalised), n where it leaves, and y, which is made as aclnnMoeAddRmsNormQuant makes it (norm_rows.h).
 #include "sandwich_norm.h"
 
 #include "aclnnop/aclnn_moe_sandwich_norm.h"
@@ -52,9 +52,6 @@ __device__ __forceinline__ float RowGate(const SandwichArgs& a, int64_t row) {
 // present one is begun (where the registers hold both, else before it is reduced the second time).  Gammas and a gate per channel stay in registers.
 // Up to 4096 values a lane has one piece, up to 12288 two on up to 768 lanes, up to 16384 four on 512: four of 9000 columns' take 71.5 us at 4096 rows
 // where two take 60.9, and more than 768 lanes have no registers for two.
-constexpr int kFewThreads = 512, kManyThreads = 768;
-constexpr int kMaxPackets = 4;
-constexpr int64_t kCus = 256;
 
 template <typename Codec, int kPackets, bool kGate>
 struct NormRows {
@@ -242,18 +239,6 @@ __global__ __launch_bounds__(kThreads) void SandwichPacketsKernel(SandwichArgs a
 
 // Rows of any length: a workgroup per row, one element at a time, the row read again behind each reduction (from the sum once that is written, by the
 // same lane: it may lie in x's or the residual's memory), squares added up in 64 bits.
-constexpr int kAnyThreads = 256;
-
-__device__ __forceinline__ double SumOfGroup(double v, double (&lds)[kAnyThreads / kWave]) {
-    v = WaveSum(v);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < kAnyThreads / kWave; ++w) v += lds[w];
-    return v;
-}
-
 template <typename Codec, typename Gamma>
 __global__ __launch_bounds__(kAnyThreads) void SandwichAnyKernel(SandwichArgs a) {
     using S = typename Codec::Storage;
@@ -326,7 +311,9 @@ class SandwichExecutor : public aclOpExecutor {
         // 42.7, 53.4 and 42.4; 8192 x 4096 38.4 with two, with one 42.6, with four 41; 8192 x 1024 13.2 with eight, with ten 14.3).  Two: 12 waves (8192 x 7168
         // 87.9 with one workgroup, with two 93.1; 8192 x 4608 59.9 with two, with three 67.7), and two workgroups where the tail's instructions want company
         // (4096 x 7167 63.0, with one 82).
-        const int64_t each = kPackets == 1 ? (threads > 4 * kWave ? 18 : 16) * kWave / threads : tail && kThreads == kFewThreads ? 2 : std::max(1, 12 * kWave / threads);
+        const int64_t each = kPackets == 1                     ? (threads > 4 * kWave ? 18 : 16) * kWave / threads
+                             : tail && kThreads == kFewThreads ? 2
+                                                               : std::max(1, 12 * kWave / threads);
         const int64_t groups = std::min<int64_t>(args.rows, kCus * each);
         const dim3 grid(static_cast<unsigned>(groups));
         if (tail) hipLaunchKernelGGL((SandwichPacketsKernel<Codec, Gamma, kPackets, kThreads, kGate, true>), grid, dim3(threads), 0, stream, args);
@@ -348,7 +335,7 @@ class SandwichExecutor : public aclOpExecutor {
             using Codec = decltype(codec);
             using Gamma = decltype(gamma);
             const int64_t lanes = (args.cols + 7) / 8;
-            if (args.cols < 8 || lanes > kMaxPackets * kFewThreads) {
+            if (args.cols < 8 || args.cols > kPacketCols) {
                 hipLaunchKernelGGL((SandwichAnyKernel<Codec, Gamma>), GridOf(args.rows), dim3(kAnyThreads), 0, stream, args);
             } else if (lanes <= kFewThreads) {
                 ForGate<Codec, Gamma, 1, kFewThreads>(stream);

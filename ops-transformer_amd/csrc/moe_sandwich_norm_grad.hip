@@ -58,8 +58,6 @@ __device__ __forceinline__ float RawRowGate(const SandwichGradArgs& a, int64_t r
     return a.gateIsFloat ? static_cast<const float*>(a.gate)[row] : Codec::Load(static_cast<const typename Codec::Storage*>(a.gate)[row]);
 }
 
-constexpr int kFewThreads = 512, kManyThreads = 768;
-
 // What is read of a row.
 template <typename Codec, int kPackets, bool kGate>
 struct GradRows {
@@ -349,18 +347,6 @@ __global__ __launch_bounds__(kThreads) void SandwichGradKernel(SandwichGradArgs 
 }
 
 // Longer rows, read behind each sum again: a workgroup a row, which leaves the pre norm's mean of the row for the columns' sums.
-constexpr int kAnyThreads = 256;
-
-__device__ __forceinline__ double SumOfGroup(double v, double (&lds)[kAnyThreads / kWave]) {
-    v = WaveSum(v);
-    __syncthreads();
-    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    v = 0.0;
-    for (int w = 0; w < kAnyThreads / kWave; ++w) v += lds[w];
-    return v;
-}
-
 // What the two kernels of long rows make of an element.
 template <typename Codec, typename Gamma>
 struct Element {
@@ -488,9 +474,6 @@ __global__ __launch_bounds__(kFinishThreads) void SandwichGradFinishKernel(Sandw
 // Rows of eight to 16384 values are one workgroup's at a time: one piece a lane up to 4096 values, two on up to 512 lanes, two on up to 768, whose 168 registers
 // hold them with the sums in LDS (4096 x 12000 bf16 138 us, 2048 x 12000 fp32 139; four pieces on 384 lanes 157 and 238; two on 1024, with 128 registers, 202
 // and 211), and four above 12288 values (3000 x 16384 156 us; an element at a time 755).
-constexpr int64_t kCus = 256;
-constexpr int kMaxPackets = 4;
-constexpr int64_t kPacketCols = 8ll * kFewThreads * kMaxPackets;
 
 class SandwichGradExecutor : public aclOpExecutor {
    public:
@@ -560,10 +543,10 @@ class SandwichGradExecutor : public aclOpExecutor {
     template <typename Codec, typename Gamma, int kPackets, int kThreads, int kGate>
     hipError_t LaunchPackets(hipStream_t stream) const {
         const bool tail = args.cols % 8 != 0;
-        if (args.pre != nullptr) {
-            return tail ? LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, true, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, true, false>(stream);
-        }
-        return tail ? LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, false, true>(stream) : LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, false, false>(stream);
+        if (args.pre != nullptr && tail) return LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, true, true>(stream);
+        if (args.pre != nullptr) return LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, true, false>(stream);
+        if (tail) return LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, false, true>(stream);
+        return LaunchKernel<Codec, Gamma, kPackets, kThreads, kGate, false, false>(stream);
     }
 
     template <typename Codec, typename Gamma, int kPackets, int kThreads>

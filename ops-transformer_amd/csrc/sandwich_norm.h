@@ -65,6 +65,24 @@ __device__ __forceinline__ void HoldPacked(Packet<Codec>& piece) {
     for (uint4& q : piece.q) asm volatile("" : "+v"(q.x), "+v"(q.y), "+v"(q.z), "+v"(q.w));
 }
 
+// Rows of eight to kPacketCols values lie on a workgroup's lanes in pieces of eight: one a lane on up to kFewThreads lanes, two on these or up to kManyThreads, four
+// on kFewThreads.  Others are read an element at a time by kAnyThreads lanes.
+constexpr int kFewThreads = 512, kManyThreads = 768, kAnyThreads = 256;
+constexpr int kMaxPackets = 4;
+constexpr int64_t kPacketCols = 8ll * kFewThreads * kMaxPackets;
+constexpr int64_t kCus = 256;
+
+// The sum over a workgroup of kAnyThreads, the same bits in every lane.
+__device__ __forceinline__ double SumOfGroup(double v, double (&lds)[kAnyThreads / kWave]) {
+    v = WaveSum(v);
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < kAnyThreads / kWave; ++w) v += lds[w];
+    return v;
+}
+
 // Where a lane's pieces of eight elements lie in a row of `cols`, at least eight.  Every lane has each of its pieces: one that would end behind the row is the
 // row's last eight elements, the first `skip` of which are other lanes' (all eight of a piece that would begin behind it; kTail: cols is no multiple of eight,
 // else there are no others).  So loads are without a branch, the compiler knows how many there are, and a wait for one row's need not be one for the
