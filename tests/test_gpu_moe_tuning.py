@@ -625,6 +625,28 @@ def test_sandwich_gate_of_one_row_for_all(aclnn, dev):
     _check_sandwich_grad(aclnn.moe_sandwich_norm_grad(*given, gate_type=1), *ins, 1, 1.0, 1.0)
 
 
+@pytest.mark.parametrize("H", [1000, 20000])
+def test_sandwich_gates_far_from_zero(aclnn, dev, H):
+    """Sigmoid gates and their slopes from nearly shut to open, each to its own precision: |gate| + 4 units for the gate, as many for 1 less it, 6 for products."""
+    T = 6
+    g = torch.Generator().manual_seed(H)
+    x, ds = torch.randn((T, H), generator=g), torch.randn((T, H), generator=g)
+    gate = 100 * (2 * torch.rand((T, H), generator=g) - 1)
+    gate[0, :6] = torch.tensor([math.inf, -math.inf, torch.finfo(torch.float32).max, torch.finfo(torch.float32).min, 0.0, -0.0])
+    open_, shut = torch.sigmoid(gate.double()), torch.sigmoid(-gate.double())
+    tol = (2 * gate.double().abs().clamp(max=90) + 8 + 6) * U
+    lost = 2.0 ** -126 * (1 + x.double().abs()) * (1 + ds.double().abs())
+    total = aclnn.moe_sandwich_norm(x.to(dev), torch.zeros((T, H), device=dev), gate=gate.to(dev), gate_type=1)[0]
+    _within(total, x.double() * open_, tol * (x.double() * open_).abs() + lost)
+    got = aclnn.moe_sandwich_norm_grad(x.to(dev), sum_grad=ds.to(dev), gate=gate.to(dev), gate_type=1)
+    _within(got[0], ds.double() * open_, tol * (ds.double() * open_).abs() + lost)
+    slope = ds.double() * x.double() * open_ * shut
+    _within(got[3], slope, tol * slope.abs() + lost)
+    row = gate[:, 6:7].clone()
+    one = aclnn.moe_sandwich_norm(x.to(dev), torch.zeros((T, H), device=dev), gate=row.to(dev), gate_type=1)[0]
+    _within(one, x.double() * open_[:, 6:7], tol[:, 6:7] * (x.double() * open_[:, 6:7]).abs() + lost)
+
+
 def test_sandwich_long_batches_and_empty_ones(aclnn, dev):
     ins = _sandwich_inputs(70000, 64, torch.bfloat16, 3, gate="each")
     _check_sandwich(*ins, aclnn.moe_sandwich_norm(*_on(dev, *ins)))
