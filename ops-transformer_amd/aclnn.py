@@ -532,7 +532,8 @@ def moe_gating_top_k_grouped(x, k, bias=None, finished=None, k_group=1, group_co
 def moe_balance_loss(x, expert_idx, seq_offsets=None, score_type=0, output_prob=True, out=None, workspace=None):
     """aclnnMoeBalanceLoss.  Returns (loss fp32 [S], counts int32 [S, E], rows int32 [S], prob fp32 [S, E] or None) of router logits x [..., E] and the
     experts picked from them, int32 [..., k], over the S sequences that seq_offsets [S + 1] (int32 or int64) cut the rows into, or over all rows as
-    one.  Rows whose first id is no expert (finished ones) and rows in no sequence do not count.  score_type 0 softmax, 1 sigmoid."""
+    one.  Rows whose first id is no expert (finished ones) and rows in no sequence do not count.  score_type 0 softmax, 1 sigmoid.  Nothing is recorded for
+    torch.autograd: the gradient is moe_gating_top_k_grouped_grad's."""
     if out is not None:
         loss, counts, rows, prob = out
     else:
@@ -562,7 +563,8 @@ def moe_sandwich_norm(x, residual, post_gamma=None, gate=None, pre_gamma=None, s
     """aclnnMoeSandwichNorm.  Returns (sum, norm, y int8, scale fp32, post_rstd fp32, pre_rstd fp32), None for those that are not there:
     sum = residual_scale * residual + branch_scale * gate * rms_norm(x) * post_gamma in x's dtype, norm = rms_norm(sum) * pre_gamma, its int8 rows with
     a scale each, and the factors 1 / sqrt(mean + epsilon) of both norms, which moe_sandwich_norm_grad takes.  gate is [H], [..., 1] or [..., H];
-    gate_type 1 takes its sigmoid.  ``out`` may carry the outputs in that order, None for those that are not wanted; its sum may be x or residual."""
+    gate_type 1 takes its sigmoid.  ``out`` may carry the outputs in that order, None for those that are not wanted; its sum may be x or residual.
+    Nothing is recorded for torch.autograd: the gradients are moe_sandwich_norm_grad's."""
     if out is not None:
         total, norm, y, scale, post_rstd, pre_rstd = out
     else:

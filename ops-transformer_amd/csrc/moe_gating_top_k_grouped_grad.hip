@@ -5,9 +5,9 @@
 // F M (1 - sum p / t) = F M eps / t: formed so, it is not the difference of two sums that cancel.  The picks' p dp goes through LDS from the lane that has
 // the pick to the one that has the expert.
 //
-// What bounds it: few rows, a launch and two round trips (256 x 8: 4.2 us, most of it the host's); many, vector instructions (16384 x 256 fp32: 10.4 us,
-// 60 % of the SIMDs' issue, where the bytes, 34.6 MB, take 6.7 at a copy's rate): a score is six instructions, its gradient ten, and four sums
-// cross the lanes.
+// What bounds it: few rows, a launch and two round trips (256 x 8: 4.4 us, most of it the host's); many, no one thing (16384 x 256 fp32: 10.4 us, where the
+// bytes, 34.6 MB, take 6.7 at a copy's rate): a score is six instructions, its gradient ten, and four sums cross the lanes, together 63 % of the SIMDs'
+// issue; and the waves wait 52 % of their cycles, for those sums and for the offsets and then the sequence's tables in front of their four rows.
 #include "router_rows.h"
 
 #include "aclnnop/aclnn_moe_gating_top_k_grouped_grad.h"
@@ -281,7 +281,7 @@ class GatingGradExecutor : public aclOpExecutor {
         ForRowLayout(args.experts, [&](auto lanes, auto pieces) {
             constexpr int kLanes = decltype(lanes)::value, kPieces = decltype(pieces)::value;
             constexpr int64_t kRowsAtOnce = kWave / kLanes;
-            // As many waves as the registers let the 256 x 4 SIMDs hold at once: 16384 x 256 10.4 us, half as many 12.9, twice 10.9, four times 12.3.
+            // Four waves for each of the 256 x 4 SIMDs: 16384 x 256 10.4 us, half as many 12.9, twice 10.9, four times 12.3.
             const int64_t waves = 4 * 1024;
             int64_t each = (args.sequences.rows + waves - 1) / waves;
             each = (each + kRowsAtOnce - 1) / kRowsAtOnce * kRowsAtOnce;
