@@ -125,6 +125,8 @@ struct ExpFrom {
 
 // sigmoid(x) and 1 - sigmoid(x), each to its own precision: |x| + 4 units of 2^-24.  (Of e^-x past fp32's range the reciprocal is 0, and below a half the
 // difference from 1 is the more exact: no value needs a case of its own.)
+// What the product's rounding leaves is not carried, as ExpFrom carries it: with it balance and gradient of 16384 x 256 logits take 3 % longer, and the gradient's
+// error, 1.2e-7 in the 2-norm, is the same, since logits are small numbers; at -20 a score has 1.4e-6.
 struct Sigmoid {
     float p, rest;
 };
