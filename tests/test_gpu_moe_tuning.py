@@ -348,6 +348,34 @@ def test_grad_rows_of_unusual_values(aclnn, dev, score):
         assert not got[1].any() and not got[8].any()
 
 
+def test_grad_strides_and_ranks(aclnn, dev):
+    """Three dimensions, views of larger tensors, rows that begin on any element; a gradient of 16 bits from picks' gradients of either type."""
+    x, idx = _router_inputs((3, 50), 33, 3, torch.bfloat16, 4, finished=0.1)
+    offsets = torch.tensor([0, 61, 61, 140], dtype=torch.int64)
+    g = torch.Generator().manual_seed(4)
+    dy, dl = torch.randn(idx.shape, generator=g), torch.rand(3, generator=g)
+    _, counts, rows, _ = _balance_want(x, idx, offsets, 1)
+    want = aclnn.moe_gating_top_k_grouped_grad(*_on(dev, x, idx, dy, dl, counts, rows, offsets), score_type=1, renorm=1)
+    assert want.shape == x.shape
+    _check_grad(want, x, idx, dy, dl, counts, rows, offsets, 1, 1, 1.0, 1e-20)
+    wide = torch.zeros((3, 50, 70), dtype=torch.bfloat16, device=dev)
+    wide[..., 5:38] = x.to(dev)
+    flat = torch.zeros(150 * 33 + 1, dtype=torch.bfloat16, device=dev)
+    flat[1:] = x.to(dev).reshape(-1)
+    ids = torch.zeros((3, 50, 6), dtype=torch.int32, device=dev)
+    ids[..., ::2] = idx.to(dev)
+    picks = dy.to(dev).transpose(0, 2).contiguous().transpose(0, 2)
+    tables = torch.stack([counts, counts], -1).to(dev)[..., 1]
+    spread = torch.stack([offsets, offsets], -1).to(dev)[:, 0]
+    for logits in (wide[..., 5:38], flat[1:].view(3, 50, 33)):
+        out = torch.zeros(150 * 33 + 3, dtype=torch.bfloat16, device=dev)
+        got = aclnn.moe_gating_top_k_grouped_grad(logits, ids[..., ::2], picks, dl.to(dev), tables, rows.to(dev), spread, score_type=1, renorm=1,
+                                                  out=out[1:-2].view(3, 50, 33))
+        assert torch.equal(got, want) and not out[0] and not out[-2:].any()
+    dy16 = dy.to(torch.bfloat16)
+    _check_grad(aclnn.moe_gating_top_k_grouped_grad(*_on(dev, x, idx, dy16)), x, idx, dy16, None, None, None, None, 0, 0, 1.0, 1e-20)
+
+
 @pytest.mark.parametrize("score", [0, 1])
 @pytest.mark.parametrize("E", [96, 2048])
 def test_grad_of_picks_with_small_scores(aclnn, dev, E, score):
@@ -863,6 +891,31 @@ def test_graph_replays(aclnn, dev):
             torch.cuda.synchronize()
             for a, b in zip(outputs, want):
                 assert torch.equal(a, b), (n, replay)
+
+
+def test_two_graphs_share_a_workspace(aclnn, dev):
+    """All four operators captured twice, on unlike inputs, with one workspace; replayed in turn, every replay against the eager outputs."""
+    both = [_calls(aclnn, dev, seed) for seed in (9, 10)]
+    want = [[t.clone() for call, outputs in calls for t in (call(None), outputs)[1]] for calls in both]
+    ws = aclnn.Workspace()
+    for calls in both:                                      # as large as any of them needs
+        for call, _ in calls:
+            call(ws)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+    side = torch.cuda.Stream()
+    for graph, calls in zip(graphs, both):
+        with torch.cuda.graph(graph, stream=side):
+            for call, _ in calls:
+                call(ws)
+    for which in (0, 1, 1, 0, 1, 0):
+        for _, outputs in both[which]:
+            for t in outputs:
+                t.fill_(3)
+        graphs[which].replay()
+        torch.cuda.synchronize()
+        for a, b in zip([t for _, outputs in both[which] for t in outputs], want[which]):
+            assert torch.equal(a, b)
 
 
 def test_two_streams_at_once(aclnn, dev):
