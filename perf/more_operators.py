@@ -261,7 +261,8 @@ def _router_grad_pass(case, s):
     experts, top_k = case["experts"], case["top_k"]
     if own:
         return _operators().moe_gating_top_k_grouped_grad(
-            s["x"], s["idx"], y_grad=s["y_grad"], loss_grad=s["loss_grad"], counts=s["counts"], rows=s["rows"], seq_offsets=s["offsets"],
+            s["x"], s["idx"], y_grad=s["y_grad"], loss_grad=s["loss_grad"], counts=s["counts"], rows=s["rows"],
+            seq_offsets=None if s["loss_grad"] is None else s["offsets"],      # the sequences are the loss's
             score_type=1 if case["score"] == "sigmoid" else 0, renorm=1 if case["renorm"] else 0, routed_scaling_factor=case["factor"],
             eps=_RENORM_EPS, out=s["out"])
     x = s["x"].float()
