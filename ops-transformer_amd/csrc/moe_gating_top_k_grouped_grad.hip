@@ -31,6 +31,8 @@ struct GradArgs {
     int32_t renorm;
     float factor;
     float eps;
+    float expertsPerPick;      // experts / k, and the other way round
+    float picksPerExpert;
     int32_t waveRows;          // rows of a wave, one behind the other
 };
 
@@ -108,9 +110,12 @@ __global__ __launch_bounds__(kGradThreads) void GatingGradKernel(GradArgs a) {
         int32_t counts[kEach];
         Row::Place(raw, a.experts, l, 0, counts);
         const float n = static_cast<float>(live);
-        const float each = live > 0 ? lossGrad * (static_cast<float>(a.experts) / static_cast<float>(a.k)) / n / n : 0.f;
+        const float each = live > 0 ? lossGrad * a.expertsPerPick / n / n : 0.f;
+        // Of the counts, their distances from the even one: what all have alike gives shares, whose sum is 1, nothing, and where a batch is spread as the loss wants it
+        // the counts' own products and their mean would cancel.
+        const uint32_t even = static_cast<uint32_t>(static_cast<int32_t>(fminf(rintf(n * a.picksPerExpert), 0x1p30f)));
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) shareGrad[i] = live > 0 ? each * static_cast<float>(counts[i]) : 0.f;
+        for (int i = 0; i < kEach; ++i) shareGrad[i] = live > 0 ? each * static_cast<float>(static_cast<int32_t>(static_cast<uint32_t>(counts[i]) - even)) : 0.f;
     };
     if (balance) {
         int64_t end, beyond;
@@ -371,6 +376,8 @@ extern "C" aclnnStatus aclnnMoeGatingTopKGroupedGradGetWorkspaceSize(
     a.renorm = static_cast<int32_t>(renorm);
     a.factor = static_cast<float>(routedScalingFactor);
     a.eps = static_cast<float>(eps);
+    a.expertsPerPick = static_cast<float>(experts) / static_cast<float>(k);
+    a.picksPerExpert = static_cast<float>(k) / static_cast<float>(experts);
     ex->SealWorkspace(0);
     *workspaceSize = ex->workspaceBytes;
     *executor = ex;

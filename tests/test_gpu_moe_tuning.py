@@ -348,6 +348,32 @@ def test_grad_rows_of_unusual_values(aclnn, dev, score):
         assert not got[1].any() and not got[8].any()
 
 
+@pytest.mark.parametrize("score", [0, 1])
+@pytest.mark.parametrize("T,E,k,dtype_name", [(512, 64, 4, "f32"), (300, 8, 8, "f32"), (2000, 250, 5, "bf16"), (900, 7, 3, "f16")])
+def test_grad_of_nearly_even_counts(aclnn, dev, T, E, k, dtype_name, score):
+    """Where a batch is spread as the loss wants it, its gradient is small, and as exact as it is small: errors are taken of the counts' distances from their
+    mean, not of the counts.  Of even counts it is nothing at all."""
+    x, _ = _router_inputs(T, E, k, TORCH[dtype_name], E)
+    idx = (torch.arange(T * k).reshape(T, k) % E).int()
+    g = torch.Generator().manual_seed(E)
+    dl = torch.tensor([0.01, 3.0])
+    offsets = torch.tensor([0, T // 3, T], dtype=torch.int32)
+    rows = torch.tensor([T // 3, T - T // 3], dtype=torch.int32)
+    even = torch.tensor([1 << 9, 1 << 19], dtype=torch.int32)[:, None].expand(2, E).contiguous()
+    for counts in (even + torch.randint(-2, 3, (2, E), generator=g, dtype=torch.int32), even):
+        # rows and picks such that the mean of the counts is k n / E, as it is where every id is an expert
+        n = torch.tensor([(1 << 9) * E // k, (1 << 19) * E // k], dtype=torch.int32)
+        got = aclnn.moe_gating_top_k_grouped_grad(*_on(dev, x, idx, None, dl, counts, n, offsets), score_type=score, x_grad_dtype=torch.float32)
+        want, mass = _grad_want(x, idx, None, dl, counts.double() - counts.double().mean(1, keepdim=True), n, offsets, score, 0, 1.0, 0.0)
+        size = mass if (counts != even).any() else torch.zeros_like(mass)
+        # (the mean of k n / E rounded to a whole number is up to a half off)
+        slack = 4 * U * (dl * E / k / n / n)[:, None].double() * torch.ones(1, E)
+        slack = torch.cat([slack[:1].expand(int(rows[0]), E), slack[1:].expand(int(rows[1]), E)])
+        _within(got, want, (6 * _score_error(x) + 10 * U) * size + slack)
+        if (1 << 19) * E % k == 0 and (1 << 9) * E % k == 0 and not (counts != even).any():
+            assert not got.any()
+
+
 def test_grad_strides_and_ranks(aclnn, dev):
     """Three dimensions, views of larger tensors, rows that begin on any element; a gradient of 16 bits from picks' gradients of either type."""
     x, idx = _router_inputs((3, 50), 33, 3, torch.bfloat16, 4, finished=0.1)
