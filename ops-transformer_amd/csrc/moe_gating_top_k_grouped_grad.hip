@@ -6,7 +6,7 @@
 // the pick to the one that has the expert.
 //
 // What bounds it: few rows, a launch and two round trips (256 x 8: 4.4 us, most of it the host's); many, no one thing (16384 x 256 fp32: 10.4 us, where the
-// bytes, 34.6 MB, take 6.7 at a copy's rate): a score is six instructions, its gradient ten, and four sums cross the lanes, together 63 % of the SIMDs'
+// bytes, 34.6 MB, take 6.7 at a copy's rate): a score is six instructions, its gradient ten, and four sums cross the lanes, together 62 % of the SIMDs'
 // issue; and the waves wait 52 % of their cycles, for those sums and for the offsets and then the sequence's tables in front of their four rows.
 #include "router_rows.h"
 

@@ -2,7 +2,7 @@
 //
 // Two reductions over a row, the second on what the first one settles: the row stays in registers from its load to its last output, so it crosses the
 // memory once, and the memory bounds it: 8192 x 7168 bf16 with a gate per channel (470 MB) 87.5 us a call, 5.37 TB/s, part of them from the memory-side cache
-// (89.7 the traced kernel); 4096 x 12000 77.3 (393 MB, 5.1 TB/s); 64 x 4096 a launch, 5.0.  Rows of 16 bits off the four-byte grid take 1.3 times as long
+// (89.2 the traced kernel); 4096 x 12000 77.3 (393 MB, 5.1 TB/s); 64 x 4096 a launch, 5.0.  Rows of 16 bits off the four-byte grid take 1.3 times as long
 // (4096 x 7167 59.7, where their bytes take 45): their loads and stores of eight elements straddle words.  int8 rows take longer than their bytes, too (8192 x 7168
 // in place of 16-bit ones 113 us).  Sums, factors, u, v and n are fp32; what is rounded is s (to the stream's type, and that rounded value is what is normalised),
 // n where it leaves, and y, which is made as aclnnMoeAddRmsNormQuant makes it (norm_rows.h).
